@@ -44,10 +44,17 @@ SIGNATURES = {
     "fni8_act_and_mul_quant_f16_ws": [_P, _I, _I, _I, _C, _P, _I, _P, _P, _I, _P],
     "fni8_rmsnorm_f16": [_P, _I, _P, _I, _P, _F, _C, _I, _I, _P, _I, _P, _I, _P],
     "fni8_rmsnorm_quant_f16": [_P, _I, _P, _I, _P, _F, _C, _I, _I, _P, _I, _P, _P, _I, _P],
+    "fni8_qk_norm_rope_f16": [_P, _I, _I, _I, _P, _I, _I, _I, _I, _I, _P, _P, _F, _C, _P, _P, _I,
+                              _I, _C, _P, _P, _P],
+    "fni8_rope_append_f16": [_P, _I, _I, _I, _P, _I, _I, _I, _P, _I, _I, _I, _I, _P, _P, _F, _C,
+                             _P, _P, _I, _I, _C, _P, _P, _P, _P, _P, _I, _I, _P, _P],
+    "fni8_paged_attention_f16": [_P, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _I, _I, _P, _I, _I,
+                                 _P, _P, _I, _I, _F, _I, _P, _P, _I, _P],
 }
 STRING_FUNCS = ("fni8_strerror", "fni8_last_error", "fni8_version")
 INT64_FUNCS = {"fni8_linear_workspace_bytes": [_I, _I, _I],
-               "fni8_act_and_mul_quant_workspace_bytes": [_I, _I]}
+               "fni8_act_and_mul_quant_workspace_bytes": [_I, _I],
+               "fni8_paged_attention_workspace_bytes": [_I, _I, _I, _I, _I, _I, _I]}
 VOID_FUNCS = {"fni8_debug_coop_wait_ticks": [_I], "fni8_debug_gemm_plan": [_I, _I, _I]}
 
 _lib = None

@@ -174,6 +174,67 @@ int check_linear(const void* x, int64_t ldx, int64_t M, int64_t K, const int8_t*
     return FNI8_OK;
 }
 
+// One of the q, k, v operands of the rows between QKV and attention.
+int check_heads(const char* name, const void* x, int64_t ld, int64_t hs, int64_t H, int64_t D) {
+    if (H == 0) return FNI8_OK;
+    REQUIRE(x, FNI8_ERR_NULL, "%s is required", name);
+    REQUIRE(hs >= D && ld >= D, FNI8_ERR_STRIDE, "%s: token or head stride < D=%lld", name,
+            (long long)D);
+    REQUIRE(aligned(x, 16) && ld % 8 == 0 && hs % 8 == 0, FNI8_ERR_ALIGN,
+            "%s must be 16-byte aligned with strides that are multiples of 8", name);
+    return FNI8_OK;
+}
+
+constexpr int64_t kMaxTokens = (int64_t)1 << 23;  // a workgroup a token and 2^32 threads a grid
+constexpr int64_t kMaxHeads = 4096;
+constexpr int64_t kMaxHeadDim = 256;
+
+int check_rows(const fni8h::QkvRows& r) {
+    REQUIRE(r.T >= 0 && r.T <= kMaxTokens, FNI8_ERR_SHAPE, "T=%lld out of range (2^23 at most)",
+            (long long)r.T);
+    REQUIRE(r.Hq >= 0 && r.Hk >= 0 && r.Hq <= kMaxHeads && r.Hk <= kMaxHeads, FNI8_ERR_SHAPE,
+            "Hq=%lld Hk=%lld out of range", (long long)r.Hq, (long long)r.Hk);
+    REQUIRE(r.D > 0 && r.D <= kMaxHeadDim && r.D % 8 == 0, FNI8_ERR_SHAPE,
+            "D=%lld must be a multiple of 8, at most 256", (long long)r.D);
+    REQUIRE(r.R >= 0 && r.R <= r.D && r.R % 2 == 0, FNI8_ERR_SHAPE,
+            "R=%lld must be even, from 0 to D=%lld", (long long)r.R, (long long)r.D);
+    REQUIRE(r.eps >= 0.0f && r.eps < __builtin_inff(), FNI8_ERR_SHAPE, "eps must be finite and >= 0");
+    int rc = check_heads("q", r.q, r.ldq, r.hsq, r.Hq, r.D);
+    if (rc) return rc;
+    rc = check_heads("k", r.k, r.ldk, r.hsk, r.Hk, r.D);
+    if (rc) return rc;
+    REQUIRE(r.Hq == 0 || r.q_out, FNI8_ERR_NULL, "q_out is required");
+    REQUIRE(aligned(r.q_weight, 16) && aligned(r.k_weight, 16) && aligned(r.q_out, 16) &&
+                aligned(r.k_out, 16),
+            FNI8_ERR_ALIGN, "weights and outputs must be 16-byte aligned");
+    if (r.R) {
+        REQUIRE(r.positions && r.cos_sin, FNI8_ERR_NULL, "positions and cos_sin are required");
+        REQUIRE(r.P > 0 && r.P < kMaxDim, FNI8_ERR_SHAPE, "P=%lld out of range", (long long)r.P);
+        REQUIRE(aligned(r.positions, 4) && aligned(r.cos_sin, 16), FNI8_ERR_ALIGN,
+                "cos_sin must be 16-byte aligned, positions element-aligned");
+    }
+    return FNI8_OK;
+}
+
+int check_cache(const void* k_cache, const void* v_cache, const float* k_scale,
+                const float* v_scale, int64_t num_pages, int64_t page_size, int64_t Hk, int64_t D) {
+    REQUIRE(k_cache && v_cache, FNI8_ERR_NULL, "k_cache and v_cache are required");
+    REQUIRE((k_scale == nullptr) == (v_scale == nullptr), FNI8_ERR_NULL,
+            "k_scale and v_scale go together");
+    REQUIRE(Hk > 0 && Hk <= kMaxHeads, FNI8_ERR_SHAPE, "Hk=%lld out of range", (long long)Hk);
+    REQUIRE(D > 0 && D <= kMaxHeadDim && D % 16 == 0, FNI8_ERR_SHAPE,
+            "D=%lld must be a multiple of 16, at most 256, with a cache", (long long)D);
+    REQUIRE(page_size >= 16 && page_size <= 65536 && (page_size & (page_size - 1)) == 0,
+            FNI8_ERR_SHAPE, "page_size=%lld must be a power of two from 16 to 65536",
+            (long long)page_size);
+    REQUIRE(num_pages > 0 && num_pages < kMaxDim / page_size, FNI8_ERR_SHAPE,
+            "num_pages=%lld out of range (num_pages * page_size < 2^31)", (long long)num_pages);
+    REQUIRE(aligned(k_cache, 16) && aligned(v_cache, 16) && aligned(k_scale, 4) &&
+                aligned(v_scale, 4),
+            FNI8_ERR_ALIGN, "caches must be 16-byte aligned, scales element-aligned");
+    return FNI8_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -629,6 +690,122 @@ int fni8_rmsnorm_quant_f16(const void* x, int64_t ldx, const void* residual, int
                                  (const uint16_t*)weight, eps, unit_offset ? 1 : 0, M, K, nullptr,
                                  0, residual ? (uint16_t*)residual_out : nullptr, ldro, xq, ldq,
                                  xs, (hipStream_t)stream);
+}
+
+int fni8_qk_norm_rope_f16(const void* q, int64_t ldq, int64_t hsq, int64_t Hq, const void* k,
+                          int64_t ldk, int64_t hsk, int64_t Hk, int64_t T, int64_t D,
+                          const void* q_weight, const void* k_weight, float eps, int unit_offset,
+                          const int32_t* positions, const float* cos_sin, int64_t P, int64_t R,
+                          int interleaved, void* q_out, void* k_out, void* stream) {
+    fni8h::g_detail[0] = 0;
+    fni8h::QkvRows r{};
+    r.q = (const uint16_t*)q; r.ldq = ldq; r.hsq = hsq; r.Hq = Hq;
+    r.k = (const uint16_t*)k; r.ldk = ldk; r.hsk = hsk; r.Hk = Hk;
+    r.T = T; r.D = D;
+    r.q_weight = (const uint16_t*)q_weight; r.k_weight = (const uint16_t*)k_weight;
+    r.eps = eps; r.unit_offset = unit_offset;
+    r.positions = positions; r.cos_sin = cos_sin; r.P = P; r.R = R; r.interleaved = interleaved;
+    r.q_out = (uint16_t*)q_out; r.k_out = (uint16_t*)k_out;
+    int rc = check_rows(r);
+    if (rc) return rc;
+    REQUIRE(Hk == 0 || k_out, FNI8_ERR_NULL, "k_out is required");
+    rc = check_device();
+    if (rc) return rc;
+    return fni8h::launch_qkv_rows(r, (hipStream_t)stream);
+}
+
+int fni8_rope_append_f16(const void* q, int64_t ldq, int64_t hsq, int64_t Hq, const void* k,
+                         int64_t ldk, int64_t hsk, int64_t Hk, const void* v, int64_t ldv,
+                         int64_t hsv, int64_t T, int64_t D, const void* q_weight,
+                         const void* k_weight, float eps, int unit_offset,
+                         const int32_t* positions, const float* cos_sin, int64_t P, int64_t R,
+                         int interleaved, void* q_out, void* k_cache, void* v_cache,
+                         float* k_scale, float* v_scale, int64_t num_pages, int64_t page_size,
+                         const int32_t* slots, void* stream) {
+    fni8h::g_detail[0] = 0;
+    fni8h::QkvRows r{};
+    r.q = (const uint16_t*)q; r.ldq = ldq; r.hsq = hsq; r.Hq = Hq;
+    r.k = (const uint16_t*)k; r.ldk = ldk; r.hsk = hsk; r.Hk = Hk;
+    r.v = (const uint16_t*)v; r.ldv = ldv; r.hsv = hsv;
+    r.T = T; r.D = D;
+    r.q_weight = (const uint16_t*)q_weight; r.k_weight = (const uint16_t*)k_weight;
+    r.eps = eps; r.unit_offset = unit_offset;
+    r.positions = positions; r.cos_sin = cos_sin; r.P = P; r.R = R; r.interleaved = interleaved;
+    r.q_out = (uint16_t*)q_out;
+    r.k_cache = k_cache; r.v_cache = v_cache; r.k_scale = k_scale; r.v_scale = v_scale;
+    r.num_pages = num_pages; r.page_size = page_size; r.slots = slots;
+    int rc = check_rows(r);
+    if (rc) return rc;
+    rc = check_cache(k_cache, v_cache, k_scale, v_scale, num_pages, page_size, Hk, D);
+    if (rc) return rc;
+    rc = check_heads("v", v, ldv, hsv, Hk, D);
+    if (rc) return rc;
+    REQUIRE(slots, FNI8_ERR_NULL, "slots is required");
+    REQUIRE(aligned(slots, 4), FNI8_ERR_ALIGN, "slots misaligned");
+    rc = check_device();
+    if (rc) return rc;
+    return fni8h::launch_qkv_rows(r, (hipStream_t)stream);
+}
+
+int fni8_paged_attention_f16(const void* q, int64_t ldq, int64_t hsq, int64_t T, int64_t Hq,
+                             int64_t Hk, int64_t D, const void* k_cache, const void* v_cache,
+                             const float* k_scale, const float* v_scale, int64_t num_pages,
+                             int64_t page_size, const int32_t* block_tables, int64_t ldt,
+                             int64_t max_pages, const int32_t* context_lens,
+                             const int32_t* cu_seqlens, int64_t B, int64_t max_seqlen, float scale,
+                             int64_t window, void* out, void* workspace, int64_t workspace_bytes,
+                             void* stream) {
+    fni8h::g_detail[0] = 0;
+    REQUIRE(out && block_tables && context_lens, FNI8_ERR_NULL,
+            "out, block_tables and context_lens are required");
+    REQUIRE(T >= 0 && T <= kMaxTokens, FNI8_ERR_SHAPE, "T=%lld out of range (2^23 at most)",
+            (long long)T);
+    REQUIRE(B > 0 && B <= 65536, FNI8_ERR_SHAPE, "B=%lld out of range (1 to 65536)", (long long)B);
+    REQUIRE(cu_seqlens || T == B, FNI8_ERR_SHAPE, "without cu_seqlens, T=%lld must equal B=%lld",
+            (long long)T, (long long)B);
+    REQUIRE(max_seqlen >= 0, FNI8_ERR_SHAPE, "max_seqlen=%lld is negative", (long long)max_seqlen);
+    int rc = check_cache(k_cache, v_cache, k_scale, v_scale, num_pages, page_size, Hk, D);
+    if (rc) return rc;
+    REQUIRE(Hq > 0 && Hq <= kMaxHeads && Hq % Hk == 0, FNI8_ERR_SHAPE,
+            "Hq=%lld must be a multiple of Hk=%lld", (long long)Hq, (long long)Hk);
+    rc = check_heads("q", q, ldq, hsq, Hq, D);
+    if (rc) return rc;
+    REQUIRE(max_pages > 0 && max_pages < kMaxDim / page_size, FNI8_ERR_SHAPE,
+            "max_pages=%lld out of range (max_pages * page_size < 2^31)", (long long)max_pages);
+    REQUIRE(ldt >= max_pages, FNI8_ERR_STRIDE, "ldt=%lld < max_pages=%lld", (long long)ldt,
+            (long long)max_pages);
+    REQUIRE(window >= 0, FNI8_ERR_SHAPE, "window=%lld is negative", (long long)window);
+    REQUIRE(scale == scale && scale > -__builtin_inff() && scale < __builtin_inff(),
+            FNI8_ERR_SHAPE, "scale must be finite");
+    REQUIRE(aligned(out, 16) && aligned(block_tables, 4) && aligned(context_lens, 4) &&
+                aligned(cu_seqlens, 4),
+            FNI8_ERR_ALIGN, "out must be 16-byte aligned, the int32 arrays element-aligned");
+    REQUIRE(workspace_bytes >= 0 && (!workspace || aligned(workspace, 256)), FNI8_ERR_ALIGN,
+            "workspace must be 256-byte aligned with a size >= 0");
+    rc = check_device();
+    if (rc) return rc;
+    fni8h::PagedAttention a{};
+    a.q = (const uint16_t*)q; a.ldq = ldq; a.hsq = hsq; a.T = T; a.Hq = Hq; a.Hk = Hk; a.D = D;
+    a.k_cache = k_cache; a.v_cache = v_cache; a.k_scale = k_scale; a.v_scale = v_scale;
+    a.num_pages = num_pages; a.page_size = page_size;
+    a.block_tables = block_tables; a.ldt = ldt; a.max_pages = max_pages;
+    a.context_lens = context_lens; a.cu_seqlens = cu_seqlens; a.B = B;
+    // one token a sequence without cu_seqlens; a bound beyond T says no more than T
+    a.max_seqlen = cu_seqlens ? (max_seqlen < T ? max_seqlen : T) : 1;
+    a.scale = scale; a.window = window; a.out = (uint16_t*)out;
+    a.work = static_cast<int8_t*>(workspace);
+    a.work_bytes = workspace ? workspace_bytes : 0;
+    return fni8h::launch_paged_attention(a, (hipStream_t)stream);
+}
+
+int64_t fni8_paged_attention_workspace_bytes(int64_t T, int64_t Hq, int64_t Hk, int64_t D,
+                                             int64_t B, int64_t max_seqlen, int64_t max_context) {
+    if (T <= 0 || T > kMaxTokens || Hk <= 0 || Hk > kMaxHeads || Hq <= 0 || Hq > kMaxHeads ||
+        Hq % Hk || D <= 0 || D > kMaxHeadDim || B <= 0 || B > 65536 || max_seqlen < 0 ||
+        max_context <= 0 || max_context >= kMaxDim)
+        return 0;
+    return fni8h::paged_attention_workspace_bytes(T, Hq, Hk, D, B, max_seqlen < T ? max_seqlen : T,
+                                                  max_context);
 }
 
 }  // extern "C"

@@ -504,5 +504,48 @@ int launch_w4a8_tile_grouped(const int8_t* aq, const float* as, const int32_t* r
 int launch_moe_route(const float* logits, int64_t ldl, int64_t T, int64_t E, int scoring,
                      const float* bias, int64_t groups, int64_t topk_group, int64_t k, int renorm,
                      float scale, uint16_t* topw, int32_t* topi, hipStream_t st);
+// Norm, rotation and cache append of a step's query, key and value rows.  Weights NULL: no
+// norm; R = 0: no rotation; slots NULL: keys go to k_out and v is unused.
+struct QkvRows {
+    const uint16_t* q;
+    int64_t ldq, hsq, Hq;
+    const uint16_t* k;
+    int64_t ldk, hsk, Hk;
+    const uint16_t* v;
+    int64_t ldv, hsv;
+    int64_t T, D;
+    const uint16_t *q_weight, *k_weight;
+    float eps;
+    int unit_offset;
+    const int32_t* positions;
+    const float* cos_sin;
+    int64_t P, R;
+    int interleaved;
+    uint16_t *q_out, *k_out;
+    void *k_cache, *v_cache;
+    float *k_scale, *v_scale;
+    int64_t num_pages, page_size;
+    const int32_t* slots;
+};
+int launch_qkv_rows(const QkvRows& r, hipStream_t st);
+struct PagedAttention {
+    const uint16_t* q;
+    int64_t ldq, hsq, T, Hq, Hk, D;
+    const void *k_cache, *v_cache;
+    const float *k_scale, *v_scale;
+    int64_t num_pages, page_size;
+    const int32_t* block_tables;
+    int64_t ldt, max_pages;
+    const int32_t *context_lens, *cu_seqlens;
+    int64_t B, max_seqlen;
+    float scale;
+    int64_t window;
+    uint16_t* out;
+    int8_t* work;
+    int64_t work_bytes;
+};
+int launch_paged_attention(const PagedAttention& a, hipStream_t st);
+int64_t paged_attention_workspace_bytes(int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t B,
+                                        int64_t max_seqlen, int64_t max_context);
 void set_error_detail(const char* fmt, ...);
 }  // namespace fni8h

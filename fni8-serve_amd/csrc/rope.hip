@@ -1,0 +1,294 @@
+// The rows between the QKV projection and attention (gfx950): an RMS norm of every query
+// and key head, rotary positions, and the append of keys and values to the paged cache,
+// in one pass over the rows.
+//
+// A row is one head of one token, D elements x.  With n = x, or
+// n = x * (1 / sqrt(sum(x^2) / D + eps)) * w with a weight (w = weight, or 1 + weight),
+// and the token's table row cos[0..R/2), sin[0..R/2):
+//   halves (a, b) = (n[i], n[i + R/2]), pairs (a, b) = (n[2i], n[2i + 1]),  i < R/2
+//   (a, b) <- (a cos[i] - b sin[i], b cos[i] + a sin[i]);  n[R..D) stays.
+// All of it in fp32 from the fp16 input to one rounding to fp16: the normed row is not
+// rounded in between.  A position outside the table gives NaN in the rotated elements.
+// A key or value row goes to its token's slot of the cache as it is (fp16), or in the
+// per-token quantization of the linears (common.h), one scale a row.  A slot outside the
+// cache (negative: padding) drops the row.
+//
+// Memory bounds it: 4 bytes an element (fp16 in and out), R * 4 a token for its table
+// row.  A row is held by LPR = 8, 16 or 32 lanes of 8 elements (16-byte accesses).  The
+// other half of a rotated pair is read a second time from the input (the L1 has it)
+// rather than exchanged between lanes: both loads are in flight together, and any R that
+// is a multiple of 16 works the same way.
+#include "common.h"
+
+namespace {
+
+using fni8::f2h;
+using fni8::h2f;
+
+struct RowArgs {
+    const uint16_t *q, *k, *v;
+    int64_t ldq, hsq, ldk, hsk, ldv, hsv;
+    int Hq, Hk, Hv, D, R, pairs, unit;
+    const uint16_t *qw, *kw;
+    float eps;
+    const int32_t* pos;
+    const float* table;
+    int64_t P;
+    uint16_t *q_out, *k_out;
+    // append: caches of `slots_n` slots in pages of 1 << page_log2; NULL slot = no cache
+    const int32_t* slot;
+    int64_t slots_n;
+    int page_log2;
+    void *kc, *vc;
+    float *ks, *vs;
+};
+
+// Sum over the LPR lanes of a row, in every one of them.
+template <int LPR>
+__device__ __forceinline__ float row_sum(float v) {
+    auto add = [](float a, int b) { return a + __builtin_bit_cast(float, b); };
+    v = add(v, fni8::dpp<fni8::kDppXor1>(__builtin_bit_cast(int, v)));
+    v = add(v, fni8::dpp<fni8::kDppXor2>(__builtin_bit_cast(int, v)));
+    v = add(v, fni8::dpp<fni8::kDppHalfMirror>(__builtin_bit_cast(int, v)));
+    if (LPR >= 16) v = add(v, fni8::dpp<fni8::kDppMirror>(__builtin_bit_cast(int, v)));
+    if (LPR >= 32) v += __shfl_xor(v, 16, 64);
+    return v;
+}
+
+template <int LPR>
+__device__ __forceinline__ uint32_t row_max(uint32_t v) {
+    auto up = [](uint32_t a, int b) { return a > (uint32_t)b ? a : (uint32_t)b; };
+    v = up(v, fni8::dpp<fni8::kDppXor1>((int)v));
+    v = up(v, fni8::dpp<fni8::kDppXor2>((int)v));
+    v = up(v, fni8::dpp<fni8::kDppHalfMirror>((int)v));
+    if (LPR >= 16) v = up(v, fni8::dpp<fni8::kDppMirror>((int)v));
+    if (LPR >= 32) v = up(v, __shfl_xor((int)v, 16, 64));
+    return v;
+}
+
+__device__ __forceinline__ float half_of(uint4 v, int i) {
+    const uint32_t w = (i >> 1) == 0 ? v.x : (i >> 1) == 1 ? v.y : (i >> 1) == 2 ? v.z : v.w;
+    return h2f((uint16_t)(i & 1 ? w >> 16 : w & 0xffffu));
+}
+
+// A block takes NR rows per group of LPR lanes of one token (blockIdx.x): rows 0..Hq are
+// query heads, then key heads, then value heads.  ALIGNED: every chunk of 8 elements is
+// rotated as a whole or not at all and its table entries are 16-byte aligned (R a multiple
+// of 16 for halves, of 8 for pairs); otherwise element by element.
+template <int LPR, int NR, bool ALIGNED>
+__global__ __launch_bounds__(256) void row_kernel(RowArgs a) {
+    constexpr int GROUPS = 256 / LPR;
+    const int64_t t = blockIdx.x;
+    const int lane = threadIdx.x & (LPR - 1), group = threadIdx.x / LPR;
+    const int e = lane * 8, half = a.R >> 1;
+    const bool mine = e < a.D;
+    const int rows = a.Hq + a.Hk + a.Hv;
+    const int row0 = blockIdx.y * (GROUPS * NR) + group;
+
+    // the lane's 8 elements of the token's angles, the same for every head
+    float c[8], s[8];
+    // where the other element of each pair lies, for halves
+    const int turn = e < half ? half : -half;
+    int64_t p = 0;
+    bool outside = false;
+    if (a.R) {
+        p = a.pos[t];
+        outside = p < 0 || p >= a.P;
+        if (outside) p = 0;
+    }
+    const float* row = a.table + p * a.R;
+    if (ALIGNED) {
+        if (e < a.R) {
+            if (a.pairs) {
+                const float4 c4 = *reinterpret_cast<const float4*>(row + e / 2);
+                const float4 s4 = *reinterpret_cast<const float4*>(row + half + e / 2);
+                const float cc[4] = {c4.x, c4.y, c4.z, c4.w}, ss[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    c[i] = cc[i / 2];
+                    s[i] = i & 1 ? ss[i / 2] : -ss[i / 2];
+                }
+            } else {
+                const float* at = row + (e < half ? e : e - half);
+                const float4 c0 = *reinterpret_cast<const float4*>(at);
+                const float4 c1 = *reinterpret_cast<const float4*>(at + 4);
+                const float4 s0 = *reinterpret_cast<const float4*>(at + half);
+                const float4 s1 = *reinterpret_cast<const float4*>(at + half + 4);
+                const float cc[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+                const float ss[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    c[i] = cc[i];
+                    s[i] = e < half ? -ss[i] : ss[i];
+                }
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int d = e + i;
+            if (d < a.R) {
+                const int n = a.pairs ? d >> 1 : d < half ? d : d - half;
+                const float sn = row[half + n];
+                c[i] = row[n];
+                s[i] = (a.pairs ? d & 1 : d >= half) ? sn : -sn;
+            }
+        }
+    }
+    if (outside)
+#pragma unroll
+        for (int i = 0; i < 8; i++) c[i] = s[i] = __builtin_nanf("");
+
+    uint4 x[NR], o[NR];
+    uint16_t other[NR][8];
+#pragma unroll
+    for (int j = 0; j < NR; j++) {
+        const int r = row0 + j * GROUPS;
+        x[j] = o[j] = make_uint4(0, 0, 0, 0);
+        if (r >= rows || !mine) continue;
+        const uint16_t* src = r < a.Hq            ? a.q + t * a.ldq + r * a.hsq
+                              : r < a.Hq + a.Hk ? a.k + t * a.ldk + (r - a.Hq) * a.hsk
+                                                : a.v + t * a.ldv + (r - a.Hq - a.Hk) * a.hsv;
+        x[j] = *reinterpret_cast<const uint4*>(src + e);
+        if (r < a.Hq + a.Hk && !a.pairs) {
+            if (ALIGNED) {
+                if (e < a.R) o[j] = *reinterpret_cast<const uint4*>(src + e + turn);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int d = e + i;
+                    other[j][i] = d < a.R ? src[d < half ? d + half : d - half] : 0;
+                }
+            }
+        }
+    }
+    int64_t slot = -1;
+    if (a.slot) {
+        slot = a.slot[t];
+        if (slot >= a.slots_n) slot = -1;
+    }
+
+#pragma unroll
+    for (int j = 0; j < NR; j++) {
+        const int r = row0 + j * GROUPS;
+        const bool is_q = r < a.Hq, is_k = !is_q && r < a.Hq + a.Hk;
+        if (r >= rows) continue;
+        uint4 y = x[j];
+        const uint16_t* w = is_q ? a.qw : a.kw;
+        if (is_q || is_k) {
+            float f[8], g[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                f[i] = half_of(x[j], i);
+                if (a.pairs)
+                    g[i] = half_of(x[j], i ^ 1);
+                else
+                    g[i] = ALIGNED ? half_of(o[j], i) : h2f(other[j][i]);
+            }
+            if (w) {
+                float ss = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; i++) ss = __builtin_fmaf(f[i], f[i], ss);
+                const float m = 1.0f / __builtin_sqrtf(row_sum<LPR>(ss) / (float)a.D + a.eps);
+                if (mine) {
+                    const uint4 w4 = *reinterpret_cast<const uint4*>(w + e);
+                    uint4 o4 = make_uint4(0, 0, 0, 0);
+                    if (ALIGNED && !a.pairs && e < a.R)
+                        o4 = *reinterpret_cast<const uint4*>(w + e + turn);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        float wi = half_of(w4, i), wo = 0.0f;
+                        if (a.pairs)
+                            wo = half_of(w4, i ^ 1);
+                        else if (ALIGNED)
+                            wo = half_of(o4, i);
+                        else if (e + i < a.R)
+                            wo = h2f(w[e + i < half ? e + i + half : e + i - half]);
+                        if (a.unit) {
+                            wi = 1.0f + wi;
+                            wo = 1.0f + wo;
+                        }
+                        f[i] = f[i] * m * wi;
+                        g[i] = g[i] * m * wo;
+                    }
+                }
+            }
+            uint32_t h[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float z = e + i < a.R ? __builtin_fmaf(f[i], c[i], g[i] * s[i]) : f[i];
+                h[i] = f2h(z);
+            }
+            y = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16,
+                           h[6] | h[7] << 16);
+        }
+        if (is_q || (is_k && !a.slot)) {
+            uint16_t* dst = is_q ? a.q_out + (t * a.Hq + r) * a.D
+                                 : a.k_out + (t * a.Hk + r - a.Hq) * a.D;
+            if (mine) *reinterpret_cast<uint4*>(dst + e) = y;
+            continue;
+        }
+        if (slot < 0) continue;
+        const int h = is_k ? r - a.Hq : r - a.Hq - a.Hk;
+        const int64_t page = slot >> a.page_log2, in = slot & ((1 << a.page_log2) - 1);
+        const int64_t at = ((page * a.Hk + h) << a.page_log2) + in;
+        void* cache = is_k ? a.kc : a.vc;
+        float* scale = is_k ? a.ks : a.vs;
+        if (!scale) {
+            if (mine) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(cache) + at * a.D + e) = y;
+            continue;
+        }
+        const uint32_t top = row_max<LPR>(fni8::amax_fold(mine ? fni8::amax_chunk(0, y) : 0));
+        const float step = fni8::row_scale_from_bits(top);
+        // a row with an infinity or NaN: codes 0 under a scale that is not finite
+        const bool live = top < 0x7c00u;
+        if (mine)
+            *reinterpret_cast<uint2*>(static_cast<int8_t*>(cache) + at * a.D + e) =
+                fni8::quant_chunk(y, step, 1.0f / step, live);
+        if (lane == 0) scale[at] = step;
+    }
+}
+
+template <int LPR, int NR>
+void launch_rows(const RowArgs& a, int64_t T, bool aligned, hipStream_t st) {
+    const int rows = a.Hq + a.Hk + a.Hv, per = 256 / LPR * NR;
+    const dim3 grid((uint32_t)T, (uint32_t)((rows + per - 1) / per));
+    if (aligned)
+        row_kernel<LPR, NR, true><<<grid, 256, 0, st>>>(a);
+    else
+        row_kernel<LPR, NR, false><<<grid, 256, 0, st>>>(a);
+}
+
+}  // namespace
+
+namespace fni8h {
+
+int launch_qkv_rows(const QkvRows& r, hipStream_t st) {
+    if (r.T == 0 || r.Hq + r.Hk == 0) return FNI8_OK;
+    RowArgs a;
+    a.q = r.q; a.ldq = r.ldq; a.hsq = r.hsq; a.Hq = (int)r.Hq;
+    a.k = r.k; a.ldk = r.ldk; a.hsk = r.hsk; a.Hk = (int)r.Hk;
+    a.v = r.v; a.ldv = r.ldv; a.hsv = r.hsv; a.Hv = r.slots ? (int)r.Hk : 0;
+    a.D = (int)r.D; a.R = (int)r.R; a.pairs = r.interleaved != 0; a.unit = r.unit_offset != 0;
+    a.qw = r.q_weight; a.kw = r.k_weight; a.eps = r.eps;
+    a.pos = r.positions; a.table = r.cos_sin; a.P = r.P;
+    a.q_out = r.q_out; a.k_out = r.k_out;
+    a.slot = r.slots; a.slots_n = r.num_pages * r.page_size;
+    a.page_log2 = r.slots ? __builtin_ctzll((uint64_t)r.page_size) : 0;
+    a.kc = r.k_cache; a.vc = r.v_cache; a.ks = r.k_scale; a.vs = r.v_scale;
+    const bool aligned = a.R % (a.pairs ? 8 : 16) == 0;
+    if (r.D <= 64)
+        launch_rows<8, 1>(a, r.T, aligned, st);
+    else if (r.D <= 128)
+        launch_rows<16, 1>(a, r.T, aligned, st);
+    else
+        launch_rows<32, 1>(a, r.T, aligned, st);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) {
+        set_error_detail("qkv rows launch: %s", hipGetErrorString(e));
+        return FNI8_ERR_LAUNCH;
+    }
+    return FNI8_OK;
+}
+
+}  // namespace fni8h

@@ -559,3 +559,222 @@ def moe_route(logits: torch.Tensor, top_k: int, scoring: str = "softmax",
                       groups, tg, top_k, int(bool(renorm)), ctypes.c_float(scale), _ptr(topw),
                       _ptr(topi), _stream(dev))
     return topw, topi
+
+
+def _heads(name: str, x: torch.Tensor):
+    """x [T, H, D] fp16 with unit inner stride and 16-byte aligned rows (a copy where it is
+    not): the tensor and its token and head strides."""
+    if x.dtype != _f16 or x.dim() != 3:
+        raise ValueError(f"{name} must be fp16 [tokens, heads, head_dim] (got {x.dtype}, "
+                         f"{tuple(x.shape)})")
+    T, H, D = x.shape
+    if D == 0 or D % 8 or D > 256:
+        raise ValueError(f"{name}: head_dim {D} must be a multiple of 8, at most 256")
+    lt, lh = (x.stride(0) if T > 1 else H * D), (x.stride(1) if H > 1 else D)
+    if x.numel() and (x.stride(2) != 1 or lt < D or lh < D or lt % 8 or lh % 8
+                      or x.data_ptr() % 16):
+        x = x.contiguous()
+        if x.data_ptr() % 16:
+            x = x.clone()
+        lt, lh = H * D, D
+    return x, max(lt, D), lh
+
+
+def _index(name: str, t: torch.Tensor, n: int | None):
+    if t.dtype not in (torch.int32, torch.int64) or t.dim() != 1 or (n is not None
+                                                                   and t.numel() != n):
+        raise ValueError(f"{name} must be int32 or int64 with {n if n is not None else 'one'} "
+                         f"entries (got {t.dtype}, {tuple(t.shape)})")
+    return t.to(torch.int32).contiguous()
+
+
+def _table(positions, cos_sin, T: int, D: int):
+    """positions int32 [T] and cos_sin fp32 [P, R], or nothing: no rotation."""
+    if (positions is None) != (cos_sin is None):
+        raise ValueError("positions and cos_sin go together")
+    if cos_sin is None:
+        return None, None, 0, 0
+    if cos_sin.dtype != torch.float32 or cos_sin.dim() != 2 or not cos_sin.is_contiguous():
+        raise ValueError("cos_sin must be a contiguous fp32 [positions, rotary_dim] tensor")
+    P, R = cos_sin.shape
+    if R % 2 or not 0 < R <= D or P == 0:
+        raise ValueError(f"cos_sin {tuple(cos_sin.shape)}: rotary_dim must be even and at most "
+                         f"head_dim {D}, with one position at least")
+    if cos_sin.data_ptr() % 16:
+        cos_sin = cos_sin.clone()
+    return _index("positions", positions, T), cos_sin, P, R
+
+
+def _head_weight(name: str, w, D: int):
+    if w is None:
+        return None
+    if w.dtype != _f16 or w.numel() != D:
+        raise ValueError(f"{name} must be fp16 with {D} entries (got {w.dtype}, {w.numel()})")
+    w = w.reshape(-1).contiguous()
+    return w.clone() if w.data_ptr() % 16 else w
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None,
+                 k_weight: torch.Tensor | None, positions: torch.Tensor | None,
+                 cos_sin: torch.Tensor | None, eps: float = 1e-6, interleaved: bool = False,
+                 unit_offset: bool = False):
+    """RMSNorm of every query and key head (a weight of None: none), then rotary positions,
+    in one pass: q [T, Hq, D], k [T, Hk, D] fp16 -> (q', k'), rounded once.
+
+    cos_sin fp32 [P, R] (RotaryEmbedding.cos_sin): row p holds the R/2 cosines, then the R/2
+    sines of position p; the first R elements of a head turn, as halves (i, i + R/2) or, with
+    interleaved, as pairs (2i, 2i + 1).  A position outside [0, P) gives NaN.  positions and
+    cos_sin of None: norms only (fni8serve/layers/rotary.py:21-55,
+    layers/gqa_attention.py:59-157)."""
+    dev = _require_cuda("qk_norm_rope", q, k, q_weight, k_weight, positions, cos_sin)
+    q, ldq, hsq = _heads("q", q)
+    k, ldk, hsk = _heads("k", k)
+    T, Hq, D = q.shape
+    Hk = k.shape[1]
+    if k.shape[0] != T or k.shape[2] != D:
+        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} differ in tokens or head_dim")
+    pos, tab, P, R = _table(positions, cos_sin, T, D)
+    q_weight = _head_weight("q_weight", q_weight, D)
+    k_weight = _head_weight("k_weight", k_weight, D)
+    q_out = torch.empty((T, Hq, D), dtype=_f16, device=dev)
+    k_out = torch.empty((T, Hk, D), dtype=_f16, device=dev)
+    if T and Hq + Hk:
+        with torch.cuda.device(dev):
+            _lib.call("fni8_qk_norm_rope_f16", _ptr(q), ldq, hsq, Hq, _ptr(k), ldk, hsk, Hk, T, D,
+                      _ptr(q_weight), _ptr(k_weight), ctypes.c_float(eps), int(bool(unit_offset)),
+                      _ptr(pos), _ptr(tab), P, R, int(bool(interleaved)), _ptr(q_out),
+                      _ptr(k_out), _stream(dev))
+    return q_out, k_out
+
+
+def rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor,
+         interleaved: bool = False):
+    """`fni8.rope` (fni8serve/layers/rotary.py:52) into new tensors: qk_norm_rope without
+    the norms."""
+    if positions is None or cos_sin is None:
+        raise ValueError("rope: positions and cos_sin are required")
+    return qk_norm_rope(q, k, None, None, positions, cos_sin, interleaved=interleaved)
+
+
+def _cache_args(k_cache, v_cache, k_scale, v_scale, Hk: int | None, D: int):
+    """Checks of a paged cache [pages, heads, page_size, head_dim]: fp16, or int8 with fp32
+    scales [pages, heads, page_size]."""
+    if (k_scale is None) != (v_scale is None):
+        raise ValueError("k_scale and v_scale go together")
+    want = _f16 if k_scale is None else torch.int8
+    for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if c.dtype != want or c.dim() != 4 or not c.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous {want} tensor [pages, heads, page_size, "
+                             f"head_dim] (got {c.dtype}, {tuple(c.shape)}; 8 bits need k_scale "
+                             "and v_scale, 16 bits none)")
+    if k_cache.shape != v_cache.shape:
+        raise ValueError(f"k_cache {tuple(k_cache.shape)} and v_cache {tuple(v_cache.shape)} differ")
+    N, H, page, dim = k_cache.shape
+    if dim != D or (Hk is not None and H != Hk):
+        raise ValueError(f"cache {tuple(k_cache.shape)} does not hold {Hk} heads of {D}")
+    if D % 16:
+        raise ValueError(f"head_dim {D} must be a multiple of 16 with a cache")
+    if page < 16 or page > 65536 or page & (page - 1):
+        raise ValueError(f"page_size {page} must be a power of two from 16 to 65536")
+    for name, s in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if s is not None and (s.dtype != torch.float32 or s.shape != (N, H, page)
+                              or not s.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous fp32 tensor {(N, H, page)}")
+    return N, H, page
+
+
+def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                positions: torch.Tensor | None, cos_sin: torch.Tensor | None,
+                k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor,
+                k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
+                q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None,
+                eps: float = 1e-6, interleaved: bool = False,
+                unit_offset: bool = False) -> torch.Tensor:
+    """qk_norm_rope with the keys, and the values as they are, appended to the paged cache in
+    the same pass: q [T, Hq, D], k and v [T, Hk, D] fp16 -> q'.
+
+    k_cache, v_cache [pages, Hk, page_size, D] are written in place at slots [T] (page *
+    page_size + offset): fp16, or int8 with the per-row scales k_scale, v_scale fp32 [pages,
+    Hk, page_size], quantized as quantize_rowwise does.  A slot outside the cache (negative:
+    padding) drops its token's rows; no slot may occur twice in a call
+    (fni8serve/engine/kv_cache.py:265,681,700,730,826)."""
+    dev = _require_cuda("rope_append", q, k, v, positions, cos_sin, k_cache, v_cache, slots,
+                        k_scale, v_scale, q_weight, k_weight)
+    q, ldq, hsq = _heads("q", q)
+    k, ldk, hsk = _heads("k", k)
+    v, ldv, hsv = _heads("v", v)
+    T, Hq, D = q.shape
+    Hk = k.shape[1]
+    if k.shape[0] != T or k.shape[2] != D or v.shape != k.shape:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} differ "
+                         "in tokens, heads or head_dim")
+    N, _, page = _cache_args(k_cache, v_cache, k_scale, v_scale, Hk, D)
+    pos, tab, P, R = _table(positions, cos_sin, T, D)
+    slots = _index("slots", slots, T)
+    q_weight = _head_weight("q_weight", q_weight, D)
+    k_weight = _head_weight("k_weight", k_weight, D)
+    q_out = torch.empty((T, Hq, D), dtype=_f16, device=dev)
+    if T:
+        with torch.cuda.device(dev):
+            _lib.call("fni8_rope_append_f16", _ptr(q), ldq, hsq, Hq, _ptr(k), ldk, hsk, Hk,
+                      _ptr(v), ldv, hsv, T, D, _ptr(q_weight), _ptr(k_weight),
+                      ctypes.c_float(eps), int(bool(unit_offset)), _ptr(pos), _ptr(tab), P, R,
+                      int(bool(interleaved)), _ptr(q_out), _ptr(k_cache), _ptr(v_cache),
+                      _ptr(k_scale), _ptr(v_scale), N, page, _ptr(slots), _stream(dev))
+    return q_out
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                    block_tables: torch.Tensor, context_lens: torch.Tensor,
+                    cu_seqlens: torch.Tensor | None = None, max_seqlen: int | None = None,
+                    k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
+                    scale: float | None = None, window: int | None = None) -> torch.Tensor:
+    """Causal attention of new tokens over the paged cache, q [T, Hq, D] -> fp16 [T, Hq, D]
+    (fni8serve/layers/gqa_attention.py:87,123,131,154,278).
+
+    Sequence s owns tokens cu_seqlens[s] .. cu_seqlens[s + 1] of q (None: one token a
+    sequence), the last of its context_lens[s] tokens; their keys and values are in the cache
+    already, token c of the sequence in page block_tables[s, c // page_size].  Query head h
+    reads key head h // (Hq / Hk).  max_seqlen bounds the new tokens of a sequence (None: not
+    known; giving it saves a launch for decoded tokens).  scale defaults to D ** -0.5; window
+    is the number of keys that a query sees, itself among them.  A query without keys and
+    tokens past cu_seqlens[-1] give 0; a token whose page is not in the cache counts as NaN."""
+    dev = _require_cuda("paged_attention", q, k_cache, v_cache, block_tables, context_lens,
+                        cu_seqlens, k_scale, v_scale)
+    q, ldq, hsq = _heads("q", q)
+    T, Hq, D = q.shape
+    N, Hk, page = _cache_args(k_cache, v_cache, k_scale, v_scale, None, D)
+    if Hq == 0 or Hk == 0 or Hq % Hk:
+        raise ValueError(f"{Hq} query heads are no multiple of {Hk} key heads")
+    if block_tables.dtype not in (torch.int32, torch.int64) or block_tables.dim() != 2:
+        raise ValueError("block_tables must be int32 or int64 [sequences, pages]")
+    B, width = block_tables.shape
+    if cu_seqlens is None and T != B:
+        raise ValueError(f"{T} tokens for {B} sequences: cu_seqlens is required")
+    if window is not None and window < 1:
+        raise ValueError(f"window {window} must be at least 1")
+    if max_seqlen is not None and max_seqlen < 0:
+        raise ValueError(f"max_seqlen {max_seqlen} is negative")
+    lens = _index("context_lens", context_lens, B)
+    cu = None if cu_seqlens is None else _index("cu_seqlens", cu_seqlens, B + 1)
+    out = torch.empty((T, Hq, D), dtype=_f16, device=dev)
+    if T == 0:
+        return out
+    if B == 0 or width == 0:
+        if B:
+            raise ValueError("block_tables has no pages")
+        return out.zero_()
+    tables = block_tables.to(torch.int32)
+    if width > 1 and tables.stride(1) != 1 or B > 1 and tables.stride(0) < width:
+        tables = tables.contiguous()
+    ldt = tables.stride(0) if B > 1 else width
+    most = T if max_seqlen is None else max_seqlen
+    nw = int(_lib.load().fni8_paged_attention_workspace_bytes(T, Hq, Hk, D, B, most, width * page))
+    work = torch.empty(nw, dtype=torch.uint8, device=dev) if nw else None
+    with torch.cuda.device(dev):
+        _lib.call("fni8_paged_attention_f16", _ptr(q), ldq, hsq, T, Hq, Hk, D, _ptr(k_cache),
+                  _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), N, page, _ptr(tables), ldt, width,
+                  _ptr(lens), _ptr(cu), B, most,
+                  ctypes.c_float(D ** -0.5 if scale is None else scale), window or 0, _ptr(out),
+                  _ptr(work), nw, _stream(dev))
+    return out

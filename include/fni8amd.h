@@ -422,6 +422,97 @@ int fni8_rmsnorm_quant_f16(const void* x, int64_t ldx, const void* residual, int
                            int8_t* xq, int64_t ldq, float* xs, void* residual_out,
                            int64_t ldro, void* stream);
 
+/*
+ * Norms of queries and keys per head and rotary positions, one pass: RMSNorm of every head
+ * with q_weight / k_weight (NULL: none), then the rotation (replaces the query and key norms
+ * of fni8serve/layers/gqa_attention.py:59-157 and `fni8.rope`,
+ * fni8serve/layers/rotary.py:21-55).
+ *   q          fp16 [T, Hq, D], strides ldq (token) and hsq (head) elements; k the same
+ *              with Hk heads.  Hq or Hk may be 0 (its pointers are then not used).
+ *              D a multiple of 8, at most 256; pointers 16-byte aligned, strides
+ *              multiples of 8 elements; T <= 2^23
+ *   q_weight, k_weight  fp16 [D], 16-byte aligned, or NULL; unit_offset: 1 + weight
+ *   positions  int32 [T]; cos_sin fp32 [P, R], 16-byte aligned: R/2 cosines, then R/2 sines
+ *              of each position; R even, R <= D (elements R.. of a head stay); R = 0: no
+ *              rotation, positions and cos_sin unused
+ *   interleaved  0: pairs (i, i + R/2); non-zero: pairs (2i, 2i + 1)
+ *   q_out      fp16 [T, Hq, D], k_out fp16 [T, Hk, D], contiguous, 16-byte aligned; must not
+ *              overlap the inputs
+ * Arithmetic: fp32 throughout, one rounding to fp16 (the normed row is not rounded before
+ * the rotation).  A position outside [0, P) gives NaN in the rotated elements.
+ */
+int fni8_qk_norm_rope_f16(const void* q, int64_t ldq, int64_t hsq, int64_t Hq, const void* k,
+                          int64_t ldk, int64_t hsk, int64_t Hk, int64_t T, int64_t D,
+                          const void* q_weight, const void* k_weight, float eps, int unit_offset,
+                          const int32_t* positions, const float* cos_sin, int64_t P, int64_t R,
+                          int interleaved, void* q_out, void* k_out, void* stream);
+
+/*
+ * fni8_qk_norm_rope_f16 with the keys, and the values as they are, written to the paged
+ * cache instead of k_out (replaces `fni8.quantize_kv_write_paged` and the 16-bit cache
+ * write, fni8serve/engine/kv_cache.py:265,681,700,730,826, and the norm and rotation
+ * launches in front of it).
+ *   v          fp16 [T, Hk, D], strides ldv, hsv
+ *   k_cache, v_cache  [num_pages, Hk, page_size, D], contiguous, 16-byte aligned: fp16, or
+ *              int8 with k_scale, v_scale fp32 [num_pages, Hk, page_size] (both or neither);
+ *              page_size a power of two from 16 to 65536; num_pages * page_size < 2^31;
+ *              D a multiple of 16
+ *   slots      int32 [T]: page * page_size + offset of each token.  A slot outside the cache
+ *              drops the token's key and value (negative: padding); its query is written
+ *              all the same.  No slot may occur twice among the tokens of a call.
+ * 8 bits: codes and scale of the fp16 row as in fni8_quantize_rowwise_f16.
+ */
+int fni8_rope_append_f16(const void* q, int64_t ldq, int64_t hsq, int64_t Hq, const void* k,
+                         int64_t ldk, int64_t hsk, int64_t Hk, const void* v, int64_t ldv,
+                         int64_t hsv, int64_t T, int64_t D, const void* q_weight,
+                         const void* k_weight, float eps, int unit_offset,
+                         const int32_t* positions, const float* cos_sin, int64_t P, int64_t R,
+                         int interleaved, void* q_out, void* k_cache, void* v_cache,
+                         float* k_scale, float* v_scale, int64_t num_pages, int64_t page_size,
+                         const int32_t* slots, void* stream);
+
+/*
+ * Attention of new tokens over the paged cache: one token a sequence (decode), a few, or a
+ * chunk of a prompt, causal, each sequence with its own length (replaces
+ * `fni8.attn_int8_decode/_verify/_varlen`, `attn_paged_decode_cached`,
+ * fni8serve/layers/gqa_attention.py:87,123,131,154,278, engine/kv_cache.py:785).
+ *   q          fp16 [T, Hq, D], strides ldq, hsq as in fni8_qk_norm_rope_f16; Hq a multiple
+ *              of Hk: query head h reads key head h / (Hq / Hk)
+ *   k_cache .. page_size  as in fni8_rope_append_f16, the new tokens' rows in place
+ *   block_tables  int32 [B, max_pages], row stride ldt: page of tokens c * page_size .. of
+ *              sequence s in entry [s, c]; entries past a sequence's length, or wholly
+ *              before its window, are not read as pages
+ *   context_lens  int32 [B]: tokens of each sequence, the new ones among them
+ *   cu_seqlens int32 [B + 1]: tokens cu[s] .. cu[s + 1] of q are sequence s's last ones;
+ *              non-decreasing from 0; NULL: one token a sequence (T = B).  Tokens from cu[B]
+ *              on are padding.
+ *   max_seqlen no sequence has more new tokens (a bound that is too small costs time only)
+ *   scale      factor of the scores; window 0, or the number of keys a query sees, itself
+ *              among them
+ *   out        fp16 [T, Hq, D], contiguous, 16-byte aligned.  A query that sees no key, and
+ *              padding, gives 0.
+ *   workspace  as in fni8_paged_attention_workspace_bytes, 256-byte aligned, any contents;
+ *              NULL or too small: the keys of one query are not split over workgroups.
+ *              One per stream.
+ * Sums and softmax statistics are fp32, the weights of the values are rounded to fp16.  A
+ * token whose page is not in the cache, or past the block table, counts as a key of NaN.
+ */
+int fni8_paged_attention_f16(const void* q, int64_t ldq, int64_t hsq, int64_t T, int64_t Hq,
+                             int64_t Hk, int64_t D, const void* k_cache, const void* v_cache,
+                             const float* k_scale, const float* v_scale, int64_t num_pages,
+                             int64_t page_size, const int32_t* block_tables, int64_t ldt,
+                             int64_t max_pages, const int32_t* context_lens,
+                             const int32_t* cu_seqlens, int64_t B, int64_t max_seqlen, float scale,
+                             int64_t window, void* out, void* workspace, int64_t workspace_bytes,
+                             void* stream);
+
+/*
+ * Workspace bytes of fni8_paged_attention_f16 (0: none) for block tables that reach
+ * max_context tokens: the parts of the sums where the keys of a query are split.
+ */
+int64_t fni8_paged_attention_workspace_bytes(int64_t T, int64_t Hq, int64_t Hk, int64_t D,
+                                             int64_t B, int64_t max_seqlen, int64_t max_context);
+
 #ifdef __cplusplus
 }
 #endif
