@@ -229,9 +229,9 @@ int check_cache(const void* k_cache, const void* v_cache, const float* k_scale,
             (long long)page_size);
     REQUIRE(num_pages > 0 && num_pages < kMaxDim / page_size, FNI8_ERR_SHAPE,
             "num_pages=%lld out of range (num_pages * page_size < 2^31)", (long long)num_pages);
-    REQUIRE(aligned(k_cache, 16) && aligned(v_cache, 16) && aligned(k_scale, 4) &&
-                aligned(v_scale, 4),
-            FNI8_ERR_ALIGN, "caches must be 16-byte aligned, scales element-aligned");
+    REQUIRE(aligned(k_cache, 16) && aligned(v_cache, 16) && aligned(k_scale, 16) &&
+                aligned(v_scale, 16),
+            FNI8_ERR_ALIGN, "caches and scales must be 16-byte aligned");
     return FNI8_OK;
 }
 
@@ -770,8 +770,8 @@ int fni8_paged_attention_f16(const void* q, int64_t ldq, int64_t hsq, int64_t T,
             "Hq=%lld must be a multiple of Hk=%lld", (long long)Hq, (long long)Hk);
     rc = check_heads("q", q, ldq, hsq, Hq, D);
     if (rc) return rc;
-    REQUIRE(max_pages > 0 && max_pages < kMaxDim / page_size, FNI8_ERR_SHAPE,
-            "max_pages=%lld out of range (max_pages * page_size < 2^31)", (long long)max_pages);
+    REQUIRE(max_pages > 0 && max_pages <= ((int64_t)1 << 30) / page_size, FNI8_ERR_SHAPE,
+            "max_pages=%lld out of range (max_pages * page_size <= 2^30)", (long long)max_pages);
     REQUIRE(ldt >= max_pages, FNI8_ERR_STRIDE, "ldt=%lld < max_pages=%lld", (long long)ldt,
             (long long)max_pages);
     REQUIRE(window >= 0, FNI8_ERR_SHAPE, "window=%lld is negative", (long long)window);
@@ -802,7 +802,7 @@ int64_t fni8_paged_attention_workspace_bytes(int64_t T, int64_t Hq, int64_t Hk, 
                                              int64_t B, int64_t max_seqlen, int64_t max_context) {
     if (T <= 0 || T > kMaxTokens || Hk <= 0 || Hk > kMaxHeads || Hq <= 0 || Hq > kMaxHeads ||
         Hq % Hk || D <= 0 || D > kMaxHeadDim || B <= 0 || B > 65536 || max_seqlen < 0 ||
-        max_context <= 0 || max_context >= kMaxDim)
+        max_context <= 0 || max_context > (int64_t)1 << 30)
         return 0;
     return fni8h::paged_attention_workspace_bytes(T, Hq, Hk, D, B, max_seqlen < T ? max_seqlen : T,
                                                   max_context);

@@ -3,90 +3,1218 @@
 // Query token i of the n new ones of a sequence of L tokens (the new ones among them)
 // stands at p = L - n + i and sees the keys j, 0 <= j <= p, j > p - window:
 //   out = sum_j softmax_j(scale * q . k_j) v_j
-// with an online softmax: running maximum m, sum l and unnormalised output o in fp32.  A
-// row that sees no key (p < 0, or no tokens) is 0.
+// with an online softmax: running maximum m, sum l and unnormalised output o in fp32, all
+// in powers of two (scores times scale * log2 e).  A row that sees no key is 0.
 //
-// The simple form: one wave a (token, query head), a lane holds 4 elements of the head,
-// keys one after another.
+// The query heads that share a key head are packed with the tokens into rows
+// r = i * group + head, so that one read of a key serves all of them.  Both kernels compute
+// S^T = K Q^T (the keys as the MFMA's rows): a lane then holds several keys of ONE query
+// row, so a row's maximum and sum need one or two lane swaps, and the weights P^T are
+// already laid out as the second operand of O^T = V^T P^T.  The MFMA's k order is free as
+// long as both operands agree, so the keys of P stay where S^T left them, and V^T is read
+// from row-major V in LDS with transposing reads (4 keys x 16 elements) in the same order.
+//
+// 8 bits: the codes go through the matrix cores as fp16 integers (exact).  A key's scale
+// multiplies its column of S.  A value's scale v_s joins the exponent instead of P:
+// P' = 2^(s + log2 v_s - m) with m the maximum of s + log2 v_s, so P' <= 1 rounds to fp16
+// like P does whatever the scale's size, and l adds P' / v_s.
+//
+// few_kernel takes sequences with few rows (decode, drafted tokens): memory bounds it, each
+// cached row is read once.  The keys of all sequences are one list of units of 128 keys,
+// cut into equal runs, one a workgroup, whatever the lengths; parts of an item that two
+// workgroups share are joined by few_join.  tile_kernel takes the others: 128 rows a
+// workgroup share K and V tiles of 64 keys in LDS; the MFMAs bound it.
 #include "common.h"
 
 namespace {
 
 using fni8::f2h;
 using fni8::h2f;
-using fni8h::PagedAttention;
 
-__device__ __forceinline__ float wave_sum(float v) {
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef __fp16 tr4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kInf = __builtin_inff();
+constexpr int kUnit = 128;      // keys of a unit of few_kernel: 32 for each of 4 waves
+constexpr int kTileRows = 128;  // rows of a workgroup of tile_kernel
+constexpr int kTileKeys = 64;
+
+struct Attn {
+    const uint16_t* q;
+    int64_t ldq, hsq;
+    const void *kc, *vc;
+    const float *ks, *vs;
+    const int32_t *tables, *lens, *cu;
+    int64_t ldt;
+    uint16_t* out;
+    float* part;
+    int T, Hq, Hk, D, group, num_pages, plog, max_pages, B, nseq, window, cap;
+    float c;       // scale * log2 e
+    int few;       // few_kernel takes sequences of at most so many rows, tile_kernel others
+    int whole;     // few_kernel: no parts, an item is one unit
+    int splits;    // tile_kernel: parts of an item at most
+    int tiles;     // of tile_kernel, at most
+};
+
+struct Seq {
+    int start, n, L;
+};
+
+__device__ __forceinline__ int bound_of(const Attn& a, int s) {
+    if (s > a.B) return a.T;
+    const int c = a.cu ? a.cu[s] : s;
+    return c < 0 ? 0 : c < a.T ? c : a.T;
+}
+
+// Sequence s; the tokens past the last one are a sequence of no keys.
+__device__ __forceinline__ Seq sequence(const Attn& a, int s) {
+    Seq q;
+    q.start = bound_of(a, s);
+    q.n = bound_of(a, s + 1) - q.start;
+    q.n = q.n > 0 ? q.n : 0;
+    q.L = 0;
+    if (s < a.B) {
+        const int L = a.lens[s];
+        // tokens past the block table count as NaN: one of them is enough
+        q.L = L < 0 ? 0 : L < a.cap ? L : a.cap;
+    }
+    return q;
+}
+
+// ---- the list of items -----------------------------------------------------------
+
+__device__ __forceinline__ int block_scan(int v, int* sh, int& total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int incl = fni8::wave_incl_scan_i32(v, lane);
+    __syncthreads();
+    if (lane == 63) sh[wave] = incl;
+    __syncthreads();
+    total = 0;
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-    return v;
+    for (int w = 0; w < 4; w++) {
+        if (w < wave) incl += sh[w];
+        total += sh[w];
+    }
+    return incl;
 }
 
-__device__ __forceinline__ int seq_start(const PagedAttention& a, int64_t s) {
-    if (s > a.B) return (int)a.T;
-    int c = a.cu_seqlens ? a.cu_seqlens[s] : (int)s;
-    c = c < 0 ? 0 : c;
-    return c > a.T ? (int)a.T : c;
+// The sequence that holds unit `target(U)` of the list of all U = sum units(s), and the
+// number of units before it.  Every thread of the block gets the same answer; false where
+// the target is not in the list.
+template <class Units, class Target>
+__device__ __forceinline__ bool find(int nseq, int* sh, Units units, Target target, int& s_out,
+                                     int& base_out, int& goal) {
+    const int tid = threadIdx.x;
+    int U = 0, mine = 0, incl = 0, total = 0;
+    for (int c = 0; c < nseq; c += 256) {
+        mine = c + tid < nseq ? units(c + tid) : 0;
+        incl = block_scan(mine, sh, total);
+        U += total;
+    }
+    goal = target(U);
+    if (goal < 0 || goal >= U) return false;
+    int base = 0;
+    if (tid == 0) sh[4] = -1;
+    __syncthreads();
+    for (int c = 0; c < nseq; c += 256) {
+        if (nseq > 256) {
+            mine = c + tid < nseq ? units(c + tid) : 0;
+            incl = block_scan(mine, sh, total);
+        }
+        const int before = base + incl - mine;
+        // (sums that overflow, from a cu_seqlens that is not one, are no place)
+        if (before >= 0 && goal >= before && goal - before < mine) {
+            sh[4] = c + tid;
+            sh[5] = before;
+        }
+        base += total;
+    }
+    __syncthreads();
+    s_out = sh[4];
+    base_out = sh[5];
+    __syncthreads();
+    return s_out >= 0;
 }
 
-__global__ __launch_bounds__(64) void simple_kernel(PagedAttention a) {
-    const int64_t t = blockIdx.x;
-    const int head = blockIdx.y, lane = threadIdx.x;
-    const int group = (int)(a.Hq / a.Hk), h = head / group;
-    const int plog = __builtin_ctzll((uint64_t)a.page_size);
-    float q[4] = {}, o[4] = {}, m = -__builtin_inff(), l = 0.0f;
-    const bool mine = lane * 4 < a.D;
-    if (mine)
-        for (int i = 0; i < 4; i++) q[i] = h2f(a.q[t * a.ldq + head * a.hsq + lane * 4 + i]);
-    int64_t s = 0;
-    while (s < a.B && seq_start(a, s + 1) <= t) s++;
-    if (s < a.B && t >= seq_start(a, s)) {
-        const int64_t n = seq_start(a, s + 1) - seq_start(a, s), L0 = a.context_lens[s],
-                      W = a.max_pages << plog, L = L0 > W + 1 ? W + 1 : L0;
-        const int64_t p = L - n + (t - seq_start(a, s));
-        int64_t j = a.window && p - a.window + 1 > 0 ? p - a.window + 1 : 0;
-        for (; j <= p; j++) {
-            const int64_t col = j >> plog;
-            int64_t page = col < a.max_pages ? a.block_tables[s * a.ldt + col] : -1;
-            const bool bad = page < 0 || page >= a.num_pages;
-            const int64_t at = (((bad ? 0 : page) * a.Hk + h) << plog) + (j & (a.page_size - 1));
-            float dot = 0.0f, v[4] = {};
-            if (mine && !bad)
-                for (int i = 0; i < 4; i++) {
-                    const int64_t e = at * a.D + lane * 4 + i;
-                    if (a.k_scale) {
-                        dot += q[i] * ((float)static_cast<const int8_t*>(a.k_cache)[e] * a.k_scale[at]);
-                        v[i] = (float)static_cast<const int8_t*>(a.v_cache)[e] * a.v_scale[at];
-                    } else {
-                        dot += q[i] * h2f(static_cast<const uint16_t*>(a.k_cache)[e]);
-                        v[i] = h2f(static_cast<const uint16_t*>(a.v_cache)[e]);
+// ---- small pieces ------------------------------------------------------------------
+
+__device__ __forceinline__ float max_xor32(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v),
+                                                    __builtin_bit_cast(uint32_t, v), false, false);
+    return __builtin_fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]),
+                           __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+__device__ __forceinline__ float max_xor16(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v),
+                                                    __builtin_bit_cast(uint32_t, v), false, false);
+    return __builtin_fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]),
+                           __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    const f32x2 v = {a, b};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, h2));  // to nearest even
+}
+
+// Four int8 codes -> four fp16 (exact): the byte, made unsigned, is the low mantissa of
+// 1024 + b; subtracting 1024 + 128 leaves the code.
+__device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    const uint32_t x = w ^ 0x80808080u;
+    const h2 off = {(_Float16)1152.0f, (_Float16)1152.0f};
+    lo = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, __builtin_amdgcn_perm(
+                                          0x64646464u, x, 0x04010400u)) - off);
+    hi = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, __builtin_amdgcn_perm(
+                                          0x64646464u, x, 0x04030402u)) - off);
+}
+
+// 16 codes -> two chunks of 8 fp16
+__device__ __forceinline__ void codes16(u32x4 w, u32x4& a, u32x4& b) {
+    uint32_t o[8];
+#pragma unroll
+    for (int i = 0; i < 4; i++) codes_to_half(w[i], o[2 * i], o[2 * i + 1]);
+    a = u32x4{o[0], o[1], o[2], o[3]};
+    b = u32x4{o[4], o[5], o[6], o[7]};
+}
+
+// log2 and reciprocal of a value's scale; a scale of 0 (a row of zeros) counts as 2^-64,
+// so that its key keeps its weight in l while its codes add nothing that shows.
+__device__ __forceinline__ void value_scale(float v, float& lv, float& rv) {
+    v = v < 0x1p-64f ? 0x1p-64f : v;
+    lv = __builtin_amdgcn_logf(v);
+    rv = 1.0f / v;
+}
+
+__device__ __forceinline__ h8 read_tr(const uint16_t* p, const uint16_t* p2) {
+    typedef __attribute__((address_space(3))) tr4 lds_tr4;
+    typedef __attribute__((address_space(3))) void lds_void;
+    const tr4 a = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr4*)(lds_void*)p);
+    const tr4 b = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr4*)(lds_void*)p2);
+    u32x4 v;
+    const uint2 x = __builtin_bit_cast(uint2, a), y = __builtin_bit_cast(uint2, b);
+    v = u32x4{x.x, x.y, y.x, y.y};
+    return __builtin_bit_cast(h8, v);
+}
+
+// Whether any of 8 fp16 is an infinity or NaN (exponent all ones).
+__device__ __forceinline__ uint32_t odd_bits(u32x4 v) {
+    uint32_t o = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) o |= ((v[i] & 0x7fff7fffu) + 0x04000400u) & 0x80008000u;
+    return o;
+}
+
+// A fragment of values with infinities or NaN, split: what is finite, and ones where a
+// +inf or NaN (`pos`), a -inf or NaN (`neg`) stands.
+__device__ __forceinline__ void split_odd(h8 v, h8& fin, h8& pos, h8& neg) {
+    const u32x4 x = __builtin_bit_cast(u32x4, v);
+    u32x4 f, p, n;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        uint32_t keep = 0, up = 0, down = 0;
+#pragma unroll
+        for (int s = 0; s < 32; s += 16) {
+            const uint32_t b = x[i] >> s & 0xffffu, one = 0x3c00u << s;
+            const bool odd = (b & 0x7c00u) == 0x7c00u, nan = odd && (b & 0x3ffu) != 0;
+            if (!odd) keep |= b << s;
+            if (odd && (nan || !(b & 0x8000u))) up |= one;
+            if (odd && (nan || (b & 0x8000u))) down |= one;
+        }
+        f[i] = keep;
+        p[i] = up;
+        n[i] = down;
+    }
+    fin = __builtin_bit_cast(h8, f);
+    pos = __builtin_bit_cast(h8, p);
+    neg = __builtin_bit_cast(h8, n);
+}
+
+// A block of 16 keys of a sequence: its page, or why there is none.
+constexpr int kNone = -1, kBad = -2;
+__device__ __forceinline__ int page_of(const Attn& a, int s, int token, int lo, int hi) {
+    if (token >= hi || token + 16 <= lo) return kNone;
+    const int col = token >> a.plog;
+    if (col >= a.max_pages) return kBad;
+    const int page = a.tables[(int64_t)s * a.ldt + col];
+    return page < 0 || page >= a.num_pages ? kBad : page;
+}
+
+// ---- few rows ----------------------------------------------------------------------
+
+// LDS bytes of a wave: its V tile (32 keys), or its rows of o when they are joined
+template <int DP, int RB>
+constexpr int few_region() {
+    return 32 * DP * 2 > 16 * RB * DP * 4 ? 32 * DP * 2 : 16 * RB * DP * 4;
+}
+template <int DP, int RB>
+constexpr int few_lds() {
+    return 4 * few_region<DP, RB>() + 4 * 2 * 16 * RB * 4 + 32;
+}
+// floats of a part: o [16 RB][DP], m, l [16 RB]
+template <int DP, int RB>
+constexpr int few_part() {
+    return 16 * RB * (DP + 2);
+}
+
+// What few_kernel makes of a sequence: its range of keys and its units.
+struct FewSeq {
+    Seq q;
+    int rows, blocks, lo, tiles, units;
+};
+template <int RB>
+__device__ __forceinline__ FewSeq few_seq(const Attn& a, int s) {
+    FewSeq f;
+    f.q = sequence(a, s);
+    f.rows = f.q.n > a.few / a.group ? 0 : f.q.n * a.group;
+    f.blocks = (f.rows + 16 * RB - 1) / (16 * RB);
+    const int first = f.q.L - f.q.n;
+    f.lo = a.window && first - a.window + 1 > 0 ? (first - a.window + 1) & ~31 : 0;
+    f.tiles = (f.q.L - f.lo + kUnit - 1) / kUnit;
+    f.tiles = f.tiles > 1 ? f.tiles : 1;
+    f.units = f.blocks * a.Hk * (a.whole ? 1 : f.tiles);
+    return f;
+}
+
+__device__ __forceinline__ int per_worker(int U) {
+    return (U + (int)gridDim.x - 1) / (int)gridDim.x;
+}
+
+template <int DP, bool I8, int RB>
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void few_kernel(Attn a) {
+    constexpr int KS = DP / 32, DB = DP / 16;
+    constexpr int KL = I8 ? DP / 64 : DP / 32, VL = KL;  // loads of 16 keys
+    constexpr int CH = DP / 8;                           // chunks of a row in LDS
+    extern __shared__ __align__(16) char smem[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int col = lane & 15, G = lane >> 4;
+    uint16_t* vt = reinterpret_cast<uint16_t*>(smem + wave * few_region<DP, RB>());
+    float* ot = reinterpret_cast<float*>(vt);
+    float* ml = reinterpret_cast<float*>(smem + 4 * few_region<DP, RB>());  // [4][2][16 RB]
+    int* sh = reinterpret_cast<int*>(ml + 4 * 2 * 16 * RB);
+
+    int s, base, u;
+    int upw = 0;
+    if (!find(
+            a.nseq, sh, [&](int i) { return few_seq<RB>(a, i).units; },
+            [&](int U) {
+                upw = per_worker(U);
+                return upw * (int)blockIdx.x;
+            },
+            s, base, u))
+        return;
+    const int first_unit = u;
+    FewSeq f = few_seq<RB>(a, s);
+    int per_item = a.whole ? 1 : f.tiles;
+    int item = (u - base) / per_item, tile = (u - base) - item * per_item;
+    int left = upw;
+
+    while (true) {
+        int nt = per_item - tile;
+        nt = nt < left ? nt : left;
+        const bool full = nt == per_item;
+        const int h = item % a.Hk, rb = item / a.Hk;
+        const int steps = a.whole ? f.tiles : nt;
+        const int row0 = rb * 16 * RB;
+        const int nrows = f.rows - row0 < 16 * RB ? f.rows - row0 : 16 * RB;
+        const int lo = a.window && f.q.L - f.q.n - a.window + 1 > 0 ? f.q.L - f.q.n - a.window + 1 : 0;
+        const int hi = f.q.L;
+        const int p0 = f.q.L - f.q.n;
+        const int pmin = p0 + row0 / a.group, pmax = p0 + (row0 + nrows - 1) / a.group;
+        const int t_first = f.lo + tile * kUnit + wave * 32;
+
+        // queries: row col of each block; the elements' order is the keys' (8 bits: two
+        // k-steps of a 16-byte load)
+        h8 q[RB][KS];
+        int prow[RB];
+#pragma unroll
+        for (int b = 0; b < RB; b++) {
+            const int r = row0 + 16 * b + col;
+            const int i = r / a.group, head = h * a.group + r - i * a.group;
+            prow[b] = r < f.rows ? p0 + i : -1;
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                const int d = I8 ? 64 * (k >> 1) + 16 * G + 8 * (k & 1) : 32 * k + 8 * G;
+                u32x4 v = {0, 0, 0, 0};
+                if (r < f.rows && d < a.D)
+                    v = *reinterpret_cast<const u32x4*>(a.q + (f.q.start + i) * a.ldq +
+                                                        head * a.hsq + d);
+                q[b][k] = __builtin_bit_cast(h8, v);
+            }
+        }
+
+        float m[RB], l[RB];
+        f32x4 o[RB][DB];
+#pragma unroll
+        for (int b = 0; b < RB; b++) {
+            m[b] = -kInf;
+            l[b] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < DB; d++) o[b][d] = f32x4{0, 0, 0, 0};
+        }
+
+        u32x4 kr[2][KL], vr[2][VL];
+        f32x4 ksr[2], vsr[2];
+        int pages = 0;  // lane j: block j & 1 of step (j >> 1) of the 32 ahead
+        int page[2];
+        auto load = [&](int i) {
+            if ((i & 31) == 0)
+                pages = i + (lane >> 1) < steps
+                            ? page_of(a, s, t_first + (i + (lane >> 1)) * kUnit + 16 * (lane & 1),
+                                      lo, hi)
+                            : kNone;
+            const int t0 = t_first + i * kUnit;
+#pragma unroll
+            for (int tb = 0; tb < 2; tb++) {
+                page[tb] = __builtin_amdgcn_readlane(pages, 2 * (i & 31) + tb);
+#pragma unroll
+                for (int j = 0; j < KL; j++) kr[tb][j] = vr[tb][j] = u32x4{0, 0, 0, 0};
+                ksr[tb] = vsr[tb] = f32x4{0, 0, 0, 0};
+                if (page[tb] < 0) continue;
+                const int tok = t0 + 16 * tb, in = tok & ((1 << a.plog) - 1);
+                const int64_t row = (((int64_t)page[tb] * a.Hk + h) << a.plog) + in;
+                if constexpr (I8) {
+                    const int8_t* kp = static_cast<const int8_t*>(a.kc) + row * a.D;
+                    const int8_t* vp = static_cast<const int8_t*>(a.vc) + row * a.D;
+#pragma unroll
+                    for (int j = 0; j < KL; j++)
+                        if (64 * j + 16 * G < a.D)
+                            kr[tb][j] = *reinterpret_cast<const u32x4*>(kp + col * a.D + 64 * j + 16 * G);
+#pragma unroll
+                    for (int j = 0; j < VL; j++) {
+                        const int c = j * 64 + lane, t = c / (DP / 16), d = 16 * (c % (DP / 16));
+                        if (d < a.D) vr[tb][j] = *reinterpret_cast<const u32x4*>(vp + t * a.D + d);
+                    }
+                    ksr[tb] = *reinterpret_cast<const f32x4*>(a.ks + row + 4 * G);
+                    vsr[tb] = *reinterpret_cast<const f32x4*>(a.vs + row + 4 * G);
+                } else {
+                    const uint16_t* kp = static_cast<const uint16_t*>(a.kc) + row * a.D;
+                    const uint16_t* vp = static_cast<const uint16_t*>(a.vc) + row * a.D;
+#pragma unroll
+                    for (int j = 0; j < KL; j++)
+                        if (32 * j + 8 * G < a.D)
+                            kr[tb][j] = *reinterpret_cast<const u32x4*>(kp + col * a.D + 32 * j + 8 * G);
+#pragma unroll
+                    for (int j = 0; j < VL; j++) {
+                        const int c = j * 64 + lane, t = c / CH, d = 8 * (c % CH);
+                        // what lies outside the range may be anything, and 0 * NaN is NaN
+                        if (d < a.D && tok + t < hi && tok + t >= lo)
+                            vr[tb][j] = *reinterpret_cast<const u32x4*>(vp + t * a.D + d);
                     }
                 }
-            const float z = bad ? __builtin_nanf("") : wave_sum(dot) * a.scale;
-            const float top = z > m || z != z ? z : m;
-            const float w = __builtin_expf(z - top), keep = m == top ? 1.0f : __builtin_expf(m - top);
-            l = l * keep + w;
-            for (int i = 0; i < 4; i++) o[i] = o[i] * keep + w * v[i];
+            }
+        };
+        // 16-byte chunk `ch` of key t of the V tile: chunks are permuted by pairs so that
+        // the 8 keys of a half wave's transposing read lie on different banks
+        auto v_at = [&](int t, int ch) {
+            const int f8 = DP == 64 ? ((t >> 1) & 3) << 1 : (t & 7) << 1;
+            return vt + t * DP + 8 * (ch ^ f8);
+        };
+
+        load(0);
+        for (int i = 0; i < steps; i++) {
+            const int t0 = t_first + i * kUnit;
+            const bool bad[2] = {page[0] == kBad, page[1] == kBad};
+            const bool none = page[0] == kNone && page[1] == kNone;
+            uint32_t odd = 0;
+#pragma unroll
+            for (int tb = 0; tb < 2; tb++)
+#pragma unroll
+                for (int j = 0; j < VL; j++) {
+                    const int c = j * 64 + lane;
+                    if constexpr (I8) {
+                        u32x4 x, y;
+                        codes16(vr[tb][j], x, y);
+                        const int t = 16 * tb + c / (DP / 16), ch = 2 * (c % (DP / 16));
+                        *reinterpret_cast<u32x4*>(v_at(t, ch)) = x;
+                        *reinterpret_cast<u32x4*>(v_at(t, ch + 1)) = y;
+                    } else {
+                        const int t = 16 * tb + c / CH, ch = c % CH;
+                        *reinterpret_cast<u32x4*>(v_at(t, ch)) = vr[tb][j];
+                        odd |= odd_bits(vr[tb][j]);
+                    }
+                }
+            f32x4 sc[RB][2];
+#pragma unroll
+            for (int tb = 0; tb < 2; tb++) {
+                h8 kf[KS];
+#pragma unroll
+                for (int j = 0; j < KL; j++) {
+                    if constexpr (I8) {
+                        u32x4 x, y;
+                        codes16(kr[tb][j], x, y);
+                        kf[2 * j] = __builtin_bit_cast(h8, x);
+                        kf[2 * j + 1] = __builtin_bit_cast(h8, y);
+                    } else {
+                        kf[j] = __builtin_bit_cast(h8, kr[tb][j]);
+                    }
+                }
+#pragma unroll
+                for (int b = 0; b < RB; b++) {
+                    f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+                    for (int k = 0; k < KS; k++)
+                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[k], q[b][k], acc, 0, 0, 0);
+                    sc[b][tb] = acc;
+                }
+            }
+            f32x4 kx[2], lv[2], rv[2];
+            if constexpr (I8)
+#pragma unroll
+                for (int tb = 0; tb < 2; tb++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        float x, y;
+                        value_scale(vsr[tb][r], x, y);
+                        lv[tb][r] = x;
+                        rv[tb][r] = y;
+                        kx[tb][r] = ksr[tb][r] * a.c;
+                    }
+            if (i + 1 < steps) load(i + 1);
+            if (none) continue;
+
+            const bool edge = t0 + 31 > pmin || (a.window && t0 <= pmax - a.window);
+            h8 p[RB];
+#pragma unroll
+            for (int b = 0; b < RB; b++) {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int tb = e >> 2, r = e & 3;
+                    if constexpr (I8)
+                        x[e] = __builtin_fmaf(sc[b][tb][r], kx[tb][r], lv[tb][r]);
+                    else
+                        x[e] = sc[b][tb][r] * a.c;
+                    if (bad[tb]) x[e] = __builtin_nanf("");
+                }
+                if (edge)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const int j = t0 + 16 * (e >> 2) + 4 * G + (e & 3);
+                        if (j > prow[b] || (a.window && j <= prow[b] - a.window)) x[e] = -kInf;
+                    }
+                float top = x[0];
+#pragma unroll
+                for (int e = 1; e < 8; e++) top = __builtin_fmaxf(top, x[e]);
+                top = max_xor32(max_xor16(top));
+                top = __builtin_fmaxf(top, m[b]);
+                const float at = top == -kInf ? 0.0f : top;
+                if (__any(top != m[b])) {
+                    const float keep = exp2_(m[b] - at);
+                    l[b] *= keep;
+#pragma unroll
+                    for (int d = 0; d < DB; d++) o[b][d] *= keep;
+                    m[b] = top;
+                }
+                float w[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    w[e] = exp2_(x[e] - at);
+                    if constexpr (I8)
+                        l[b] += w[e] == 0.0f ? 0.0f : w[e] * rv[e >> 2][e & 3];
+                    else
+                        l[b] += w[e];
+                }
+                const u32x4 pk = {pack2(w[0], w[1]), pack2(w[2], w[3]), pack2(w[4], w[5]),
+                                  pack2(w[6], w[7])};
+                p[b] = __builtin_bit_cast(h8, pk);
+            }
+            // values that are not finite under a mask: see split_odd
+            const bool split = edge && __any(odd != 0);
+            const int tr = col >> 2, dd = 4 * (col & 3);
+#pragma unroll
+            for (int d = 0; d < DB; d++) {
+                const int t = 4 * G + tr, ch = 2 * d + (dd >> 3);
+                h8 v = read_tr(v_at(t, ch) + (dd & 7), v_at(t + 16, ch) + (dd & 7));
+                if (split) {
+                    h8 fin, pos, neg;
+                    split_odd(v, fin, pos, neg);
+                    v = fin;
+#pragma unroll
+                    for (int b = 0; b < RB; b++) {
+                        h8 seen;
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            const int j = t0 + 16 * (e >> 2) + 4 * G + (e & 3);
+                            seen[e] = j > prow[b] || (a.window && j <= prow[b] - a.window)
+                                          ? (_Float16)0.0f : (_Float16)1.0f;
+                        }
+                        const f32x4 z = {0, 0, 0, 0};
+                        const f32x4 up = __builtin_amdgcn_mfma_f32_16x16x32_f16(pos, seen, z, 0, 0, 0);
+                        const f32x4 dn = __builtin_amdgcn_mfma_f32_16x16x32_f16(neg, seen, z, 0, 0, 0);
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            if (up[r] > 0.0f) o[b][d][r] += kInf;
+                            if (dn[r] > 0.0f) o[b][d][r] -= kInf;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int b = 0; b < RB; b++)
+                    o[b][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[b], o[b][d], 0, 0, 0);
+            }
+        }
+
+        // join the four waves: o rows in LDS (16-byte pieces permuted against bank conflicts)
+#pragma unroll
+        for (int b = 0; b < RB; b++) {
+            l[b] += __shfl_xor(l[b], 16, 64);
+            l[b] += __shfl_xor(l[b], 32, 64);
+            if (G == 0) {
+                ml[(wave * 2) * 16 * RB + 16 * b + col] = m[b];
+                ml[(wave * 2 + 1) * 16 * RB + 16 * b + col] = l[b];
+            }
+#pragma unroll
+            for (int d = 0; d < DB; d++) {
+                const int c4 = (4 * d + G) ^ (col & 7);
+                *reinterpret_cast<f32x4*>(ot + (16 * b + col) * DP + 4 * c4) = o[b][d];
+            }
+        }
+        __syncthreads();
+        const int D4 = a.D >> 2;
+        float* part = a.part + (int64_t)(2 * blockIdx.x + (first_unit == u ? 0 : 1)) * few_part<DP, RB>();
+        for (int e = threadIdx.x; e < nrows * D4; e += 256) {
+            const int r = e / D4, d4 = e - r * D4;
+            float top = -kInf, wm[4];
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                wm[w] = ml[(w * 2) * 16 * RB + r];
+                top = __builtin_fmaxf(top, wm[w]);
+            }
+            const float at = top == -kInf ? 0.0f : top;
+            float sum = 0.0f;
+            f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const float k = exp2_(wm[w] - at);
+                sum += k * ml[(w * 2 + 1) * 16 * RB + r];
+                acc += k * *reinterpret_cast<const f32x4*>(
+                               smem + w * few_region<DP, RB>() + (r * DP + 4 * (d4 ^ (r & 7))) * 4);
+            }
+            if (full) {
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                const int rr = row0 + r, i = rr / a.group, head = h * a.group + rr - i * a.group;
+                uint2 y = {pack2(acc[0] * inv, acc[1] * inv), pack2(acc[2] * inv, acc[3] * inv)};
+                if (sum == 0.0f) y = uint2{0, 0};
+                *reinterpret_cast<uint2*>(a.out + ((int64_t)(f.q.start + i) * a.Hq + head) * a.D +
+                                          4 * d4) = y;
+            } else {
+                *reinterpret_cast<f32x4*>(part + r * DP + 4 * d4) = acc;
+                if (d4 == 0) {
+                    part[16 * RB * DP + r] = top;
+                    part[16 * RB * DP + 16 * RB + r] = sum;
+                }
+            }
+        }
+        left -= nt;
+        u += nt;
+        if (left <= 0) return;
+        tile = 0;
+        if (++item >= f.blocks * a.Hk) {
+            do {
+                if (++s >= a.nseq) return;
+                f = few_seq<RB>(a, s);
+            } while (f.units == 0);
+            item = 0;
+            per_item = a.whole ? 1 : f.tiles;
+        }
+        __syncthreads();  // the rows of o have been read
+    }
+}
+
+// Joins the parts of the item that run `blockIdx.x` began and did not finish.
+template <int DP, int RB>
+__global__ __launch_bounds__(256) void few_join(Attn a) {
+    __shared__ int sh[8];
+    int s, base, u, upw = 0;
+    if (!find(
+            a.nseq, sh, [&](int i) { return few_seq<RB>(a, i).units; },
+            [&](int U) {
+                upw = per_worker(U);
+                const int end = upw * ((int)blockIdx.x + 1);
+                return end < U ? end - 1 : -1;  // the last run ends its item
+            },
+            s, base, u))
+        return;
+    const FewSeq f = few_seq<RB>(a, s);
+    const int item = (u - base) / f.tiles, begin = base + item * f.tiles, end = begin + f.tiles;
+    const int w0 = blockIdx.x;
+    if (end <= u + 1 || begin < w0 * upw) return;  // finished, or another run began it
+    const int w1 = (end - 1) / upw;
+    const int h = item % a.Hk, row0 = item / a.Hk * 16 * RB;
+    const int nrows = f.rows - row0 < 16 * RB ? f.rows - row0 : 16 * RB;
+    const int D4 = a.D >> 2;
+    auto slot = [&](int w) {
+        return a.part + (int64_t)(2 * w + (w == w0 && begin != w0 * upw ? 1 : 0)) * few_part<DP, RB>();
+    };
+    for (int e = threadIdx.x; e < nrows * D4; e += 256) {
+        const int r = e / D4, d4 = e - r * D4;
+        float top = -kInf;
+        for (int w = w0; w <= w1; w++) top = __builtin_fmaxf(top, slot(w)[16 * RB * DP + r]);
+        const float at = top == -kInf ? 0.0f : top;
+        float sum = 0.0f;
+        f32x4 acc = {0, 0, 0, 0};
+        for (int w = w0; w <= w1; w++) {
+            const float* p = slot(w);
+            const float k = exp2_(p[16 * RB * DP + r] - at);
+            sum += k * p[16 * RB * DP + 16 * RB + r];
+            acc += k * *reinterpret_cast<const f32x4*>(p + r * DP + 4 * d4);
+        }
+        const float inv = 1.0f / sum;
+        const int rr = row0 + r, i = rr / a.group, head = h * a.group + rr - i * a.group;
+        uint2 y = {pack2(acc[0] * inv, acc[1] * inv), pack2(acc[2] * inv, acc[3] * inv)};
+        if (sum == 0.0f) y = uint2{0, 0};
+        *reinterpret_cast<uint2*>(a.out + ((int64_t)(f.q.start + i) * a.Hq + head) * a.D + 4 * d4) = y;
+    }
+}
+
+// ---- tiles of 128 rows -------------------------------------------------------------
+
+// 16 bytes a lane, global -> LDS at `lds` + lane * 16.  The wait is the caller's.
+__device__ __forceinline__ void copy16(uint32_t lds, const void* src) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                 :: "s"(lds), "v"(src) : "memory", "m0");
+}
+
+__device__ const uint4 kZeros = {0, 0, 0, 0};
+__device__ const uint4 kNaNs = {0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u};
+
+template <int DP, bool I8>
+constexpr int tile_lds() {
+    return 2 * 2 * kTileKeys * DP * 2 + (I8 ? 2 * 3 * kTileKeys * 4 : 0) + 32;
+}
+
+// The item of a workgroup of tile_kernel and tile_join.
+struct TileItem {
+    Seq q;
+    int s, rows, tile, h, lo, hi, kt0, kt1, per, parts;
+    int index;  // of the parts
+};
+
+// Tiles of all sequences from the last to the first: a causal tile's keys grow with its
+// rows, and the longest ones begin first.
+__device__ __forceinline__ bool tile_item(const Attn& a, int id, int h, int* sh, TileItem& t) {
+    auto tiles = [&](int s) {
+        const Seq q = sequence(a, s);
+        return q.n > a.few / a.group
+                   ? (int)(((int64_t)q.n * a.group + kTileRows - 1) / kTileRows) : 0;
+    };
+    int base, goal;
+    if (!find(a.nseq, sh, tiles, [&](int N) { return N - 1 - id; }, t.s, base, goal) ||
+        goal >= a.tiles)
+        return false;
+    t.q = sequence(a, t.s);
+    t.rows = t.q.n * a.group;
+    t.tile = goal - base;
+    t.h = h;
+    const int i0 = t.tile * kTileRows / a.group;
+    int i1 = (t.tile * kTileRows + kTileRows - 1) / a.group;
+    i1 = i1 < t.q.n ? i1 : t.q.n - 1;
+    const int p0 = t.q.L - t.q.n;
+    t.hi = p0 + i1 + 1 > 0 ? p0 + i1 + 1 : 0;
+    t.lo = a.window && p0 + i0 - a.window + 1 > 0 ? p0 + i0 - a.window + 1 : 0;
+    t.kt0 = t.lo / kTileKeys;
+    t.kt1 = (t.hi + kTileKeys - 1) / kTileKeys;
+    const int n = t.kt1 > t.kt0 ? t.kt1 - t.kt0 : 0;
+    // a part has four tiles of keys at least
+    t.parts = n / 4 < a.splits ? (n / 4 > 1 ? n / 4 : 1) : a.splits;
+    t.per = (n + t.parts - 1) / t.parts;
+    t.index = goal * a.Hk + h;
+    return true;
+}
+
+template <int DP>
+constexpr int tile_part() {
+    return kTileRows * (DP + 2);
+}
+
+template <int DP, bool I8>
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
+    constexpr int KS = DP / 16, DB = DP / 32, CH = DP / 8;
+    constexpr int TB = kTileKeys * DP * 2;  // bytes of a K or V tile
+    constexpr int NL = I8 ? DP / 64 : DP / 32;
+    extern __shared__ __align__(16) char smem[];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 31, H = lane >> 5;
+    float* scales = reinterpret_cast<float*>(smem + 4 * TB);  // [2][3][64]
+    int* sh = reinterpret_cast<int*>(smem + tile_lds<DP, I8>() - 32);
+
+    // a key head's items are neighbours modulo the heads: with the round-robin dispatch
+    // over the 8 XCDs they share an L2 where the heads divide 8
+    const int h = blockIdx.x % a.Hk, rest = blockIdx.x / a.Hk;
+    const int split = rest % a.splits;
+    TileItem t;
+    if (!tile_item(a, rest / a.splits, h, sh, t) || split >= t.parts) return;
+    const int first = t.kt0 + split * t.per;
+    const int last = first + t.per < t.kt1 ? first + t.per : t.kt1;
+
+    const int row0 = t.tile * kTileRows + wave * 32;
+    const int p0 = t.q.L - t.q.n;
+    const int nrows = t.rows - row0 < 32 ? t.rows - row0 : 32;  // may be 0 or less
+    const int pmin = p0 + row0 / a.group;
+    const int pmax = nrows > 0 ? p0 + (row0 + nrows - 1) / a.group : -1;
+    int prow = -1;
+    h8 q[KS];
+    const int r = row0 + col, qi = r / a.group, head = h * a.group + r - qi * a.group;
+    if (r < t.rows) prow = p0 + qi;
+#pragma unroll
+    for (int k = 0; k < KS; k++) {
+        u32x4 v = {0, 0, 0, 0};
+        if (r < t.rows && 16 * k + 8 * H < a.D)
+            v = *reinterpret_cast<const u32x4*>(a.q + (t.q.start + qi) * a.ldq + head * a.hsq +
+                                                16 * k + 8 * H);
+        q[k] = __builtin_bit_cast(h8, v);
+    }
+
+    // chunk ch of key t: K rows are read by 32 keys at one chunk, V rows by 4 keys at 4
+    // chunks (transposing); both permutations put those on different banks
+    auto k_swz = [](int t) { return DP == 64 ? (t >> 1) & 7 : t & 15; };
+    auto v_swz = [](int t) { return DP == 64 ? ((t >> 1) & 1) << 2 : (t & 3) << 2; };
+
+    int pages = 0;  // lane j: the wave's 16 keys of tile (kt & ~63) + j, counted from `first`
+    u32x4 kr[I8 ? NL : 1], vr[I8 ? NL : 1];
+    float ksr = 0.0f, vsr = 1.0f;
+    auto begin = [&](int kt, int buf) {
+        const int i = kt - first;
+        if ((i & 63) == 0)
+            pages = kt + lane < last ? page_of(a, t.s, (kt + lane) * kTileKeys + 16 * wave, t.lo, t.hi)
+                                     : kNone;
+        const int page = __builtin_amdgcn_readlane(pages, i & 63);
+        const int tok = kt * kTileKeys + 16 * wave;
+        const int64_t row = (((int64_t)(page < 0 ? 0 : page) * a.Hk + h) << a.plog) +
+                            (tok & ((1 << a.plog) - 1));
+        if constexpr (I8) {
+#pragma unroll
+            for (int j = 0; j < NL; j++) {
+                const int c = j * 64 + lane, k = c / (DP / 16), d = 16 * (c % (DP / 16));
+                kr[j] = vr[j] = u32x4{0, 0, 0, 0};
+                if (page >= 0 && d < a.D) {
+                    const int64_t at = (row + k) * a.D + d;
+                    kr[j] = *reinterpret_cast<const u32x4*>(static_cast<const int8_t*>(a.kc) + at);
+                    vr[j] = *reinterpret_cast<const u32x4*>(static_cast<const int8_t*>(a.vc) + at);
+                }
+            }
+            ksr = page == kBad ? __builtin_nanf("") : 0.0f;
+            vsr = 1.0f;
+            if (page >= 0) {
+                ksr = a.ks[row + (lane & 15)];
+                vsr = a.vs[row + (lane & 15)];
+            }
+        } else {
+            const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)smem;
+            const uint32_t kd = base + buf * 2 * TB + 16 * wave * DP * 2;
+#pragma unroll
+            for (int j = 0; j < NL; j++) {
+                const int c = j * 64 + lane, k = c / CH, in = c % CH;
+                const int dk = 8 * (in ^ k_swz(16 * wave + k)), dv = 8 * (in ^ v_swz(16 * wave + k));
+                const void* ks = static_cast<const uint16_t*>(a.kc) + (row + k) * a.D + dk;
+                const void* vs = static_cast<const uint16_t*>(a.vc) + (row + k) * a.D + dv;
+                if (page < 0 || dk >= a.D) ks = page == kBad && dk < a.D ? &kNaNs : &kZeros;
+                // what lies outside the range may be anything, and 0 * NaN is NaN
+                if (page < 0 || dv >= a.D || tok + k >= t.hi || tok + k < t.lo) vs = &kZeros;
+                copy16(kd + j * 1024, ks);
+                copy16(kd + TB + j * 1024, vs);
+            }
+        }
+    };
+    auto finish = [&](int buf) {
+        if constexpr (I8) {
+            char* kt = smem + buf * 2 * TB;
+#pragma unroll
+            for (int j = 0; j < NL; j++) {
+                const int c = j * 64 + lane, k = 16 * wave + c / (DP / 16), ch = 2 * (c % (DP / 16));
+                u32x4 x, y;
+                codes16(kr[j], x, y);
+                char* at = kt + k * DP * 2;
+                *reinterpret_cast<u32x4*>(at + 16 * (ch ^ k_swz(k))) = x;
+                *reinterpret_cast<u32x4*>(at + 16 * ((ch + 1) ^ k_swz(k))) = y;
+                codes16(vr[j], x, y);
+                *reinterpret_cast<u32x4*>(at + TB + 16 * (ch ^ v_swz(k))) = x;
+                *reinterpret_cast<u32x4*>(at + TB + 16 * ((ch + 1) ^ v_swz(k))) = y;
+            }
+            if (lane < 16) {
+                float lv, rv;
+                value_scale(vsr, lv, rv);
+                float* sc = scales + buf * 3 * kTileKeys + 16 * wave + lane;
+                sc[0] = ksr * a.c;
+                sc[kTileKeys] = lv;
+                sc[2 * kTileKeys] = rv;
+            }
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+    };
+
+    float m = -kInf, l = 0.0f;
+    f32x16 o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; d++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) o[d][e] = 0.0f;
+
+    auto compute = [&](int kt, int buf) {
+        const int t0 = kt * kTileKeys;
+        if (t0 > pmax || (a.window && t0 + kTileKeys - 1 <= pmin - a.window)) return;
+        const char* kb = smem + buf * 2 * TB;
+        const char* vb = kb + TB;
+        const float* sc = scales + buf * 3 * kTileKeys;
+        f32x16 s[2];
+#pragma unroll
+        for (int tb = 0; tb < 2; tb++) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) s[tb][e] = 0.0f;
+            const int k = 32 * tb + col;
+#pragma unroll
+            for (int i = 0; i < KS; i++) {
+                const u32x4 v = *reinterpret_cast<const u32x4*>(kb + k * DP * 2 +
+                                                                16 * ((2 * i + H) ^ k_swz(k)));
+                s[tb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, v), q[i],
+                                                               s[tb], 0, 0, 0);
+            }
+        }
+        // element e of block tb is key 32 tb + 8 (e / 4) + 4 H + e % 4
+#pragma unroll
+        for (int tb = 0; tb < 2; tb++)
+#pragma unroll
+            for (int e4 = 0; e4 < 4; e4++) {
+                if constexpr (I8) {
+                    const int at = 32 * tb + 8 * e4 + 4 * H;
+                    const f32x4 kx = *reinterpret_cast<const f32x4*>(sc + at);
+                    const f32x4 lv = *reinterpret_cast<const f32x4*>(sc + kTileKeys + at);
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        s[tb][4 * e4 + e] = __builtin_fmaf(s[tb][4 * e4 + e], kx[e], lv[e]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) s[tb][4 * e4 + e] *= a.c;
+                }
+            }
+        const bool edge = t0 + kTileKeys - 1 > pmin || (a.window && t0 <= pmax - a.window);
+        if (edge)
+#pragma unroll
+            for (int tb = 0; tb < 2; tb++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const int j = t0 + 32 * tb + 8 * (e >> 2) + 4 * H + (e & 3);
+                    if (j > prow || (a.window && j <= prow - a.window)) s[tb][e] = -kInf;
+                }
+        float top = s[0][0];
+#pragma unroll
+        for (int tb = 0; tb < 2; tb++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) top = __builtin_fmaxf(top, s[tb][e]);
+        top = __builtin_fmaxf(max_xor32(top), m);
+        const float at = top == -kInf ? 0.0f : top;
+        if (__any(top != m)) {
+            const float keep = exp2_(m - at);
+            l *= keep;
+#pragma unroll
+            for (int d = 0; d < DB; d++) o[d] *= keep;
             m = top;
         }
+        h8 p[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            float w[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                w[e] = exp2_(s[k >> 1][8 * (k & 1) + e] - at);
+                if constexpr (!I8) l += w[e];
+            }
+            if constexpr (I8) {
+#pragma unroll
+                for (int e4 = 0; e4 < 2; e4++) {
+                    const f32x4 rv = *reinterpret_cast<const f32x4*>(
+                        sc + 2 * kTileKeys + 32 * (k >> 1) + 16 * (k & 1) + 8 * e4 + 4 * H);
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        l += w[4 * e4 + e] == 0.0f ? 0.0f : w[4 * e4 + e] * rv[e];
+                }
+            }
+            const u32x4 pk = {pack2(w[0], w[1]), pack2(w[2], w[3]), pack2(w[4], w[5]),
+                              pack2(w[6], w[7])};
+            p[k] = __builtin_bit_cast(h8, pk);
+        }
+        // value fragment of 32 elements (block d) and keys 16 k + {4 H .., 8 + 4 H ..}
+        auto value = [&](int d, int k) {
+            const int tk = 16 * k + 4 * H + ((lane & 15) >> 2);
+            const int dd = 32 * d + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+            const char* p1 = vb + tk * DP * 2 + 16 * ((dd >> 3) ^ v_swz(tk)) + 2 * (dd & 7);
+            const char* p2 = vb + (tk + 8) * DP * 2 + 16 * ((dd >> 3) ^ v_swz(tk + 8)) + 2 * (dd & 7);
+            return read_tr(reinterpret_cast<const uint16_t*>(p1), reinterpret_cast<const uint16_t*>(p2));
+        };
+        bool split_v = false;
+        if (!I8 && edge) {
+            uint32_t odd = 0;
+#pragma unroll
+            for (int d = 0; d < DB; d++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) odd |= odd_bits(__builtin_bit_cast(u32x4, value(d, k)));
+            split_v = __any(odd != 0);
+        }
+        if (split_v) {  // values that are not finite under a mask: see split_odd
+#pragma unroll 1
+            for (int k = 0; k < 4; k++) {
+                h8 seen;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int j = t0 + 16 * k + 8 * (e >> 2) + 4 * H + (e & 3);
+                    seen[e] = j > prow || (a.window && j <= prow - a.window) ? (_Float16)0.0f
+                                                                             : (_Float16)1.0f;
+                }
+#pragma unroll
+                for (int d = 0; d < DB; d++) {
+                    h8 fin, pos, neg;
+                    split_odd(value(d, k), fin, pos, neg);
+                    f32x16 z;
+#pragma unroll
+                    for (int e = 0; e < 16; e++) z[e] = 0.0f;
+                    const f32x16 up = __builtin_amdgcn_mfma_f32_32x32x16_f16(pos, seen, z, 0, 0, 0);
+                    const f32x16 dn = __builtin_amdgcn_mfma_f32_32x32x16_f16(neg, seen, z, 0, 0, 0);
+                    const h8 pk = k == 0 ? p[0] : k == 1 ? p[1] : k == 2 ? p[2] : p[3];
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fin, pk, o[d], 0, 0, 0);
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        if (up[e] > 0.0f) o[d][e] += kInf;
+                        if (dn[e] > 0.0f) o[d][e] -= kInf;
+                    }
+                }
+            }
+            return;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+            for (int d = 0; d < DB; d++)
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(value(d, k), p[k], o[d], 0, 0, 0);
+    };
+
+    if (first < last) {
+        begin(first, 0);
+        finish(0);
+        __syncthreads();
+        for (int kt = first; kt < last; kt++) {
+            const int buf = (kt - first) & 1;
+            if (kt + 1 < last) begin(kt + 1, buf ^ 1);
+            compute(kt, buf);
+            if (kt + 1 < last) finish(buf ^ 1);
+            __syncthreads();
+        }
     }
-    if (mine)
-        for (int i = 0; i < 4; i++)
-            a.out[(t * a.Hq + head) * a.D + lane * 4 + i] = f2h(l == 0.0f ? 0.0f : o[i] / l);
+
+    l += __shfl_xor(l, 32, 64);
+    if (r >= t.rows) return;
+    if (t.parts > 1) {
+        float* part = a.part + ((int64_t)t.index * a.splits + split) * tile_part<DP>();
+        const int pr = wave * 32 + col;
+#pragma unroll
+        for (int d = 0; d < DB; d++)
+#pragma unroll
+            for (int e4 = 0; e4 < 4; e4++) {
+                const f32x4 v = {o[d][4 * e4], o[d][4 * e4 + 1], o[d][4 * e4 + 2], o[d][4 * e4 + 3]};
+                *reinterpret_cast<f32x4*>(part + pr * DP + 32 * d + 8 * e4 + 4 * H) = v;
+            }
+        if (H == 0) {
+            part[kTileRows * DP + pr] = m;
+            part[kTileRows * DP + kTileRows + pr] = l;
+        }
+        return;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    uint16_t* dst = a.out + ((int64_t)(t.q.start + qi) * a.Hq + head) * a.D;
+#pragma unroll
+    for (int d = 0; d < DB; d++)
+#pragma unroll
+        for (int e4 = 0; e4 < 4; e4++) {
+            const int at = 32 * d + 8 * e4 + 4 * H;
+            uint2 y = {pack2(o[d][4 * e4] * inv, o[d][4 * e4 + 1] * inv),
+                       pack2(o[d][4 * e4 + 2] * inv, o[d][4 * e4 + 3] * inv)};
+            if (l == 0.0f) y = uint2{0, 0};
+            if (at < a.D) *reinterpret_cast<uint2*>(dst + at) = y;
+        }
+}
+
+// Joins the parts of an item of tile_kernel, 32 rows a workgroup.
+template <int DP>
+__global__ __launch_bounds__(256) void tile_join(Attn a) {
+    __shared__ int sh[8];
+    const int quarter = blockIdx.x & 3, id = blockIdx.x >> 2;
+    TileItem t;
+    if (!tile_item(a, id / a.Hk, id % a.Hk, sh, t) || t.parts <= 1) return;
+    const float* parts = a.part + (int64_t)t.index * a.splits * tile_part<DP>();
+    const int D4 = a.D >> 2;
+    for (int e = threadIdx.x; e < 32 * D4; e += 256) {
+        const int pr = quarter * 32 + e / D4, d4 = e % D4, r = t.tile * kTileRows + pr;
+        if (r >= t.rows) return;
+        float top = -kInf;
+        for (int w = 0; w < t.parts; w++)
+            top = __builtin_fmaxf(top, parts[w * tile_part<DP>() + kTileRows * DP + pr]);
+        const float at = top == -kInf ? 0.0f : top;
+        float sum = 0.0f;
+        f32x4 acc = {0, 0, 0, 0};
+        for (int w = 0; w < t.parts; w++) {
+            const float* p = parts + w * tile_part<DP>();
+            const float k = exp2_(p[kTileRows * DP + pr] - at);
+            sum += k * p[kTileRows * DP + kTileRows + pr];
+            acc += k * *reinterpret_cast<const f32x4*>(p + pr * DP + 4 * d4);
+        }
+        const float inv = 1.0f / sum;
+        const int i = r / a.group, head = t.h * a.group + r - i * a.group;
+        uint2 y = {pack2(acc[0] * inv, acc[1] * inv), pack2(acc[2] * inv, acc[3] * inv)};
+        if (sum == 0.0f) y = uint2{0, 0};
+        *reinterpret_cast<uint2*>(a.out + ((int64_t)(t.q.start + i) * a.Hq + head) * a.D + 4 * d4) = y;
+    }
+}
+
+// ---- host --------------------------------------------------------------------------
+
+// How a call is cut up, from what the host knows.
+struct Plan {
+    int rb;               // 16-row blocks of few_kernel's rows
+    int few;              // rows of a sequence that few_kernel takes at most
+    bool use_few, use_tile;
+    int64_t workers;      // of few_kernel
+    int64_t tiles;        // of 128 rows, at most
+    int splits;
+    int64_t bytes;
+};
+
+int padded_dim(int64_t D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
+
+Plan plan_of(int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t B, int64_t most,
+             int64_t max_context) {
+    const int64_t group = Hq / Hk, rows = most * group, DP = padded_dim(D);
+    Plan p{};
+    p.rb = rows <= 32 && rows > 16 ? 2 : 1;
+    p.use_tile = rows > 32;
+    // one sequence of many rows: nothing is left for few_kernel but padding, which the
+    // tiles take too
+    p.use_few = !p.use_tile || B > 1;
+    p.few = !p.use_tile ? 1 << 30 : p.use_few ? 16 * p.rb : 0;
+    const int64_t units = (max_context + 1 + kUnit - 1) / kUnit;
+    p.workers = (B + 1 + T * group / (16 * p.rb)) * Hk * units;
+    p.workers = p.workers < 512 ? p.workers : 512;
+    p.tiles = T * group / kTileRows + B + 1;
+    const int64_t items = p.tiles * Hk;
+    p.splits = items >= 384 ? 1 : (int)(512 / items);
+    if (p.splits > 16) p.splits = 16;
+    if (p.use_few) p.bytes += p.workers * 2 * 16 * p.rb * (DP + 2) * 4;
+    if (p.use_tile && p.splits > 1) {
+        const int64_t b = items * p.splits * kTileRows * (DP + 2) * 4;
+        p.bytes = p.bytes > b ? p.bytes : b;
+    }
+    return p;
+}
+
+template <class K>
+int allow_lds(K kernel, int bytes) {
+    static bool done[64];
+    int dev = 0;
+    (void)hipGetDevice(&dev);
+    if (dev >= 0 && dev < 64 && done[dev]) return FNI8_OK;
+    const hipError_t e = hipFuncSetAttribute((const void*)kernel,
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != hipSuccess) {
+        fni8h::set_error_detail("LDS attribute (%d bytes): %s", bytes, hipGetErrorString(e));
+        return FNI8_ERR_LAUNCH;
+    }
+    if (dev >= 0 && dev < 64) done[dev] = true;
+    return FNI8_OK;
+}
+
+template <int DP, bool I8, int RB>
+int run_few(const Attn& a, int64_t workers, hipStream_t st) {
+    const auto kern = few_kernel<DP, I8, RB>;
+    constexpr int lds = few_lds<DP, RB>();
+    const int rc = allow_lds(kern, lds);
+    if (rc) return rc;
+    kern<<<dim3((uint32_t)workers), 256, lds, st>>>(a);
+    if (!a.whole && workers > 1) few_join<DP, RB><<<dim3((uint32_t)workers), 256, 0, st>>>(a);
+    return FNI8_OK;
+}
+
+template <int DP, bool I8>
+int run_tile(const Attn& a, int64_t tiles, hipStream_t st) {
+    const auto kern = tile_kernel<DP, I8>;
+    constexpr int lds = tile_lds<DP, I8>();
+    const int rc = allow_lds(kern, lds);
+    if (rc) return rc;
+    kern<<<dim3((uint32_t)(tiles * a.Hk * a.splits)), 256, lds, st>>>(a);
+    if (a.splits > 1) tile_join<DP><<<dim3((uint32_t)(tiles * a.Hk * 4)), 256, 0, st>>>(a);
+    return FNI8_OK;
+}
+
+template <int DP, bool I8>
+int run_all(Attn a, const Plan& p, hipStream_t st) {
+    // few_kernel and its join have read their parts before the tiles' are written
+    if (p.use_few) {
+        a.whole = a.part == nullptr;
+        const int64_t grid = a.whole ? (a.nseq + (p.use_tile ? 0 : (int64_t)a.T * a.group / (16 * p.rb))) * a.Hk
+                                     : p.workers;
+        const int rc = p.rb == 1 ? run_few<DP, I8, 1>(a, grid, st) : run_few<DP, I8, 2>(a, grid, st);
+        if (rc) return rc;
+    }
+    if (p.use_tile) {
+        a.splits = a.part ? p.splits : 1;
+        return run_tile<DP, I8>(a, p.tiles, st);
+    }
+    return FNI8_OK;
 }
 
 }  // namespace
 
 namespace fni8h {
 
-int64_t paged_attention_workspace_bytes(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t,
-                                        int64_t) {
-    return 0;
+int64_t paged_attention_workspace_bytes(int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t B,
+                                        int64_t max_seqlen, int64_t max_context) {
+    return (plan_of(T, Hq, Hk, D, B, max_seqlen, max_context).bytes + 255) & ~(int64_t)255;
 }
 
-int launch_paged_attention(const PagedAttention& a, hipStream_t st) {
-    if (a.T == 0) return FNI8_OK;
-    simple_kernel<<<dim3((uint32_t)a.T, (uint32_t)a.Hq), 64, 0, st>>>(a);
+int launch_paged_attention(const PagedAttention& p, hipStream_t st) {
+    if (p.T == 0) return FNI8_OK;
+    const int64_t context = p.max_pages * p.page_size;
+    const Plan plan = plan_of(p.T, p.Hq, p.Hk, p.D, p.B, p.max_seqlen, context);
+    const int64_t group = p.Hq / p.Hk;
+    // the units' sums are 32 bits, a grid has 2^32 threads
+    const int64_t items = (p.B + 1 + (plan.use_tile ? 0 : p.T * group / (16 * plan.rb))) * p.Hk;
+    if (items * ((context + kUnit) / kUnit) >= (int64_t)1 << 31 || items >= (int64_t)1 << 24 ||
+        plan.tiles * p.Hk >= (int64_t)1 << 24) {
+        set_error_detail("T=%lld tokens of %lld sequences and %lld keys are too many for one call",
+                         (long long)p.T, (long long)p.B, (long long)context);
+        return FNI8_ERR_SHAPE;
+    }
+    Attn a{};
+    a.q = p.q; a.ldq = p.ldq; a.hsq = p.hsq;
+    a.kc = p.k_cache; a.vc = p.v_cache; a.ks = p.k_scale; a.vs = p.v_scale;
+    a.tables = p.block_tables; a.lens = p.context_lens; a.cu = p.cu_seqlens; a.ldt = p.ldt;
+    a.out = p.out;
+    a.T = (int)p.T; a.Hq = (int)p.Hq; a.Hk = (int)p.Hk; a.D = (int)p.D; a.group = (int)group;
+    a.num_pages = (int)p.num_pages;
+    a.plog = __builtin_ctzll((uint64_t)p.page_size);
+    a.max_pages = (int)p.max_pages;
+    a.B = (int)p.B;
+    a.nseq = p.cu_seqlens ? a.B + 1 : a.B;
+    // a window that reaches past every key is none
+    a.window = p.window > context ? 0 : (int)p.window;
+    a.cap = (int)context + 1;
+    a.c = p.scale * 1.44269504088896340736f;
+    a.few = plan.few;
+    a.splits = 1;
+    a.tiles = (int)plan.tiles;
+    if (plan.bytes && p.work_bytes >= plan.bytes) a.part = reinterpret_cast<float*>(p.work);
+    int rc;
+    switch (padded_dim(p.D)) {
+        case 64: rc = p.k_scale ? run_all<64, true>(a, plan, st) : run_all<64, false>(a, plan, st); break;
+        case 128: rc = p.k_scale ? run_all<128, true>(a, plan, st) : run_all<128, false>(a, plan, st); break;
+        default: rc = p.k_scale ? run_all<256, true>(a, plan, st) : run_all<256, false>(a, plan, st);
+    }
+    if (rc) return rc;
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) {
         set_error_detail("paged_attention launch: %s", hipGetErrorString(e));

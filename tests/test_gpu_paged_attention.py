@@ -181,7 +181,7 @@ def test_chunk_with_a_page_outside_the_cache(ops, cuda):
     q = _q(200, 4, 128, 1)
     k, v, _, _, tables = ref.paged(lens, 16, 2, 128, 2)
     want, tol = ref.attention(q, k, v, tables, lens, starts)
-    tables[0, 10] = k.shape[0]
+    tables[0, 10] = k.shape[0]  # the first page past the cache
     want[60:] = math.nan  # tokens from 160 on see page 10
     ref.within(_run(ops, q, (k, v, None, None, tables), lens, starts), want, tol)
 
