@@ -43,6 +43,7 @@ constexpr float kInf = __builtin_inff();
 constexpr int kUnit = 128;      // keys of a unit of few_kernel: 32 for each of 4 waves
 constexpr int kTileRows = 128;  // rows of a workgroup of tile_kernel
 constexpr int kTileKeys = 64;
+constexpr float kLag = 8.0f;
 
 struct Attn {
     const uint16_t* q;
@@ -116,6 +117,7 @@ __device__ __forceinline__ bool find(int nseq, int* sh, Units units, Target targ
         incl = block_scan(mine, sh, total);
         U += total;
     }
+    U = __builtin_amdgcn_readfirstlane(U);  // wave-uniform from here on, in scalar registers
     goal = target(U);
     if (goal < 0 || goal >= U) return false;
     int base = 0;
@@ -135,8 +137,8 @@ __device__ __forceinline__ bool find(int nseq, int* sh, Units units, Target targ
         base += total;
     }
     __syncthreads();
-    s_out = sh[4];
-    base_out = sh[5];
+    s_out = __builtin_amdgcn_readfirstlane(sh[4]);
+    base_out = __builtin_amdgcn_readfirstlane(sh[5]);
     __syncthreads();
     return s_out >= 0;
 }
@@ -210,30 +212,26 @@ __device__ __forceinline__ uint32_t odd_bits(u32x4 v) {
     return o;
 }
 
-// A fragment of values with infinities or NaN, split: what is finite, and ones where a
-// +inf or NaN (`pos`), a -inf or NaN (`neg`) stands.
-__device__ __forceinline__ void split_odd(h8 v, h8& fin, h8& pos, h8& neg) {
-    const u32x4 x = __builtin_bit_cast(u32x4, v);
-    u32x4 f, p, n;
+// 8 fp16 with 0 in the place of infinities and NaN.
+__device__ __forceinline__ u32x4 finite_part(u32x4 v) {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        uint32_t keep = 0, up = 0, down = 0;
-#pragma unroll
-        for (int s = 0; s < 32; s += 16) {
-            const uint32_t b = x[i] >> s & 0xffffu, one = 0x3c00u << s;
-            const bool odd = (b & 0x7c00u) == 0x7c00u, nan = odd && (b & 0x3ffu) != 0;
-            if (!odd) keep |= b << s;
-            if (odd && (nan || !(b & 0x8000u))) up |= one;
-            if (odd && (nan || (b & 0x8000u))) down |= one;
-        }
-        f[i] = keep;
-        p[i] = up;
-        n[i] = down;
+        if ((v[i] & 0x7c00u) == 0x7c00u) v[i] &= 0xffff0000u;
+        if ((v[i] & 0x7c000000u) == 0x7c000000u) v[i] &= 0xffffu;
     }
-    fin = __builtin_bit_cast(h8, f);
-    pos = __builtin_bit_cast(h8, p);
-    neg = __builtin_bit_cast(h8, n);
+    return v;
 }
+
+// The fp16 in half `hi` of w where it is an infinity or NaN, else 0.
+__device__ __forceinline__ float odd_part(uint32_t w, int hi) {
+    const uint32_t b = hi ? w >> 16 : w & 0xffffu;
+    return (b & 0x7c00u) == 0x7c00u ? h2f((uint16_t)b) : 0.0f;
+}
+
+// Masks and values that are not finite: the weight of a key that a row does not see is 0,
+// but 0 times an infinity or NaN is NaN.  Where a tile that some row sees in part only holds
+// such a value, the tile's values are made finite before the product, and the rows that see
+// the key get the value added afterwards, read once more from the cache.
 
 // A block of 16 keys of a sequence: its page, or why there is none.
 constexpr int kNone = -1, kBad = -2;
@@ -291,7 +289,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void few_kernel(Attn a) {
     constexpr int KL = I8 ? DP / 64 : DP / 32, VL = KL;  // loads of 16 keys
     constexpr int CH = DP / 8;                           // chunks of a row in LDS
     extern __shared__ __align__(16) char smem[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, G = lane >> 4;
     uint16_t* vt = reinterpret_cast<uint16_t*>(smem + wave * few_region<DP, RB>());
     float* ot = reinterpret_cast<float*>(vt);
@@ -421,7 +420,23 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void few_kernel(Attn a) {
             const int t0 = t_first + i * kUnit;
             const bool bad[2] = {page[0] == kBad, page[1] == kBad};
             const bool none = page[0] == kNone && page[1] == kNone;
-            uint32_t odd = 0;
+            const bool edge = t0 + 31 > pmin || (a.window && t0 <= pmax - a.window);
+            bool odd = false;
+            const int held[2] = {page[0], page[1]};
+            if constexpr (!I8)
+                if (edge) {
+                    uint32_t bits = 0;
+#pragma unroll
+                    for (int tb = 0; tb < 2; tb++)
+#pragma unroll
+                        for (int j = 0; j < VL; j++) bits |= odd_bits(vr[tb][j]);
+                    odd = __any(bits != 0);
+                    if (odd)
+#pragma unroll
+                        for (int tb = 0; tb < 2; tb++)
+#pragma unroll
+                            for (int j = 0; j < VL; j++) vr[tb][j] = finite_part(vr[tb][j]);
+                }
 #pragma unroll
             for (int tb = 0; tb < 2; tb++)
 #pragma unroll
@@ -436,7 +451,6 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void few_kernel(Attn a) {
                     } else {
                         const int t = 16 * tb + c / CH, ch = c % CH;
                         *reinterpret_cast<u32x4*>(v_at(t, ch)) = vr[tb][j];
-                        odd |= odd_bits(vr[tb][j]);
                     }
                 }
             f32x4 sc[RB][2];
@@ -478,7 +492,6 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void few_kernel(Attn a) {
             if (i + 1 < steps) load(i + 1);
             if (none) continue;
 
-            const bool edge = t0 + 31 > pmin || (a.window && t0 <= pmax - a.window);
             h8 p[RB];
 #pragma unroll
             for (int b = 0; b < RB; b++) {
@@ -524,40 +537,35 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void few_kernel(Attn a) {
                                   pack2(w[6], w[7])};
                 p[b] = __builtin_bit_cast(h8, pk);
             }
-            // values that are not finite under a mask: see split_odd
-            const bool split = edge && __any(odd != 0);
             const int tr = col >> 2, dd = 4 * (col & 3);
 #pragma unroll
             for (int d = 0; d < DB; d++) {
                 const int t = 4 * G + tr, ch = 2 * d + (dd >> 3);
-                h8 v = read_tr(v_at(t, ch) + (dd & 7), v_at(t + 16, ch) + (dd & 7));
-                if (split) {
-                    h8 fin, pos, neg;
-                    split_odd(v, fin, pos, neg);
-                    v = fin;
-#pragma unroll
-                    for (int b = 0; b < RB; b++) {
-                        h8 seen;
-#pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            const int j = t0 + 16 * (e >> 2) + 4 * G + (e & 3);
-                            seen[e] = j > prow[b] || (a.window && j <= prow[b] - a.window)
-                                          ? (_Float16)0.0f : (_Float16)1.0f;
-                        }
-                        const f32x4 z = {0, 0, 0, 0};
-                        const f32x4 up = __builtin_amdgcn_mfma_f32_16x16x32_f16(pos, seen, z, 0, 0, 0);
-                        const f32x4 dn = __builtin_amdgcn_mfma_f32_16x16x32_f16(neg, seen, z, 0, 0, 0);
-#pragma unroll
-                        for (int r = 0; r < 4; r++) {
-                            if (up[r] > 0.0f) o[b][d][r] += kInf;
-                            if (dn[r] > 0.0f) o[b][d][r] -= kInf;
-                        }
-                    }
-                }
+                const h8 v = read_tr(v_at(t, ch) + (dd & 7), v_at(t + 16, ch) + (dd & 7));
 #pragma unroll
                 for (int b = 0; b < RB; b++)
                     o[b][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[b], o[b][d], 0, 0, 0);
             }
+            if (odd)
+#pragma unroll 1
+                for (int t = 0; t < 32; t++) {
+                    const int pg = t < 16 ? held[0] : held[1], j = t0 + t;
+                    if (pg < 0) continue;
+                    const int64_t row = (((int64_t)pg * a.Hk + h) << a.plog) + (j & ((1 << a.plog) - 1));
+                    const uint16_t* vp = static_cast<const uint16_t*>(a.vc) + row * a.D + 4 * G;
+#pragma unroll
+                    for (int d = 0; d < DB; d++) {
+                        if (16 * d >= a.D) continue;
+                        const uint2 w = *reinterpret_cast<const uint2*>(vp + 16 * d);
+#pragma unroll
+                        for (int b = 0; b < RB; b++) {
+                            if (j > prow[b] || (a.window && j <= prow[b] - a.window)) continue;
+#pragma unroll
+                            for (int r = 0; r < 4; r++)
+                                o[b][d][r] += odd_part(r < 2 ? w.x : w.y, r & 1);
+                        }
+                    }
+                }
         }
 
         // join the four waves: o rows in LDS (16-byte pieces permuted against bank conflicts)
@@ -681,6 +689,34 @@ __device__ __forceinline__ void copy16(uint32_t lds, const void* src) {
                  :: "s"(lds), "v"(src) : "memory", "m0");
 }
 
+// A wave-uniform address in scalar registers, wherever it was computed.
+__device__ __forceinline__ const void* scalar(const void* p) {
+    const uint64_t u = (uint64_t)(uintptr_t)p;
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)u);
+    const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(u >> 32));
+    return reinterpret_cast<const void*>((uintptr_t)((uint64_t)hi << 32 | lo));
+}
+
+// The same with a wave-uniform base and a byte offset a lane.
+__device__ __forceinline__ void copy16_s(uint32_t lds, const void* base, uint32_t voff) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :: "s"(lds), "v"(voff), "s"(base) : "memory", "m0");
+}
+
+// 16 bytes of LDS at a byte offset, and a value fragment: 4 keys at `off`, 4 eight rows on
+typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+typedef __attribute__((address_space(3))) tr4 lds_tr4;
+__device__ __forceinline__ h8 lds_read16(uint32_t off) {
+    return __builtin_bit_cast(h8, *reinterpret_cast<lds_u32x4*>(off));
+}
+__device__ __forceinline__ h8 lds_read_tr(uint32_t off, uint32_t off2) {
+    const tr4 a = __builtin_amdgcn_ds_read_tr16_b64_v4f16(reinterpret_cast<lds_tr4*>(off));
+    const tr4 b = __builtin_amdgcn_ds_read_tr16_b64_v4f16(reinterpret_cast<lds_tr4*>(off2));
+    const uint2 x = __builtin_bit_cast(uint2, a), y = __builtin_bit_cast(uint2, b);
+    const u32x4 v = {x.x, x.y, y.x, y.y};
+    return __builtin_bit_cast(h8, v);
+}
+
 __device__ const uint4 kZeros = {0, 0, 0, 0};
 __device__ const uint4 kNaNs = {0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u};
 
@@ -777,6 +813,32 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
     auto k_swz = [](int t) { return DP == 64 ? (t >> 1) & 7 : t & 15; };
     auto v_swz = [](int t) { return DP == 64 ? ((t >> 1) & 1) << 2 : (t & 3) << 2; };
 
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)smem;
+    // The permutations split into a part of the lane and one of the fragment, so a fragment's
+    // address is one of a few registers and a constant.
+    constexpr int KA = KS < 8 ? KS : 8, VA = DB < 4 ? DB : 4;
+    uint32_t k_addr[KA], v_addr[VA];
+#pragma unroll
+    for (int i = 0; i < KA; i++) k_addr[i] = lds0 + col * DP * 2 + 16 * ((2 * i + H) ^ k_swz(col));
+#pragma unroll
+    for (int d = 0; d < VA; d++) {
+        const int tk = 4 * H + ((lane & 15) >> 2);
+        const int dd = 32 * d + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+        v_addr[d] = lds0 + TB + tk * DP * 2 + 16 * ((dd >> 3) ^ v_swz(tk)) + 2 * (dd & 7);
+    }
+    // byte offsets of the wave's copies from its first row's
+    uint32_t k_off[I8 ? 1 : NL], v_off = 0;
+    if constexpr (!I8) {
+#pragma unroll
+        for (int j = 0; j < NL; j++) {
+            const int c = j * 64 + lane, k = c / CH, in = c % CH;
+            k_off[j] = (k * DP + 8 * (in ^ k_swz(16 * wave + k))) * 2;
+        }
+        v_off = (lane / CH * DP + 8 * (lane % CH ^ v_swz(lane / CH))) * 2;
+    }
+    // copy j takes the next 1024 bytes; rows of 512 bytes change the permutation with it
+    auto v_off_of = [&](int j) { return (DP == 256 && (j & 1) ? v_off ^ 128 : v_off) + j * 1024; };
+
     int pages = 0;  // lane j: the wave's 16 keys of tile (kt & ~63) + j, counted from `first`
     u32x4 kr[I8 ? NL : 1], vr[I8 ? NL : 1];
     float ksr = 0.0f, vsr = 1.0f;
@@ -807,8 +869,16 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
                 vsr = a.vs[row + (lane & 15)];
             }
         } else {
-            const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)smem;
-            const uint32_t kd = base + buf * 2 * TB + 16 * wave * DP * 2;
+            const uint32_t kd = lds0 + buf * 2 * TB + 16 * wave * DP * 2;
+            if (page >= 0 && a.D == DP && tok >= t.lo && tok + 16 <= t.hi) {
+                const void* kp = scalar(static_cast<const uint16_t*>(a.kc) + row * DP);
+                const void* vp = scalar(static_cast<const uint16_t*>(a.vc) + row * DP);
+#pragma unroll
+                for (int j = 0; j < NL; j++) copy16_s(kd + j * 1024, kp, k_off[j]);
+#pragma unroll
+                for (int j = 0; j < NL; j++) copy16_s(kd + TB + j * 1024, vp, v_off_of(j));
+                return;
+            }
 #pragma unroll
             for (int j = 0; j < NL; j++) {
                 const int c = j * 64 + lane, k = c / CH, in = c % CH;
@@ -861,22 +931,18 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
     auto compute = [&](int kt, int buf) {
         const int t0 = kt * kTileKeys;
         if (t0 > pmax || (a.window && t0 + kTileKeys - 1 <= pmin - a.window)) return;
-        const char* kb = smem + buf * 2 * TB;
-        const char* vb = kb + TB;
+        const uint32_t at_buf = buf * 2 * TB;
         const float* sc = scales + buf * 3 * kTileKeys;
         f32x16 s[2];
 #pragma unroll
         for (int tb = 0; tb < 2; tb++) {
 #pragma unroll
             for (int e = 0; e < 16; e++) s[tb][e] = 0.0f;
-            const int k = 32 * tb + col;
 #pragma unroll
-            for (int i = 0; i < KS; i++) {
-                const u32x4 v = *reinterpret_cast<const u32x4*>(kb + k * DP * 2 +
-                                                                16 * ((2 * i + H) ^ k_swz(k)));
-                s[tb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, v), q[i],
-                                                               s[tb], 0, 0, 0);
-            }
+            for (int i = 0; i < KS; i++)
+                s[tb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                    lds_read16(k_addr[i % KA] + at_buf + 32 * tb * DP * 2 + i / KA * 256), q[i],
+                    s[tb], 0, 0, 0);
         }
         // element e of block tb is key 32 tb + 8 (e / 4) + 4 H + e % 4
 #pragma unroll
@@ -909,15 +975,17 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
         for (int tb = 0; tb < 2; tb++)
 #pragma unroll
             for (int e = 0; e < 16; e++) top = __builtin_fmaxf(top, s[tb][e]);
-        top = __builtin_fmaxf(max_xor32(top), m);
-        const float at = top == -kInf ? 0.0f : top;
-        if (__any(top != m)) {
-            const float keep = exp2_(m - at);
+        top = max_xor32(top);
+        // m need not be the maximum: it may lag by kLag, weights are at most 2^kLag then
+        if (__any(top > m + kLag)) {
+            top = __builtin_fmaxf(top, m);
+            const float keep = exp2_(m - (top == -kInf ? 0.0f : top));
             l *= keep;
 #pragma unroll
             for (int d = 0; d < DB; d++) o[d] *= keep;
             m = top;
         }
+        const float at = m == -kInf ? 0.0f : m;
         h8 p[4];
 #pragma unroll
         for (int k = 0; k < 4; k++) {
@@ -943,56 +1011,56 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
         }
         // value fragment of 32 elements (block d) and keys 16 k + {4 H .., 8 + 4 H ..}
         auto value = [&](int d, int k) {
-            const int tk = 16 * k + 4 * H + ((lane & 15) >> 2);
-            const int dd = 32 * d + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-            const char* p1 = vb + tk * DP * 2 + 16 * ((dd >> 3) ^ v_swz(tk)) + 2 * (dd & 7);
-            const char* p2 = vb + (tk + 8) * DP * 2 + 16 * ((dd >> 3) ^ v_swz(tk + 8)) + 2 * (dd & 7);
-            return read_tr(reinterpret_cast<const uint16_t*>(p1), reinterpret_cast<const uint16_t*>(p2));
+            const uint32_t at = v_addr[d % VA] + at_buf + 16 * k * DP * 2 + d / VA * 256;
+            return lds_read_tr(at, at + 8 * DP * 2);
         };
-        bool split_v = false;
-        if (!I8 && edge) {
-            uint32_t odd = 0;
-#pragma unroll
-            for (int d = 0; d < DB; d++)
-#pragma unroll
-                for (int k = 0; k < 4; k++) odd |= odd_bits(__builtin_bit_cast(u32x4, value(d, k)));
-            split_v = __any(odd != 0);
-        }
-        if (split_v) {  // values that are not finite under a mask: see split_odd
-#pragma unroll 1
-            for (int k = 0; k < 4; k++) {
-                h8 seen;
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const int j = t0 + 16 * k + 8 * (e >> 2) + 4 * H + (e & 3);
-                    seen[e] = j > prow || (a.window && j <= prow - a.window) ? (_Float16)0.0f
-                                                                             : (_Float16)1.0f;
-                }
-#pragma unroll
-                for (int d = 0; d < DB; d++) {
-                    h8 fin, pos, neg;
-                    split_odd(value(d, k), fin, pos, neg);
-                    f32x16 z;
-#pragma unroll
-                    for (int e = 0; e < 16; e++) z[e] = 0.0f;
-                    const f32x16 up = __builtin_amdgcn_mfma_f32_32x32x16_f16(pos, seen, z, 0, 0, 0);
-                    const f32x16 dn = __builtin_amdgcn_mfma_f32_32x32x16_f16(neg, seen, z, 0, 0, 0);
-                    const h8 pk = k == 0 ? p[0] : k == 1 ? p[1] : k == 2 ? p[2] : p[3];
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fin, pk, o[d], 0, 0, 0);
-#pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        if (up[e] > 0.0f) o[d][e] += kInf;
-                        if (dn[e] > 0.0f) o[d][e] -= kInf;
-                    }
-                }
-            }
-            return;
-        }
 #pragma unroll
         for (int k = 0; k < 4; k++)
 #pragma unroll
             for (int d = 0; d < DB; d++)
                 o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(value(d, k), p[k], o[d], 0, 0, 0);
+    };
+
+    // What lies at the edge of some row of the workgroup (the same for its four waves).
+    const int wg_pmin = p0 + t.tile * kTileRows / a.group, wg_pmax = t.hi - 1;
+    // Makes the wave's 16 keys of a V tile finite; whether it changed any.
+    auto clean = [&](int buf) {
+        u32x4 v[DP / 32];
+        uint32_t bits = 0;
+        const uint32_t at = lds0 + buf * 2 * TB + TB + 16 * wave * DP * 2 + lane * 16;
+#pragma unroll
+        for (int j = 0; j < DP / 32; j++) {
+            v[j] = __builtin_bit_cast(u32x4, lds_read16(at + j * 1024));
+            bits |= odd_bits(v[j]);
+        }
+        if (!__any(bits != 0)) return 0;
+#pragma unroll
+        for (int j = 0; j < DP / 32; j++)
+            *reinterpret_cast<lds_u32x4*>(at + j * 1024) = finite_part(v[j]);
+        return 1;
+    };
+    auto restore = [&](int kt) {
+#pragma unroll 1
+        for (int i = 0; i < kTileKeys; i++) {
+            const int j = kt * kTileKeys + i;
+            if (j > pmax || j < t.lo) continue;
+            const int page = __builtin_amdgcn_readfirstlane(page_of(a, t.s, j & ~15, t.lo, t.hi));
+            if (page < 0) continue;
+            const int64_t row = (((int64_t)page * a.Hk + h) << a.plog) + (j & ((1 << a.plog) - 1));
+            const uint16_t* vp = static_cast<const uint16_t*>(a.vc) + row * a.D + 4 * H;
+            const bool sees = j <= prow && !(a.window && j <= prow - a.window);
+#pragma unroll
+            for (int d = 0; d < DB; d++)
+#pragma unroll
+                for (int e4 = 0; e4 < 4; e4++) {
+                    uint2 w = {0, 0};
+                    if (sees && 32 * d + 8 * e4 < a.D)
+                        w = *reinterpret_cast<const uint2*>(vp + 32 * d + 8 * e4);
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        o[d][4 * e4 + e] += odd_part(e < 2 ? w.x : w.y, e & 1);
+                }
+        }
     };
 
     if (first < last) {
@@ -1002,7 +1070,16 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
         for (int kt = first; kt < last; kt++) {
             const int buf = (kt - first) & 1;
             if (kt + 1 < last) begin(kt + 1, buf ^ 1);
+            bool odd = false;
+            if (!I8 && (kt * kTileKeys + kTileKeys - 1 > wg_pmin ||
+                        (a.window && kt * kTileKeys <= wg_pmax - a.window))) {
+                const int mine = clean(buf);
+                if (lane == 0) sh[wave] = mine;
+                __syncthreads();
+                odd = sh[0] | sh[1] | sh[2] | sh[3];
+            }
             compute(kt, buf);
+            if (!I8 && odd) restore(kt);
             if (kt + 1 < last) finish(buf ^ 1);
             __syncthreads();
         }
@@ -1091,8 +1168,9 @@ Plan plan_of(int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t B, int64_t mo
              int64_t max_context) {
     const int64_t group = Hq / Hk, rows = most * group, DP = padded_dim(D);
     Plan p{};
-    p.rb = rows <= 32 && rows > 16 ? 2 : 1;
-    p.use_tile = rows > 32;
+    // two blocks of 16 rows keep their sums in registers up to 128 elements
+    p.rb = DP <= 128 && rows <= 32 && rows > 16 ? 2 : 1;
+    p.use_tile = rows > 16 * p.rb;
     // one sequence of many rows: nothing is left for few_kernel but padding, which the
     // tiles take too
     p.use_few = !p.use_tile || B > 1;
@@ -1157,7 +1235,11 @@ int run_all(Attn a, const Plan& p, hipStream_t st) {
         a.whole = a.part == nullptr;
         const int64_t grid = a.whole ? (a.nseq + (p.use_tile ? 0 : (int64_t)a.T * a.group / (16 * p.rb))) * a.Hk
                                      : p.workers;
-        const int rc = p.rb == 1 ? run_few<DP, I8, 1>(a, grid, st) : run_few<DP, I8, 2>(a, grid, st);
+        int rc;
+        if constexpr (DP <= 128)
+            rc = p.rb == 1 ? run_few<DP, I8, 1>(a, grid, st) : run_few<DP, I8, 2>(a, grid, st);
+        else
+            rc = run_few<DP, I8, 1>(a, grid, st);
         if (rc) return rc;
     }
     if (p.use_tile) {
