@@ -44,6 +44,15 @@ constexpr int kUnit = 128;      // keys of a unit of few_kernel: 32 for each of 
 constexpr int kTileRows = 128;  // rows of a workgroup of tile_kernel
 constexpr int kTileKeys = 64;
 constexpr float kLag = 8.0f;
+constexpr int kWorkers = 768;  // of few_kernel at most: three a CU
+
+// What join_kernel does: part p of an item, o [rows][DP], m, l [rows], lies in slot `first`
+// (p = 0) or next + (p - 1) * step.
+struct Join {
+    int parts;  // 0: nothing to do
+    int first, next, step;
+    int start, row0, nrows, h;
+};
 
 struct Attn {
     const uint16_t* q;
@@ -53,13 +62,13 @@ struct Attn {
     const int32_t *tables, *lens, *cu;
     int64_t ldt;
     uint16_t* out;
+    Join* joins;
     float* part;
     int T, Hq, Hk, D, group, num_pages, plog, max_pages, B, nseq, window, cap;
     float c;       // scale * log2 e
     int few;       // few_kernel takes sequences of at most so many rows, tile_kernel others
     int whole;     // few_kernel: no parts, an item is one unit
     int splits;    // tile_kernel: parts of an item at most
-    int tiles;     // of tile_kernel, at most
 };
 
 struct Seq {
@@ -190,17 +199,20 @@ __device__ __forceinline__ void codes16(u32x4 w, u32x4& a, u32x4& b) {
 __device__ __forceinline__ void value_scale(float v, float& lv, float& rv) {
     v = v < 0x1p-64f ? 0x1p-64f : v;
     lv = __builtin_amdgcn_logf(v);
-    rv = 1.0f / v;
+    rv = __builtin_amdgcn_rcpf(v);
 }
 
-__device__ __forceinline__ h8 read_tr(const uint16_t* p, const uint16_t* p2) {
-    typedef __attribute__((address_space(3))) tr4 lds_tr4;
-    typedef __attribute__((address_space(3))) void lds_void;
-    const tr4 a = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr4*)(lds_void*)p);
-    const tr4 b = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr4*)(lds_void*)p2);
-    u32x4 v;
+// 16 bytes of LDS at a byte offset, and a value fragment: 4 keys at `off`, 4 at `off2`
+typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+typedef __attribute__((address_space(3))) tr4 lds_tr4;
+__device__ __forceinline__ h8 lds_read16(uint32_t off) {
+    return __builtin_bit_cast(h8, *reinterpret_cast<lds_u32x4*>(off));
+}
+__device__ __forceinline__ h8 lds_read_tr(uint32_t off, uint32_t off2) {
+    const tr4 a = __builtin_amdgcn_ds_read_tr16_b64_v4f16(reinterpret_cast<lds_tr4*>(off));
+    const tr4 b = __builtin_amdgcn_ds_read_tr16_b64_v4f16(reinterpret_cast<lds_tr4*>(off2));
     const uint2 x = __builtin_bit_cast(uint2, a), y = __builtin_bit_cast(uint2, b);
-    v = u32x4{x.x, x.y, y.x, y.y};
+    const u32x4 v = {x.x, x.y, y.x, y.y};
     return __builtin_bit_cast(h8, v);
 }
 
@@ -260,6 +272,11 @@ constexpr int few_part() {
     return 16 * RB * (DP + 2);
 }
 
+// Workgroups a CU, by the registers: codes of 8 bits take half as many on their way
+constexpr int few_waves(int dp, bool i8, int rb) {
+    return dp > 128 ? 1 : rb == 1 && (i8 || dp == 64) ? 3 : 2;
+}
+
 // What few_kernel makes of a sequence: its range of keys and its units.
 struct FewSeq {
     Seq q;
@@ -284,19 +301,23 @@ __device__ __forceinline__ int per_worker(int U) {
 }
 
 template <int DP, bool I8, int RB>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void few_kernel(Attn a) {
+__global__ __launch_bounds__(256, few_waves(DP, I8, RB)) void few_kernel(Attn a) {
     constexpr int KS = DP / 32, DB = DP / 16;
     constexpr int KL = I8 ? DP / 64 : DP / 32, VL = KL;  // loads of 16 keys
     constexpr int CH = DP / 8;                           // chunks of a row in LDS
+    constexpr int ES = I8 ? 1 : 2, RC = DP * ES / 16;    // 16-byte pieces of a cached row
+    constexpr bool AHEAD = false;
     extern __shared__ __align__(16) char smem[];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, G = lane >> 4;
+    const uint32_t k_off = col * a.D * ES + 16 * G;
     uint16_t* vt = reinterpret_cast<uint16_t*>(smem + wave * few_region<DP, RB>());
     float* ot = reinterpret_cast<float*>(vt);
     float* ml = reinterpret_cast<float*>(smem + 4 * few_region<DP, RB>());  // [4][2][16 RB]
     int* sh = reinterpret_cast<int*>(ml + 4 * 2 * 16 * RB);
 
+    if (!a.whole && threadIdx.x == 0) a.joins[blockIdx.x].parts = 0;
     int s, base, u;
     int upw = 0;
     if (!find(
@@ -357,11 +378,16 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void few_kernel(Attn a) {
             for (int d = 0; d < DB; d++) o[b][d] = f32x4{0, 0, 0, 0};
         }
 
-        u32x4 kr[2][KL], vr[2][VL];
-        f32x4 ksr[2], vsr[2];
+        struct Step {  // a wave's 32 keys on their way
+            u32x4 kr[2][KL], vr[2][VL];
+            f32x4 ksr[2], vsr[2];
+            int page[2];
+        };
         int pages = 0;  // lane j: block j & 1 of step (j >> 1) of the 32 ahead
-        int page[2];
-        auto load = [&](int i) {
+        auto load = [&](int i, Step& n) {
+            auto &kr = n.kr, &vr = n.vr;
+            auto &ksr = n.ksr, &vsr = n.vsr;
+            auto& page = n.page;
             if ((i & 31) == 0)
                 pages = i + (lane >> 1) < steps
                             ? page_of(a, s, t_first + (i + (lane >> 1)) * kUnit + 16 * (lane & 1),
@@ -377,46 +403,49 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void few_kernel(Attn a) {
                 if (page[tb] < 0) continue;
                 const int tok = t0 + 16 * tb, in = tok & ((1 << a.plog) - 1);
                 const int64_t row = (((int64_t)page[tb] * a.Hk + h) << a.plog) + in;
+                const char* kp = static_cast<const char*>(a.kc) + row * a.D * ES;
+                const char* vp = static_cast<const char*>(a.vc) + row * a.D * ES;
                 if constexpr (I8) {
-                    const int8_t* kp = static_cast<const int8_t*>(a.kc) + row * a.D;
-                    const int8_t* vp = static_cast<const int8_t*>(a.vc) + row * a.D;
-#pragma unroll
-                    for (int j = 0; j < KL; j++)
-                        if (64 * j + 16 * G < a.D)
-                            kr[tb][j] = *reinterpret_cast<const u32x4*>(kp + col * a.D + 64 * j + 16 * G);
-#pragma unroll
-                    for (int j = 0; j < VL; j++) {
-                        const int c = j * 64 + lane, t = c / (DP / 16), d = 16 * (c % (DP / 16));
-                        if (d < a.D) vr[tb][j] = *reinterpret_cast<const u32x4*>(vp + t * a.D + d);
-                    }
                     ksr[tb] = *reinterpret_cast<const f32x4*>(a.ks + row + 4 * G);
                     vsr[tb] = *reinterpret_cast<const f32x4*>(a.vs + row + 4 * G);
-                } else {
-                    const uint16_t* kp = static_cast<const uint16_t*>(a.kc) + row * a.D;
-                    const uint16_t* vp = static_cast<const uint16_t*>(a.vc) + row * a.D;
+                }
+                if (a.D == DP && (I8 || (tok >= lo && tok + 16 <= hi))) {
 #pragma unroll
                     for (int j = 0; j < KL; j++)
-                        if (32 * j + 8 * G < a.D)
-                            kr[tb][j] = *reinterpret_cast<const u32x4*>(kp + col * a.D + 32 * j + 8 * G);
+                        kr[tb][j] = *reinterpret_cast<const u32x4*>(kp + k_off + 64 * j);
+#pragma unroll
+                    for (int j = 0; j < VL; j++)
+                        vr[tb][j] = *reinterpret_cast<const u32x4*>(vp + 16 * lane + 1024 * j);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < KL; j++)
+                        if (64 * j + 16 * G < a.D * ES)
+                            kr[tb][j] = *reinterpret_cast<const u32x4*>(kp + k_off + 64 * j);
 #pragma unroll
                     for (int j = 0; j < VL; j++) {
-                        const int c = j * 64 + lane, t = c / CH, d = 8 * (c % CH);
+                        const int c = j * 64 + lane, t = c / RC, d = 16 * (c % RC);
                         // what lies outside the range may be anything, and 0 * NaN is NaN
-                        if (d < a.D && tok + t < hi && tok + t >= lo)
-                            vr[tb][j] = *reinterpret_cast<const u32x4*>(vp + t * a.D + d);
+                        if (d < a.D * ES && (I8 || (tok + t < hi && tok + t >= lo)))
+                            vr[tb][j] = *reinterpret_cast<const u32x4*>(
+                                vp + (uint32_t)(t * a.D * ES + d));
                     }
                 }
             }
         };
-        // 16-byte chunk `ch` of key t of the V tile: chunks are permuted by pairs so that
-        // the 8 keys of a half wave's transposing read lie on different banks
-        auto v_at = [&](int t, int ch) {
-            const int f8 = DP == 64 ? ((t >> 1) & 3) << 1 : (t & 7) << 1;
-            return vt + t * DP + 8 * (ch ^ f8);
-        };
-
-        load(0);
-        for (int i = 0; i < steps; i++) {
+        // The V tile: chunk ch of key t lies at chunk ch ^ f(t), f = 2 (t & 7), or
+        // 2 ((t >> 1) & 3) for rows of 128 bytes: the 8 keys of a half wave's transposing
+        // read lie on different banks.  Seen from a lane the permutation is an exclusive or
+        // with constants on its first address.
+        const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)vt;
+        auto f_of = [](int t) { return DP == 64 ? ((t >> 1) & 3) << 1 : (t & 7) << 1; };
+        const int wt = I8 ? lane / (DP / 16) : lane / CH, wc = I8 ? 2 * (lane % (DP / 16)) : lane % CH;
+        const uint32_t w_addr = lds0 + wt * DP * 2 + 16 * (wc ^ f_of(wt));
+        const int rt = 4 * G + (col >> 2);
+        const uint32_t r_addr = lds0 + rt * DP * 2 + 16 * (((col & 3) >> 1) ^ f_of(rt)) + 8 * (col & 1);
+        auto step = [&](int i, Step& n) {
+            auto &kr = n.kr, &vr = n.vr;
+            auto &ksr = n.ksr, &vsr = n.vsr;
+            auto& page = n.page;
             const int t0 = t_first + i * kUnit;
             const bool bad[2] = {page[0] == kBad, page[1] == kBad};
             const bool none = page[0] == kNone && page[1] == kNone;
@@ -437,20 +466,22 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void few_kernel(Attn a) {
 #pragma unroll
                             for (int j = 0; j < VL; j++) vr[tb][j] = finite_part(vr[tb][j]);
                 }
+            uint32_t wa = w_addr, ra = r_addr;
+            asm volatile("" : "+v"(wa), "+v"(ra));  // computed here, not kept in registers
 #pragma unroll
             for (int tb = 0; tb < 2; tb++)
 #pragma unroll
                 for (int j = 0; j < VL; j++) {
-                    const int c = j * 64 + lane;
+                    constexpr int rows = I8 ? 64 / (DP / 16) : 64 / CH;  // of one load
+                    const int t = 16 * tb + j * rows;
+                    const uint32_t at = (wa ^ (16 * f_of(t))) + t * DP * 2;
                     if constexpr (I8) {
                         u32x4 x, y;
                         codes16(vr[tb][j], x, y);
-                        const int t = 16 * tb + c / (DP / 16), ch = 2 * (c % (DP / 16));
-                        *reinterpret_cast<u32x4*>(v_at(t, ch)) = x;
-                        *reinterpret_cast<u32x4*>(v_at(t, ch + 1)) = y;
+                        *reinterpret_cast<lds_u32x4*>(at) = x;
+                        *reinterpret_cast<lds_u32x4*>(at ^ 16) = y;
                     } else {
-                        const int t = 16 * tb + c / CH, ch = c % CH;
-                        *reinterpret_cast<u32x4*>(v_at(t, ch)) = vr[tb][j];
+                        *reinterpret_cast<lds_u32x4*>(at) = vr[tb][j];
                     }
                 }
             f32x4 sc[RB][2];
@@ -489,8 +520,9 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void few_kernel(Attn a) {
                         rv[tb][r] = y;
                         kx[tb][r] = ksr[tb][r] * a.c;
                     }
-            if (i + 1 < steps) load(i + 1);
-            if (none) continue;
+            if constexpr (!AHEAD)
+                if (i + 1 < steps) load(i + 1, n);  // its registers are free from here on
+            if (none) return;
 
             h8 p[RB];
 #pragma unroll
@@ -515,15 +547,16 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void few_kernel(Attn a) {
 #pragma unroll
                 for (int e = 1; e < 8; e++) top = __builtin_fmaxf(top, x[e]);
                 top = max_xor32(max_xor16(top));
-                top = __builtin_fmaxf(top, m[b]);
-                const float at = top == -kInf ? 0.0f : top;
-                if (__any(top != m[b])) {
-                    const float keep = exp2_(m[b] - at);
+                // m may lag behind the maximum by kLag: weights are at most 2^kLag
+                if (__any(top > m[b] + kLag)) {
+                    top = __builtin_fmaxf(top, m[b]);
+                    const float keep = exp2_(m[b] - (top == -kInf ? 0.0f : top));
                     l[b] *= keep;
 #pragma unroll
                     for (int d = 0; d < DB; d++) o[b][d] *= keep;
                     m[b] = top;
                 }
+                const float at = m[b] == -kInf ? 0.0f : m[b];
                 float w[8];
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
@@ -537,11 +570,10 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void few_kernel(Attn a) {
                                   pack2(w[6], w[7])};
                 p[b] = __builtin_bit_cast(h8, pk);
             }
-            const int tr = col >> 2, dd = 4 * (col & 3);
 #pragma unroll
             for (int d = 0; d < DB; d++) {
-                const int t = 4 * G + tr, ch = 2 * d + (dd >> 3);
-                const h8 v = read_tr(v_at(t, ch) + (dd & 7), v_at(t + 16, ch) + (dd & 7));
+                const uint32_t at = (ra ^ (d % 8 * 32)) + d / 8 * 256;
+                const h8 v = lds_read_tr(at, at + 16 * DP * 2);
 #pragma unroll
                 for (int b = 0; b < RB; b++)
                     o[b][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[b], o[b][d], 0, 0, 0);
@@ -566,6 +598,21 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void few_kernel(Attn a) {
                         }
                     }
                 }
+        };
+        if constexpr (AHEAD) {  // one step is on its way while another is computed
+            Step sa, sb;
+            load(0, sa);
+            for (int i = 0; i < steps; i += 2) {
+                if (i + 1 < steps) load(i + 1, sb);
+                step(i, sa);
+                if (i + 1 >= steps) break;
+                if (i + 2 < steps) load(i + 2, sa);
+                step(i + 1, sb);
+            }
+        } else {
+            Step sa;
+            load(0, sa);
+            for (int i = 0; i < steps; i++) step(i, sa);
         }
 
         // join the four waves: o rows in LDS (16-byte pieces permuted against bank conflicts)
@@ -619,6 +666,11 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void few_kernel(Attn a) {
                 }
             }
         }
+        if (!full && tile == 0 && threadIdx.x == 0) {  // this run begins an item, others end it
+            const int w0 = blockIdx.x, w1 = (u + per_item - 1) / upw;
+            a.joins[w0] = Join{w1 - w0 + 1, 2 * w0 + (first_unit == u ? 0 : 1), 2 * w0 + 2, 2,
+                               f.q.start, row0, nrows, h};
+        }
         left -= nt;
         u += nt;
         if (left <= 0) return;
@@ -635,50 +687,64 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void few_kernel(Attn a) {
     }
 }
 
-// Joins the parts of the item that run `blockIdx.x` began and did not finish.
-template <int DP, int RB>
-__global__ __launch_bounds__(256) void few_join(Attn a) {
-    __shared__ int sh[8];
-    int s, base, u, upw = 0;
-    if (!find(
-            a.nseq, sh, [&](int i) { return few_seq<RB>(a, i).units; },
-            [&](int U) {
-                upw = per_worker(U);
-                const int end = upw * ((int)blockIdx.x + 1);
-                return end < U ? end - 1 : -1;  // the last run ends its item
-            },
-            s, base, u))
-        return;
-    const FewSeq f = few_seq<RB>(a, s);
-    const int item = (u - base) / f.tiles, begin = base + item * f.tiles, end = begin + f.tiles;
-    const int w0 = blockIdx.x;
-    if (end <= u + 1 || begin < w0 * upw) return;  // finished, or another run began it
-    const int w1 = (end - 1) / upw;
-    const int h = item % a.Hk, row0 = item / a.Hk * 16 * RB;
-    const int nrows = f.rows - row0 < 16 * RB ? f.rows - row0 : 16 * RB;
-    const int D4 = a.D >> 2;
-    auto slot = [&](int w) {
-        return a.part + (int64_t)(2 * w + (w == w0 && begin != w0 * upw ? 1 : 0)) * few_part<DP, RB>();
+// Joins an item's parts, a wave a row: 64 parts' weights at a time, one a lane, then the
+// parts of o, DP / 4 lanes each, several in flight.
+template <int DP>
+__global__ __launch_bounds__(256) void join_kernel(Attn a, int part_rows) {
+    constexpr int LP = DP / 4, NG = 64 / LP;  // lanes of a part, parts at a time
+    const Join j = a.joins[blockIdx.x];
+    const int lane = threadIdx.x & 63, r = blockIdx.y * 4 + (threadIdx.x >> 6);
+    if (r >= j.nrows || j.parts == 0) return;
+    const int64_t size = (int64_t)part_rows * (DP + 2);
+    const int d4 = lane % LP, grp = lane / LP;
+    auto slot = [&](int p) {
+        return a.part + size * (p == 0 ? j.first : j.next + (p - 1) * j.step);
     };
-    for (int e = threadIdx.x; e < nrows * D4; e += 256) {
-        const int r = e / D4, d4 = e - r * D4;
-        float top = -kInf;
-        for (int w = w0; w <= w1; w++) top = __builtin_fmaxf(top, slot(w)[16 * RB * DP + r]);
-        const float at = top == -kInf ? 0.0f : top;
-        float sum = 0.0f;
-        f32x4 acc = {0, 0, 0, 0};
-        for (int w = w0; w <= w1; w++) {
-            const float* p = slot(w);
-            const float k = exp2_(p[16 * RB * DP + r] - at);
-            sum += k * p[16 * RB * DP + 16 * RB + r];
-            acc += k * *reinterpret_cast<const f32x4*>(p + r * DP + 4 * d4);
+    float top = -kInf, sum = 0.0f;
+    f32x4 acc = {0, 0, 0, 0};
+    for (int c = 0; c < j.parts; c += 64) {
+        const int n = j.parts - c < 64 ? j.parts - c : 64;
+        float m = -kInf, l = 0.0f;
+        if (lane < n) {
+            const float* p = slot(c + lane) + part_rows * DP;
+            m = p[r];
+            l = p[part_rows + r];
         }
-        const float inv = 1.0f / sum;
-        const int rr = row0 + r, i = rr / a.group, head = h * a.group + rr - i * a.group;
-        uint2 y = {pack2(acc[0] * inv, acc[1] * inv), pack2(acc[2] * inv, acc[3] * inv)};
-        if (sum == 0.0f) y = uint2{0, 0};
-        *reinterpret_cast<uint2*>(a.out + ((int64_t)(f.q.start + i) * a.Hq + head) * a.D + 4 * d4) = y;
+        float t = __builtin_fmaxf(top, m);
+        t = max_xor32(max_xor16(t));
+#pragma unroll
+        for (int x = 8; x > 0; x >>= 1) t = __builtin_fmaxf(t, __shfl_xor(t, x, 64));
+        const float at = t == -kInf ? 0.0f : t;
+        const float keep = exp2_(top - at), w = exp2_(m - at);
+        acc *= keep;
+        float wl = w * l;
+#pragma unroll
+        for (int x = 32; x > 0; x >>= 1) wl += __shfl_xor(wl, x, 64);
+        sum = sum * keep + wl;
+        top = t;
+        constexpr int U = 8;
+        for (int i = 0; i < n; i += U * NG) {
+            f32x4 v[U];
+#pragma unroll
+            for (int k = 0; k < U; k++) {
+                const int p = i + k * NG + grp;
+                v[k] = f32x4{0, 0, 0, 0};
+                if (p < n) v[k] = *reinterpret_cast<const f32x4*>(slot(c + p) + r * DP + 4 * d4);
+            }
+#pragma unroll
+            for (int k = 0; k < U; k++) acc += __shfl(w, (i + k * NG + grp) & 63, 64) * v[k];
+        }
     }
+#pragma unroll
+    for (int x = 32; x >= LP; x >>= 1)
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[e] += __shfl_xor(acc[e], x, 64);
+    if (grp != 0 || 4 * d4 >= a.D) return;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const int rr = j.row0 + r, i = rr / a.group, head = j.h * a.group + rr - i * a.group;
+    uint2 y = {pack2(acc[0] * inv, acc[1] * inv), pack2(acc[2] * inv, acc[3] * inv)};
+    if (sum == 0.0f) y = uint2{0, 0};
+    *reinterpret_cast<uint2*>(a.out + ((int64_t)(j.start + i) * a.Hq + head) * a.D + 4 * d4) = y;
 }
 
 // ---- tiles of 128 rows -------------------------------------------------------------
@@ -703,20 +769,6 @@ __device__ __forceinline__ void copy16_s(uint32_t lds, const void* base, uint32_
                  :: "s"(lds), "v"(voff), "s"(base) : "memory", "m0");
 }
 
-// 16 bytes of LDS at a byte offset, and a value fragment: 4 keys at `off`, 4 eight rows on
-typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
-typedef __attribute__((address_space(3))) tr4 lds_tr4;
-__device__ __forceinline__ h8 lds_read16(uint32_t off) {
-    return __builtin_bit_cast(h8, *reinterpret_cast<lds_u32x4*>(off));
-}
-__device__ __forceinline__ h8 lds_read_tr(uint32_t off, uint32_t off2) {
-    const tr4 a = __builtin_amdgcn_ds_read_tr16_b64_v4f16(reinterpret_cast<lds_tr4*>(off));
-    const tr4 b = __builtin_amdgcn_ds_read_tr16_b64_v4f16(reinterpret_cast<lds_tr4*>(off2));
-    const uint2 x = __builtin_bit_cast(uint2, a), y = __builtin_bit_cast(uint2, b);
-    const u32x4 v = {x.x, x.y, y.x, y.y};
-    return __builtin_bit_cast(h8, v);
-}
-
 __device__ const uint4 kZeros = {0, 0, 0, 0};
 __device__ const uint4 kNaNs = {0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u};
 
@@ -725,11 +777,10 @@ constexpr int tile_lds() {
     return 2 * 2 * kTileKeys * DP * 2 + (I8 ? 2 * 3 * kTileKeys * 4 : 0) + 32;
 }
 
-// The item of a workgroup of tile_kernel and tile_join.
+// The item of a workgroup of tile_kernel.
 struct TileItem {
     Seq q;
     int s, rows, tile, h, lo, hi, kt0, kt1, per, parts;
-    int index;  // of the parts
 };
 
 // Tiles of all sequences from the last to the first: a causal tile's keys grow with its
@@ -741,8 +792,7 @@ __device__ __forceinline__ bool tile_item(const Attn& a, int id, int h, int* sh,
                    ? (int)(((int64_t)q.n * a.group + kTileRows - 1) / kTileRows) : 0;
     };
     int base, goal;
-    if (!find(a.nseq, sh, tiles, [&](int N) { return N - 1 - id; }, t.s, base, goal) ||
-        goal >= a.tiles)
+    if (!find(a.nseq, sh, tiles, [&](int N) { return N - 1 - id; }, t.s, base, goal))
         return false;
     t.q = sequence(a, t.s);
     t.rows = t.q.n * a.group;
@@ -760,7 +810,6 @@ __device__ __forceinline__ bool tile_item(const Attn& a, int id, int h, int* sh,
     // a part has four tiles of keys at least
     t.parts = n / 4 < a.splits ? (n / 4 > 1 ? n / 4 : 1) : a.splits;
     t.per = (n + t.parts - 1) / t.parts;
-    t.index = goal * a.Hk + h;
     return true;
 }
 
@@ -785,8 +834,18 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
     // over the 8 XCDs they share an L2 where the heads divide 8
     const int h = blockIdx.x % a.Hk, rest = blockIdx.x / a.Hk;
     const int split = rest % a.splits;
-    TileItem t;
-    if (!tile_item(a, rest / a.splits, h, sh, t) || split >= t.parts) return;
+    TileItem t{};
+    const bool found = tile_item(a, rest / a.splits, h, sh, t);
+    const int index = rest / a.splits * a.Hk + h;
+    if (a.splits > 1 && split == 0 && threadIdx.x == 0) {
+        const int tile_row0 = t.tile * kTileRows;
+        Join j{0, 0, 0, 0, 0, 0, 0, 0};
+        if (found && t.parts > 1)
+            j = Join{t.parts, index * a.splits, index * a.splits + 1, 1, t.q.start, tile_row0,
+                     t.rows - tile_row0 < kTileRows ? t.rows - tile_row0 : kTileRows, h};
+        a.joins[index] = j;
+    }
+    if (!found || split >= t.parts) return;
     const int first = t.kt0 + split * t.per;
     const int last = first + t.per < t.kt1 ? first + t.per : t.kt1;
 
@@ -1088,7 +1147,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
     l += __shfl_xor(l, 32, 64);
     if (r >= t.rows) return;
     if (t.parts > 1) {
-        float* part = a.part + ((int64_t)t.index * a.splits + split) * tile_part<DP>();
+        float* part = a.part + ((int64_t)index * a.splits + split) * tile_part<DP>();
         const int pr = wave * 32 + col;
 #pragma unroll
         for (int d = 0; d < DB; d++)
@@ -1117,38 +1176,6 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
         }
 }
 
-// Joins the parts of an item of tile_kernel, 32 rows a workgroup.
-template <int DP>
-__global__ __launch_bounds__(256) void tile_join(Attn a) {
-    __shared__ int sh[8];
-    const int quarter = blockIdx.x & 3, id = blockIdx.x >> 2;
-    TileItem t;
-    if (!tile_item(a, id / a.Hk, id % a.Hk, sh, t) || t.parts <= 1) return;
-    const float* parts = a.part + (int64_t)t.index * a.splits * tile_part<DP>();
-    const int D4 = a.D >> 2;
-    for (int e = threadIdx.x; e < 32 * D4; e += 256) {
-        const int pr = quarter * 32 + e / D4, d4 = e % D4, r = t.tile * kTileRows + pr;
-        if (r >= t.rows) return;
-        float top = -kInf;
-        for (int w = 0; w < t.parts; w++)
-            top = __builtin_fmaxf(top, parts[w * tile_part<DP>() + kTileRows * DP + pr]);
-        const float at = top == -kInf ? 0.0f : top;
-        float sum = 0.0f;
-        f32x4 acc = {0, 0, 0, 0};
-        for (int w = 0; w < t.parts; w++) {
-            const float* p = parts + w * tile_part<DP>();
-            const float k = exp2_(p[kTileRows * DP + pr] - at);
-            sum += k * p[kTileRows * DP + kTileRows + pr];
-            acc += k * *reinterpret_cast<const f32x4*>(p + pr * DP + 4 * d4);
-        }
-        const float inv = 1.0f / sum;
-        const int i = r / a.group, head = t.h * a.group + r - i * a.group;
-        uint2 y = {pack2(acc[0] * inv, acc[1] * inv), pack2(acc[2] * inv, acc[3] * inv)};
-        if (sum == 0.0f) y = uint2{0, 0};
-        *reinterpret_cast<uint2*>(a.out + ((int64_t)(t.q.start + i) * a.Hq + head) * a.D + 4 * d4) = y;
-    }
-}
-
 // ---- host --------------------------------------------------------------------------
 
 // How a call is cut up, from what the host knows.
@@ -1159,8 +1186,10 @@ struct Plan {
     int64_t workers;      // of few_kernel
     int64_t tiles;        // of 128 rows, at most
     int splits;
-    int64_t bytes;
+    int64_t joins, bytes;  // of the workspace: Join records, and the records and parts
 };
+
+int64_t join_bytes(int64_t n) { return (n * (int64_t)sizeof(Join) + 255) & ~(int64_t)255; }
 
 int padded_dim(int64_t D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
@@ -1177,16 +1206,21 @@ Plan plan_of(int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t B, int64_t mo
     p.few = !p.use_tile ? 1 << 30 : p.use_few ? 16 * p.rb : 0;
     const int64_t units = (max_context + 1 + kUnit - 1) / kUnit;
     p.workers = (B + 1 + T * group / (16 * p.rb)) * Hk * units;
-    p.workers = p.workers < 512 ? p.workers : 512;
+    p.workers = p.workers < kWorkers ? p.workers : kWorkers;
     p.tiles = T * group / kTileRows + B + 1;
     const int64_t items = p.tiles * Hk;
     p.splits = items >= 384 ? 1 : (int)(512 / items);
     if (p.splits > 16) p.splits = 16;
-    if (p.use_few) p.bytes += p.workers * 2 * 16 * p.rb * (DP + 2) * 4;
+    if (p.use_few) {
+        p.joins = p.workers;
+        p.bytes = p.workers * 2 * 16 * p.rb * (DP + 2) * 4;
+    }
     if (p.use_tile && p.splits > 1) {
         const int64_t b = items * p.splits * kTileRows * (DP + 2) * 4;
+        p.joins = p.joins > items ? p.joins : items;
         p.bytes = p.bytes > b ? p.bytes : b;
     }
+    p.bytes += join_bytes(p.joins);
     return p;
 }
 
@@ -1209,11 +1243,13 @@ int allow_lds(K kernel, int bytes) {
 template <int DP, bool I8, int RB>
 int run_few(const Attn& a, int64_t workers, hipStream_t st) {
     const auto kern = few_kernel<DP, I8, RB>;
+    if (!a.whole && workers > 256 * few_waves(DP, I8, RB)) workers = 256 * few_waves(DP, I8, RB);
     constexpr int lds = few_lds<DP, RB>();
     const int rc = allow_lds(kern, lds);
     if (rc) return rc;
     kern<<<dim3((uint32_t)workers), 256, lds, st>>>(a);
-    if (!a.whole && workers > 1) few_join<DP, RB><<<dim3((uint32_t)workers), 256, 0, st>>>(a);
+    if (!a.whole && workers > 1)
+        join_kernel<DP><<<dim3((uint32_t)workers, 4 * RB), 256, 0, st>>>(a, 16 * RB);
     return FNI8_OK;
 }
 
@@ -1224,7 +1260,8 @@ int run_tile(const Attn& a, int64_t tiles, hipStream_t st) {
     const int rc = allow_lds(kern, lds);
     if (rc) return rc;
     kern<<<dim3((uint32_t)(tiles * a.Hk * a.splits)), 256, lds, st>>>(a);
-    if (a.splits > 1) tile_join<DP><<<dim3((uint32_t)(tiles * a.Hk * 4)), 256, 0, st>>>(a);
+    if (a.splits > 1)
+        join_kernel<DP><<<dim3((uint32_t)(tiles * a.Hk), kTileRows / 4), 256, 0, st>>>(a, kTileRows);
     return FNI8_OK;
 }
 
@@ -1288,8 +1325,10 @@ int launch_paged_attention(const PagedAttention& p, hipStream_t st) {
     a.c = p.scale * 1.44269504088896340736f;
     a.few = plan.few;
     a.splits = 1;
-    a.tiles = (int)plan.tiles;
-    if (plan.bytes && p.work_bytes >= plan.bytes) a.part = reinterpret_cast<float*>(p.work);
+    if (plan.bytes && p.work_bytes >= plan.bytes) {
+        a.joins = reinterpret_cast<Join*>(p.work);
+        a.part = reinterpret_cast<float*>(p.work + join_bytes(plan.joins));
+    }
     int rc;
     switch (padded_dim(p.D)) {
         case 64: rc = p.k_scale ? run_all<64, true>(a, plan, st) : run_all<64, false>(a, plan, st); break;
