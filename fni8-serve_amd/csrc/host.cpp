@@ -22,6 +22,8 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 
+#include <cmath>
+
 #include "../../include/fni8amd.h"
 
 namespace {
@@ -466,10 +468,185 @@ PyObject* py_moe(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// Heads [T, H, D] fp16 as they lie: unit inner stride, 16-byte aligned rows.
+struct Heads {
+    const void* p;
+    int64_t T, H, D, lt, lh;
+};
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+Heads heads(const Tensor& x) {
+    need(x.scalar_type() == at::kHalf && x.dim() == 3 && x.numel() > 0 && x.stride(2) == 1);
+    Heads h{x.data_ptr(), x.size(0), x.size(1), x.size(2), 0, 0};
+    h.lt = h.T > 1 ? x.stride(0) : h.H * h.D;
+    h.lh = h.H > 1 ? x.stride(1) : h.D;
+    need(h.D % 8 == 0 && h.D <= 256 && h.lt >= h.D && h.lh >= h.D && h.lt % 8 == 0 &&
+         h.lh % 8 == 0 && aligned16(h.p));
+    return h;
+}
+
+const int32_t* index32(const Tensor& t, const Tensor& x, int64_t n) {
+    same(t, x, at::kInt);
+    need(t.dim() == 1 && t.numel() == n);
+    return static_cast<const int32_t*>(t.data_ptr());
+}
+
+// What the rows between QKV and attention share: weights, positions, table.
+struct RowArgs {
+    const void *qw = nullptr, *kw = nullptr;
+    const int32_t* pos = nullptr;
+    const float* table = nullptr;
+    int64_t P = 0, R = 0;
+    float eps = 0;
+    int pairs = 0, unit = 0;
+};
+RowArgs row_args(PyObject* const* a, const Tensor& q, int64_t T, int64_t D) {
+    RowArgs r;
+    for (int i = 0; i < 2; i++)
+        if (a[i] != Py_None) {
+            const Tensor& w = plain(a[i]);
+            same(w, q, at::kHalf);
+            need(w.numel() == D && aligned16(w.data_ptr()));
+            (i ? r.kw : r.qw) = w.data_ptr();
+        }
+    need((a[2] == Py_None) == (a[3] == Py_None));
+    if (a[2] != Py_None) {
+        r.pos = index32(plain(a[2]), q, T);
+        const Tensor& t = plain(a[3]);
+        same(t, q, at::kFloat);
+        need(t.dim() == 2 && aligned16(t.data_ptr()) && t.size(0) > 0 && t.size(1) > 0 &&
+             t.size(1) <= D && t.size(1) % 2 == 0);
+        r.table = static_cast<const float*>(t.data_ptr());
+        r.P = t.size(0);
+        r.R = t.size(1);
+    }
+    r.eps = (float)real(a[4]);
+    r.pairs = PyObject_IsTrue(a[5]);
+    r.unit = PyObject_IsTrue(a[6]);
+    return r;
+}
+
+// norm_rope(q, k, q_weight, k_weight, positions, cos_sin, eps, interleaved, unit_offset)
+PyObject* py_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return entry(a, n, 9, [](PyObject* const* a) {
+        const Tensor &q = plain(a[0]), &k = plain(a[1]);
+        const Heads hq = heads(q), hk = heads(k);
+        need(hk.T == hq.T && hk.D == hq.D && k.device() == q.device());
+        const RowArgs r = row_args(a + 2, q, hq.T, hq.D);
+        return [q, k, hq, hk, r] {
+            c10::DeviceGuard guard(q.device());
+            Several out;
+            out.t[out.n++] = at::empty(q.sizes(), q.options());
+            out.t[out.n++] = at::empty(k.sizes(), k.options());
+            check("fni8_qk_norm_rope_f16",
+                  fni8_qk_norm_rope_f16(hq.p, hq.lt, hq.lh, hq.H, hk.p, hk.lt, hk.lh, hk.H, hq.T,
+                                        hq.D, r.qw, r.kw, r.eps, r.unit, r.pos, r.table, r.P, r.R,
+                                        r.pairs, out.t[0].data_ptr(), out.t[1].data_ptr(),
+                                        stream_of(q)));
+            return out;
+        };
+    });
+}
+
+// A paged cache [pages, H, page_size, D], fp16 or int8 with fp32 scales.
+struct Cache {
+    void *k, *v;
+    float *ks = nullptr, *vs = nullptr;
+    int64_t pages, page, H;
+};
+Cache cache_of(PyObject* pk, PyObject* pv, PyObject* pks, PyObject* pvs, const Tensor& q, int64_t D) {
+    const Tensor &k = plain(pk), &v = plain(pv);
+    need((pks == Py_None) == (pvs == Py_None));
+    const bool i8 = pks != Py_None;
+    same(k, q, i8 ? at::kChar : at::kHalf);
+    same(v, q, i8 ? at::kChar : at::kHalf);
+    need(k.dim() == 4 && k.sizes() == v.sizes() && k.size(3) == D && k.numel() > 0);
+    Cache c{k.data_ptr(), v.data_ptr(), nullptr, nullptr, k.size(0), k.size(2), k.size(1)};
+    if (i8) {
+        const Tensor &ks = plain(pks), &vs = plain(pvs);
+        same(ks, q, at::kFloat);
+        same(vs, q, at::kFloat);
+        need(ks.dim() == 3 && ks.sizes() == k.sizes().slice(0, 3) && vs.sizes() == ks.sizes());
+        c.ks = static_cast<float*>(ks.data_ptr());
+        c.vs = static_cast<float*>(vs.data_ptr());
+    }
+    return c;
+}
+
+// rope_append(q, k, v, k_cache, v_cache, k_scale, v_scale, slots, q_weight, k_weight,
+//             positions, cos_sin, eps, interleaved, unit_offset)
+PyObject* py_rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return entry(a, n, 15, [](PyObject* const* a) {
+        const Tensor &q = plain(a[0]), &k = plain(a[1]), &v = plain(a[2]);
+        const Heads hq = heads(q), hk = heads(k), hv = heads(v);
+        need(hk.T == hq.T && hk.D == hq.D && hv.T == hq.T && hv.H == hk.H && hv.D == hq.D &&
+             k.device() == q.device() && v.device() == q.device());
+        const Cache c = cache_of(a[3], a[4], a[5], a[6], q, hq.D);
+        need(c.H == hk.H);
+        const int32_t* slots = index32(plain(a[7]), q, hq.T);
+        const RowArgs r = row_args(a + 8, q, hq.T, hq.D);
+        return [q, hq, hk, hv, c, slots, r] {
+            c10::DeviceGuard guard(q.device());
+            Tensor out = at::empty(q.sizes(), q.options());
+            check("fni8_rope_append_f16",
+                  fni8_rope_append_f16(hq.p, hq.lt, hq.lh, hq.H, hk.p, hk.lt, hk.lh, hk.H, hv.p,
+                                       hv.lt, hv.lh, hq.T, hq.D, r.qw, r.kw, r.eps, r.unit, r.pos,
+                                       r.table, r.P, r.R, r.pairs, out.data_ptr(), c.k, c.v, c.ks,
+                                       c.vs, c.pages, c.page, slots, stream_of(q)));
+            return One{out};
+        };
+    });
+}
+
+// paged_attention(q, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens,
+//                 cu_seqlens, max_seqlen, scale, window)
+PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return entry(a, n, 11, [](PyObject* const* a) {
+        const Tensor &q = plain(a[0]), &tables = plain(a[5]);
+        const Heads h = heads(q);
+        const Cache c = cache_of(a[1], a[2], a[3], a[4], q, h.D);
+        need(tables.scalar_type() == at::kInt && tables.device() == q.device() &&
+             tables.dim() == 2 && tables.numel() > 0);
+        const int64_t B = tables.size(0), W = tables.size(1);
+        need((W == 1 || tables.stride(1) == 1) && (B == 1 || tables.stride(0) >= W));
+        const int64_t ldt = B == 1 ? W : tables.stride(0);
+        const int32_t* lens = index32(plain(a[6]), q, B);
+        const int32_t* cu = a[7] == Py_None ? nullptr : index32(plain(a[7]), q, B + 1);
+        need(cu || h.T == B);
+        int64_t most = h.T;
+        if (a[8] != Py_None) {
+            most = integer(a[8]);
+            need(most >= 0);
+        }
+        const float scale = a[9] == Py_None ? (float)std::pow((double)h.D, -0.5) : (float)real(a[9]);
+        int64_t window = 0;
+        if (a[10] != Py_None) {
+            window = integer(a[10]);
+            need(window >= 1);
+        }
+        const int32_t* tp = static_cast<const int32_t*>(tables.data_ptr());
+        return [q, h, c, tp, ldt, B, W, lens, cu, most, scale, window] {
+            c10::DeviceGuard guard(q.device());
+            Tensor out = at::empty(q.sizes(), q.options());
+            const int64_t nw = fni8_paged_attention_workspace_bytes(h.T, h.H, c.H, h.D, B, most,
+                                                                    W * c.page);
+            Scratch sc;
+            sc.take(nw);
+            if (nw) sc.alloc(q);
+            check("fni8_paged_attention_f16",
+                  fni8_paged_attention_f16(h.p, h.lt, h.lh, h.T, h.H, c.H, h.D, c.k, c.v, c.ks,
+                                           c.vs, c.pages, c.page, tp, ldt, W, lens, cu, B, most,
+                                           scale, window, out.data_ptr(),
+                                           nw ? sc.at_<void>(0) : nullptr, nw, stream_of(q)));
+            return One{out};
+        };
+    });
+}
+
 #define FNI8_METHOD(name) \
     {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FNI8_METHOD(linear), FNI8_METHOD(gemm), FNI8_METHOD(mlp),
-                         FNI8_METHOD(rmsnorm), FNI8_METHOD(moe), {nullptr, nullptr, 0, nullptr}};
+                         FNI8_METHOD(rmsnorm), FNI8_METHOD(moe), FNI8_METHOD(norm_rope),
+                         FNI8_METHOD(rope_append), FNI8_METHOD(paged_attention), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods,
                       nullptr, nullptr, nullptr, nullptr};
 

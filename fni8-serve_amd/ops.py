@@ -11,8 +11,8 @@ device, allocates its outputs and scratch from torch's caching allocator, and
 never synchronises, so the calls can be captured in a HIP graph.  GPU tensors
 are required: there is no CPU or PyTorch fallback here.
 
-`linear`, `gemm_w8a8`, `gemm_w4a8`, `rmsnorm`, `rmsnorm_quant` and the chains
-`gated_mlp` and `sparse_moe` run in native host code (`_host`, csrc/host.cpp) when
+`linear`, `gemm_w8a8`, `gemm_w4a8`, `rmsnorm`, `rmsnorm_quant`, `rope`, `qk_norm_rope`,
+`rope_append`, `paged_attention` and the chains `gated_mlp` and `sparse_moe` run in native host code (`_host`, csrc/host.cpp) when
 every tensor is a plain GPU tensor in the layout the kernels take; the Python below
 is the general way (strided, converted or refused arguments).  A LinearW8A8 call at
 one token took 17 us of Python for 4.3 us of kernel on an MI355X host; natively a
@@ -626,6 +626,11 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
     interleaved, as pairs (2i, 2i + 1).  A position outside [0, P) gives NaN.  positions and
     cos_sin of None: norms only (fni8serve/layers/rotary.py:21-55,
     layers/gqa_attention.py:59-157)."""
+    if q.is_cuda:
+        out = _lib.host().norm_rope(q, k, q_weight, k_weight, positions, cos_sin, eps, interleaved,
+                                    unit_offset)
+        if out is not None:
+            return out
     dev = _require_cuda("qk_norm_rope", q, k, q_weight, k_weight, positions, cos_sin)
     q, ldq, hsq = _heads("q", q)
     k, ldk, hsk = _heads("k", k)
@@ -698,6 +703,11 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     Hk, page_size], quantized as quantize_rowwise does.  A slot outside the cache (negative:
     padding) drops its token's rows; no slot may occur twice in a call
     (fni8serve/engine/kv_cache.py:265,681,700,730,826)."""
+    if q.is_cuda:
+        out = _lib.host().rope_append(q, k, v, k_cache, v_cache, k_scale, v_scale, slots, q_weight,
+                                      k_weight, positions, cos_sin, eps, interleaved, unit_offset)
+        if out is not None:
+            return out
     dev = _require_cuda("rope_append", q, k, v, positions, cos_sin, k_cache, v_cache, slots,
                         k_scale, v_scale, q_weight, k_weight)
     q, ldq, hsq = _heads("q", q)
@@ -739,6 +749,11 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     known; giving it saves a launch for decoded tokens).  scale defaults to D ** -0.5; window
     is the number of keys that a query sees, itself among them.  A query without keys and
     tokens past cu_seqlens[-1] give 0; a token whose page is not in the cache counts as NaN."""
+    if q.is_cuda:
+        out = _lib.host().paged_attention(q, k_cache, v_cache, k_scale, v_scale, block_tables,
+                                          context_lens, cu_seqlens, max_seqlen, scale, window)
+        if out is not None:
+            return out
     dev = _require_cuda("paged_attention", q, k_cache, v_cache, block_tables, context_lens,
                         cu_seqlens, k_scale, v_scale)
     q, ldq, hsq = _heads("q", q)
