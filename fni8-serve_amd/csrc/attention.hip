@@ -66,7 +66,7 @@ struct Attn {
     float* part;
     int T, Hq, Hk, D, group, num_pages, plog, max_pages, B, nseq, window, cap;
     float c;       // scale * log2 e
-    int few;       // few_kernel takes sequences of at most so many rows, tile_kernel others
+    int few;       // few_kernel takes sequences of at most so many new tokens, tile_kernel others
     int whole;     // few_kernel: no parts, an item is one unit
     int splits;    // tile_kernel: parts of an item at most
 };
@@ -114,15 +114,33 @@ __device__ __forceinline__ int block_scan(int v, int* sh, int& total) {
 }
 
 // The sequence that holds unit `target(U)` of the list of all U = sum units(s), and the
-// number of units before it.  Every thread of the block gets the same answer; false where
-// the target is not in the list.
+// number of units before it.  Every thread of the block gets the same answer, in scalar
+// registers; false where the target is not in the list.  sh: 16 words of LDS.
 template <class Units, class Target>
 __device__ __forceinline__ bool find(int nseq, int* sh, Units units, Target target, int& s_out,
-                                     int& base_out, int& goal) {
+                                     int& base_out, int& goal, Seq& q_out) {
     const int tid = threadIdx.x;
     int U = 0, mine = 0, incl = 0, total = 0;
+    Seq q{0, 0, 0};
+    if (nseq <= 64) {  // every wave by itself
+        const int lane = tid & 63;
+        if (lane < nseq) mine = units(lane, q);
+        incl = fni8::wave_incl_scan_i32(mine, lane);
+        U = __builtin_amdgcn_readlane(incl, 63);
+        goal = target(U);
+        if (goal < 0 || goal >= U) return false;
+        const uint64_t at = __ballot(incl >= mine && goal >= incl - mine && goal < incl);
+        if (!at) return false;
+        s_out = __builtin_ctzll(at);
+        base_out = __builtin_amdgcn_readlane(incl - mine, s_out);
+        q_out.start = __builtin_amdgcn_readlane(q.start, s_out);
+        q_out.n = __builtin_amdgcn_readlane(q.n, s_out);
+        q_out.L = __builtin_amdgcn_readlane(q.L, s_out);
+        return true;
+    }
+    if (tid == 0) sh[4] = -1;
     for (int c = 0; c < nseq; c += 256) {
-        mine = c + tid < nseq ? units(c + tid) : 0;
+        mine = c + tid < nseq ? units(c + tid, q) : 0;
         incl = block_scan(mine, sh, total);
         U += total;
     }
@@ -130,11 +148,9 @@ __device__ __forceinline__ bool find(int nseq, int* sh, Units units, Target targ
     goal = target(U);
     if (goal < 0 || goal >= U) return false;
     int base = 0;
-    if (tid == 0) sh[4] = -1;
-    __syncthreads();
     for (int c = 0; c < nseq; c += 256) {
         if (nseq > 256) {
-            mine = c + tid < nseq ? units(c + tid) : 0;
+            mine = c + tid < nseq ? units(c + tid, q) : 0;
             incl = block_scan(mine, sh, total);
         }
         const int before = base + incl - mine;
@@ -142,12 +158,18 @@ __device__ __forceinline__ bool find(int nseq, int* sh, Units units, Target targ
         if (before >= 0 && goal >= before && goal - before < mine) {
             sh[4] = c + tid;
             sh[5] = before;
+            sh[6] = q.start;
+            sh[7] = q.n;
+            sh[8] = q.L;
         }
         base += total;
     }
     __syncthreads();
     s_out = __builtin_amdgcn_readfirstlane(sh[4]);
     base_out = __builtin_amdgcn_readfirstlane(sh[5]);
+    q_out.start = __builtin_amdgcn_readfirstlane(sh[6]);
+    q_out.n = __builtin_amdgcn_readfirstlane(sh[7]);
+    q_out.L = __builtin_amdgcn_readfirstlane(sh[8]);
     __syncthreads();
     return s_out >= 0;
 }
@@ -264,7 +286,7 @@ constexpr int few_region() {
 }
 template <int DP, int RB>
 constexpr int few_lds() {
-    return 4 * few_region<DP, RB>() + 4 * 2 * 16 * RB * 4 + 32;
+    return 4 * few_region<DP, RB>() + 4 * 2 * 16 * RB * 4 + 64;
 }
 // floats of a part: o [16 RB][DP], m, l [16 RB]
 template <int DP, int RB>
@@ -283,10 +305,10 @@ struct FewSeq {
     int rows, blocks, lo, tiles, units;
 };
 template <int RB>
-__device__ __forceinline__ FewSeq few_seq(const Attn& a, int s) {
+__device__ __forceinline__ FewSeq few_seq(const Attn& a, const Seq& q) {
     FewSeq f;
-    f.q = sequence(a, s);
-    f.rows = f.q.n > a.few / a.group ? 0 : f.q.n * a.group;
+    f.q = q;
+    f.rows = f.q.n > a.few ? 0 : f.q.n * a.group;
     f.blocks = (f.rows + 16 * RB - 1) / (16 * RB);
     const int first = f.q.L - f.q.n;
     f.lo = a.window && first - a.window + 1 > 0 ? (first - a.window + 1) & ~31 : 0;
@@ -318,18 +340,22 @@ __global__ __launch_bounds__(256, few_waves(DP, I8, RB)) void few_kernel(Attn a)
     int* sh = reinterpret_cast<int*>(ml + 4 * 2 * 16 * RB);
 
     if (!a.whole && threadIdx.x == 0) a.joins[blockIdx.x].parts = 0;
-    int s, base, u;
-    int upw = 0;
+    int s, base, u, upw = 0;
+    Seq sq;
     if (!find(
-            a.nseq, sh, [&](int i) { return few_seq<RB>(a, i).units; },
+            a.nseq, sh,
+            [&](int i, Seq& q) {
+                q = sequence(a, i);
+                return few_seq<RB>(a, q).units;
+            },
             [&](int U) {
                 upw = per_worker(U);
                 return upw * (int)blockIdx.x;
             },
-            s, base, u))
+            s, base, u, sq))
         return;
     const int first_unit = u;
-    FewSeq f = few_seq<RB>(a, s);
+    FewSeq f = few_seq<RB>(a, sq);
     int per_item = a.whole ? 1 : f.tiles;
     int item = (u - base) / per_item, tile = (u - base) - item * per_item;
     int left = upw;
@@ -678,7 +704,7 @@ __global__ __launch_bounds__(256, few_waves(DP, I8, RB)) void few_kernel(Attn a)
         if (++item >= f.blocks * a.Hk) {
             do {
                 if (++s >= a.nseq) return;
-                f = few_seq<RB>(a, s);
+                f = few_seq<RB>(a, sequence(a, s));
             } while (f.units == 0);
             item = 0;
             per_item = a.whole ? 1 : f.tiles;
@@ -774,7 +800,7 @@ __device__ const uint4 kNaNs = {0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e0
 
 template <int DP, bool I8>
 constexpr int tile_lds() {
-    return 2 * 2 * kTileKeys * DP * 2 + (I8 ? 2 * 3 * kTileKeys * 4 : 0) + 32;
+    return 2 * 2 * kTileKeys * DP * 2 + (I8 ? 2 * 3 * kTileKeys * 4 : 0) + 64;
 }
 
 // The item of a workgroup of tile_kernel.
@@ -786,15 +812,14 @@ struct TileItem {
 // Tiles of all sequences from the last to the first: a causal tile's keys grow with its
 // rows, and the longest ones begin first.
 __device__ __forceinline__ bool tile_item(const Attn& a, int id, int h, int* sh, TileItem& t) {
-    auto tiles = [&](int s) {
-        const Seq q = sequence(a, s);
-        return q.n > a.few / a.group
+    auto tiles = [&](int s, Seq& q) {
+        q = sequence(a, s);
+        return q.n > a.few
                    ? (int)(((int64_t)q.n * a.group + kTileRows - 1) / kTileRows) : 0;
     };
     int base, goal;
-    if (!find(a.nseq, sh, tiles, [&](int N) { return N - 1 - id; }, t.s, base, goal))
+    if (!find(a.nseq, sh, tiles, [&](int N) { return N - 1 - id; }, t.s, base, goal, t.q))
         return false;
-    t.q = sequence(a, t.s);
     t.rows = t.q.n * a.group;
     t.tile = goal - base;
     t.h = h;
@@ -828,7 +853,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, H = lane >> 5;
     float* scales = reinterpret_cast<float*>(smem + 4 * TB);  // [2][3][64]
-    int* sh = reinterpret_cast<int*>(smem + tile_lds<DP, I8>() - 32);
+    int* sh = reinterpret_cast<int*>(smem + tile_lds<DP, I8>() - 64);
 
     // a key head's items are neighbours modulo the heads: with the round-robin dispatch
     // over the 8 XCDs they share an L2 where the heads divide 8
@@ -1181,7 +1206,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
 // How a call is cut up, from what the host knows.
 struct Plan {
     int rb;               // 16-row blocks of few_kernel's rows
-    int few;              // rows of a sequence that few_kernel takes at most
+    int64_t few;          // new tokens of a sequence that few_kernel takes at most
     bool use_few, use_tile;
     int64_t workers;      // of few_kernel
     int64_t tiles;        // of 128 rows, at most
@@ -1203,7 +1228,7 @@ Plan plan_of(int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t B, int64_t mo
     // one sequence of many rows: nothing is left for few_kernel but padding, which the
     // tiles take too
     p.use_few = !p.use_tile || B > 1;
-    p.few = !p.use_tile ? 1 << 30 : p.use_few ? 16 * p.rb : 0;
+    p.few = !p.use_tile ? 1 << 30 : p.use_few ? 16 * p.rb / group : 0;
     const int64_t units = (max_context + 1 + kUnit - 1) / kUnit;
     p.workers = (B + 1 + T * group / (16 * p.rb)) * Hk * units;
     p.workers = p.workers < kWorkers ? p.workers : kWorkers;
@@ -1323,7 +1348,7 @@ int launch_paged_attention(const PagedAttention& p, hipStream_t st) {
     a.window = p.window > context ? 0 : (int)p.window;
     a.cap = (int)context + 1;
     a.c = p.scale * 1.44269504088896340736f;
-    a.few = plan.few;
+    a.few = (int)plan.few;
     a.splits = 1;
     if (plan.bytes && p.work_bytes >= plan.bytes) {
         a.joins = reinterpret_cast<Join*>(p.work);
