@@ -41,7 +41,6 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kInf = __builtin_inff();
 constexpr int kUnit = 128;      // keys of a unit of few_kernel: 32 for each of 4 waves
-constexpr int kTileRows = 128;  // rows of a workgroup of tile_kernel
 constexpr int kTileKeys = 64;
 constexpr float kLag = 8.0f;
 constexpr int kWorkers = 768;  // of few_kernel at most: three a CU
@@ -65,7 +64,8 @@ struct Attn {
     Join* joins;
     float* part;
     int T, Hq, Hk, D, group, num_pages, plog, max_pages, B, nseq, window, cap;
-    float c;       // scale * log2 e
+    float c;       // |scale| * log2 e, not 0
+    uint32_t flip; // sign bits of two fp16 where the scale is negative: the queries' signs
     int few;       // few_kernel takes sequences of at most so many new tokens, tile_kernel others
     int whole;     // few_kernel: no parts, an item is one unit
     int splits;    // tile_kernel: parts of an item at most
@@ -98,6 +98,7 @@ __device__ __forceinline__ Seq sequence(const Attn& a, int s) {
 
 // ---- the list of items -----------------------------------------------------------
 
+template <int NW>
 __device__ __forceinline__ int block_scan(int v, int* sh, int& total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int incl = fni8::wave_incl_scan_i32(v, lane);
@@ -106,7 +107,7 @@ __device__ __forceinline__ int block_scan(int v, int* sh, int& total) {
     __syncthreads();
     total = 0;
 #pragma unroll
-    for (int w = 0; w < 4; w++) {
+    for (int w = 0; w < NW; w++) {
         if (w < wave) incl += sh[w];
         total += sh[w];
     }
@@ -116,7 +117,7 @@ __device__ __forceinline__ int block_scan(int v, int* sh, int& total) {
 // The sequence that holds unit `target(U)` of the list of all U = sum units(s), and the
 // number of units before it.  Every thread of the block gets the same answer, in scalar
 // registers; false where the target is not in the list.  sh: 16 words of LDS.
-template <class Units, class Target>
+template <int NW, class Units, class Target>
 __device__ __forceinline__ bool find(int nseq, int* sh, Units units, Target target, int& s_out,
                                      int& base_out, int& goal, Seq& q_out) {
     const int tid = threadIdx.x;
@@ -138,38 +139,38 @@ __device__ __forceinline__ bool find(int nseq, int* sh, Units units, Target targ
         q_out.L = __builtin_amdgcn_readlane(q.L, s_out);
         return true;
     }
-    if (tid == 0) sh[4] = -1;
-    for (int c = 0; c < nseq; c += 256) {
+    if (tid == 0) sh[8] = -1;
+    for (int c = 0; c < nseq; c += 64 * NW) {
         mine = c + tid < nseq ? units(c + tid, q) : 0;
-        incl = block_scan(mine, sh, total);
+        incl = block_scan<NW>(mine, sh, total);
         U += total;
     }
     U = __builtin_amdgcn_readfirstlane(U);  // wave-uniform from here on, in scalar registers
     goal = target(U);
     if (goal < 0 || goal >= U) return false;
     int base = 0;
-    for (int c = 0; c < nseq; c += 256) {
-        if (nseq > 256) {
+    for (int c = 0; c < nseq; c += 64 * NW) {
+        if (nseq > 64 * NW) {
             mine = c + tid < nseq ? units(c + tid, q) : 0;
-            incl = block_scan(mine, sh, total);
+            incl = block_scan<NW>(mine, sh, total);
         }
         const int before = base + incl - mine;
         // (sums that overflow, from a cu_seqlens that is not one, are no place)
         if (before >= 0 && goal >= before && goal - before < mine) {
-            sh[4] = c + tid;
-            sh[5] = before;
-            sh[6] = q.start;
-            sh[7] = q.n;
-            sh[8] = q.L;
+            sh[8] = c + tid;
+            sh[9] = before;
+            sh[10] = q.start;
+            sh[11] = q.n;
+            sh[12] = q.L;
         }
         base += total;
     }
     __syncthreads();
-    s_out = __builtin_amdgcn_readfirstlane(sh[4]);
-    base_out = __builtin_amdgcn_readfirstlane(sh[5]);
-    q_out.start = __builtin_amdgcn_readfirstlane(sh[6]);
-    q_out.n = __builtin_amdgcn_readfirstlane(sh[7]);
-    q_out.L = __builtin_amdgcn_readfirstlane(sh[8]);
+    s_out = __builtin_amdgcn_readfirstlane(sh[8]);
+    base_out = __builtin_amdgcn_readfirstlane(sh[9]);
+    q_out.start = __builtin_amdgcn_readfirstlane(sh[10]);
+    q_out.n = __builtin_amdgcn_readfirstlane(sh[11]);
+    q_out.L = __builtin_amdgcn_readfirstlane(sh[12]);
     __syncthreads();
     return s_out >= 0;
 }
@@ -342,7 +343,7 @@ __global__ __launch_bounds__(256, few_waves(DP, I8, RB)) void few_kernel(Attn a)
     if (!a.whole && threadIdx.x == 0) a.joins[blockIdx.x].parts = 0;
     int s, base, u, upw = 0;
     Seq sq;
-    if (!find(
+    if (!find<4>(
             a.nseq, sh,
             [&](int i, Seq& q) {
                 q = sequence(a, i);
@@ -378,11 +379,15 @@ __global__ __launch_bounds__(256, few_waves(DP, I8, RB)) void few_kernel(Attn a)
         // k-steps of a 16-byte load)
         h8 q[RB][KS];
         int prow[RB];
+        uint32_t span[RB], seen0[RB];
 #pragma unroll
         for (int b = 0; b < RB; b++) {
             const int r = row0 + 16 * b + col;
             const int i = r / a.group, head = h * a.group + r - i * a.group;
             prow[b] = r < f.rows ? p0 + i : -1;
+            // it sees the keys j with prow - span < j <= prow: one unsigned comparison
+            span[b] = prow[b] < 0 ? 0 : a.window ? a.window : prow[b] + 1;
+            seen0[b] = 4 * G - (prow[b] + 1 - (int)span[b]);
 #pragma unroll
             for (int k = 0; k < KS; k++) {
                 const int d = I8 ? 64 * (k >> 1) + 16 * G + 8 * (k & 1) : 32 * k + 8 * G;
@@ -390,6 +395,7 @@ __global__ __launch_bounds__(256, few_waves(DP, I8, RB)) void few_kernel(Attn a)
                 if (r < f.rows && d < a.D)
                     v = *reinterpret_cast<const u32x4*>(a.q + (f.q.start + i) * a.ldq +
                                                         head * a.hsq + d);
+                v ^= a.flip;
                 q[b][k] = __builtin_bit_cast(h8, v);
             }
         }
@@ -566,8 +572,7 @@ __global__ __launch_bounds__(256, few_waves(DP, I8, RB)) void few_kernel(Attn a)
                 if (edge)
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
-                        const int j = t0 + 16 * (e >> 2) + 4 * G + (e & 3);
-                        if (j > prow[b] || (a.window && j <= prow[b] - a.window)) x[e] = -kInf;
+                        if (seen0[b] + t0 + 16 * (e >> 2) + (e & 3) >= span[b]) x[e] = -kInf;
                     }
                 float top = x[0];
 #pragma unroll
@@ -617,7 +622,7 @@ __global__ __launch_bounds__(256, few_waves(DP, I8, RB)) void few_kernel(Attn a)
                         const uint2 w = *reinterpret_cast<const uint2*>(vp + 16 * d);
 #pragma unroll
                         for (int b = 0; b < RB; b++) {
-                            if (j > prow[b] || (a.window && j <= prow[b] - a.window)) continue;
+                            if (j - (prow[b] + 1 - (int)span[b]) >= span[b]) continue;
 #pragma unroll
                             for (int r = 0; r < 4; r++)
                                 o[b][d][r] += odd_part(r < 2 ? w.x : w.y, r & 1);
@@ -781,6 +786,20 @@ __device__ __forceinline__ void copy16(uint32_t lds, const void* src) {
                  :: "s"(lds), "v"(src) : "memory", "m0");
 }
 
+// Waits until at most N of the wave's copies (and other loads) are on their way.
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+    asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory");
+}
+
+// A workgroup barrier that leaves copies on their way (__syncthreads waits for all of
+// them); LDS reads of the stage that is copied into next have returned by then.
+__device__ __forceinline__ void barrier_all() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
 // A wave-uniform address in scalar registers, wherever it was computed.
 __device__ __forceinline__ const void* scalar(const void* p) {
     const uint64_t u = (uint64_t)(uintptr_t)p;
@@ -798,9 +817,13 @@ __device__ __forceinline__ void copy16_s(uint32_t lds, const void* base, uint32_
 __device__ const uint4 kZeros = {0, 0, 0, 0};
 __device__ const uint4 kNaNs = {0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u};
 
-template <int DP, bool I8>
+// Stages of K and V tiles: as many as fit where the copies need no registers
+constexpr int tile_stages(int dp, bool i8, int nw) {
+    return i8 || dp == 256 || (dp == 128 && nw == 4) ? 2 : 4;
+}
+template <int DP, bool I8, int NW>
 constexpr int tile_lds() {
-    return 2 * 2 * kTileKeys * DP * 2 + (I8 ? 2 * 3 * kTileKeys * 4 : 0) + 64;
+    return tile_stages(DP, I8, NW) * 2 * kTileKeys * DP * 2 + (I8 ? 2 * 3 * kTileKeys * 4 : 0) + 64;
 }
 
 // The item of a workgroup of tile_kernel.
@@ -811,20 +834,22 @@ struct TileItem {
 
 // Tiles of all sequences from the last to the first: a causal tile's keys grow with its
 // rows, and the longest ones begin first.
+template <int NW>
 __device__ __forceinline__ bool tile_item(const Attn& a, int id, int h, int* sh, TileItem& t) {
+    constexpr int BM = 32 * NW;
     auto tiles = [&](int s, Seq& q) {
         q = sequence(a, s);
         return q.n > a.few
-                   ? (int)(((int64_t)q.n * a.group + kTileRows - 1) / kTileRows) : 0;
+                   ? (int)(((int64_t)q.n * a.group + BM - 1) / BM) : 0;
     };
     int base, goal;
-    if (!find(a.nseq, sh, tiles, [&](int N) { return N - 1 - id; }, t.s, base, goal, t.q))
+    if (!find<NW>(a.nseq, sh, tiles, [&](int N) { return N - 1 - id; }, t.s, base, goal, t.q))
         return false;
     t.rows = t.q.n * a.group;
     t.tile = goal - base;
     t.h = h;
-    const int i0 = t.tile * kTileRows / a.group;
-    int i1 = (t.tile * kTileRows + kTileRows - 1) / a.group;
+    const int i0 = t.tile * BM / a.group;
+    int i1 = (t.tile * BM + BM - 1) / a.group;
     i1 = i1 < t.q.n ? i1 : t.q.n - 1;
     const int p0 = t.q.L - t.q.n;
     t.hi = p0 + i1 + 1 > 0 ? p0 + i1 + 1 : 0;
@@ -838,43 +863,40 @@ __device__ __forceinline__ bool tile_item(const Attn& a, int id, int h, int* sh,
     return true;
 }
 
-template <int DP>
-constexpr int tile_part() {
-    return kTileRows * (DP + 2);
-}
-
-template <int DP, bool I8>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
+template <int DP, bool I8, int NW>
+__global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
+    constexpr int BM = 32 * NW, KW = kTileKeys / NW;  // rows of a workgroup, keys a wave copies
+    constexpr int S = tile_stages(DP, I8, NW);
     constexpr int KS = DP / 16, DB = DP / 32, CH = DP / 8;
     constexpr int TB = kTileKeys * DP * 2;  // bytes of a K or V tile
-    constexpr int NL = I8 ? DP / 64 : DP / 32;
+    constexpr int NL = KW * DP * (I8 ? 1 : 2) / 1024;  // copies of a wave and tile, K or V
     extern __shared__ __align__(16) char smem[];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, H = lane >> 5;
-    float* scales = reinterpret_cast<float*>(smem + 4 * TB);  // [2][3][64]
-    int* sh = reinterpret_cast<int*>(smem + tile_lds<DP, I8>() - 64);
+    float* scales = reinterpret_cast<float*>(smem + 2 * S * TB);  // [2][3][64]
+    int* sh = reinterpret_cast<int*>(smem + tile_lds<DP, I8, NW>() - 64);
 
     // a key head's items are neighbours modulo the heads: with the round-robin dispatch
     // over the 8 XCDs they share an L2 where the heads divide 8
     const int h = blockIdx.x % a.Hk, rest = blockIdx.x / a.Hk;
     const int split = rest % a.splits;
     TileItem t{};
-    const bool found = tile_item(a, rest / a.splits, h, sh, t);
+    const bool found = tile_item<NW>(a, rest / a.splits, h, sh, t);
     const int index = rest / a.splits * a.Hk + h;
     if (a.splits > 1 && split == 0 && threadIdx.x == 0) {
-        const int tile_row0 = t.tile * kTileRows;
+        const int tile_row0 = t.tile * BM;
         Join j{0, 0, 0, 0, 0, 0, 0, 0};
         if (found && t.parts > 1)
             j = Join{t.parts, index * a.splits, index * a.splits + 1, 1, t.q.start, tile_row0,
-                     t.rows - tile_row0 < kTileRows ? t.rows - tile_row0 : kTileRows, h};
+                     t.rows - tile_row0 < BM ? t.rows - tile_row0 : BM, h};
         a.joins[index] = j;
     }
     if (!found || split >= t.parts) return;
     const int first = t.kt0 + split * t.per;
     const int last = first + t.per < t.kt1 ? first + t.per : t.kt1;
 
-    const int row0 = t.tile * kTileRows + wave * 32;
+    const int row0 = t.tile * BM + wave * 32;
     const int p0 = t.q.L - t.q.n;
     const int nrows = t.rows - row0 < 32 ? t.rows - row0 : 32;  // may be 0 or less
     const int pmin = p0 + row0 / a.group;
@@ -889,8 +911,14 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
         if (r < t.rows && 16 * k + 8 * H < a.D)
             v = *reinterpret_cast<const u32x4*>(a.q + (t.q.start + qi) * a.ldq + head * a.hsq +
                                                 16 * k + 8 * H);
+        v ^= a.flip;
+        asm volatile("" : "+v"(v));  // waited for here, not in the loop among the copies
         q[k] = __builtin_bit_cast(h8, v);
     }
+
+    // the row sees the keys j with prow - span < j <= prow: one unsigned comparison
+    const uint32_t span = prow < 0 ? 0 : a.window ? a.window : prow + 1;
+    const uint32_t seen0 = 4 * H - (prow + 1 - (int)span);
 
     // chunk ch of key t: K rows are read by 32 keys at one chunk, V rows by 4 keys at 4
     // chunks (transposing); both permutations put those on different banks
@@ -916,23 +944,26 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
 #pragma unroll
         for (int j = 0; j < NL; j++) {
             const int c = j * 64 + lane, k = c / CH, in = c % CH;
-            k_off[j] = (k * DP + 8 * (in ^ k_swz(16 * wave + k))) * 2;
+            k_off[j] = (k * DP + 8 * (in ^ k_swz(KW * wave + k))) * 2;
         }
         v_off = (lane / CH * DP + 8 * (lane % CH ^ v_swz(lane / CH))) * 2;
     }
     // copy j takes the next 1024 bytes; rows of 512 bytes change the permutation with it
     auto v_off_of = [&](int j) { return (DP == 256 && (j & 1) ? v_off ^ 128 : v_off) + j * 1024; };
 
-    int pages = 0;  // lane j: the wave's 16 keys of tile (kt & ~63) + j, counted from `first`
+    int pages = 0;  // lane j: the page of the wave's keys of tile (kt & ~63) + j, from `first`
     u32x4 kr[I8 ? NL : 1], vr[I8 ? NL : 1];
     float ksr = 0.0f, vsr = 1.0f;
     auto begin = [&](int kt, int buf) {
         const int i = kt - first;
-        if ((i & 63) == 0)
-            pages = kt + lane < last ? page_of(a, t.s, (kt + lane) * kTileKeys + 16 * wave, t.lo, t.hi)
+        if ((i & 63) == 0) {
+            pages = kt + lane < last ? page_of(a, t.s, (kt + lane) * kTileKeys + (KW * wave & ~15),
+                                               t.lo, t.hi)
                                      : kNone;
+            asm volatile("" : "+v"(pages));  // waited for here
+        }
         const int page = __builtin_amdgcn_readlane(pages, i & 63);
-        const int tok = kt * kTileKeys + 16 * wave;
+        const int tok = kt * kTileKeys + KW * wave;
         const int64_t row = (((int64_t)(page < 0 ? 0 : page) * a.Hk + h) << a.plog) +
                             (tok & ((1 << a.plog) - 1));
         if constexpr (I8) {
@@ -949,12 +980,12 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
             ksr = page == kBad ? __builtin_nanf("") : 0.0f;
             vsr = 1.0f;
             if (page >= 0) {
-                ksr = a.ks[row + (lane & 15)];
-                vsr = a.vs[row + (lane & 15)];
+                ksr = a.ks[row + lane % KW];
+                vsr = a.vs[row + lane % KW];
             }
         } else {
-            const uint32_t kd = lds0 + buf * 2 * TB + 16 * wave * DP * 2;
-            if (page >= 0 && a.D == DP && tok >= t.lo && tok + 16 <= t.hi) {
+            const uint32_t kd = lds0 + buf * 2 * TB + KW * wave * DP * 2;
+            if (page >= 0 && a.D == DP && tok >= t.lo && tok + KW <= t.hi) {
                 const void* kp = scalar(static_cast<const uint16_t*>(a.kc) + row * DP);
                 const void* vp = scalar(static_cast<const uint16_t*>(a.vc) + row * DP);
 #pragma unroll
@@ -966,7 +997,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
 #pragma unroll
             for (int j = 0; j < NL; j++) {
                 const int c = j * 64 + lane, k = c / CH, in = c % CH;
-                const int dk = 8 * (in ^ k_swz(16 * wave + k)), dv = 8 * (in ^ v_swz(16 * wave + k));
+                const int dk = 8 * (in ^ k_swz(KW * wave + k)), dv = 8 * (in ^ v_swz(KW * wave + k));
                 const void* ks = static_cast<const uint16_t*>(a.kc) + (row + k) * a.D + dk;
                 const void* vs = static_cast<const uint16_t*>(a.vc) + (row + k) * a.D + dv;
                 if (page < 0 || dk >= a.D) ks = page == kBad && dk < a.D ? &kNaNs : &kZeros;
@@ -982,7 +1013,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
             char* kt = smem + buf * 2 * TB;
 #pragma unroll
             for (int j = 0; j < NL; j++) {
-                const int c = j * 64 + lane, k = 16 * wave + c / (DP / 16), ch = 2 * (c % (DP / 16));
+                const int c = j * 64 + lane, k = KW * wave + c / (DP / 16), ch = 2 * (c % (DP / 16));
                 u32x4 x, y;
                 codes16(kr[j], x, y);
                 char* at = kt + k * DP * 2;
@@ -992,20 +1023,19 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
                 *reinterpret_cast<u32x4*>(at + TB + 16 * (ch ^ v_swz(k))) = x;
                 *reinterpret_cast<u32x4*>(at + TB + 16 * ((ch + 1) ^ v_swz(k))) = y;
             }
-            if (lane < 16) {
+            if (lane < KW) {
                 float lv, rv;
                 value_scale(vsr, lv, rv);
-                float* sc = scales + buf * 3 * kTileKeys + 16 * wave + lane;
+                float* sc = scales + buf * 3 * kTileKeys + KW * wave + lane;
                 sc[0] = ksr * a.c;
                 sc[kTileKeys] = lv;
                 sc[2 * kTileKeys] = rv;
             }
-        } else {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
     };
 
-    float m = -kInf, l = 0.0f;
+    // m counts once a key was seen: limit, of the exponents over it, is -inf before
+    float m = 0.0f, l = 0.0f, limit = -kInf;
     f32x16 o[DB];
 #pragma unroll
     for (int d = 0; d < DB; d++)
@@ -1015,20 +1045,39 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
     auto compute = [&](int kt, int buf) {
         const int t0 = kt * kTileKeys;
         if (t0 > pmax || (a.window && t0 + kTileKeys - 1 <= pmin - a.window)) return;
-        const uint32_t at_buf = buf * 2 * TB;
         const float* sc = scales + buf * 3 * kTileKeys;
+        uint32_t ka[KA], va[VA];
+#pragma unroll
+        for (int i = 0; i < KA; i++) {
+            ka[i] = k_addr[i] + buf * 2 * TB;
+            asm volatile("" : "+v"(ka[i]));  // what follows is in the reads' constants
+        }
+#pragma unroll
+        for (int d = 0; d < VA; d++) {
+            va[d] = v_addr[d] + buf * 2 * TB;
+            asm volatile("" : "+v"(va[d]));
+        }
         f32x16 s[2];
 #pragma unroll
-        for (int tb = 0; tb < 2; tb++) {
+        for (int tb = 0; tb < 2; tb++)
 #pragma unroll
             for (int e = 0; e < 16; e++) s[tb][e] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < KS; i++)
+        for (int i = 0; i < KS; i++)
+#pragma unroll
+            for (int tb = 0; tb < 2; tb++)
                 s[tb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-                    lds_read16(k_addr[i % KA] + at_buf + 32 * tb * DP * 2 + i / KA * 256), q[i],
-                    s[tb], 0, 0, 0);
+                    lds_read16(ka[i % KA] + 32 * tb * DP * 2 + i / KA * 256), q[i], s[tb], 0, 0, 0);
+        // four fragments ahead of the product that uses them
+        constexpr int kDs = 0x100, kMfma = 0x8;
+        __builtin_amdgcn_sched_group_barrier(kDs, 4, 0);
+#pragma unroll
+        for (int i = 0; i < 2 * KS - 4; i++) {
+            __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(kDs, 1, 0);
         }
-        // element e of block tb is key 32 tb + 8 (e / 4) + 4 H + e % 4
+        __builtin_amdgcn_sched_group_barrier(kMfma, 4, 0);
+        // element e of block tb is key 32 tb + 8 (e / 4) + 4 H + e % 4: its exponent
 #pragma unroll
         for (int tb = 0; tb < 2; tb++)
 #pragma unroll
@@ -1039,10 +1088,11 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
                     const f32x4 lv = *reinterpret_cast<const f32x4*>(sc + kTileKeys + at);
 #pragma unroll
                     for (int e = 0; e < 4; e++)
-                        s[tb][4 * e4 + e] = __builtin_fmaf(s[tb][4 * e4 + e], kx[e], lv[e]);
+                        s[tb][4 * e4 + e] = __builtin_fmaf(s[tb][4 * e4 + e], kx[e], lv[e]) - m;
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) s[tb][4 * e4 + e] *= a.c;
+                    for (int e = 0; e < 4; e++)
+                        s[tb][4 * e4 + e] = __builtin_fmaf(s[tb][4 * e4 + e], a.c, -m);
                 }
             }
         const bool edge = t0 + kTileKeys - 1 > pmin || (a.window && t0 <= pmax - a.window);
@@ -1051,8 +1101,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
             for (int tb = 0; tb < 2; tb++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
-                    const int j = t0 + 32 * tb + 8 * (e >> 2) + 4 * H + (e & 3);
-                    if (j > prow || (a.window && j <= prow - a.window)) s[tb][e] = -kInf;
+                    if (seen0 + t0 + 32 * tb + 8 * (e >> 2) + (e & 3) >= span) s[tb][e] = -kInf;
                 }
         float top = s[0][0];
 #pragma unroll
@@ -1061,22 +1110,26 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
             for (int e = 0; e < 16; e++) top = __builtin_fmaxf(top, s[tb][e]);
         top = max_xor32(top);
         // m need not be the maximum: it may lag by kLag, weights are at most 2^kLag then
-        if (__any(top > m + kLag)) {
-            top = __builtin_fmaxf(top, m);
-            const float keep = exp2_(m - (top == -kInf ? 0.0f : top));
+        if (__any(top > limit)) {
+            const float up = top > limit ? top : 0.0f;
+            const float keep = limit < 0.0f ? 1.0f : exp2_(-up);  // nothing summed yet: 1
             l *= keep;
 #pragma unroll
             for (int d = 0; d < DB; d++) o[d] *= keep;
-            m = top;
+#pragma unroll
+            for (int tb = 0; tb < 2; tb++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) s[tb][e] -= up;
+            m += up;
+            if (top > limit) limit = kLag;
         }
-        const float at = m == -kInf ? 0.0f : m;
         h8 p[4];
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             float w[8];
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                w[e] = exp2_(s[k >> 1][8 * (k & 1) + e] - at);
+                w[e] = exp2_(s[k >> 1][8 * (k & 1) + e]);
                 if constexpr (!I8) l += w[e];
             }
             if constexpr (I8) {
@@ -1095,7 +1148,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
         }
         // value fragment of 32 elements (block d) and keys 16 k + {4 H .., 8 + 4 H ..}
         auto value = [&](int d, int k) {
-            const uint32_t at = v_addr[d % VA] + at_buf + 16 * k * DP * 2 + d / VA * 256;
+            const uint32_t at = va[d % VA] + 16 * k * DP * 2 + d / VA * 256;
             return lds_read_tr(at, at + 8 * DP * 2);
         };
 #pragma unroll
@@ -1106,20 +1159,21 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
     };
 
     // What lies at the edge of some row of the workgroup (the same for its four waves).
-    const int wg_pmin = p0 + t.tile * kTileRows / a.group, wg_pmax = t.hi - 1;
-    // Makes the wave's 16 keys of a V tile finite; whether it changed any.
+    const int wg_pmin = p0 + t.tile * BM / a.group, wg_pmax = t.hi - 1;
+    // Makes the V rows that the wave copied finite; whether it changed any.
     auto clean = [&](int buf) {
-        u32x4 v[DP / 32];
+        constexpr int N = KW * DP * 2 / 1024;
+        u32x4 v[N];
         uint32_t bits = 0;
-        const uint32_t at = lds0 + buf * 2 * TB + TB + 16 * wave * DP * 2 + lane * 16;
+        const uint32_t at = lds0 + buf * 2 * TB + TB + KW * wave * DP * 2 + lane * 16;
 #pragma unroll
-        for (int j = 0; j < DP / 32; j++) {
+        for (int j = 0; j < N; j++) {
             v[j] = __builtin_bit_cast(u32x4, lds_read16(at + j * 1024));
             bits |= odd_bits(v[j]);
         }
         if (!__any(bits != 0)) return 0;
 #pragma unroll
-        for (int j = 0; j < DP / 32; j++)
+        for (int j = 0; j < N; j++)
             *reinterpret_cast<lds_u32x4*>(at + j * 1024) = finite_part(v[j]);
         return 1;
     };
@@ -1132,7 +1186,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
             if (page < 0) continue;
             const int64_t row = (((int64_t)page * a.Hk + h) << a.plog) + (j & ((1 << a.plog) - 1));
             const uint16_t* vp = static_cast<const uint16_t*>(a.vc) + row * a.D + 4 * H;
-            const bool sees = j <= prow && !(a.window && j <= prow - a.window);
+            const bool sees = j - (prow + 1 - (int)span) < span;
 #pragma unroll
             for (int d = 0; d < DB; d++)
 #pragma unroll
@@ -1147,32 +1201,51 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
         }
     };
 
-    if (first < last) {
-        begin(first, 0);
-        finish(0);
-        __syncthreads();
+    if constexpr (I8) {  // one tile ahead in registers
+        if (first < last) {
+            begin(first, 0);
+            finish(0);
+            __syncthreads();
+        }
         for (int kt = first; kt < last; kt++) {
             const int buf = (kt - first) & 1;
-            if (kt + 1 < last) begin(kt + 1, buf ^ 1);
-            bool odd = false;
-            if (!I8 && (kt * kTileKeys + kTileKeys - 1 > wg_pmin ||
-                        (a.window && kt * kTileKeys <= wg_pmax - a.window))) {
-                const int mine = clean(buf);
-                if (lane == 0) sh[wave] = mine;
-                __syncthreads();
-                odd = sh[0] | sh[1] | sh[2] | sh[3];
-            }
+            if (kt + 1 < last) begin(kt + 1, 0);
             compute(kt, buf);
-            if (!I8 && odd) restore(kt);
             if (kt + 1 < last) finish(buf ^ 1);
             __syncthreads();
+        }
+    } else {  // S - 1 tiles on their way
+        for (int i = 0; i < S - 1; i++)
+            if (first + i < last) begin(first + i, i);
+        int stage = 0, into = S - 1;
+        for (int kt = first; kt < last; kt++) {
+            // every wave's copies of this tile have landed, and the stage that the next
+            // copies go to has been read
+            if (kt + S - 1 <= last)
+                wait_copies<2 * NL * (S - 2)>();
+            else
+                wait_copies<0>();
+            barrier_all();
+            if (kt + S - 1 < last) begin(kt + S - 1, into);
+            bool odd = false;
+            if (kt * kTileKeys + kTileKeys - 1 > wg_pmin ||
+                (a.window && kt * kTileKeys <= wg_pmax - a.window)) {
+                const int mine = clean(stage);
+                if (lane == 0) sh[wave] = mine;
+                __syncthreads();
+                for (int w = 0; w < NW; w++) odd |= sh[w] != 0;
+            }
+            compute(kt, stage);
+            if (odd) restore(kt);
+            stage = stage + 1 == S ? 0 : stage + 1;
+            into = into + 1 == S ? 0 : into + 1;
         }
     }
 
     l += __shfl_xor(l, 32, 64);
     if (r >= t.rows) return;
     if (t.parts > 1) {
-        float* part = a.part + ((int64_t)index * a.splits + split) * tile_part<DP>();
+        float* part = a.part + ((int64_t)index * a.splits + split) * (BM * (DP + 2));
         const int pr = wave * 32 + col;
 #pragma unroll
         for (int d = 0; d < DB; d++)
@@ -1182,8 +1255,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
                 *reinterpret_cast<f32x4*>(part + pr * DP + 32 * d + 8 * e4 + 4 * H) = v;
             }
         if (H == 0) {
-            part[kTileRows * DP + pr] = m;
-            part[kTileRows * DP + kTileRows + pr] = l;
+            part[BM * DP + pr] = limit < 0.0f ? -kInf : m;
+            part[BM * DP + BM + pr] = l;
         }
         return;
     }
@@ -1209,7 +1282,8 @@ struct Plan {
     int64_t few;          // new tokens of a sequence that few_kernel takes at most
     bool use_few, use_tile;
     int64_t workers;      // of few_kernel
-    int64_t tiles;        // of 128 rows, at most
+    int waves;            // of tile_kernel: 32 rows each
+    int64_t tiles;        // of that many rows, at most
     int splits;
     int64_t joins, bytes;  // of the workspace: Join records, and the records and parts
 };
@@ -1232,7 +1306,10 @@ Plan plan_of(int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t B, int64_t mo
     const int64_t units = (max_context + 1 + kUnit - 1) / kUnit;
     p.workers = (B + 1 + T * group / (16 * p.rb)) * Hk * units;
     p.workers = p.workers < kWorkers ? p.workers : kWorkers;
-    p.tiles = T * group / kTileRows + B + 1;
+    // eight waves share a tile of keys where that leaves an item for every CU
+    p.waves = DP == 128 && T * group / 256 * Hk >= 256 ? 8 : 4;
+    const int rows_of = 32 * p.waves;
+    p.tiles = T * group / rows_of + B + 1;
     const int64_t items = p.tiles * Hk;
     p.splits = items >= 384 ? 1 : (int)(512 / items);
     if (p.splits > 16) p.splits = 16;
@@ -1241,7 +1318,7 @@ Plan plan_of(int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t B, int64_t mo
         p.bytes = p.workers * 2 * 16 * p.rb * (DP + 2) * 4;
     }
     if (p.use_tile && p.splits > 1) {
-        const int64_t b = items * p.splits * kTileRows * (DP + 2) * 4;
+        const int64_t b = items * p.splits * rows_of * (DP + 2) * 4;
         p.joins = p.joins > items ? p.joins : items;
         p.bytes = p.bytes > b ? p.bytes : b;
     }
@@ -1278,15 +1355,15 @@ int run_few(const Attn& a, int64_t workers, hipStream_t st) {
     return FNI8_OK;
 }
 
-template <int DP, bool I8>
+template <int DP, bool I8, int NW>
 int run_tile(const Attn& a, int64_t tiles, hipStream_t st) {
-    const auto kern = tile_kernel<DP, I8>;
-    constexpr int lds = tile_lds<DP, I8>();
+    const auto kern = tile_kernel<DP, I8, NW>;
+    constexpr int lds = tile_lds<DP, I8, NW>();
     const int rc = allow_lds(kern, lds);
     if (rc) return rc;
-    kern<<<dim3((uint32_t)(tiles * a.Hk * a.splits)), 256, lds, st>>>(a);
+    kern<<<dim3((uint32_t)(tiles * a.Hk * a.splits)), 64 * NW, lds, st>>>(a);
     if (a.splits > 1)
-        join_kernel<DP><<<dim3((uint32_t)(tiles * a.Hk), kTileRows / 4), 256, 0, st>>>(a, kTileRows);
+        join_kernel<DP><<<dim3((uint32_t)(tiles * a.Hk), 8 * NW), 256, 0, st>>>(a, 32 * NW);
     return FNI8_OK;
 }
 
@@ -1306,7 +1383,9 @@ int run_all(Attn a, const Plan& p, hipStream_t st) {
     }
     if (p.use_tile) {
         a.splits = a.part ? p.splits : 1;
-        return run_tile<DP, I8>(a, p.tiles, st);
+        if constexpr (DP == 128)
+            if (p.waves == 8) return run_tile<DP, I8, 8>(a, p.tiles, st);
+        return run_tile<DP, I8, 4>(a, p.tiles, st);
     }
     return FNI8_OK;
 }
@@ -1347,7 +1426,11 @@ int launch_paged_attention(const PagedAttention& p, hipStream_t st) {
     // a window that reaches past every key is none
     a.window = p.window > context ? 0 : (int)p.window;
     a.cap = (int)context + 1;
-    a.c = p.scale * 1.44269504088896340736f;
+    // a positive factor, so that the largest product is the largest exponent; a scale of 0
+    // stays one that makes every exponent 0, but 0 * -inf
+    a.c = __builtin_fabsf(p.scale) * 1.44269504088896340736f;
+    a.c = a.c > 1e-30f ? a.c : 1e-30f;
+    a.flip = p.scale < 0.0f ? 0x80008000u : 0;
     a.few = (int)plan.few;
     a.splits = 1;
     if (plan.bytes && p.work_bytes >= plan.bytes) {

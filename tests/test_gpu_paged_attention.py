@@ -81,6 +81,15 @@ def test_chunks(ops, cuda, new, old, Hq, Hk, D, page, int8):
     _check(ops, new, [a + b for a, b in zip(new, old)], Hq, Hk, D, page, int8, seed=D + len(new))
 
 
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("new,old,window", [([300], [277], None), ([130, 1, 200, 3], [0, 500, 65, 9], None),
+                                            ([260, 40], [100, 0], 70)])
+def test_chunks_of_many_heads(ops, cuda, new, old, window, int8):
+    """Enough rows for workgroups of eight waves."""
+    _check(ops, new, [a + b for a, b in zip(new, old)], 256, 32, 128, 32, int8, seed=len(new),
+           window=window)
+
+
 @pytest.mark.parametrize("window", [1, 2, 17, 64, 100, 5000])
 def test_window(ops, cuda, window):
     _check(ops, [1, 1, 1], [5, 300, 1200], 4, 2, 128, 16, window=window)
@@ -150,6 +159,7 @@ def test_values_of_later_tokens_stay_hidden(ops, cuda, new):
         cache[tables[0, at // 16], 1, at % 16, 5] = value
         got = _run(ops, q, (k, v, None, None, tables), lens, starts)
         cache[tables[0, at // 16], 1, at % 16, 5] = kept
+        # equal but for the sign of a zero
         assert torch.equal(got[:new // 2], clean[:new // 2])
         assert torch.equal(got[:, :2], clean[:, :2])  # the other key head
         hit = got[new // 2:, 2:]
@@ -220,6 +230,26 @@ def test_scale_argument_and_views(ops, cuda):
                               more.cuda()[:, 1:1 + tables.shape[1]], torch.tensor(lens).cuda(),
                               torch.tensor(starts).cuda(), scale=0.3)
     ref.within(got, want, tol)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.2, 3.0])
+@pytest.mark.parametrize("int8", [False, True])
+def test_any_scale(ops, cuda, scale, int8):
+    _check(ops, [1, 2], [300, 70], 4, 2, 128, 16, int8, scale=scale)
+    _check(ops, [90, 40], [150, 40], 4, 2, 64, 16, int8, scale=scale)
+
+
+@pytest.mark.parametrize("shift", [-300.0, 300.0])
+def test_scores_far_from_zero(ops, cuda, shift):
+    """Every key the same large part along the queries: exponents of hundreds, in one part
+    and in several."""
+    for new, lens in (([1, 1], [40, 5000]), ([150], [2000])):
+        starts = _starts(new)
+        q = _q(sum(new), 4, 64, 2)
+        k, v, _, _, tables = ref.paged(lens, 16, 2, 64, 3)
+        q[..., 0], k[..., 0] = 16.0, shift / 16.0
+        want, tol = ref.attention(q, k, v, tables, lens, starts, scale=1.0)
+        ref.within(_run(ops, q, (k, v, None, None, tables), lens, starts, scale=1.0), want, tol)
 
 
 def test_many_sequences(ops, cuda):
