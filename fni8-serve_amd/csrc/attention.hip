@@ -41,6 +41,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kInf = __builtin_inff();
 constexpr int kUnit = 128;      // keys of a unit of few_kernel: 32 for each of 4 waves
+constexpr int kTileRows = 128;  // of a workgroup of tile_kernel: 32 a wave
 constexpr int kTileKeys = 64;
 constexpr float kLag = 8.0f;
 constexpr int kWorkers = 768;  // of few_kernel at most: three a CU
@@ -98,7 +99,6 @@ __device__ __forceinline__ Seq sequence(const Attn& a, int s) {
 
 // ---- the list of items -----------------------------------------------------------
 
-template <int NW>
 __device__ __forceinline__ int block_scan(int v, int* sh, int& total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int incl = fni8::wave_incl_scan_i32(v, lane);
@@ -107,7 +107,7 @@ __device__ __forceinline__ int block_scan(int v, int* sh, int& total) {
     __syncthreads();
     total = 0;
 #pragma unroll
-    for (int w = 0; w < NW; w++) {
+    for (int w = 0; w < 4; w++) {
         if (w < wave) incl += sh[w];
         total += sh[w];
     }
@@ -117,7 +117,7 @@ __device__ __forceinline__ int block_scan(int v, int* sh, int& total) {
 // The sequence that holds unit `target(U)` of the list of all U = sum units(s), and the
 // number of units before it.  Every thread of the block gets the same answer, in scalar
 // registers; false where the target is not in the list.  sh: 16 words of LDS.
-template <int NW, class Units, class Target>
+template <class Units, class Target>
 __device__ __forceinline__ bool find(int nseq, int* sh, Units units, Target target, int& s_out,
                                      int& base_out, int& goal, Seq& q_out) {
     const int tid = threadIdx.x;
@@ -140,19 +140,19 @@ __device__ __forceinline__ bool find(int nseq, int* sh, Units units, Target targ
         return true;
     }
     if (tid == 0) sh[8] = -1;
-    for (int c = 0; c < nseq; c += 64 * NW) {
+    for (int c = 0; c < nseq; c += 256) {
         mine = c + tid < nseq ? units(c + tid, q) : 0;
-        incl = block_scan<NW>(mine, sh, total);
+        incl = block_scan(mine, sh, total);
         U += total;
     }
     U = __builtin_amdgcn_readfirstlane(U);  // wave-uniform from here on, in scalar registers
     goal = target(U);
     if (goal < 0 || goal >= U) return false;
     int base = 0;
-    for (int c = 0; c < nseq; c += 64 * NW) {
-        if (nseq > 64 * NW) {
+    for (int c = 0; c < nseq; c += 256) {
+        if (nseq > 256) {
             mine = c + tid < nseq ? units(c + tid, q) : 0;
-            incl = block_scan<NW>(mine, sh, total);
+            incl = block_scan(mine, sh, total);
         }
         const int before = base + incl - mine;
         // (sums that overflow, from a cu_seqlens that is not one, are no place)
@@ -278,6 +278,14 @@ __device__ __forceinline__ int page_of(const Attn& a, int s, int token, int lo, 
     return page < 0 || page >= a.num_pages ? kBad : page;
 }
 
+// 16 bytes that are read once.  Past the caches where ONCE: 64 sequences, 1 GB of 16 bits,
+// 189 -> 175 us; codes of 8 bits, whose lines two loads share, 49 -> 56.
+template <bool ONCE>
+__device__ __forceinline__ u32x4 stream(const char* p) {
+    const u32x4* q = reinterpret_cast<const u32x4*>(p);
+    return ONCE ? __builtin_nontemporal_load(q) : *q;
+}
+
 // ---- few rows ----------------------------------------------------------------------
 
 // LDS bytes of a wave: its V tile (32 keys), or its rows of o when they are joined
@@ -295,9 +303,9 @@ constexpr int few_part() {
     return 16 * RB * (DP + 2);
 }
 
-// Workgroups a CU, by the registers: codes of 8 bits take half as many on their way
-constexpr int few_waves(int dp, bool i8, int rb) {
-    return dp > 128 ? 1 : rb == 1 && (i8 || dp == 64) ? 3 : 2;
+// Workgroups a CU, by the registers
+constexpr int few_waves(int dp, int rb) {
+    return dp > 128 ? 1 : rb == 1 && dp == 64 ? 3 : 2;
 }
 
 // What few_kernel makes of a sequence: its range of keys and its units.
@@ -315,7 +323,7 @@ __device__ __forceinline__ FewSeq few_seq(const Attn& a, const Seq& q) {
     f.lo = a.window && first - a.window + 1 > 0 ? (first - a.window + 1) & ~31 : 0;
     f.tiles = (f.q.L - f.lo + kUnit - 1) / kUnit;
     f.tiles = f.tiles > 1 ? f.tiles : 1;
-    f.units = f.blocks * a.Hk * (a.whole ? 1 : f.tiles);
+    f.units = f.blocks * a.Hk * (a.whole ? 1 : f.tiles + 1);
     return f;
 }
 
@@ -324,7 +332,7 @@ __device__ __forceinline__ int per_worker(int U) {
 }
 
 template <int DP, bool I8, int RB>
-__global__ __launch_bounds__(256, few_waves(DP, I8, RB)) void few_kernel(Attn a) {
+__global__ __launch_bounds__(256, few_waves(DP, RB)) void few_kernel(Attn a) {
     constexpr int KS = DP / 32, DB = DP / 16;
     constexpr int KL = I8 ? DP / 64 : DP / 32, VL = KL;  // loads of 16 keys
     constexpr int CH = DP / 8;                           // chunks of a row in LDS
@@ -343,7 +351,7 @@ __global__ __launch_bounds__(256, few_waves(DP, I8, RB)) void few_kernel(Attn a)
     if (!a.whole && threadIdx.x == 0) a.joins[blockIdx.x].parts = 0;
     int s, base, u, upw = 0;
     Seq sq;
-    if (!find<4>(
+    if (!find(
             a.nseq, sh,
             [&](int i, Seq& q) {
                 q = sequence(a, i);
@@ -357,16 +365,19 @@ __global__ __launch_bounds__(256, few_waves(DP, I8, RB)) void few_kernel(Attn a)
         return;
     const int first_unit = u;
     FewSeq f = few_seq<RB>(a, sq);
-    int per_item = a.whole ? 1 : f.tiles;
+    int per_item = a.whole ? 1 : f.tiles + 1;
     int item = (u - base) / per_item, tile = (u - base) - item * per_item;
     int left = upw;
 
     while (true) {
+        // an item's last unit has no keys: it stands for the time of its beginning and end
         int nt = per_item - tile;
         nt = nt < left ? nt : left;
-        const bool full = nt == per_item;
+        const int real = a.whole || nt < f.tiles - tile ? nt : f.tiles - tile;
+        const bool full = a.whole || real == f.tiles;
+        if (real > 0) {
         const int h = item % a.Hk, rb = item / a.Hk;
-        const int steps = a.whole ? f.tiles : nt;
+        const int steps = a.whole ? f.tiles : real;
         const int row0 = rb * 16 * RB;
         const int nrows = f.rows - row0 < 16 * RB ? f.rows - row0 : 16 * RB;
         const int lo = a.window && f.q.L - f.q.n - a.window + 1 > 0 ? f.q.L - f.q.n - a.window + 1 : 0;
@@ -443,11 +454,9 @@ __global__ __launch_bounds__(256, few_waves(DP, I8, RB)) void few_kernel(Attn a)
                 }
                 if (a.D == DP && (I8 || (tok >= lo && tok + 16 <= hi))) {
 #pragma unroll
-                    for (int j = 0; j < KL; j++)
-                        kr[tb][j] = *reinterpret_cast<const u32x4*>(kp + k_off + 64 * j);
+                    for (int j = 0; j < KL; j++) kr[tb][j] = stream<!I8>(kp + k_off + 64 * j);
 #pragma unroll
-                    for (int j = 0; j < VL; j++)
-                        vr[tb][j] = *reinterpret_cast<const u32x4*>(vp + 16 * lane + 1024 * j);
+                    for (int j = 0; j < VL; j++) vr[tb][j] = stream<!I8>(vp + 16 * lane + 1024 * j);
                 } else {
 #pragma unroll
                     for (int j = 0; j < KL; j++)
@@ -698,9 +707,10 @@ __global__ __launch_bounds__(256, few_waves(DP, I8, RB)) void few_kernel(Attn a)
             }
         }
         if (!full && tile == 0 && threadIdx.x == 0) {  // this run begins an item, others end it
-            const int w0 = blockIdx.x, w1 = (u + per_item - 1) / upw;
+            const int w0 = blockIdx.x, w1 = (u + f.tiles - 1) / upw;
             a.joins[w0] = Join{w1 - w0 + 1, 2 * w0 + (first_unit == u ? 0 : 1), 2 * w0 + 2, 2,
                                f.q.start, row0, nrows, h};
+        }
         }
         left -= nt;
         u += nt;
@@ -712,7 +722,7 @@ __global__ __launch_bounds__(256, few_waves(DP, I8, RB)) void few_kernel(Attn a)
                 f = few_seq<RB>(a, sequence(a, s));
             } while (f.units == 0);
             item = 0;
-            per_item = a.whole ? 1 : f.tiles;
+            per_item = a.whole ? 1 : f.tiles + 1;
         }
         __syncthreads();  // the rows of o have been read
     }
@@ -724,58 +734,94 @@ template <int DP>
 __global__ __launch_bounds__(256) void join_kernel(Attn a, int part_rows) {
     constexpr int LP = DP / 4, NG = 64 / LP;  // lanes of a part, parts at a time
     const Join j = a.joins[blockIdx.x];
-    const int lane = threadIdx.x & 63, r = blockIdx.y * 4 + (threadIdx.x >> 6);
-    if (r >= j.nrows || j.parts == 0) return;
+    if (j.parts == 0) return;
+    const int lane = threadIdx.x & 63;
     const int64_t size = (int64_t)part_rows * (DP + 2);
     const int d4 = lane % LP, grp = lane / LP;
     auto slot = [&](int p) {
         return a.part + size * (p == 0 ? j.first : j.next + (p - 1) * j.step);
     };
-    float top = -kInf, sum = 0.0f;
-    f32x4 acc = {0, 0, 0, 0};
-    for (int c = 0; c < j.parts; c += 64) {
-        const int n = j.parts - c < 64 ? j.parts - c : 64;
-        float m = -kInf, l = 0.0f;
-        if (lane < n) {
-            const float* p = slot(c + lane) + part_rows * DP;
-            m = p[r];
-            l = p[part_rows + r];
-        }
-        float t = __builtin_fmaxf(top, m);
-        t = max_xor32(max_xor16(t));
-#pragma unroll
-        for (int x = 8; x > 0; x >>= 1) t = __builtin_fmaxf(t, __shfl_xor(t, x, 64));
-        const float at = t == -kInf ? 0.0f : t;
-        const float keep = exp2_(top - at), w = exp2_(m - at);
-        acc *= keep;
-        float wl = w * l;
-#pragma unroll
-        for (int x = 32; x > 0; x >>= 1) wl += __shfl_xor(wl, x, 64);
-        sum = sum * keep + wl;
-        top = t;
-        constexpr int U = 8;
-        for (int i = 0; i < n; i += U * NG) {
-            f32x4 v[U];
-#pragma unroll
-            for (int k = 0; k < U; k++) {
-                const int p = i + k * NG + grp;
-                v[k] = f32x4{0, 0, 0, 0};
-                if (p < n) v[k] = *reinterpret_cast<const f32x4*>(slot(c + p) + r * DP + 4 * d4);
+    for (int r = blockIdx.y * 4 + (threadIdx.x >> 6); r < j.nrows; r += 4 * gridDim.y) {
+        float top = -kInf, sum = 0.0f;
+        f32x4 acc = {0, 0, 0, 0};
+        for (int c = 0; c < j.parts; c += 64) {
+            const int n = j.parts - c < 64 ? j.parts - c : 64;
+            float m = -kInf, l = 0.0f;
+            if (lane < n) {
+                const float* p = slot(c + lane) + part_rows * DP;
+                m = p[r];
+                l = p[part_rows + r];
             }
+            float t = __builtin_fmaxf(top, m);
+            t = max_xor32(max_xor16(t));
 #pragma unroll
-            for (int k = 0; k < U; k++) acc += __shfl(w, (i + k * NG + grp) & 63, 64) * v[k];
+            for (int x = 8; x > 0; x >>= 1) t = __builtin_fmaxf(t, __shfl_xor(t, x, 64));
+            const float at = t == -kInf ? 0.0f : t;
+            const float keep = exp2_(top - at), w = exp2_(m - at);
+            acc *= keep;
+            float wl = w * l;
+#pragma unroll
+            for (int x = 32; x > 0; x >>= 1) wl += __shfl_xor(wl, x, 64);
+            sum = sum * keep + wl;
+            top = t;
+            constexpr int U = 8;
+            for (int i = 0; i < n; i += U * NG) {
+                f32x4 v[U];
+#pragma unroll
+                for (int k = 0; k < U; k++) {
+                    const int p = i + k * NG + grp;
+                    v[k] = f32x4{0, 0, 0, 0};
+                    if (p < n) v[k] = *reinterpret_cast<const f32x4*>(slot(c + p) + r * DP + 4 * d4);
+                }
+#pragma unroll
+                for (int k = 0; k < U; k++) acc += __shfl(w, (i + k * NG + grp) & 63, 64) * v[k];
+            }
         }
+#pragma unroll
+        for (int x = 32; x >= LP; x >>= 1)
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[e] += __shfl_xor(acc[e], x, 64);
+        if (grp != 0 || 4 * d4 >= a.D) continue;
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const int rr = j.row0 + r, i = rr / a.group, head = j.h * a.group + rr - i * a.group;
+        uint2 y = {pack2(acc[0] * inv, acc[1] * inv), pack2(acc[2] * inv, acc[3] * inv)};
+        if (sum == 0.0f) y = uint2{0, 0};
+        *reinterpret_cast<uint2*>(a.out + ((int64_t)(j.start + i) * a.Hq + head) * a.D + 4 * d4) = y;
     }
-#pragma unroll
-    for (int x = 32; x >= LP; x >>= 1)
-#pragma unroll
-        for (int e = 0; e < 4; e++) acc[e] += __shfl_xor(acc[e], x, 64);
-    if (grp != 0 || 4 * d4 >= a.D) return;
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const int rr = j.row0 + r, i = rr / a.group, head = j.h * a.group + rr - i * a.group;
-    uint2 y = {pack2(acc[0] * inv, acc[1] * inv), pack2(acc[2] * inv, acc[3] * inv)};
-    if (sum == 0.0f) y = uint2{0, 0};
-    *reinterpret_cast<uint2*>(a.out + ((int64_t)(j.start + i) * a.Hq + head) * a.D + 4 * d4) = y;
+}
+
+// The same for the many rows and few parts of tile_kernel's items: DP / 4 lanes a row, 32
+// rows a workgroup.  (A wave a row spends its time on the exchange of the weights: 45 us of
+// 76 for 480 items of two parts.)
+template <int DP>
+__global__ __launch_bounds__(256) void join_tile_kernel(Attn a) {
+    constexpr int LP = DP / 4, RP = 256 / LP;  // lanes of a row, rows at a time
+    const Join j = a.joins[blockIdx.x];
+    if (j.parts == 0) return;
+    const int d4 = threadIdx.x % LP;
+    if (4 * d4 >= a.D) return;
+    const float* parts = a.part + (int64_t)j.first * (kTileRows * (DP + 2));
+    for (int r = blockIdx.y * 32 + threadIdx.x / LP; r < (int)blockIdx.y * 32 + 32 && r < j.nrows;
+         r += RP) {
+        float top = -kInf, sum = 0.0f;
+        f32x4 acc = {0, 0, 0, 0};
+#pragma unroll 4
+        for (int p = 0; p < j.parts; p++)
+            top = __builtin_fmaxf(top, parts[p * (kTileRows * (DP + 2)) + kTileRows * DP + r]);
+        const float at = top == -kInf ? 0.0f : top;
+#pragma unroll 4
+        for (int p = 0; p < j.parts; p++) {
+            const float* part = parts + p * (kTileRows * (DP + 2));
+            const float k = exp2_(part[kTileRows * DP + r] - at);
+            sum += k * part[kTileRows * (DP + 1) + r];
+            acc += k * *reinterpret_cast<const f32x4*>(part + r * DP + 4 * d4);
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const int rr = j.row0 + r, i = rr / a.group, head = j.h * a.group + rr - i * a.group;
+        uint2 y = {pack2(acc[0] * inv, acc[1] * inv), pack2(acc[2] * inv, acc[3] * inv)};
+        if (sum == 0.0f) y = uint2{0, 0};
+        *reinterpret_cast<uint2*>(a.out + ((int64_t)(j.start + i) * a.Hq + head) * a.D + 4 * d4) = y;
+    }
 }
 
 // ---- tiles of 128 rows -------------------------------------------------------------
@@ -817,13 +863,11 @@ __device__ __forceinline__ void copy16_s(uint32_t lds, const void* base, uint32_
 __device__ const uint4 kZeros = {0, 0, 0, 0};
 __device__ const uint4 kNaNs = {0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u};
 
-// Stages of K and V tiles: as many as fit where the copies need no registers
-constexpr int tile_stages(int dp, bool i8, int nw) {
-    return i8 || dp == 256 || (dp == 128 && nw == 4) ? 2 : 4;
-}
-template <int DP, bool I8, int NW>
+// Stages of K and V tiles: two workgroups a CU share its LDS at 128 elements, three at 64
+constexpr int tile_stages(int dp, bool i8) { return dp == 64 && !i8 ? 3 : 2; }
+template <int DP, bool I8>
 constexpr int tile_lds() {
-    return tile_stages(DP, I8, NW) * 2 * kTileKeys * DP * 2 + (I8 ? 2 * 3 * kTileKeys * 4 : 0) + 64;
+    return tile_stages(DP, I8) * 2 * kTileKeys * DP * 2 + (I8 ? 2 * 3 * kTileKeys * 4 : 0) + 64;
 }
 
 // The item of a workgroup of tile_kernel.
@@ -834,22 +878,20 @@ struct TileItem {
 
 // Tiles of all sequences from the last to the first: a causal tile's keys grow with its
 // rows, and the longest ones begin first.
-template <int NW>
 __device__ __forceinline__ bool tile_item(const Attn& a, int id, int h, int* sh, TileItem& t) {
-    constexpr int BM = 32 * NW;
     auto tiles = [&](int s, Seq& q) {
         q = sequence(a, s);
         return q.n > a.few
-                   ? (int)(((int64_t)q.n * a.group + BM - 1) / BM) : 0;
+                   ? (int)(((int64_t)q.n * a.group + kTileRows - 1) / kTileRows) : 0;
     };
     int base, goal;
-    if (!find<NW>(a.nseq, sh, tiles, [&](int N) { return N - 1 - id; }, t.s, base, goal, t.q))
+    if (!find(a.nseq, sh, tiles, [&](int N) { return N - 1 - id; }, t.s, base, goal, t.q))
         return false;
     t.rows = t.q.n * a.group;
     t.tile = goal - base;
     t.h = h;
-    const int i0 = t.tile * BM / a.group;
-    int i1 = (t.tile * BM + BM - 1) / a.group;
+    const int i0 = t.tile * kTileRows / a.group;
+    int i1 = (t.tile * kTileRows + kTileRows - 1) / a.group;
     i1 = i1 < t.q.n ? i1 : t.q.n - 1;
     const int p0 = t.q.L - t.q.n;
     t.hi = p0 + i1 + 1 > 0 ? p0 + i1 + 1 : 0;
@@ -863,10 +905,10 @@ __device__ __forceinline__ bool tile_item(const Attn& a, int id, int h, int* sh,
     return true;
 }
 
-template <int DP, bool I8, int NW>
-__global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
-    constexpr int BM = 32 * NW, KW = kTileKeys / NW;  // rows of a workgroup, keys a wave copies
-    constexpr int S = tile_stages(DP, I8, NW);
+template <int DP, bool I8>
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
+    constexpr int KW = kTileKeys / 4;  // keys that a wave copies
+    constexpr int S = tile_stages(DP, I8);
     constexpr int KS = DP / 16, DB = DP / 32, CH = DP / 8;
     constexpr int TB = kTileKeys * DP * 2;  // bytes of a K or V tile
     constexpr int NL = KW * DP * (I8 ? 1 : 2) / 1024;  // copies of a wave and tile, K or V
@@ -875,28 +917,28 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void tile_kernel(Attn a
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, H = lane >> 5;
     float* scales = reinterpret_cast<float*>(smem + 2 * S * TB);  // [2][3][64]
-    int* sh = reinterpret_cast<int*>(smem + tile_lds<DP, I8, NW>() - 64);
+    int* sh = reinterpret_cast<int*>(smem + tile_lds<DP, I8>() - 64);
 
     // a key head's items are neighbours modulo the heads: with the round-robin dispatch
     // over the 8 XCDs they share an L2 where the heads divide 8
     const int h = blockIdx.x % a.Hk, rest = blockIdx.x / a.Hk;
     const int split = rest % a.splits;
     TileItem t{};
-    const bool found = tile_item<NW>(a, rest / a.splits, h, sh, t);
+    const bool found = tile_item(a, rest / a.splits, h, sh, t);
     const int index = rest / a.splits * a.Hk + h;
     if (a.splits > 1 && split == 0 && threadIdx.x == 0) {
-        const int tile_row0 = t.tile * BM;
+        const int tile_row0 = t.tile * kTileRows;
         Join j{0, 0, 0, 0, 0, 0, 0, 0};
         if (found && t.parts > 1)
             j = Join{t.parts, index * a.splits, index * a.splits + 1, 1, t.q.start, tile_row0,
-                     t.rows - tile_row0 < BM ? t.rows - tile_row0 : BM, h};
+                     t.rows - tile_row0 < kTileRows ? t.rows - tile_row0 : kTileRows, h};
         a.joins[index] = j;
     }
     if (!found || split >= t.parts) return;
     const int first = t.kt0 + split * t.per;
     const int last = first + t.per < t.kt1 ? first + t.per : t.kt1;
 
-    const int row0 = t.tile * BM + wave * 32;
+    const int row0 = t.tile * kTileRows + wave * 32;
     const int p0 = t.q.L - t.q.n;
     const int nrows = t.rows - row0 < 32 ? t.rows - row0 : 32;  // may be 0 or less
     const int pmin = p0 + row0 / a.group;
@@ -912,9 +954,18 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void tile_kernel(Attn a
             v = *reinterpret_cast<const u32x4*>(a.q + (t.q.start + qi) * a.ldq + head * a.hsq +
                                                 16 * k + 8 * H);
         v ^= a.flip;
-        asm volatile("" : "+v"(v));  // waited for here, not in the loop among the copies
         q[k] = __builtin_bit_cast(h8, v);
     }
+    // the queries, asked for before the first copies, waited for behind them and not in the
+    // loop, where a wait for a load is one for every copy
+    auto queries_landed = [&] {
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            u32x4 v = __builtin_bit_cast(u32x4, q[k]);
+            asm volatile("" : "+v"(v));
+            q[k] = __builtin_bit_cast(h8, v);
+        }
+    };
 
     // the row sees the keys j with prow - span < j <= prow: one unsigned comparison
     const uint32_t span = prow < 0 ? 0 : a.window ? a.window : prow + 1;
@@ -938,35 +989,87 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void tile_kernel(Attn a
         const int dd = 32 * d + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
         v_addr[d] = lds0 + TB + tk * DP * 2 + 16 * ((dd >> 3) ^ v_swz(tk)) + 2 * (dd & 7);
     }
-    // byte offsets of the wave's copies from its first row's
-    uint32_t k_off[I8 ? 1 : NL], v_off = 0;
-    if constexpr (!I8) {
+    // Byte offsets of the wave's copies (16 bits) from its first row; elements past the head's
+    // are zeros in K, and in V, where they only reach sums that nobody reads, the row's first.
+    uint32_t k_off[I8 ? 1 : NL], v_off[I8 ? 1 : NL], k_pad = 0;
+    if constexpr (!I8)
 #pragma unroll
         for (int j = 0; j < NL; j++) {
-            const int c = j * 64 + lane, k = c / CH, in = c % CH;
-            k_off[j] = (k * DP + 8 * (in ^ k_swz(KW * wave + k))) * 2;
+            const int c = j * 64 + lane, k = c / CH;
+            const int dk = 8 * (c % CH ^ k_swz(KW * wave + k)), dv = 8 * (c % CH ^ v_swz(KW * wave + k));
+            k_off[j] = (k * a.D + dk) * 2;
+            v_off[j] = (k * a.D + (dv < a.D ? dv : 0)) * 2;
+            if (dk >= a.D) k_pad |= 1u << j;
         }
-        v_off = (lane / CH * DP + 8 * (lane % CH ^ v_swz(lane / CH))) * 2;
-    }
-    // copy j takes the next 1024 bytes; rows of 512 bytes change the permutation with it
-    auto v_off_of = [&](int j) { return (DP == 256 && (j & 1) ? v_off ^ 128 : v_off) + j * 1024; };
 
-    int pages = 0;  // lane j: the page of the wave's keys of tile (kt & ~63) + j, from `first`
-    u32x4 kr[I8 ? NL : 1], vr[I8 ? NL : 1];
-    float ksr = 0.0f, vsr = 1.0f;
-    auto begin = [&](int kt, int buf) {
+    // Lane j: where the wave's rows of tile j of the 64 ahead begin in the caches (elements).
+    // whole: the tiles whose rows all lie in the range and on a page of the cache.
+    int64_t rows_ahead = 0;
+    uint64_t whole = 0;
+    struct Rows {
+        int64_t row;
+        bool whole;
+    };
+    auto rows_of = [&](int kt) {
         const int i = kt - first;
         if ((i & 63) == 0) {
-            pages = kt + lane < last ? page_of(a, t.s, (kt + lane) * kTileKeys + (KW * wave & ~15),
-                                               t.lo, t.hi)
-                                     : kNone;
-            asm volatile("" : "+v"(pages));  // waited for here
+            const int tok = (kt + lane) * kTileKeys + KW * wave;
+            const int page = kt + lane < last ? page_of(a, t.s, tok & ~15, t.lo, t.hi) : kNone;
+            rows_ahead = (((int64_t)(page < 0 ? 0 : page) * a.Hk + h) << a.plog) +
+                         (tok & ((1 << a.plog) - 1));
+            whole = __ballot(page >= 0 && tok >= t.lo && tok + KW <= t.hi);
         }
-        const int page = __builtin_amdgcn_readlane(pages, i & 63);
+        Rows r;
+        const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)rows_ahead, i & 63);
+        const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(rows_ahead >> 32), i & 63);
+        r.row = (int64_t)((uint64_t)hi << 32 | lo);
+        r.whole = whole >> (i & 63) & 1;
+        return r;
+    };
+    u32x4 kr[I8 ? NL : 1], vr[I8 ? NL : 1];
+    float ksr = 0.0f, vsr = 1.0f;
+    // Begins the copies of the wave's rows of a K or V tile (16 bits).
+    auto copy_keys = [&](int kt, int stage, Rows r) {
+        const uint32_t to = lds0 + stage * 2 * TB + KW * wave * DP * 2;
+        const char* p = static_cast<const char*>(scalar(static_cast<const uint16_t*>(a.kc) + r.row * a.D));
+        if (r.whole && a.D == DP) {
+#pragma unroll
+            for (int j = 0; j < NL; j++) copy16_s(to + j * 1024, p, k_off[j]);
+            return;
+        }
+        const int page = r.whole ? 0 : page_of(a, t.s, (kt * kTileKeys + KW * wave) & ~15, t.lo, t.hi);
+#pragma unroll
+        for (int j = 0; j < NL; j++) {
+            const bool pad = k_pad >> j & 1;
+            const void* src = p + k_off[j];
+            if (pad || page < 0) src = page == kBad && !pad ? &kNaNs : &kZeros;
+            copy16(to + j * 1024, src);
+        }
+    };
+    auto copy_values = [&](int kt, int stage, Rows r) {
+        const uint32_t to = lds0 + stage * 2 * TB + TB + KW * wave * DP * 2;
+        const char* p = static_cast<const char*>(scalar(static_cast<const uint16_t*>(a.vc) + r.row * a.D));
+        if (r.whole) {
+#pragma unroll
+            for (int j = 0; j < NL; j++) copy16_s(to + j * 1024, p, v_off[j]);
+            return;
+        }
         const int tok = kt * kTileKeys + KW * wave;
-        const int64_t row = (((int64_t)(page < 0 ? 0 : page) * a.Hk + h) << a.plog) +
-                            (tok & ((1 << a.plog) - 1));
+        const int page = page_of(a, t.s, tok & ~15, t.lo, t.hi);
+#pragma unroll
+        for (int j = 0; j < NL; j++) {
+            const int k = (j * 64 + lane) / CH;
+            const void* src = p + v_off[j];
+            // what lies outside the range may be anything, and 0 * NaN is NaN
+            if (page < 0 || tok + k >= t.hi || tok + k < t.lo) src = &kZeros;
+            copy16(to + j * 1024, src);
+        }
+    };
+    auto begin = [&](int kt, int stage) {
+        const Rows rw = rows_of(kt);
         if constexpr (I8) {
+            const int64_t row = rw.row;
+            const int page = rw.whole ? 0 : page_of(a, t.s, (kt * kTileKeys + KW * wave) & ~15, t.lo, t.hi);
 #pragma unroll
             for (int j = 0; j < NL; j++) {
                 const int c = j * 64 + lane, k = c / (DP / 16), d = 16 * (c % (DP / 16));
@@ -984,28 +1087,8 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void tile_kernel(Attn a
                 vsr = a.vs[row + lane % KW];
             }
         } else {
-            const uint32_t kd = lds0 + buf * 2 * TB + KW * wave * DP * 2;
-            if (page >= 0 && a.D == DP && tok >= t.lo && tok + KW <= t.hi) {
-                const void* kp = scalar(static_cast<const uint16_t*>(a.kc) + row * DP);
-                const void* vp = scalar(static_cast<const uint16_t*>(a.vc) + row * DP);
-#pragma unroll
-                for (int j = 0; j < NL; j++) copy16_s(kd + j * 1024, kp, k_off[j]);
-#pragma unroll
-                for (int j = 0; j < NL; j++) copy16_s(kd + TB + j * 1024, vp, v_off_of(j));
-                return;
-            }
-#pragma unroll
-            for (int j = 0; j < NL; j++) {
-                const int c = j * 64 + lane, k = c / CH, in = c % CH;
-                const int dk = 8 * (in ^ k_swz(KW * wave + k)), dv = 8 * (in ^ v_swz(KW * wave + k));
-                const void* ks = static_cast<const uint16_t*>(a.kc) + (row + k) * a.D + dk;
-                const void* vs = static_cast<const uint16_t*>(a.vc) + (row + k) * a.D + dv;
-                if (page < 0 || dk >= a.D) ks = page == kBad && dk < a.D ? &kNaNs : &kZeros;
-                // what lies outside the range may be anything, and 0 * NaN is NaN
-                if (page < 0 || dv >= a.D || tok + k >= t.hi || tok + k < t.lo) vs = &kZeros;
-                copy16(kd + j * 1024, ks);
-                copy16(kd + TB + j * 1024, vs);
-            }
+            copy_keys(kt, stage, rw);
+            copy_values(kt, stage, rw);
         }
     };
     auto finish = [&](int buf) {
@@ -1042,41 +1125,54 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void tile_kernel(Attn a
 #pragma unroll
         for (int e = 0; e < 16; e++) o[d][e] = 0.0f;
 
-    auto compute = [&](int kt, int buf) {
+    // A tile is computed in three steps: the products S^T = K Q^T, the weights, and the
+    // products with the values.  A wave skips tiles that none of its rows sees.
+    f32x16 s[2];
+    h8 p[4];
+    auto active = [&](int kt) {
         const int t0 = kt * kTileKeys;
-        if (t0 > pmax || (a.window && t0 + kTileKeys - 1 <= pmin - a.window)) return;
-        const float* sc = scales + buf * 3 * kTileKeys;
-        uint32_t ka[KA], va[VA];
+        return t0 <= pmax && !(a.window && t0 + kTileKeys - 1 <= pmin - a.window);
+    };
+    constexpr int kArithmetic = 0x6;  // what passes a scheduling barrier: reads and products do not
+    uint32_t ka[KA], va[VA];
+    auto at_stage = [&](int stage, uint32_t (&out)[KA], const uint32_t (&from)[KA]) {
 #pragma unroll
         for (int i = 0; i < KA; i++) {
-            ka[i] = k_addr[i] + buf * 2 * TB;
-            asm volatile("" : "+v"(ka[i]));  // what follows is in the reads' constants
+            out[i] = from[i] + stage * 2 * TB;
+            asm volatile("" : "+v"(out[i]));  // what follows is in the reads' constants
         }
+    };
+    auto v_at_stage = [&](int stage) {
 #pragma unroll
         for (int d = 0; d < VA; d++) {
-            va[d] = v_addr[d] + buf * 2 * TB;
+            va[d] = v_addr[d] + stage * 2 * TB;
             asm volatile("" : "+v"(va[d]));
         }
-        f32x16 s[2];
+    };
+    // Fragment i of 2 KS: 16 elements of 32 keys.  Four are read ahead of their products.
+    h8 kf[4];
+    auto key_fragment = [&](int i) {
+        return lds_read16(ka[(i >> 1) % KA] + 32 * (i & 1) * DP * 2 + (i >> 1) / KA * 256);
+    };
+    auto first_keys = [&] {
+#pragma unroll
+        for (int i = 0; i < 4; i++) kf[i] = key_fragment(i);
+    };
+    auto scores = [&] {
 #pragma unroll
         for (int tb = 0; tb < 2; tb++)
 #pragma unroll
             for (int e = 0; e < 16; e++) s[tb][e] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < KS; i++)
-#pragma unroll
-            for (int tb = 0; tb < 2; tb++)
-                s[tb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-                    lds_read16(ka[i % KA] + 32 * tb * DP * 2 + i / KA * 256), q[i], s[tb], 0, 0, 0);
-        // four fragments ahead of the product that uses them
-        constexpr int kDs = 0x100, kMfma = 0x8;
-        __builtin_amdgcn_sched_group_barrier(kDs, 4, 0);
-#pragma unroll
-        for (int i = 0; i < 2 * KS - 4; i++) {
-            __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(kDs, 1, 0);
+        for (int i = 0; i < 2 * KS; i++) {
+            s[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i & 3], q[i >> 1], s[i & 1], 0, 0, 0);
+            if (i + 4 < 2 * KS) kf[i & 3] = key_fragment(i + 4);
+            __builtin_amdgcn_sched_barrier(kArithmetic);
         }
-        __builtin_amdgcn_sched_group_barrier(kMfma, 4, 0);
+    };
+    auto weights = [&](int kt, int buf) {
+        const int t0 = kt * kTileKeys;
+        const float* sc = scales + buf * 3 * kTileKeys;
         // element e of block tb is key 32 tb + 8 (e / 4) + 4 H + e % 4: its exponent
 #pragma unroll
         for (int tb = 0; tb < 2; tb++)
@@ -1123,7 +1219,6 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void tile_kernel(Attn a
             m += up;
             if (top > limit) limit = kLag;
         }
-        h8 p[4];
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             float w[8];
@@ -1146,20 +1241,56 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void tile_kernel(Attn a
                               pack2(w[6], w[7])};
             p[k] = __builtin_bit_cast(h8, pk);
         }
-        // value fragment of 32 elements (block d) and keys 16 k + {4 H .., 8 + 4 H ..}
-        auto value = [&](int d, int k) {
-            const uint32_t at = va[d % VA] + 16 * k * DP * 2 + d / VA * 256;
-            return lds_read_tr(at, at + 8 * DP * 2);
-        };
+    };
+    // Fragments of V: block d of 32 elements, keys 16 k + {4 H .., 8 + 4 H ..}, in groups of
+    // up to four blocks.  Two groups are read ahead of their products.
+    constexpr int GD = DB < 4 ? DB : 4, GK = DB / GD;  // blocks of a group, groups of 16 keys
+    h8 vf[2][GD];
+    auto value_group = [&](int g) {
 #pragma unroll
-        for (int k = 0; k < 4; k++)
+        for (int i = 0; i < GD; i++) {
+            const uint32_t at = va[i] + 16 * (g / GK) * DP * 2 + g % GK * 256;
+            vf[g & 1][i] = lds_read_tr(at, at + 8 * DP * 2);
+        }
+    };
+    auto first_values = [&](int stage) {
+        v_at_stage(stage);
+        value_group(0);
+        value_group(1);
+    };
+    auto values = [&](auto ahead) {
 #pragma unroll
-            for (int d = 0; d < DB; d++)
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(value(d, k), p[k], o[d], 0, 0, 0);
+        for (int g = 0; g < 4 * GK; g++) {
+#pragma unroll
+            for (int i = 0; i < GD; i++) {
+                f32x16& acc = o[g % GK * GD + i];
+                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[g & 1][i], p[g / GK], acc, 0, 0, 0);
+            }
+            __builtin_amdgcn_sched_barrier(kArithmetic);
+            if (g + 2 < 4 * GK) value_group(g + 2);
+            if (g + 2 == 4 * GK) ahead();
+            __builtin_amdgcn_sched_barrier(kArithmetic);
+        }
+    };
+    auto compute = [&](int kt, int stage) {
+        if (!active(kt)) return;
+        at_stage(stage, ka, k_addr);
+        first_keys();
+        scores();
+        // (where the registers allow it, on their way while the weights are computed)
+        constexpr bool early = !I8 && DP <= 128;
+        if constexpr (early) first_values(stage);
+        weights(kt, stage);
+        if constexpr (!early) first_values(stage);
+        values([] {});
     };
 
     // What lies at the edge of some row of the workgroup (the same for its four waves).
-    const int wg_pmin = p0 + t.tile * BM / a.group, wg_pmax = t.hi - 1;
+    const int wg_pmin = p0 + t.tile * kTileRows / a.group, wg_pmax = t.hi - 1;
+    auto at_edge = [&](int kt) {
+        return kt * kTileKeys + kTileKeys - 1 > wg_pmin ||
+               (a.window && kt * kTileKeys <= wg_pmax - a.window);
+    };
     // Makes the V rows that the wave copied finite; whether it changed any.
     auto clean = [&](int buf) {
         constexpr int N = KW * DP * 2 / 1024;
@@ -1205,6 +1336,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void tile_kernel(Attn a
         if (first < last) {
             begin(first, 0);
             finish(0);
+            queries_landed();
             __syncthreads();
         }
         for (int kt = first; kt < last; kt++) {
@@ -1217,6 +1349,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void tile_kernel(Attn a
     } else {  // S - 1 tiles on their way
         for (int i = 0; i < S - 1; i++)
             if (first + i < last) begin(first + i, i);
+        queries_landed();
         int stage = 0, into = S - 1;
         for (int kt = first; kt < last; kt++) {
             // every wave's copies of this tile have landed, and the stage that the next
@@ -1228,12 +1361,11 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void tile_kernel(Attn a
             barrier_all();
             if (kt + S - 1 < last) begin(kt + S - 1, into);
             bool odd = false;
-            if (kt * kTileKeys + kTileKeys - 1 > wg_pmin ||
-                (a.window && kt * kTileKeys <= wg_pmax - a.window)) {
+            if (at_edge(kt)) {
                 const int mine = clean(stage);
                 if (lane == 0) sh[wave] = mine;
                 __syncthreads();
-                for (int w = 0; w < NW; w++) odd |= sh[w] != 0;
+                for (int w = 0; w < 4; w++) odd |= sh[w] != 0;
             }
             compute(kt, stage);
             if (odd) restore(kt);
@@ -1245,7 +1377,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void tile_kernel(Attn a
     l += __shfl_xor(l, 32, 64);
     if (r >= t.rows) return;
     if (t.parts > 1) {
-        float* part = a.part + ((int64_t)index * a.splits + split) * (BM * (DP + 2));
+        float* part = a.part + ((int64_t)index * a.splits + split) * (kTileRows * (DP + 2));
         const int pr = wave * 32 + col;
 #pragma unroll
         for (int d = 0; d < DB; d++)
@@ -1255,8 +1387,8 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void tile_kernel(Attn a
                 *reinterpret_cast<f32x4*>(part + pr * DP + 32 * d + 8 * e4 + 4 * H) = v;
             }
         if (H == 0) {
-            part[BM * DP + pr] = limit < 0.0f ? -kInf : m;
-            part[BM * DP + BM + pr] = l;
+            part[kTileRows * DP + pr] = limit < 0.0f ? -kInf : m;
+            part[kTileRows * DP + kTileRows + pr] = l;
         }
         return;
     }
@@ -1281,9 +1413,9 @@ struct Plan {
     int rb;               // 16-row blocks of few_kernel's rows
     int64_t few;          // new tokens of a sequence that few_kernel takes at most
     bool use_few, use_tile;
+    int64_t most_rows;    // of a sequence in few_kernel that keeps to the bound
     int64_t workers;      // of few_kernel
-    int waves;            // of tile_kernel: 32 rows each
-    int64_t tiles;        // of that many rows, at most
+    int64_t tiles;        // of kTileRows rows, at most
     int splits;
     int64_t joins, bytes;  // of the workspace: Join records, and the records and parts
 };
@@ -1293,12 +1425,13 @@ int64_t join_bytes(int64_t n) { return (n * (int64_t)sizeof(Join) + 255) & ~(int
 int padded_dim(int64_t D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
 Plan plan_of(int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t B, int64_t most,
-             int64_t max_context) {
+             int64_t max_context, int64_t window = 0) {
     const int64_t group = Hq / Hk, rows = most * group, DP = padded_dim(D);
     Plan p{};
     // two blocks of 16 rows keep their sums in registers up to 128 elements
     p.rb = DP <= 128 && rows <= 32 && rows > 16 ? 2 : 1;
     p.use_tile = rows > 16 * p.rb;
+    p.most_rows = rows < 1 ? 1 : rows < 16 * p.rb ? rows : 16 * p.rb;
     // one sequence of many rows: nothing is left for few_kernel but padding, which the
     // tiles take too
     p.use_few = !p.use_tile || B > 1;
@@ -1306,19 +1439,25 @@ Plan plan_of(int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t B, int64_t mo
     const int64_t units = (max_context + 1 + kUnit - 1) / kUnit;
     p.workers = (B + 1 + T * group / (16 * p.rb)) * Hk * units;
     p.workers = p.workers < kWorkers ? p.workers : kWorkers;
-    // eight waves share a tile of keys where that leaves an item for every CU
-    p.waves = DP == 128 && T * group / 256 * Hk >= 256 ? 8 : 4;
-    const int rows_of = 32 * p.waves;
-    p.tiles = T * group / rows_of + B + 1;
+    p.tiles = T * group / kTileRows + B + 1;
     const int64_t items = p.tiles * Hk;
-    p.splits = items >= 384 ? 1 : (int)(512 / items);
+    // Parts of an item so that the items fill the CUs' 512 places once; 2048 keys and more of
+    // sequences of their own length, twice, so that the long ones do not end last (8
+    // sequences of up to 8500 tokens 277 -> 230 us, 16 of few tokens 139 -> 80; a window
+    // makes the lengths equal: 41.5 us, in two parts 54).
+    const int64_t full = ((T * group + kTileRows - 1) / kTileRows + B / 2) * Hk;
+    const int64_t reach = window && window < max_context ? window : max_context;
+    p.splits = (int)(B > 1 && !window ? (1024 + full - 1) / full : 512 / full);
+    const int64_t most_parts = reach / (4 * kTileKeys);  // of four tiles of keys at least
+    if (p.splits > most_parts) p.splits = (int)most_parts;
     if (p.splits > 16) p.splits = 16;
+    if (p.splits < 1) p.splits = 1;
     if (p.use_few) {
         p.joins = p.workers;
         p.bytes = p.workers * 2 * 16 * p.rb * (DP + 2) * 4;
     }
     if (p.use_tile && p.splits > 1) {
-        const int64_t b = items * p.splits * rows_of * (DP + 2) * 4;
+        const int64_t b = items * p.splits * kTileRows * (DP + 2) * 4;
         p.joins = p.joins > items ? p.joins : items;
         p.bytes = p.bytes > b ? p.bytes : b;
     }
@@ -1343,27 +1482,28 @@ int allow_lds(K kernel, int bytes) {
 }
 
 template <int DP, bool I8, int RB>
-int run_few(const Attn& a, int64_t workers, hipStream_t st) {
+int run_few(const Attn& a, int64_t workers, int64_t most_rows, hipStream_t st) {
     const auto kern = few_kernel<DP, I8, RB>;
-    if (!a.whole && workers > 256 * few_waves(DP, I8, RB)) workers = 256 * few_waves(DP, I8, RB);
+    if (!a.whole && workers > 256 * few_waves(DP, RB)) workers = 256 * few_waves(DP, RB);
     constexpr int lds = few_lds<DP, RB>();
     const int rc = allow_lds(kern, lds);
     if (rc) return rc;
     kern<<<dim3((uint32_t)workers), 256, lds, st>>>(a);
     if (!a.whole && workers > 1)
-        join_kernel<DP><<<dim3((uint32_t)workers, 4 * RB), 256, 0, st>>>(a, 16 * RB);
+        join_kernel<DP><<<dim3((uint32_t)workers, (uint32_t)((most_rows + 3) / 4)), 256, 0, st>>>(
+            a, 16 * RB);
     return FNI8_OK;
 }
 
-template <int DP, bool I8, int NW>
+template <int DP, bool I8>
 int run_tile(const Attn& a, int64_t tiles, hipStream_t st) {
-    const auto kern = tile_kernel<DP, I8, NW>;
-    constexpr int lds = tile_lds<DP, I8, NW>();
+    const auto kern = tile_kernel<DP, I8>;
+    constexpr int lds = tile_lds<DP, I8>();
     const int rc = allow_lds(kern, lds);
     if (rc) return rc;
-    kern<<<dim3((uint32_t)(tiles * a.Hk * a.splits)), 64 * NW, lds, st>>>(a);
+    kern<<<dim3((uint32_t)(tiles * a.Hk * a.splits)), 256, lds, st>>>(a);
     if (a.splits > 1)
-        join_kernel<DP><<<dim3((uint32_t)(tiles * a.Hk), 8 * NW), 256, 0, st>>>(a, 32 * NW);
+        join_tile_kernel<DP><<<dim3((uint32_t)(tiles * a.Hk), kTileRows / 32), 256, 0, st>>>(a);
     return FNI8_OK;
 }
 
@@ -1376,16 +1516,15 @@ int run_all(Attn a, const Plan& p, hipStream_t st) {
                                      : p.workers;
         int rc;
         if constexpr (DP <= 128)
-            rc = p.rb == 1 ? run_few<DP, I8, 1>(a, grid, st) : run_few<DP, I8, 2>(a, grid, st);
+            rc = p.rb == 1 ? run_few<DP, I8, 1>(a, grid, p.most_rows, st)
+                           : run_few<DP, I8, 2>(a, grid, p.most_rows, st);
         else
-            rc = run_few<DP, I8, 1>(a, grid, st);
+            rc = run_few<DP, I8, 1>(a, grid, p.most_rows, st);
         if (rc) return rc;
     }
     if (p.use_tile) {
         a.splits = a.part ? p.splits : 1;
-        if constexpr (DP == 128)
-            if (p.waves == 8) return run_tile<DP, I8, 8>(a, p.tiles, st);
-        return run_tile<DP, I8, 4>(a, p.tiles, st);
+        return run_tile<DP, I8>(a, p.tiles, st);
     }
     return FNI8_OK;
 }
@@ -1402,11 +1541,11 @@ int64_t paged_attention_workspace_bytes(int64_t T, int64_t Hq, int64_t Hk, int64
 int launch_paged_attention(const PagedAttention& p, hipStream_t st) {
     if (p.T == 0) return FNI8_OK;
     const int64_t context = p.max_pages * p.page_size;
-    const Plan plan = plan_of(p.T, p.Hq, p.Hk, p.D, p.B, p.max_seqlen, context);
+    const Plan plan = plan_of(p.T, p.Hq, p.Hk, p.D, p.B, p.max_seqlen, context, p.window);
     const int64_t group = p.Hq / p.Hk;
     // the units' sums are 32 bits, a grid has 2^32 threads
     const int64_t items = (p.B + 1 + (plan.use_tile ? 0 : p.T * group / (16 * plan.rb))) * p.Hk;
-    if (items * ((context + kUnit) / kUnit) >= (int64_t)1 << 31 || items >= (int64_t)1 << 24 ||
+    if (items * ((context + kUnit) / kUnit + 1) >= (int64_t)1 << 31 || items >= (int64_t)1 << 24 ||
         plan.tiles * p.Hk >= (int64_t)1 << 24) {
         set_error_detail("T=%lld tokens of %lld sequences and %lld keys are too many for one call",
                          (long long)p.T, (long long)p.B, (long long)context);
