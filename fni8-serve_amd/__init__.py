@@ -12,7 +12,15 @@ callers):
                                   (activation.py:24, norm.py:51), and their
                                   forms fused with the next linear's
                                   quantization (act_and_mul_quant, rmsnorm_quant)
-    LinearW8A8, GatedMLP, SparseMoE, LMHead, RMSNorm and the weight helpers
+    rope, qk_norm_rope, rope_append, paged_attention
+                                  what lies between a layer's QKV and O linears
+                                  (rotary.py:52, gqa_attention.py:59-157): rotary
+                                  positions, with the norms of queries and keys,
+                                  with the append to the paged cache, and
+                                  attention over that cache
+    LinearW8A8, GatedMLP, SparseMoE, LMHead, RMSNorm, RotaryEmbedding, GQAAttention
+                                  and the weight helpers
+    PagedKVCache, Step            the cache, fp16 or int8, and one call's tokens
     save_fni8, FQWriter, FQReader the `.fni8` checkpoint container
     load_fni8_checkpoint, load_fni8_state_dict, checkpoint_info
                                   the loader (fni8serve/loader.py:19-69)
@@ -32,19 +40,26 @@ from .ops import (  # noqa: F401
     linear_with_intermediates,
     moe_combine,
     moe_sort,
+    paged_attention,
+    qk_norm_rope,
     quantize_rowwise,
     rmsnorm,
     rmsnorm_quant,
+    rope,
+    rope_append,
 )
 from .qtensor import QTensor  # noqa: F401
 from .container import FQReader, FQWriter, save_fni8  # noqa: F401
+from .kv_cache import PagedKVCache, Step  # noqa: F401
 from .loader import checkpoint_info, load_fni8_checkpoint, load_fni8_state_dict  # noqa: F401
 from .quant import quantize_int8_rowwise  # noqa: F401
 from .layers import (  # noqa: F401
     NF4_CODEBOOK,
     GatedMLP,
     GeluAndMul,
+    GQAAttention,
     RMSNorm,
+    RotaryEmbedding,
     SiluAndMul,
     get_act_and_mul,
     LinearW8A8,
@@ -65,5 +80,6 @@ __all__ = [
     "qkv_weight", "gate_up_weight", "save_fni8", "FQWriter", "FQReader", "load_fni8_checkpoint",
     "load_fni8_state_dict", "checkpoint_info", "act_and_mul", "act_and_mul_quant", "rmsnorm",
     "rmsnorm_quant", "RMSNorm", "SiluAndMul", "GeluAndMul", "get_act_and_mul", "gemm_w4a8",
-    "gemm_quantized",
+    "gemm_quantized", "rope", "qk_norm_rope", "rope_append", "paged_attention", "PagedKVCache",
+    "Step", "RotaryEmbedding", "GQAAttention",
 ]

@@ -585,7 +585,13 @@ def _index(name: str, t: torch.Tensor, n: int | None):
                                                                    and t.numel() != n):
         raise ValueError(f"{name} must be int32 or int64 with {n if n is not None else 'one'} "
                          f"entries (got {t.dtype}, {tuple(t.shape)})")
-    return t.to(torch.int32).contiguous()
+    return _int32(t).contiguous()
+
+
+def _int32(t: torch.Tensor):
+    """64-bit positions, slots, pages or lengths in 32 bits; what lies outside stays outside
+    every table and cache."""
+    return t if t.dtype == torch.int32 else t.clamp(-1, 2 ** 31 - 1).to(torch.int32)
 
 
 def _table(positions, cos_sin, T: int, D: int):
@@ -779,7 +785,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         if B:
             raise ValueError("block_tables has no pages")
         return out.zero_()
-    tables = block_tables.to(torch.int32)
+    tables = _int32(block_tables)
     if width > 1 and tables.stride(1) != 1 or B > 1 and tables.stride(0) < width:
         tables = tables.contiguous()
     ldt = tables.stride(0) if B > 1 else width
