@@ -19,12 +19,13 @@
 // P' = 2^(s + log2 v_s - m) with m the maximum of s + log2 v_s, so P' <= 1 rounds to fp16
 // like P does whatever the scale's size, and l adds P' / v_s.
 //
-// few_kernel takes sequences with few rows (decode, drafted tokens): memory bounds it, each
+// few_work takes sequences with few rows (decode, drafted tokens): memory bounds it, each
 // cached row is read once.  The keys of all sequences are one list of units of 128 keys,
 // cut into equal runs, one a workgroup, whatever the lengths; parts of an item that two
 // workgroups share are joined by join_kernel.  tile_kernel takes the others: 128 rows a
 // workgroup share K and V tiles of 64 keys in LDS; the MFMAs, and the card's power under
-// them, bound it.
+// them, bound it.  A batch of both kinds is one launch, so that the reads of the one pass
+// beside the products of the other.
 #include "common.h"
 
 namespace {
@@ -41,11 +42,17 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kInf = __builtin_inff();
-constexpr int kUnit = 128;      // keys of a unit of few_kernel: 32 for each of 4 waves
+constexpr int kUnit = 128;      // keys of a unit of few_work: 32 for each of 4 waves
 constexpr int kTileRows = 128;  // of a workgroup of tile_kernel: 32 a wave
 constexpr int kTileKeys = 64;
 constexpr float kLag = 8.0f;
-constexpr int kWorkers = 768;  // of few_kernel at most: three a CU
+constexpr int kWorkers = 768;  // of few_work at most: three a CU
+// Beside tiles: one a CU, the tiles have the rest of it.  Decoded tokens beside one chunk, in
+// two launches, one with 512 workers and one with 256 (us): 120 of 2000 to 16000 keys beside
+// 2000 tokens 1060, 1020, 969; 63 of up to 8500 beside 512 229, 216, 231, of 8 bits 247, 242,
+// 226; 15 of up to 2000 beside 384 58, 51, 51.  Only chunks, 8 bits, 64 of 450 tokens: 2059,
+// 2134, 2143.
+constexpr int kMixedWorkers = 256;
 
 // What join_kernel does: part p of an item, o [rows][DP], m, l [rows], lies in slot `first`
 // (p = 0) or next + (p - 1) * step.
@@ -63,13 +70,14 @@ struct Attn {
     const int32_t *tables, *lens, *cu;
     int64_t ldt;
     uint16_t* out;
-    Join* joins;
-    float* part;
+    Join *joins, *tile_joins;
+    float *part, *tile_part;
     int T, Hq, Hk, D, group, num_pages, plog, max_pages, B, nseq, window, cap;
     float c;       // |scale| * log2 e, not 0
     uint32_t flip; // sign bits of two fp16 where the scale is negative: the queries' signs
-    int few;       // few_kernel takes sequences of at most so many new tokens, tile_kernel others
-    int whole;     // few_kernel: no parts, an item is one unit
+    int few;       // few_work takes sequences of at most so many new tokens, tiles the others
+    int workers;   // workgroups of few_work
+    int whole;     // few_work: no parts, an item is one unit
     int splits;    // tile_kernel: parts of an item at most
 };
 
@@ -309,7 +317,7 @@ constexpr int few_waves(int dp, int rb) {
     return dp > 128 ? 1 : rb == 1 && dp == 64 ? 3 : 2;
 }
 
-// What few_kernel makes of a sequence: its range of keys and its units.
+// What few_work makes of a sequence: its range of keys and its units.
 struct FewSeq {
     Seq q;
     int rows, blocks, lo, tiles, units;
@@ -328,17 +336,13 @@ __device__ __forceinline__ FewSeq few_seq(const Attn& a, const Seq& q) {
     return f;
 }
 
-__device__ __forceinline__ int per_worker(int U) {
-    return (U + (int)gridDim.x - 1) / (int)gridDim.x;
-}
-
+// The work of one of a.workers workgroups.
 template <int DP, bool I8, int RB>
-__global__ __launch_bounds__(256, few_waves(DP, RB)) void few_kernel(Attn a) {
+__device__ __forceinline__ void few_work(const Attn& a, const int worker, char* smem) {
     constexpr int KS = DP / 32, DB = DP / 16;
     constexpr int KL = I8 ? DP / 64 : DP / 32, VL = KL;  // loads of 16 keys
     constexpr int CH = DP / 8;                           // chunks of a row in LDS
     constexpr int ES = I8 ? 1 : 2, RC = DP * ES / 16;    // 16-byte pieces of a cached row
-    extern __shared__ __align__(16) char smem[];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, G = lane >> 4;
@@ -348,7 +352,7 @@ __global__ __launch_bounds__(256, few_waves(DP, RB)) void few_kernel(Attn a) {
     float* ml = reinterpret_cast<float*>(smem + 4 * few_region<DP, RB>());  // [4][2][16 RB]
     int* sh = reinterpret_cast<int*>(ml + 4 * 2 * 16 * RB);
 
-    if (!a.whole && threadIdx.x == 0) a.joins[blockIdx.x].parts = 0;
+    if (!a.whole && threadIdx.x == 0) a.joins[worker].parts = 0;
     int s, base, u, upw = 0;
     Seq sq;
     if (!find(
@@ -358,8 +362,8 @@ __global__ __launch_bounds__(256, few_waves(DP, RB)) void few_kernel(Attn a) {
                 return few_seq<RB>(a, q).units;
             },
             [&](int U) {
-                upw = per_worker(U);
-                return upw * (int)blockIdx.x;
+                upw = (U + a.workers - 1) / a.workers;
+                return upw * worker;
             },
             s, base, u, sq))
         return;
@@ -659,7 +663,7 @@ __global__ __launch_bounds__(256, few_waves(DP, RB)) void few_kernel(Attn a) {
         }
         __syncthreads();
         const int D4 = a.D >> 2;
-        float* part = a.part + (int64_t)(2 * blockIdx.x + (first_unit == u ? 0 : 1)) * few_part<DP, RB>();
+        float* part = a.part + (int64_t)(2 * worker + (first_unit == u ? 0 : 1)) * few_part<DP, RB>();
         for (int e = threadIdx.x; e < nrows * D4; e += 256) {
             const int r = e / D4, d4 = e - r * D4;
             float top = -kInf, wm[4];
@@ -694,7 +698,7 @@ __global__ __launch_bounds__(256, few_waves(DP, RB)) void few_kernel(Attn a) {
             }
         }
         if (!full && tile == 0 && threadIdx.x == 0) {  // this run begins an item, others end it
-            const int w0 = blockIdx.x, w1 = (u + f.tiles - 1) / upw;
+            const int w0 = worker, w1 = (u + f.tiles - 1) / upw;
             a.joins[w0] = Join{w1 - w0 + 1, 2 * w0 + (first_unit == u ? 0 : 1), 2 * w0 + 2, 2,
                                f.q.start, row0, nrows, h};
         }
@@ -715,12 +719,18 @@ __global__ __launch_bounds__(256, few_waves(DP, RB)) void few_kernel(Attn a) {
     }
 }
 
+template <int DP, bool I8, int RB>
+__global__ __launch_bounds__(256, few_waves(DP, RB)) void few_kernel(Attn a) {
+    extern __shared__ __align__(16) char smem[];
+    few_work<DP, I8, RB>(a, blockIdx.x, smem);
+}
+
 // Joins an item's parts, a wave a row: 64 parts' weights at a time, one a lane, then the
 // parts of o, DP / 4 lanes each, several in flight.
 template <int DP>
-__global__ __launch_bounds__(256) void join_kernel(Attn a, int part_rows) {
+__device__ __forceinline__ void join_few(const Attn& a, int worker, int part_rows) {
     constexpr int LP = DP / 4, NG = 64 / LP;  // lanes of a part, parts at a time
-    const Join j = a.joins[blockIdx.x];
+    const Join j = a.joins[worker];
     if (j.parts == 0) return;
     const int lane = threadIdx.x & 63;
     const int64_t size = (int64_t)part_rows * (DP + 2);
@@ -781,13 +791,13 @@ __global__ __launch_bounds__(256) void join_kernel(Attn a, int part_rows) {
 // rows a workgroup.  (A wave a row spends its time on the exchange of the weights: 45 us of
 // 76 for 480 items of two parts.)
 template <int DP>
-__global__ __launch_bounds__(256) void join_tile_kernel(Attn a) {
+__device__ __forceinline__ void join_tile(const Attn& a, int item) {
     constexpr int LP = DP / 4, RP = 256 / LP;  // lanes of a row, rows at a time
-    const Join j = a.joins[blockIdx.x];
+    const Join j = a.tile_joins[item];
     if (j.parts == 0) return;
     const int d4 = threadIdx.x % LP;
     if (4 * d4 >= a.D) return;
-    const float* parts = a.part + (int64_t)j.first * (kTileRows * (DP + 2));
+    const float* parts = a.tile_part + (int64_t)j.first * (kTileRows * (DP + 2));
     for (int r = blockIdx.y * 32 + threadIdx.x / LP; r < (int)blockIdx.y * 32 + 32 && r < j.nrows;
          r += RP) {
         float top = -kInf, sum = 0.0f;
@@ -809,6 +819,15 @@ __global__ __launch_bounds__(256) void join_tile_kernel(Attn a) {
         if (sum == 0.0f) y = uint2{0, 0};
         *reinterpret_cast<uint2*>(a.out + ((int64_t)(j.start + i) * a.Hq + head) * a.D + 4 * d4) = y;
     }
+}
+
+// grid.x: few_work's workers, then the tiles' items
+template <int DP>
+__global__ __launch_bounds__(256) void join_kernel(Attn a, int part_rows) {
+    if ((int)blockIdx.x < a.workers)
+        join_few<DP>(a, blockIdx.x, part_rows);
+    else
+        join_tile<DP>(a, blockIdx.x - a.workers);
 }
 
 // ---- tiles of 128 rows -------------------------------------------------------------
@@ -856,6 +875,9 @@ template <int DP, bool I8>
 constexpr int tile_lds() {
     return tile_stages(DP, I8) * 2 * kTileKeys * DP * 2 + (I8 ? 2 * 3 * kTileKeys * 4 : 0) + 64;
 }
+
+// Workgroups a CU, by the registers
+constexpr int tile_waves(int dp, bool mixed) { return mixed ? few_waves(dp, 1) : dp > 128 ? 1 : 2; }
 
 // The item of a workgroup of tile_kernel.
 struct TileItem {
@@ -914,8 +936,10 @@ __device__ __forceinline__ bool tile_item(const Attn& a, int id, int h, int* sh,
     return true;
 }
 
-template <int DP, bool I8>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
+// MIXED: the first a.workers workgroups take the sequences of few rows, whose reads pass
+// beside the products of the others.
+template <int DP, bool I8, bool MIXED>
+__global__ __launch_bounds__(256, tile_waves(DP, MIXED)) void tile_kernel(Attn a) {
     constexpr int KW = kTileKeys / 4;  // keys that a wave copies
     constexpr int S = tile_stages(DP, I8);
     constexpr int KS = DP / 16, DB = DP / 32, CH = DP / 8;
@@ -928,9 +952,15 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
     float* scales = reinterpret_cast<float*>(smem + 2 * S * TB);  // [2][3][64]
     int* sh = reinterpret_cast<int*>(smem + tile_lds<DP, I8>() - 64);
 
+    if constexpr (MIXED)
+        if ((int)blockIdx.x < a.workers) {
+            few_work<DP, I8, 1>(a, blockIdx.x, smem);
+            return;
+        }
+    const int id = blockIdx.x - (MIXED ? a.workers : 0);
     // a key head's items are neighbours modulo the heads: with the round-robin dispatch
     // over the 8 XCDs they share an L2 where the heads divide 8
-    const int h = blockIdx.x % a.Hk, rest = blockIdx.x / a.Hk;
+    const int h = id % a.Hk, rest = id / a.Hk;
     const int split = rest % a.splits;
     TileItem t{};
     const bool found = tile_item(a, rest / a.splits, h, sh, t);
@@ -941,7 +971,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
         if (found && t.parts > 1)
             j = Join{t.parts, index * a.splits, index * a.splits + 1, 1, t.q.start, tile_row0,
                      t.rows - tile_row0 < kTileRows ? t.rows - tile_row0 : kTileRows, h};
-        a.joins[index] = j;
+        a.tile_joins[index] = j;
     }
     if (!found || split >= t.parts) return;
     const int first = t.kt0 + split * t.per;
@@ -1386,7 +1416,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
     l += __shfl_xor(l, 32, 64);
     if (r >= t.rows) return;
     if (t.parts > 1) {
-        float* part = a.part + ((int64_t)index * a.splits + split) * (kTileRows * (DP + 2));
+        float* part = a.tile_part + ((int64_t)index * a.splits + split) * (kTileRows * (DP + 2));
         const int pr = wave * 32 + col;
 #pragma unroll
         for (int d = 0; d < DB; d++)
@@ -1419,17 +1449,16 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void tile_kernel(Attn a) {
 
 // How a call is cut up, from what the host knows.
 struct Plan {
-    int rb;               // 16-row blocks of few_kernel's rows
-    int64_t few;          // new tokens of a sequence that few_kernel takes at most
+    int rb;               // 16-row blocks of few_work's rows
+    int64_t few;          // new tokens of a sequence that few_work takes at most
     bool use_few, use_tile;
-    int64_t most_rows;    // of a sequence in few_kernel that keeps to the bound
-    int64_t workers;      // of few_kernel
+    int64_t most_rows;    // of a sequence in few_work that keeps to the bound
+    int64_t workers;      // of few_work
     int64_t tiles;        // of kTileRows rows, at most
     int splits;
-    int64_t joins, bytes;  // of the workspace: Join records, and the records and parts
+    // of the workspace: Join records and parts of few_work, the same of the tiles
+    int64_t joins, part, tile_joins, tile_part, bytes;
 };
-
-int64_t join_bytes(int64_t n) { return (n * (int64_t)sizeof(Join) + 255) & ~(int64_t)255; }
 
 int padded_dim(int64_t D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
@@ -1441,13 +1470,14 @@ Plan plan_of(int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t B, int64_t mo
     p.rb = DP <= 128 && rows <= 32 && rows > 16 ? 2 : 1;
     p.use_tile = rows > 16 * p.rb;
     p.most_rows = rows < 1 ? 1 : rows < 16 * p.rb ? rows : 16 * p.rb;
-    // one sequence of many rows: nothing is left for few_kernel but padding, which the
+    // one sequence of many rows: nothing is left for few_work but padding, which the
     // tiles take too
     p.use_few = !p.use_tile || B > 1;
     p.few = !p.use_tile ? 1 << 30 : p.use_few ? 16 * p.rb / group : 0;
     const int64_t units = (max_context + 1 + kUnit - 1) / kUnit;
     p.workers = (B + 1 + T * group / (16 * p.rb)) * Hk * units;
-    p.workers = p.workers < kWorkers ? p.workers : kWorkers;
+    const int64_t most_workers = p.use_tile ? kMixedWorkers : kWorkers;
+    p.workers = !p.use_few ? 0 : p.workers < most_workers ? p.workers : most_workers;
     p.tiles = T * group / kTileRows + B + 1;
     const int64_t items = p.tiles * Hk;
     // Parts of an item so that the items fill the CUs' 512 places once; 2048 keys and more of
@@ -1461,16 +1491,15 @@ Plan plan_of(int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t B, int64_t mo
     if (p.splits > most_parts) p.splits = (int)most_parts;
     if (p.splits > 16) p.splits = 16;
     if (p.splits < 1) p.splits = 1;
-    if (p.use_few) {
-        p.joins = p.workers;
-        p.bytes = p.workers * 2 * 16 * p.rb * (DP + 2) * 4;
-    }
+    // in this order, each a multiple of 256 bytes
+    const auto round = [](int64_t n) { return (n + 255) & ~(int64_t)255; };
+    p.joins = round(p.workers * (int64_t)sizeof(Join));
+    p.part = round(p.workers * 2 * 16 * p.rb * (DP + 2) * 4);
     if (p.use_tile && p.splits > 1) {
-        const int64_t b = items * p.splits * kTileRows * (DP + 2) * 4;
-        p.joins = p.joins > items ? p.joins : items;
-        p.bytes = p.bytes > b ? p.bytes : b;
+        p.tile_joins = round(items * (int64_t)sizeof(Join));
+        p.tile_part = round(items * p.splits * kTileRows * (DP + 2) * 4);
     }
-    p.bytes += join_bytes(p.joins);
+    p.bytes = p.joins + p.part + p.tile_joins + p.tile_part;
     return p;
 }
 
@@ -1490,51 +1519,45 @@ int allow_lds(K kernel, int bytes) {
     return FNI8_OK;
 }
 
-template <int DP, bool I8, int RB>
-int run_few(const Attn& a, int64_t workers, int64_t most_rows, hipStream_t st) {
-    const auto kern = few_kernel<DP, I8, RB>;
-    if (!a.whole && workers > 256 * few_waves(DP, RB)) workers = 256 * few_waves(DP, RB);
-    constexpr int lds = few_lds<DP, RB>();
-    const int rc = allow_lds(kern, lds);
-    if (rc) return rc;
-    kern<<<dim3((uint32_t)workers), 256, lds, st>>>(a);
-    if (!a.whole && workers > 1)
-        join_kernel<DP><<<dim3((uint32_t)workers, (uint32_t)((most_rows + 3) / 4)), 256, 0, st>>>(
-            a, 16 * RB);
-    return FNI8_OK;
+template <class K>
+int run(K kernel, const Attn& a, int64_t grid, int lds, hipStream_t st) {
+    const int rc = allow_lds(kernel, lds);
+    if (rc == FNI8_OK) kernel<<<dim3((uint32_t)grid), 256, lds, st>>>(a);
+    return rc;
 }
 
-template <int DP, bool I8>
-int run_tile(const Attn& a, int64_t tiles, hipStream_t st) {
-    const auto kern = tile_kernel<DP, I8>;
-    constexpr int lds = tile_lds<DP, I8>();
-    const int rc = allow_lds(kern, lds);
-    if (rc) return rc;
-    kern<<<dim3((uint32_t)(tiles * a.Hk * a.splits)), 256, lds, st>>>(a);
-    if (a.splits > 1)
-        join_tile_kernel<DP><<<dim3((uint32_t)(tiles * a.Hk), kTileRows / 32), 256, 0, st>>>(a);
-    return FNI8_OK;
+template <int DP, bool I8, int RB>
+int run_few(Attn& a, hipStream_t st) {
+    if (!a.whole && a.workers > 256 * few_waves(DP, RB)) a.workers = 256 * few_waves(DP, RB);
+    return run(few_kernel<DP, I8, RB>, a, a.workers, few_lds<DP, RB>(), st);
 }
 
 template <int DP, bool I8>
 int run_all(Attn a, const Plan& p, hipStream_t st) {
-    // few_kernel and its join have read their parts before the tiles' are written
-    if (p.use_few) {
-        a.whole = a.part == nullptr;
-        const int64_t grid = a.whole ? (a.nseq + (p.use_tile ? 0 : (int64_t)a.T * a.group / (16 * p.rb))) * a.Hk
-                                     : p.workers;
-        int rc;
+    a.whole = a.part == nullptr;
+    a.workers = (int)p.workers;
+    if (a.whole && p.use_few)
+        a.workers = (int)((a.nseq + (p.use_tile ? 0 : (int64_t)a.T * a.group / (16 * p.rb))) * a.Hk);
+    a.splits = a.whole ? 1 : p.splits;
+    const int64_t items = p.tiles * a.Hk;
+    int rc;
+    if (!p.use_tile) {
         if constexpr (DP <= 128)
-            rc = p.rb == 1 ? run_few<DP, I8, 1>(a, grid, p.most_rows, st)
-                           : run_few<DP, I8, 2>(a, grid, p.most_rows, st);
+            rc = p.rb == 1 ? run_few<DP, I8, 1>(a, st) : run_few<DP, I8, 2>(a, st);
         else
-            rc = run_few<DP, I8, 1>(a, grid, p.most_rows, st);
-        if (rc) return rc;
+            rc = run_few<DP, I8, 1>(a, st);
+    } else if (p.use_few) {
+        rc = run(tile_kernel<DP, I8, true>, a, a.workers + items * a.splits, tile_lds<DP, I8>(), st);
+    } else {
+        rc = run(tile_kernel<DP, I8, false>, a, items * a.splits, tile_lds<DP, I8>(), st);
     }
-    if (p.use_tile) {
-        a.splits = a.part ? p.splits : 1;
-        return run_tile<DP, I8>(a, p.tiles, st);
-    }
+    if (rc || a.whole) return rc;
+    const bool few_parts = a.workers > 1, tile_parts = p.use_tile && a.splits > 1;
+    if (!few_parts && !tile_parts) return FNI8_OK;
+    // four of few_work's rows or 32 of a tile's a workgroup
+    const int64_t y = tile_parts ? kTileRows / 32 : (p.most_rows + 3) / 4;
+    join_kernel<DP><<<dim3((uint32_t)(a.workers + (tile_parts ? items : 0)), (uint32_t)y), 256, 0, st>>>(
+        a, 16 * p.rb);
     return FNI8_OK;
 }
 
@@ -1580,10 +1603,12 @@ int launch_paged_attention(const PagedAttention& p, hipStream_t st) {
     a.c = a.c > 1e-30f ? a.c : 1e-30f;
     a.flip = p.scale < 0.0f ? 0x80008000u : 0;
     a.few = (int)plan.few;
-    a.splits = 1;
     if (plan.bytes && p.work_bytes >= plan.bytes) {
-        a.joins = reinterpret_cast<Join*>(p.work);
-        a.part = reinterpret_cast<float*>(p.work + join_bytes(plan.joins));
+        int8_t* at = p.work;
+        a.joins = reinterpret_cast<Join*>(at);
+        a.part = reinterpret_cast<float*>(at += plan.joins);
+        a.tile_joins = reinterpret_cast<Join*>(at += plan.part);
+        a.tile_part = reinterpret_cast<float*>(at += plan.tile_joins);
     }
     int rc;
     switch (padded_dim(p.D)) {
