@@ -749,6 +749,18 @@ __device__ __forceinline__ void join_few(const Attn& a, int worker, int part_row
                 m = p[r];
                 l = p[part_rows + r];
             }
+            // the first parts of o are on their way while the weights are made
+            constexpr int U = 8;
+            f32x4 v[U];
+            auto fetch = [&](int i) {
+#pragma unroll
+                for (int k = 0; k < U; k++) {
+                    const int p = i + k * NG + grp;
+                    v[k] = f32x4{0, 0, 0, 0};
+                    if (p < n) v[k] = *reinterpret_cast<const f32x4*>(slot(c + p) + r * DP + 4 * d4);
+                }
+            };
+            fetch(0);
             float t = __builtin_fmaxf(top, m);
             t = max_xor32(max_xor16(t));
 #pragma unroll
@@ -761,15 +773,8 @@ __device__ __forceinline__ void join_few(const Attn& a, int worker, int part_row
             for (int x = 32; x > 0; x >>= 1) wl += __shfl_xor(wl, x, 64);
             sum = sum * keep + wl;
             top = t;
-            constexpr int U = 8;
             for (int i = 0; i < n; i += U * NG) {
-                f32x4 v[U];
-#pragma unroll
-                for (int k = 0; k < U; k++) {
-                    const int p = i + k * NG + grp;
-                    v[k] = f32x4{0, 0, 0, 0};
-                    if (p < n) v[k] = *reinterpret_cast<const f32x4*>(slot(c + p) + r * DP + 4 * d4);
-                }
+                if (i > 0) fetch(i);
 #pragma unroll
                 for (int k = 0; k < U; k++) acc += __shfl(w, (i + k * NG + grp) & 63, 64) * v[k];
             }
