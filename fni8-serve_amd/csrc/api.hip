@@ -180,6 +180,8 @@ int check_heads(const char* name, const void* x, int64_t ld, int64_t hs, int64_t
     REQUIRE(x, FNI8_ERR_NULL, "%s is required", name);
     REQUIRE(hs >= D && ld >= D, FNI8_ERR_STRIDE, "%s: token or head stride < D=%lld", name,
             (long long)D);
+    REQUIRE(hs < (int64_t)1 << 32, FNI8_ERR_STRIDE, "%s: head stride %lld >= 2^32", name,
+            (long long)hs);
     REQUIRE(aligned(x, 16) && ld % 8 == 0 && hs % 8 == 0, FNI8_ERR_ALIGN,
             "%s must be 16-byte aligned with strides that are multiples of 8", name);
     return FNI8_OK;

@@ -14,7 +14,10 @@
 // cache (negative: padding) drops the row.
 //
 // Memory bounds it: 4 bytes an element (fp16 in and out), R * 4 a token for its table
-// row.  A row is held by LPR = 8, 16 or 32 lanes of 8 elements (16-byte accesses).  The
+// row.  The vector instructions come next, so a row has one form whatever its pairs, its
+// weight and its R: (x c w + x' s w') m with the other element x' of the pair, c = 1 and
+// s = -0 where nothing turns (x + 0 * -0 is x, its sign included), and w = m = 1 without a
+// weight.  A row is held by LPR = 8, 16 or 32 lanes of 8 elements (16-byte accesses).  The
 // other half of a rotated pair is read a second time from the input (the L1 has it)
 // rather than exchanged between lanes: both loads are in flight together, and any R that
 // is a multiple of 16 works the same way.
@@ -27,7 +30,8 @@ using fni8::h2f;
 
 struct RowArgs {
     const uint16_t *q, *k, *v;
-    int64_t ldq, hsq, ldk, hsk, ldv, hsv;
+    int64_t ldq, ldk, ldv;
+    uint32_t hsq, hsk, hsv;
     int Hq, Hk, Hv, D, R, pairs, unit;
     const uint16_t *qw, *kw;
     float eps, inv_d;
@@ -71,24 +75,63 @@ __device__ __forceinline__ float half_of(uint4 v, int i) {
     return h2f((uint16_t)(i & 1 ? w >> 16 : w & 0xffffu));
 }
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    const f32x2 v = {a, b};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, h2));  // to nearest even
+}
+
+// The other elements of the pairs of the 8 elements from e on, `self`, of the row at src; 0
+// where nothing turns.
+template <bool ALIGNED>
+__device__ __forceinline__ uint4 others(const uint16_t* src, uint4 self, int e, int R, int pairs) {
+    const int half = R >> 1;
+    auto turned = [](uint32_t w) { return w >> 16 | w << 16; };
+    uint4 o = make_uint4(0, 0, 0, 0);
+    if (ALIGNED) {
+        if (e >= R) return o;
+        if (pairs)
+            return make_uint4(turned(self.x), turned(self.y), turned(self.z), turned(self.w));
+        return *reinterpret_cast<const uint4*>(src + (e < half ? e + half : e - half));
+    }
+    uint32_t h[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        h[i] = 0;
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const int d = e + 2 * i + k;
+            if (d >= R) continue;
+            const int at = pairs ? d ^ 1 : d < half ? d + half : d - half;
+            h[i] |= (uint32_t)src[at] << 16 * k;
+        }
+    }
+    return make_uint4(h[0], h[1], h[2], h[3]);
+}
+
 // A block takes NR rows per group of LPR lanes of one token (blockIdx.x): rows 0..Hq are
 // query heads, then key heads, then value heads.  ALIGNED: every chunk of 8 elements is
 // rotated as a whole or not at all and its table entries are 16-byte aligned (R a multiple
 // of 16 for halves, of 8 for pairs); otherwise element by element.
-template <int LPR, int NR, bool ALIGNED>
+// NORM: some row has a weight.
+template <int LPR, int NR, bool ALIGNED, bool NORM>
 __global__ __launch_bounds__(256) void row_kernel(RowArgs a) {
     constexpr int GROUPS = 256 / LPR;
     const int64_t t = blockIdx.x;
     const int lane = threadIdx.x & (LPR - 1), group = threadIdx.x / LPR;
-    const int e = lane * 8, half = a.R >> 1;
+    const int e = lane * 8;
     const bool mine = e < a.D;
     const int rows = a.Hq + a.Hk + a.Hv;
     const int row0 = blockIdx.y * (GROUPS * NR) + group;
 
     // the lane's 8 elements of the token's angles, the same for every head
     float c[8], s[8];
-    // where the other element of each pair lies, for halves
-    const int turn = e < half ? half : -half;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        c[i] = 1.0f;
+        s[i] = -0.0f;
+    }
     int64_t p = 0;
     bool outside = false;
     if (a.R) {
@@ -96,6 +139,7 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs a) {
         outside = p < 0 || p >= a.P;
         if (outside) p = 0;
     }
+    const int half = a.R >> 1;
     const float* row = a.table + p * a.R;
     if (ALIGNED) {
         if (e < a.R) {
@@ -137,30 +181,22 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs a) {
     }
     if (outside)
 #pragma unroll
-        for (int i = 0; i < 8; i++) c[i] = s[i] = __builtin_nanf("");
+        for (int i = 0; i < 8; i++)
+            if (e + i < a.R) c[i] = s[i] = __builtin_nanf("");
 
+    const uint16_t *q = a.q + t * a.ldq, *k = a.k + t * a.ldk, *v = a.v + t * a.ldv;
     uint4 x[NR], o[NR];
-    uint16_t other[NR][8];
 #pragma unroll
     for (int j = 0; j < NR; j++) {
         const int r = row0 + j * GROUPS;
         x[j] = o[j] = make_uint4(0, 0, 0, 0);
         if (r >= rows || !mine) continue;
-        const uint16_t* src = r < a.Hq            ? a.q + t * a.ldq + r * a.hsq
-                              : r < a.Hq + a.Hk ? a.k + t * a.ldk + (r - a.Hq) * a.hsk
-                                                : a.v + t * a.ldv + (r - a.Hq - a.Hk) * a.hsv;
+        const bool is_q = r < a.Hq, turns = r < a.Hq + a.Hk;
+        const uint32_t h = is_q ? r : turns ? r - a.Hq : r - a.Hq - a.Hk;
+        const uint32_t hs = is_q ? a.hsq : turns ? a.hsk : a.hsv;
+        const uint16_t* src = (is_q ? q : turns ? k : v) + (uint64_t)h * hs;
         x[j] = *reinterpret_cast<const uint4*>(src + e);
-        if (r < a.Hq + a.Hk && !a.pairs) {
-            if (ALIGNED) {
-                if (e < a.R) o[j] = *reinterpret_cast<const uint4*>(src + e + turn);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int d = e + i;
-                    other[j][i] = d < a.R ? src[d < half ? d + half : d - half] : 0;
-                }
-            }
-        }
+        if (turns) o[j] = others<ALIGNED>(src, x[j], e, a.R, a.pairs);
     }
     int64_t slot = -1;
     if (a.slot) {
@@ -174,53 +210,37 @@ __global__ __launch_bounds__(256) void row_kernel(RowArgs a) {
         const bool is_q = r < a.Hq, is_k = !is_q && r < a.Hq + a.Hk;
         if (r >= rows) continue;
         uint4 y = x[j];
-        const uint16_t* w = is_q ? a.qw : a.kw;
         if (is_q || is_k) {
-            float f[8], g[8];
+            float f[8], g[8], z[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 f[i] = half_of(x[j], i);
-                if (a.pairs)
-                    g[i] = half_of(x[j], i ^ 1);
-                else
-                    g[i] = ALIGNED ? half_of(o[j], i) : h2f(other[j][i]);
+                g[i] = half_of(o[j], i);
             }
-            if (w) {
+            if (NORM) {
+                const uint16_t* w = is_q ? a.qw : a.kw;
                 float ss = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 8; i++) ss = __builtin_fmaf(f[i], f[i], ss);
                 const float m = __builtin_amdgcn_rsqf(__builtin_fmaf(row_sum<LPR>(ss), a.inv_d, a.eps));
-                if (mine) {
-                    const uint4 w4 = *reinterpret_cast<const uint4*>(w + e);
-                    uint4 o4 = make_uint4(0, 0, 0, 0);
-                    if (ALIGNED && !a.pairs && e < a.R)
-                        o4 = *reinterpret_cast<const uint4*>(w + e + turn);
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        float wi = half_of(w4, i), wo = 0.0f;
-                        if (a.pairs)
-                            wo = half_of(w4, i ^ 1);
-                        else if (ALIGNED)
-                            wo = half_of(o4, i);
-                        else if (e + i < a.R)
-                            wo = h2f(w[e + i < half ? e + i + half : e + i - half]);
-                        if (a.unit) {
-                            wi = 1.0f + wi;
-                            wo = 1.0f + wo;
-                        }
-                        f[i] = f[i] * m * wi;
-                        g[i] = g[i] * m * wo;
-                    }
+                const uint32_t one = a.unit ? 0 : 0x3c003c00u;
+                uint4 w4 = make_uint4(one, one, one, one), o4 = w4;
+                if (w && mine) {
+                    w4 = *reinterpret_cast<const uint4*>(w + e);
+                    o4 = others<ALIGNED>(w, w4, e, a.R, a.pairs);
                 }
-            }
-            uint32_t h[8];
+                const float scale = w ? m : 1.0f, unit = a.unit ? 1.0f : 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float z = e + i < a.R ? __builtin_fmaf(f[i], c[i], g[i] * s[i]) : f[i];
-                h[i] = f2h(z);
+                for (int i = 0; i < 8; i++) {
+                    const float wc = (unit + half_of(w4, i)) * c[i], ws = (unit + half_of(o4, i)) * s[i];
+                    z[i] = __builtin_fmaf(f[i], wc, g[i] * ws) * scale;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) z[i] = __builtin_fmaf(f[i], c[i], g[i] * s[i]);
             }
-            y = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16,
-                           h[6] | h[7] << 16);
+            y = make_uint4(pack2(z[0], z[1]), pack2(z[2], z[3]), pack2(z[4], z[5]),
+                           pack2(z[6], z[7]));
         }
         if (is_q || (is_k && !a.slot)) {
             uint16_t* dst = is_q ? a.q_out + (t * a.Hq + r) * a.D
@@ -253,10 +273,10 @@ template <int LPR, int NR>
 void launch_rows(const RowArgs& a, int64_t T, bool aligned, hipStream_t st) {
     const int rows = a.Hq + a.Hk + a.Hv, per = 256 / LPR * NR;
     const dim3 grid((uint32_t)T, (uint32_t)((rows + per - 1) / per));
-    if (aligned)
-        row_kernel<LPR, NR, true><<<grid, 256, 0, st>>>(a);
-    else
-        row_kernel<LPR, NR, false><<<grid, 256, 0, st>>>(a);
+    const bool norm = a.qw || a.kw;
+    const auto kernel = aligned ? norm ? row_kernel<LPR, NR, true, true> : row_kernel<LPR, NR, true, false>
+                                : norm ? row_kernel<LPR, NR, false, true> : row_kernel<LPR, NR, false, false>;
+    kernel<<<grid, 256, 0, st>>>(a);
 }
 
 }  // namespace
@@ -266,9 +286,9 @@ namespace fni8h {
 int launch_qkv_rows(const QkvRows& r, hipStream_t st) {
     if (r.T == 0 || r.Hq + r.Hk == 0) return FNI8_OK;
     RowArgs a;
-    a.q = r.q; a.ldq = r.ldq; a.hsq = r.hsq; a.Hq = (int)r.Hq;
-    a.k = r.k; a.ldk = r.ldk; a.hsk = r.hsk; a.Hk = (int)r.Hk;
-    a.v = r.v; a.ldv = r.ldv; a.hsv = r.hsv; a.Hv = r.slots ? (int)r.Hk : 0;
+    a.q = r.q; a.ldq = r.ldq; a.hsq = (uint32_t)r.hsq; a.Hq = (int)r.Hq;
+    a.k = r.k; a.ldk = r.ldk; a.hsk = (uint32_t)r.hsk; a.Hk = (int)r.Hk;
+    a.v = r.v; a.ldv = r.ldv; a.hsv = (uint32_t)r.hsv; a.Hv = r.slots ? (int)r.Hk : 0;
     a.D = (int)r.D; a.R = (int)r.R; a.pairs = r.interleaved != 0; a.unit = r.unit_offset != 0;
     a.qw = r.q_weight; a.kw = r.k_weight; a.eps = r.eps; a.inv_d = 1.0f / (float)r.D;
     a.pos = r.positions; a.table = r.cos_sin; a.P = r.P;
