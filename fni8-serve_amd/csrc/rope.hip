@@ -297,9 +297,9 @@ int launch_qkv_rows(const QkvRows& r, hipStream_t st) {
     a.page_log2 = r.slots ? __builtin_ctzll((uint64_t)r.page_size) : 0;
     a.kc = r.k_cache; a.vc = r.v_cache; a.ks = r.k_scale; a.vs = r.v_scale;
     const bool aligned = a.R % (a.pairs ? 8 : 16) == 0;
-    // three rows a lane share the angles and keep more loads in flight: 40 rows of 128 a token
-    // take 5.0 us at 256 tokens either way (5.9 with three), 9.5 at 1024, and 25 -> 23.5 at
-    // 4096
+    // three rows a lane group share the angles and keep more loads in flight: 40 rows of 128 a
+    // token, one against three, take 5.3 and 5.5 us at 64 tokens, 7.3 and 6.9 at 1024, 11.0
+    // and 9.7 at 2048, 18.0 and 16.9 at 4096, 35 and 28 (6.1 TB/s) at 8192
     const bool many = r.T * (a.Hq + a.Hk + a.Hv) >= 32768;
     if (r.D <= 64)
         many ? launch_rows<8, 3>(a, r.T, aligned, st) : launch_rows<8, 1>(a, r.T, aligned, st);

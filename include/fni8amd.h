@@ -454,8 +454,8 @@ int fni8_qk_norm_rope_f16(const void* q, int64_t ldq, int64_t hsq, int64_t Hq, c
  * launches in front of it).
  *   v          fp16 [T, Hk, D], strides ldv, hsv
  *   k_cache, v_cache  [num_pages, Hk, page_size, D], contiguous, 16-byte aligned: fp16, or
- *              int8 with k_scale, v_scale fp32 [num_pages, Hk, page_size] (both or neither);
- *              page_size a power of two from 16 to 65536; num_pages * page_size < 2^31;
+ *              int8 with k_scale, v_scale fp32 [num_pages, Hk, page_size], 16-byte aligned
+ *              (both or neither); page_size a power of two from 16 to 65536; num_pages * page_size < 2^31;
  *              D a multiple of 16
  *   slots      int32 [T]: page * page_size + offset of each token.  A slot outside the cache
  *              drops the token's key and value (negative: padding); its query is written
@@ -478,16 +478,18 @@ int fni8_rope_append_f16(const void* q, int64_t ldq, int64_t hsq, int64_t Hq, co
  * fni8serve/layers/gqa_attention.py:87,123,131,154,278, engine/kv_cache.py:785).
  *   q          fp16 [T, Hq, D], strides ldq, hsq as in fni8_qk_norm_rope_f16; Hq a multiple
  *              of Hk: query head h reads key head h / (Hq / Hk)
- *   k_cache .. page_size  as in fni8_rope_append_f16, the new tokens' rows in place
+ *   k_cache .. page_size  as in fni8_rope_append_f16, the new tokens' rows in place; scales
+ *              are not negative.  Places that hold no token may hold anything.
  *   block_tables  int32 [B, max_pages], row stride ldt: page of tokens c * page_size .. of
  *              sequence s in entry [s, c]; entries past a sequence's length, or wholly
- *              before its window, are not read as pages
+ *              before its window, are not read as pages; max_pages * page_size <= 2^30,
+ *              B <= 65536.  Pages may be shared by sequences.
  *   context_lens  int32 [B]: tokens of each sequence, the new ones among them
  *   cu_seqlens int32 [B + 1]: tokens cu[s] .. cu[s + 1] of q are sequence s's last ones;
  *              non-decreasing from 0; NULL: one token a sequence (T = B).  Tokens from cu[B]
  *              on are padding.
  *   max_seqlen no sequence has more new tokens (a bound that is too small costs time only)
- *   scale      factor of the scores; window 0, or the number of keys a query sees, itself
+ *   scale      factor of the scores, finite; window 0, or the number of keys a query sees, itself
  *              among them
  *   out        fp16 [T, Hq, D], contiguous, 16-byte aligned.  A query that sees no key, and
  *              padding, gives 0.
@@ -496,6 +498,9 @@ int fni8_rope_append_f16(const void* q, int64_t ldq, int64_t hsq, int64_t Hq, co
  *              One per stream.
  * Sums and softmax statistics are fp32, the weights of the values are rounded to fp16.  A
  * token whose page is not in the cache, or past the block table, counts as a key of NaN.
+ * Infinities and NaN in keys and values reach the queries that see them, and no others.
+ * More work units than 2^31 (about B * Hk * max_pages * page_size / 128) are refused with
+ * FNI8_ERR_SHAPE.
  */
 int fni8_paged_attention_f16(const void* q, int64_t ldq, int64_t hsq, int64_t T, int64_t Hq,
                              int64_t Hk, int64_t D, const void* k_cache, const void* v_cache,
