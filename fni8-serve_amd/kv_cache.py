@@ -58,7 +58,7 @@ class PagedKVCache:
 
     def step(self, block_tables: torch.Tensor, new: list[int], total: list[int]) -> Step:
         """The step that brings `new[s]` tokens to sequence s, the last of its `total[s]`.
-        block_tables [sequences, pages] on the cache's device."""
+        block_tables [sequences, pages]: the pages of each sequence's tokens, in order."""
         if len(new) != len(total) or len(new) != block_tables.shape[0]:
             raise ValueError(f"{len(new)} new and {len(total)} total lengths for "
                              f"{block_tables.shape[0]} block tables")
@@ -77,7 +77,7 @@ class PagedKVCache:
         host = torch.tensor(seq + pos + list(total) + cu, dtype=torch.int32)
         ints = (host.pin_memory() if dev.type == "cuda" else host).to(dev, non_blocking=True)
         seq, pos, lens, cu = ints.split([len(seq), len(seq), len(total), len(cu)])
-        tables = ops._int32(block_tables)
+        tables = ops._int32(block_tables).to(dev)
         return Step(pos, self.slots(tables, seq, pos), tables, lens, cu, max(new, default=0))
 
     def slots(self, block_tables: torch.Tensor, sequences: torch.Tensor,

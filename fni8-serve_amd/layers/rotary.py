@@ -16,7 +16,8 @@ stretches the positions for long contexts:
                                         attention_factor (Peng et al., YaRN, 2023)
 
 forward(q, k, positions) rotates [T, heads, head_dim] tensors into new ones: fp16 on the
-GPU through the kernel (`ops.rope`), anything else in fp32 by torch, as RMSNorm does.
+GPU through the kernel (`ops.rope`), anything else in fp32 by torch, as RMSNorm does.  A
+position outside the table gives NaN.
 """
 from __future__ import annotations
 
@@ -86,7 +87,10 @@ class RotaryEmbedding(nn.Module):
         return self
 
     def _rotate(self, x: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
-        cos, sin = self.cos_sin[positions.long()].unsqueeze(1).chunk(2, -1)
+        pos, last = positions.long(), self.cos_sin.shape[0] - 1
+        rows = self.cos_sin[pos.clamp(0, last)]
+        rows = rows.masked_fill(((pos < 0) | (pos > last)).unsqueeze(-1), math.nan)
+        cos, sin = rows.unsqueeze(1).chunk(2, -1)
         y = x.float()
         turn, rest = y[..., :self.rotary_dim], y[..., self.rotary_dim:]
         a, b = (turn[..., 0::2], turn[..., 1::2]) if self.interleaved else turn.chunk(2, -1)

@@ -748,8 +748,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     """Causal attention of new tokens over the paged cache, q [T, Hq, D] -> fp16 [T, Hq, D]
     (fni8serve/layers/gqa_attention.py:87,123,131,154,278).
 
-    Sequence s owns tokens cu_seqlens[s] .. cu_seqlens[s + 1] of q (None: one token a
-    sequence), the last of its context_lens[s] tokens; their keys and values are in the cache
+    Sequence s owns tokens cu_seqlens[s] .. cu_seqlens[s + 1] of q (from 0 on, not
+    decreasing; None: one token a sequence), the last of its context_lens[s] tokens; their keys and values are in the cache
     already, token c of the sequence in page block_tables[s, c // page_size].  Query head h
     reads key head h // (Hq / Hk).  max_seqlen bounds the new tokens of a sequence (None: not
     known; giving it saves a launch for decoded tokens).  scale defaults to D ** -0.5; window

@@ -194,6 +194,14 @@ def test_two_graphs_and_two_streams_at_once(pkg, cuda):
             assert torch.equal(out, w) and all(torch.equal(t, w) for t in got)
 
 
+def test_block_tables_on_the_host(pkg, cuda):
+    layer = _layer(pkg)
+    cache, tables = _cache(pkg, layer, [40, 20], 16, torch.float16)
+    a, b = cache.step(tables, [3, 1], [33, 20]), cache.step(tables.cpu(), [3, 1], [33, 20])
+    assert all(torch.equal(getattr(a, f), getattr(b, f)) for f in
+               ("positions", "slots", "block_tables", "context_lens", "cu_seqlens"))
+
+
 def test_the_current_stream_orders_the_calls(pkg, cuda):
     """Inputs made on a side stream behind slow work: the calls run on that stream."""
     layer = _layer(pkg)
@@ -302,6 +310,16 @@ def test_alignment_of_scales(pkg, cuda):
     off = torch.empty(ks.numel() + 1, device="cuda")[1:].view(ks.shape)
     with pytest.raises(ValueError, match="align"):
         pkg.paged_attention(q, kc, vc, tables, lens, k_scale=off, v_scale=vs)
+
+
+def test_too_many_workgroups_are_refused(pkg, cuda):
+    """Items of both kinds whose sum has no grid, though each kind alone has one."""
+    from importlib import import_module
+    lib = import_module("fni8serve_amd._lib").load()
+    f, B, T, Hk = ctypes.c_void_p(0x1000), 65536, 65536, 130  # nothing is read
+    rc = lib.fni8_paged_attention_f16(f, Hk * 16, 16, T, Hk, Hk, 16, f, f, None, None, 8, 16, f, 1,
+                                      1, f, f, B, 40, ctypes.c_float(1.0), 0, f, None, 0, None)
+    assert rc == -2 and b"too many" in lib.fni8_last_error()
 
 
 @pytest.mark.parametrize("new,lens", [([1] * 4, [900, 3, 0, 5000]), ([3, 5], [700, 5]),

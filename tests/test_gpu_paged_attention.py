@@ -85,7 +85,7 @@ def test_chunks(ops, cuda, new, old, Hq, Hk, D, page, int8):
 @pytest.mark.parametrize("new,old,window", [([300], [277], None), ([130, 1, 200, 3], [0, 500, 65, 9], None),
                                             ([260, 40], [100, 0], 70)])
 def test_chunks_of_many_heads(ops, cuda, new, old, window, int8):
-    """Enough rows for workgroups of eight waves."""
+    """Rows for more workgroups than the CUs hold at once."""
     _check(ops, new, [a + b for a, b in zip(new, old)], 256, 32, 128, 32, int8, seed=len(new),
            window=window)
 
@@ -258,6 +258,15 @@ def test_many_sequences(ops, cuda):
     _check(ops, [1] * 700, lens, 2, 1, 64, 16)
     new = [i % 3 for i in range(600)]
     _check(ops, new, [n + i % 50 for i, n in enumerate(new)], 4, 2, 64, 16, most=None)
+
+
+@pytest.mark.parametrize("B", [63, 64, 65, 300])
+@pytest.mark.parametrize("window", [None, 50])
+def test_chunks_and_single_tokens_of_many_sequences(ops, cuda, B, window):
+    """Sequences as many as a wave's lanes, one fewer and more, of lengths that repeat."""
+    new = [(1, 40, 0, 33, 2, 70)[i % 6] for i in range(B)]
+    lens = [n + (0, 100, 7)[i % 3] for i, n in enumerate(new)]
+    _check(ops, new, lens, 4, 1, 64, 16, int8=B == 65, seed=B, window=window)
 
 
 def test_long_cache_offsets(ops, cuda):

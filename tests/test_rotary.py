@@ -68,6 +68,13 @@ def test_rotary_refusals(pkg):
             pkg.RotaryEmbedding(**args)
 
 
+def test_positions_outside_the_table_on_the_cpu(pkg):
+    rot = pkg.RotaryEmbedding(16, 8, rotary_dim=8)
+    q, _ = rot(torch.ones(4, 2, 16), torch.ones(4, 1, 16), torch.tensor([0, -1, 8, 1 << 40]))
+    assert q[0].isfinite().all() and q[1:, :, :8].isnan().all()
+    assert (q[..., 8:] == 1).all()
+
+
 def test_table_stays_fp32(pkg):
     rot = pkg.RotaryEmbedding(64, 8)
     kept = rot.cos_sin.clone()
