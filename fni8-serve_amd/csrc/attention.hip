@@ -46,6 +46,11 @@ constexpr int kUnit = 128;      // keys of a unit of few_work: 32 for each of 4 
 constexpr int kTileRows = 128;  // of a workgroup of tile_kernel: 32 a wave
 constexpr int kTileKeys = 64;
 constexpr float kLag = 8.0f;
+// Block tables of so few units: an item is one workgroup's, and no join is launched.  One
+// decoded token a sequence, 8 key heads of 128, whole against split (us): 1 sequence of 100,
+// 250, 380, 500 keys 8.1, 10.1, 11.1, 12.1 against 9.6, 11.5, 11.5, 11.6 (8 bits 7.7, 9.6,
+// 11.4, 13.1 against 9.1, 10.9, 11.0, 11.0); 64 of 380 21.4 against 23.1.
+constexpr int kWholeUnits = 3;
 constexpr int kWorkers = 768;  // of few_work at most: three a CU
 // Beside tiles: one a CU, the tiles have the rest of it.  Decoded tokens beside one chunk, in
 // two launches, one with 512 workers and one with 256 (us): 120 of 2000 to 16000 keys beside
@@ -1458,6 +1463,7 @@ struct Plan {
     int64_t few;          // new tokens of a sequence that few_work takes at most
     bool use_few, use_tile;
     int64_t most_rows;    // of a sequence in few_work that keeps to the bound
+    bool whole;           // few_work splits no item
     int64_t workers;      // of few_work
     int64_t tiles;        // of kTileRows rows, at most
     int splits;
@@ -1480,6 +1486,7 @@ Plan plan_of(int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t B, int64_t mo
     p.use_few = !p.use_tile || B > 1;
     p.few = !p.use_tile ? 1 << 30 : p.use_few ? 16 * p.rb / group : 0;
     const int64_t units = (max_context + 1 + kUnit - 1) / kUnit;
+    p.whole = units <= kWholeUnits;
     p.workers = (B + 1 + T * group / (16 * p.rb)) * Hk * units;
     const int64_t most_workers = p.use_tile ? kMixedWorkers : kWorkers;
     p.workers = !p.use_few ? 0 : p.workers < most_workers ? p.workers : most_workers;
@@ -1498,8 +1505,10 @@ Plan plan_of(int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t B, int64_t mo
     if (p.splits < 1) p.splits = 1;
     // in this order, each a multiple of 256 bytes
     const auto round = [](int64_t n) { return (n + 255) & ~(int64_t)255; };
-    p.joins = round(p.workers * (int64_t)sizeof(Join));
-    p.part = round(p.workers * 2 * 16 * p.rb * (DP + 2) * 4);
+    if (!p.whole) {
+        p.joins = round(p.workers * (int64_t)sizeof(Join));
+        p.part = round(p.workers * 2 * 16 * p.rb * (DP + 2) * 4);
+    }
     if (p.use_tile && p.splits > 1) {
         p.tile_joins = round(items * (int64_t)sizeof(Join));
         p.tile_part = round(items * p.splits * kTileRows * (DP + 2) * 4);
@@ -1539,11 +1548,12 @@ int run_few(Attn& a, hipStream_t st) {
 
 template <int DP, bool I8>
 int run_all(Attn a, const Plan& p, hipStream_t st) {
-    a.whole = a.part == nullptr;
+    const bool parts = a.joins != nullptr;  // there is a workspace
+    a.whole = p.whole || !parts;
     a.workers = (int)p.workers;
     if (a.whole && p.use_few)
         a.workers = (int)((a.nseq + (p.use_tile ? 0 : (int64_t)a.T * a.group / (16 * p.rb))) * a.Hk);
-    a.splits = a.whole ? 1 : p.splits;
+    a.splits = parts ? p.splits : 1;
     const int64_t items = p.tiles * a.Hk;
     int rc;
     if (!p.use_tile) {
@@ -1556,7 +1566,8 @@ int run_all(Attn a, const Plan& p, hipStream_t st) {
     } else {
         rc = run(tile_kernel<DP, I8, false>, a, items * a.splits, tile_lds<DP, I8>(), st);
     }
-    if (rc || a.whole) return rc;
+    if (rc) return rc;
+    if (a.whole) a.workers = 0;  // none that leaves parts
     const bool few_parts = a.workers > 1, tile_parts = p.use_tile && a.splits > 1;
     if (!few_parts && !tile_parts) return FNI8_OK;
     // four of few_work's rows or 32 of a tile's a workgroup
