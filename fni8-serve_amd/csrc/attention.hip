@@ -67,6 +67,17 @@ struct Join {
     int start, row0, nrows, h;
 };
 
+// Division of 0 <= n < 2^31 by a divisor d that the host knows (Granlund and Montgomery,
+// 1994): with 2^shift the next power of two from d on and mul = floor(2^(32 + shift) / d) -
+// 2^32 + 1, n / d = (hi32(n mul) + n) >> shift.  Eight divisions stand before the first load
+// of a workgroup.
+struct Div {
+    uint32_t mul, shift;
+};
+__device__ __forceinline__ int over(int n, Div d) {
+    return (int)((__umulhi((uint32_t)n, d.mul) + (uint32_t)n) >> d.shift);
+}
+
 struct Attn {
     const uint16_t* q;
     int64_t ldq, hsq;
@@ -80,6 +91,7 @@ struct Attn {
     int T, Hq, Hk, D, group, num_pages, plog, max_pages, B, nseq, window, cap;
     float c;       // |scale| * log2 e, not 0
     uint32_t flip; // sign bits of two fp16 where the scale is negative: the queries' signs
+    Div by_group, by_heads, by_splits, by_quads;  // group, Hk, splits, D / 4
     int few;       // few_work takes sequences of at most so many new tokens, tiles the others
     int workers;   // workgroups of few_work
     int whole;     // few_work: no parts, an item is one unit
@@ -385,14 +397,14 @@ __device__ __forceinline__ void few_work(const Attn& a, const int worker, char* 
         const int real = a.whole || nt < f.tiles - tile ? nt : f.tiles - tile;
         const bool full = a.whole || real == f.tiles;
         if (real > 0) {
-        const int h = item % a.Hk, rb = item / a.Hk;
+        const int rb = over(item, a.by_heads), h = item - rb * a.Hk;
         const int steps = a.whole ? f.tiles : real;
         const int row0 = rb * 16 * RB;
         const int nrows = f.rows - row0 < 16 * RB ? f.rows - row0 : 16 * RB;
         const int lo = a.window && f.q.L - f.q.n - a.window + 1 > 0 ? f.q.L - f.q.n - a.window + 1 : 0;
         const int hi = f.q.L;
         const int p0 = f.q.L - f.q.n;
-        const int pmin = p0 + row0 / a.group, pmax = p0 + (row0 + nrows - 1) / a.group;
+        const int pmin = p0 + over(row0, a.by_group), pmax = p0 + over(row0 + nrows - 1, a.by_group);
         const int t_first = f.lo + tile * kUnit + wave * 32;
 
         // queries: row col of each block; the elements' order is the keys' (8 bits: two
@@ -403,7 +415,7 @@ __device__ __forceinline__ void few_work(const Attn& a, const int worker, char* 
 #pragma unroll
         for (int b = 0; b < RB; b++) {
             const int r = row0 + 16 * b + col;
-            const int i = r / a.group, head = h * a.group + r - i * a.group;
+            const int i = over(r, a.by_group), head = h * a.group + r - i * a.group;
             prow[b] = r < f.rows ? p0 + i : -1;
             // it sees the keys j with prow - span < j <= prow: one unsigned comparison
             span[b] = prow[b] < 0 ? 0 : a.window ? a.window : prow[b] + 1;
@@ -670,7 +682,7 @@ __device__ __forceinline__ void few_work(const Attn& a, const int worker, char* 
         const int D4 = a.D >> 2;
         float* part = a.part + (int64_t)(2 * worker + (first_unit == u ? 0 : 1)) * few_part<DP, RB>();
         for (int e = threadIdx.x; e < nrows * D4; e += 256) {
-            const int r = e / D4, d4 = e - r * D4;
+            const int r = over(e, a.by_quads), d4 = e - r * D4;
             float top = -kInf, wm[4];
 #pragma unroll
             for (int w = 0; w < 4; w++) {
@@ -689,7 +701,7 @@ __device__ __forceinline__ void few_work(const Attn& a, const int worker, char* 
             }
             if (full) {
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                const int rr = row0 + r, i = rr / a.group, head = h * a.group + rr - i * a.group;
+                const int rr = row0 + r, i = over(rr, a.by_group), head = h * a.group + rr - i * a.group;
                 uint2 y = {pack2(acc[0] * inv, acc[1] * inv), pack2(acc[2] * inv, acc[3] * inv)};
                 if (sum == 0.0f) y = uint2{0, 0};
                 *reinterpret_cast<uint2*>(a.out + ((int64_t)(f.q.start + i) * a.Hq + head) * a.D +
@@ -790,7 +802,7 @@ __device__ __forceinline__ void join_few(const Attn& a, int worker, int part_row
             for (int e = 0; e < 4; e++) acc[e] += __shfl_xor(acc[e], x, 64);
         if (grp != 0 || 4 * d4 >= a.D) continue;
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        const int rr = j.row0 + r, i = rr / a.group, head = j.h * a.group + rr - i * a.group;
+        const int rr = j.row0 + r, i = over(rr, a.by_group), head = j.h * a.group + rr - i * a.group;
         uint2 y = {pack2(acc[0] * inv, acc[1] * inv), pack2(acc[2] * inv, acc[3] * inv)};
         if (sum == 0.0f) y = uint2{0, 0};
         *reinterpret_cast<uint2*>(a.out + ((int64_t)(j.start + i) * a.Hq + head) * a.D + 4 * d4) = y;
@@ -824,7 +836,7 @@ __device__ __forceinline__ void join_tile(const Attn& a, int item) {
             acc += k * *reinterpret_cast<const f32x4*>(part + r * DP + 4 * d4);
         }
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        const int rr = j.row0 + r, i = rr / a.group, head = j.h * a.group + rr - i * a.group;
+        const int rr = j.row0 + r, i = over(rr, a.by_group), head = j.h * a.group + rr - i * a.group;
         uint2 y = {pack2(acc[0] * inv, acc[1] * inv), pack2(acc[2] * inv, acc[3] * inv)};
         if (sum == 0.0f) y = uint2{0, 0};
         *reinterpret_cast<uint2*>(a.out + ((int64_t)(j.start + i) * a.Hq + head) * a.D + 4 * d4) = y;
@@ -931,8 +943,8 @@ __device__ __forceinline__ bool tile_item(const Attn& a, int id, int h, int* sh,
     }
     t.rows = t.q.n * a.group;
     t.h = h;
-    const int i0 = t.tile * kTileRows / a.group;
-    int i1 = (t.tile * kTileRows + kTileRows - 1) / a.group;
+    const int i0 = over(t.tile * kTileRows, a.by_group);
+    int i1 = over(t.tile * kTileRows + kTileRows - 1, a.by_group);
     i1 = i1 < t.q.n ? i1 : t.q.n - 1;
     const int p0 = t.q.L - t.q.n;
     t.hi = p0 + i1 + 1 > 0 ? p0 + i1 + 1 : 0;
@@ -970,11 +982,11 @@ __global__ __launch_bounds__(256, tile_waves(DP, MIXED)) void tile_kernel(Attn a
     const int id = blockIdx.x - (MIXED ? a.workers : 0);
     // a key head's items are neighbours modulo the heads: with the round-robin dispatch
     // over the 8 XCDs they share an L2 where the heads divide 8
-    const int h = id % a.Hk, rest = id / a.Hk;
-    const int split = rest % a.splits;
+    const int rest = over(id, a.by_heads), h = id - rest * a.Hk;
+    const int item = over(rest, a.by_splits), split = rest - item * a.splits;
     TileItem t{};
-    const bool found = tile_item(a, rest / a.splits, h, sh, t);
-    const int index = rest / a.splits * a.Hk + h;
+    const bool found = tile_item(a, item, h, sh, t);
+    const int index = item * a.Hk + h;
     if (a.splits > 1 && split == 0 && threadIdx.x == 0) {
         const int tile_row0 = t.tile * kTileRows;
         Join j{0, 0, 0, 0, 0, 0, 0, 0};
@@ -990,11 +1002,11 @@ __global__ __launch_bounds__(256, tile_waves(DP, MIXED)) void tile_kernel(Attn a
     const int row0 = t.tile * kTileRows + wave * 32;
     const int p0 = t.q.L - t.q.n;
     const int nrows = t.rows - row0 < 32 ? t.rows - row0 : 32;  // may be 0 or less
-    const int pmin = p0 + row0 / a.group;
-    const int pmax = nrows > 0 ? p0 + (row0 + nrows - 1) / a.group : -1;
+    const int pmin = p0 + over(row0, a.by_group);
+    const int pmax = nrows > 0 ? p0 + over(row0 + nrows - 1, a.by_group) : -1;
     int prow = -1;
     h8 q[KS];
-    const int r = row0 + col, qi = r / a.group, head = h * a.group + r - qi * a.group;
+    const int r = row0 + col, qi = over(r, a.by_group), head = h * a.group + r - qi * a.group;
     if (r < t.rows) prow = p0 + qi;
 #pragma unroll
     for (int k = 0; k < KS; k++) {
@@ -1335,7 +1347,7 @@ __global__ __launch_bounds__(256, tile_waves(DP, MIXED)) void tile_kernel(Attn a
     };
 
     // What lies at the edge of some row of the workgroup (the same for its four waves).
-    const int wg_pmin = p0 + t.tile * kTileRows / a.group, wg_pmax = t.hi - 1;
+    const int wg_pmin = p0 + over(t.tile * kTileRows, a.by_group), wg_pmax = t.hi - 1;
     auto at_edge = [&](int kt) {
         return kt * kTileKeys + kTileKeys - 1 > wg_pmin ||
                (a.window && kt * kTileKeys <= wg_pmax - a.window);
@@ -1471,6 +1483,12 @@ struct Plan {
     int64_t joins, part, tile_joins, tile_part, bytes;
 };
 
+Div div_by(int64_t d) {
+    uint32_t shift = 0;
+    while (((int64_t)1 << shift) < d) shift++;
+    return {(uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << shift) - (uint64_t)d)) / (uint64_t)d + 1), shift};
+}
+
 int padded_dim(int64_t D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
 Plan plan_of(int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t B, int64_t most,
@@ -1554,6 +1572,7 @@ int run_all(Attn a, const Plan& p, hipStream_t st) {
     if (a.whole && p.use_few)
         a.workers = (int)((a.nseq + (p.use_tile ? 0 : (int64_t)a.T * a.group / (16 * p.rb))) * a.Hk);
     a.splits = parts ? p.splits : 1;
+    a.by_splits = div_by(a.splits);
     const int64_t items = p.tiles * a.Hk;
     int rc;
     if (!p.use_tile) {
@@ -1605,6 +1624,7 @@ int launch_paged_attention(const PagedAttention& p, hipStream_t st) {
     a.tables = p.block_tables; a.lens = p.context_lens; a.cu = p.cu_seqlens; a.ldt = p.ldt;
     a.out = p.out;
     a.T = (int)p.T; a.Hq = (int)p.Hq; a.Hk = (int)p.Hk; a.D = (int)p.D; a.group = (int)group;
+    a.by_group = div_by(group); a.by_heads = div_by(p.Hk); a.by_quads = div_by(p.D / 4);
     a.num_pages = (int)p.num_pages;
     a.plog = __builtin_ctzll((uint64_t)p.page_size);
     a.max_pages = (int)p.max_pages;
