@@ -101,6 +101,17 @@ struct Attn {
 struct Seq {
     int start, n, L;
 };
+// Where a token stands as a query: its own position, but past the block table (a.cap - 1
+// tokens) that of the first token there.  That one is a key of NaN, which such a query sees
+// whatever its window; the queries before it keep their positions and never see it.
+__device__ __forceinline__ int position(const Attn& a, const Seq& q, int i) {
+    const int p = q.L - q.n + i;
+    return p < a.cap - 1 ? p : a.cap - 1;
+}
+// The keys that any of its queries can see, from 0 on.
+__device__ __forceinline__ int keys_of(const Attn& a, const Seq& q) {
+    return q.L < a.cap ? q.L : a.cap;
+}
 
 __device__ __forceinline__ int bound_of(const Attn& a, int s) {
     if (s > a.B) return a.T;
@@ -117,8 +128,7 @@ __device__ __forceinline__ Seq sequence(const Attn& a, int s) {
     q.L = 0;
     if (s < a.B) {
         const int L = a.lens[s];
-        // tokens past the block table count as NaN: one of them is enough
-        q.L = L < 0 ? 0 : L < a.cap ? L : a.cap;
+        q.L = L < 0 ? 0 : L;
     }
     return q;
 }
@@ -345,9 +355,9 @@ __device__ __forceinline__ FewSeq few_seq(const Attn& a, const Seq& q) {
     f.q = q;
     f.rows = f.q.n > a.few ? 0 : f.q.n * a.group;
     f.blocks = (f.rows + 16 * RB - 1) / (16 * RB);
-    const int first = f.q.L - f.q.n;
+    const int first = position(a, f.q, 0);
     f.lo = a.window && first - a.window + 1 > 0 ? (first - a.window + 1) & ~31 : 0;
-    f.tiles = (f.q.L - f.lo + kUnit - 1) / kUnit;
+    f.tiles = (keys_of(a, f.q) - f.lo + kUnit - 1) / kUnit;
     f.tiles = f.tiles > 1 ? f.tiles : 1;
     f.units = f.blocks * a.Hk * (a.whole ? 1 : f.tiles + 1);
     return f;
@@ -401,10 +411,11 @@ __device__ __forceinline__ void few_work(const Attn& a, const int worker, char* 
         const int steps = a.whole ? f.tiles : real;
         const int row0 = rb * 16 * RB;
         const int nrows = f.rows - row0 < 16 * RB ? f.rows - row0 : 16 * RB;
-        const int lo = a.window && f.q.L - f.q.n - a.window + 1 > 0 ? f.q.L - f.q.n - a.window + 1 : 0;
-        const int hi = f.q.L;
-        const int p0 = f.q.L - f.q.n;
-        const int pmin = p0 + over(row0, a.by_group), pmax = p0 + over(row0 + nrows - 1, a.by_group);
+        const int first = position(a, f.q, 0);
+        const int lo = a.window && first - a.window + 1 > 0 ? first - a.window + 1 : 0;
+        const int hi = keys_of(a, f.q);
+        const int pmin = position(a, f.q, over(row0, a.by_group));
+        const int pmax = position(a, f.q, over(row0 + nrows - 1, a.by_group));
         const int t_first = f.lo + tile * kUnit + wave * 32;
 
         // queries: row col of each block; the elements' order is the keys' (8 bits: two
@@ -416,7 +427,7 @@ __device__ __forceinline__ void few_work(const Attn& a, const int worker, char* 
         for (int b = 0; b < RB; b++) {
             const int r = row0 + 16 * b + col;
             const int i = over(r, a.by_group), head = h * a.group + r - i * a.group;
-            prow[b] = r < f.rows ? p0 + i : -1;
+            prow[b] = r < f.rows ? position(a, f.q, i) : -1;
             // it sees the keys j with prow - span < j <= prow: one unsigned comparison
             span[b] = prow[b] < 0 ? 0 : a.window ? a.window : prow[b] + 1;
             seen0[b] = 4 * G - (prow[b] + 1 - (int)span[b]);
@@ -946,9 +957,9 @@ __device__ __forceinline__ bool tile_item(const Attn& a, int id, int h, int* sh,
     const int i0 = over(t.tile * kTileRows, a.by_group);
     int i1 = over(t.tile * kTileRows + kTileRows - 1, a.by_group);
     i1 = i1 < t.q.n ? i1 : t.q.n - 1;
-    const int p0 = t.q.L - t.q.n;
-    t.hi = p0 + i1 + 1 > 0 ? p0 + i1 + 1 : 0;
-    t.lo = a.window && p0 + i0 - a.window + 1 > 0 ? p0 + i0 - a.window + 1 : 0;
+    const int p0 = position(a, t.q, i0), p1 = position(a, t.q, i1);
+    t.hi = p1 + 1 > 0 ? p1 + 1 : 0;
+    t.lo = a.window && p0 - a.window + 1 > 0 ? p0 - a.window + 1 : 0;
     t.kt0 = t.lo / kTileKeys;
     t.kt1 = (t.hi + kTileKeys - 1) / kTileKeys;
     const int n = t.kt1 > t.kt0 ? t.kt1 - t.kt0 : 0;
@@ -1000,14 +1011,13 @@ __global__ __launch_bounds__(256, tile_waves(DP, MIXED)) void tile_kernel(Attn a
     const int last = first + t.per < t.kt1 ? first + t.per : t.kt1;
 
     const int row0 = t.tile * kTileRows + wave * 32;
-    const int p0 = t.q.L - t.q.n;
     const int nrows = t.rows - row0 < 32 ? t.rows - row0 : 32;  // may be 0 or less
-    const int pmin = p0 + over(row0, a.by_group);
-    const int pmax = nrows > 0 ? p0 + over(row0 + nrows - 1, a.by_group) : -1;
+    const int pmin = position(a, t.q, over(row0, a.by_group));
+    const int pmax = nrows > 0 ? position(a, t.q, over(row0 + nrows - 1, a.by_group)) : -1;
     int prow = -1;
     h8 q[KS];
     const int r = row0 + col, qi = over(r, a.by_group), head = h * a.group + r - qi * a.group;
-    if (r < t.rows) prow = p0 + qi;
+    if (r < t.rows) prow = position(a, t.q, qi);
 #pragma unroll
     for (int k = 0; k < KS; k++) {
         u32x4 v = {0, 0, 0, 0};
@@ -1347,7 +1357,7 @@ __global__ __launch_bounds__(256, tile_waves(DP, MIXED)) void tile_kernel(Attn a
     };
 
     // What lies at the edge of some row of the workgroup (the same for its four waves).
-    const int wg_pmin = p0 + over(t.tile * kTileRows, a.by_group), wg_pmax = t.hi - 1;
+    const int wg_pmin = position(a, t.q, over(t.tile * kTileRows, a.by_group)), wg_pmax = t.hi - 1;
     auto at_edge = [&](int kt) {
         return kt * kTileKeys + kTileKeys - 1 > wg_pmin ||
                (a.window && kt * kTileKeys <= wg_pmax - a.window);
