@@ -4,7 +4,8 @@
 // stands at p = L - n + i and sees the keys j, 0 <= j <= p, j > p - window:
 //   out = sum_j softmax_j(scale * q . k_j) v_j
 // with an online softmax: running maximum m, sum l and unnormalised output o in fp32, all
-// in powers of two (scores times scale * log2 e).  A row that sees no key is 0.
+// in powers of two (scores times scale * log2 e).  A row that sees no key (p < 0: it always
+// sees its own) is 0; one whose scores are all -inf has the sum 0 and gives 0 / 0, NaN.
 //
 // The query heads that share a key head are packed with the tokens into rows
 // r = i * group + head, so that one read of a key serves all of them.  Both kernels compute
@@ -65,6 +66,7 @@ struct Join {
     int parts;  // 0: nothing to do
     int first, next, step;
     int start, row0, nrows, h;
+    int p0;  // position of the sequence's first new token
 };
 
 // Division of 0 <= n < 2^31 by a divisor d that the host knows (Granlund and Montgomery,
@@ -711,10 +713,10 @@ __device__ __forceinline__ void few_work(const Attn& a, const int worker, char* 
                                smem + w * few_region<DP, RB>() + (r * DP + 4 * (d4 ^ (r & 7))) * 4);
             }
             if (full) {
-                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                const float inv = 1.0f / sum;
                 const int rr = row0 + r, i = over(rr, a.by_group), head = h * a.group + rr - i * a.group;
                 uint2 y = {pack2(acc[0] * inv, acc[1] * inv), pack2(acc[2] * inv, acc[3] * inv)};
-                if (sum == 0.0f) y = uint2{0, 0};
+                if (position(a, f.q, i) < 0) y = uint2{0, 0};
                 *reinterpret_cast<uint2*>(a.out + ((int64_t)(f.q.start + i) * a.Hq + head) * a.D +
                                           4 * d4) = y;
             } else {
@@ -728,7 +730,7 @@ __device__ __forceinline__ void few_work(const Attn& a, const int worker, char* 
         if (!full && tile == 0 && threadIdx.x == 0) {  // this run begins an item, others end it
             const int w0 = worker, w1 = (u + f.tiles - 1) / upw;
             a.joins[w0] = Join{w1 - w0 + 1, 2 * w0 + (first_unit == u ? 0 : 1), 2 * w0 + 2, 2,
-                               f.q.start, row0, nrows, h};
+                               f.q.start, row0, nrows, h, f.q.L - f.q.n};
         }
         }
         left -= nt;
@@ -812,10 +814,10 @@ __device__ __forceinline__ void join_few(const Attn& a, int worker, int part_row
 #pragma unroll
             for (int e = 0; e < 4; e++) acc[e] += __shfl_xor(acc[e], x, 64);
         if (grp != 0 || 4 * d4 >= a.D) continue;
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const float inv = 1.0f / sum;
         const int rr = j.row0 + r, i = over(rr, a.by_group), head = j.h * a.group + rr - i * a.group;
         uint2 y = {pack2(acc[0] * inv, acc[1] * inv), pack2(acc[2] * inv, acc[3] * inv)};
-        if (sum == 0.0f) y = uint2{0, 0};
+        if (j.p0 + i < 0) y = uint2{0, 0};
         *reinterpret_cast<uint2*>(a.out + ((int64_t)(j.start + i) * a.Hq + head) * a.D + 4 * d4) = y;
     }
 }
@@ -846,10 +848,10 @@ __device__ __forceinline__ void join_tile(const Attn& a, int item) {
             sum += k * part[kTileRows * (DP + 1) + r];
             acc += k * *reinterpret_cast<const f32x4*>(part + r * DP + 4 * d4);
         }
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const float inv = 1.0f / sum;
         const int rr = j.row0 + r, i = over(rr, a.by_group), head = j.h * a.group + rr - i * a.group;
         uint2 y = {pack2(acc[0] * inv, acc[1] * inv), pack2(acc[2] * inv, acc[3] * inv)};
-        if (sum == 0.0f) y = uint2{0, 0};
+        if (j.p0 + i < 0) y = uint2{0, 0};
         *reinterpret_cast<uint2*>(a.out + ((int64_t)(j.start + i) * a.Hq + head) * a.D + 4 * d4) = y;
     }
 }
@@ -1000,10 +1002,11 @@ __global__ __launch_bounds__(256, tile_waves(DP, MIXED)) void tile_kernel(Attn a
     const int index = item * a.Hk + h;
     if (a.splits > 1 && split == 0 && threadIdx.x == 0) {
         const int tile_row0 = t.tile * kTileRows;
-        Join j{0, 0, 0, 0, 0, 0, 0, 0};
+        Join j{};
         if (found && t.parts > 1)
             j = Join{t.parts, index * a.splits, index * a.splits + 1, 1, t.q.start, tile_row0,
-                     t.rows - tile_row0 < kTileRows ? t.rows - tile_row0 : kTileRows, h};
+                     t.rows - tile_row0 < kTileRows ? t.rows - tile_row0 : kTileRows, h,
+                     t.q.L - t.q.n};
         a.tile_joins[index] = j;
     }
     if (!found || split >= t.parts) return;
@@ -1463,7 +1466,7 @@ __global__ __launch_bounds__(256, tile_waves(DP, MIXED)) void tile_kernel(Attn a
         }
         return;
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float inv = 1.0f / l;
     uint16_t* dst = a.out + ((int64_t)(t.q.start + qi) * a.Hq + head) * a.D;
 #pragma unroll
     for (int d = 0; d < DB; d++)
@@ -1472,7 +1475,7 @@ __global__ __launch_bounds__(256, tile_waves(DP, MIXED)) void tile_kernel(Attn a
             const int at = 32 * d + 8 * e4 + 4 * H;
             uint2 y = {pack2(o[d][4 * e4] * inv, o[d][4 * e4 + 1] * inv),
                        pack2(o[d][4 * e4 + 2] * inv, o[d][4 * e4 + 3] * inv)};
-            if (l == 0.0f) y = uint2{0, 0};
+            if (prow < 0) y = uint2{0, 0};
             if (at < a.D) *reinterpret_cast<uint2*>(dst + at) = y;
         }
 }

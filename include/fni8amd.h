@@ -499,7 +499,8 @@ int fni8_rope_append_f16(const void* q, int64_t ldq, int64_t hsq, int64_t Hq, co
  * Sums and softmax statistics are fp32, the weights of the values are rounded to fp16.  A
  * token whose page is not in the cache, or past the block table, counts as a key of NaN;
  * the tokens before it are not moved by it.
- * Infinities and NaN in keys and values reach the queries that see them, and no others.
+ * Infinities and NaN in keys and values reach the queries that see them, and no others; a
+ * query whose scores are all -infinity has no softmax and gives NaN.
  * More work units than 2^31 (about B * Hk * max_pages * page_size / 128) are refused with
  * FNI8_ERR_SHAPE.
  */
