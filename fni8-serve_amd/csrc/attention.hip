@@ -27,6 +27,8 @@
 // workgroup share K and V tiles of 64 keys in LDS; the MFMAs, and the card's power under
 // them, bound it.  A batch of both kinds is one launch, so that the reads of the one pass
 // beside the products of the other.
+#include <atomic>
+
 #include "common.h"
 
 namespace {
@@ -1548,25 +1550,26 @@ Plan plan_of(int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t B, int64_t mo
     return p;
 }
 
-template <class K>
-int allow_lds(K kernel, int bytes) {
-    static bool done[64];
+// The LDS limit is an attribute of a kernel on a device: a flag for each pair.
+template <auto kernel>
+int allow_lds(int bytes) {
+    static std::atomic<bool> done[64];
     int dev = 0;
     (void)hipGetDevice(&dev);
-    if (dev >= 0 && dev < 64 && done[dev]) return FNI8_OK;
+    if (dev >= 0 && dev < 64 && done[dev].load(std::memory_order_relaxed)) return FNI8_OK;
     const hipError_t e = hipFuncSetAttribute((const void*)kernel,
                                              hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != hipSuccess) {
         fni8h::set_error_detail("LDS attribute (%d bytes): %s", bytes, hipGetErrorString(e));
         return FNI8_ERR_LAUNCH;
     }
-    if (dev >= 0 && dev < 64) done[dev] = true;
+    if (dev >= 0 && dev < 64) done[dev].store(true, std::memory_order_relaxed);
     return FNI8_OK;
 }
 
-template <class K>
-int run(K kernel, const Attn& a, int64_t grid, int lds, hipStream_t st) {
-    const int rc = allow_lds(kernel, lds);
+template <auto kernel>
+int run(const Attn& a, int64_t grid, int lds, hipStream_t st) {
+    const int rc = allow_lds<kernel>(lds);
     if (rc == FNI8_OK) kernel<<<dim3((uint32_t)grid), 256, lds, st>>>(a);
     return rc;
 }
@@ -1574,7 +1577,7 @@ int run(K kernel, const Attn& a, int64_t grid, int lds, hipStream_t st) {
 template <int DP, bool I8, int RB>
 int run_few(Attn& a, hipStream_t st) {
     if (!a.whole && a.workers > 256 * few_waves(DP, RB)) a.workers = 256 * few_waves(DP, RB);
-    return run(few_kernel<DP, I8, RB>, a, a.workers, few_lds<DP, RB>(), st);
+    return run<few_kernel<DP, I8, RB>>(a, a.workers, few_lds<DP, RB>(), st);
 }
 
 template <int DP, bool I8>
@@ -1594,9 +1597,9 @@ int run_all(Attn a, const Plan& p, hipStream_t st) {
         else
             rc = run_few<DP, I8, 1>(a, st);
     } else if (p.use_few) {
-        rc = run(tile_kernel<DP, I8, true>, a, a.workers + items * a.splits, tile_lds<DP, I8>(), st);
+        rc = run<tile_kernel<DP, I8, true>>(a, a.workers + items * a.splits, tile_lds<DP, I8>(), st);
     } else {
-        rc = run(tile_kernel<DP, I8, false>, a, items * a.splits, tile_lds<DP, I8>(), st);
+        rc = run<tile_kernel<DP, I8, false>>(a, items * a.splits, tile_lds<DP, I8>(), st);
     }
     if (rc) return rc;
     if (a.whole) a.workers = 0;  // none that leaves parts
