@@ -617,6 +617,7 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
             most = integer(a[8]);
             need(most >= 0);
         }
+        if (!cu) most = 1;
         const float scale = a[9] == Py_None ? (float)std::pow((double)h.D, -0.5) : (float)real(a[9]);
         int64_t window = 0;
         if (a[10] != Py_None) {

@@ -752,7 +752,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     decreasing; None: one token a sequence), the last of its context_lens[s] tokens; their keys and values are in the cache
     already, token c of the sequence in page block_tables[s, c // page_size].  Query head h
     reads key head h // (Hq / Hk).  max_seqlen bounds the new tokens of a sequence (None: not
-    known; giving it saves a launch for decoded tokens).  scale defaults to D ** -0.5; window
+    known; giving it saves time for decoded tokens; without cu_seqlens it is 1 whatever it
+    says).  scale defaults to D ** -0.5; window
     is the number of keys that a query sees, itself among them.  A query without keys and
     tokens past cu_seqlens[-1] give 0; a token whose page is not in the cache counts as NaN."""
     if q.is_cuda:
@@ -789,7 +790,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if width > 1 and tables.stride(1) != 1 or B > 1 and tables.stride(0) < width:
         tables = tables.contiguous()
     ldt = tables.stride(0) if B > 1 else width
-    most = T if max_seqlen is None else max_seqlen
+    most = 1 if cu is None else T if max_seqlen is None else max_seqlen
     nw = int(_lib.load().fni8_paged_attention_workspace_bytes(T, Hq, Hk, D, B, most, width * page))
     work = torch.empty(nw, dtype=torch.uint8, device=dev) if nw else None
     with torch.cuda.device(dev):

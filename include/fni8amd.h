@@ -488,7 +488,8 @@ int fni8_rope_append_f16(const void* q, int64_t ldq, int64_t hsq, int64_t Hq, co
  *   cu_seqlens int32 [B + 1]: tokens cu[s] .. cu[s + 1] of q are sequence s's last ones;
  *              non-decreasing from 0; NULL: one token a sequence (T = B).  Tokens from cu[B]
  *              on are padding.
- *   max_seqlen no sequence has more new tokens (a bound that is too small costs time only)
+ *   max_seqlen no sequence has more new tokens (a bound that is too small costs time only);
+ *              without cu_seqlens it is taken as 1
  *   scale      factor of the scores, finite; window 0, or the number of keys a query sees, itself
  *              among them
  *   out        fp16 [T, Hq, D], contiguous, 16-byte aligned.  A query that sees no key, and
@@ -515,7 +516,8 @@ int fni8_paged_attention_f16(const void* q, int64_t ldq, int64_t hsq, int64_t T,
 
 /*
  * Workspace bytes of fni8_paged_attention_f16 (0: none) for block tables that reach
- * max_context tokens: the parts of the sums where the keys of a query are split.
+ * max_context tokens: the parts of the sums where the keys of a query are split.  max_seqlen
+ * is that of the call; 1 for a call without cu_seqlens.  Any window may use it.
  */
 int64_t fni8_paged_attention_workspace_bytes(int64_t T, int64_t Hq, int64_t Hk, int64_t D,
                                              int64_t B, int64_t max_seqlen, int64_t max_context);

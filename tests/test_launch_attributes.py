@@ -80,7 +80,8 @@ for c in json.loads(sys.argv[3]):
     n = size(T, Hq, Hk, D, B, most, width * page) if c.get("work", True) else 0
     stand_in.forget()
     rc = call(f, Hq * D, D, T, Hq, Hk, D, f, f, scale, scale, 1 << 10, page, f, width, width, f,
-              None if c.get("cu") is False else f, B, most, 0.1, 0, f, f if n else None, n, None)
+              None if c.get("cu") is False else f, B, most, 0.1, c.get("window", 0), f,
+              f if n else None, n + (c.get("more", 0) if n else 0), None)
     lines = [[int(x) for x in l.split()] for l in stand_in.recorded().decode().splitlines()]
     out.append({"rc": rc, "work": n, "launches": lines})
 print(json.dumps(out))
@@ -127,3 +128,17 @@ def test_each_kernel_gets_its_own_lds_limit(pkg, launches):
                     assert limit >= lds, (c, lds, limit)
                     seen.add((c["D"], lds))
     assert {D for D, _ in seen} == {128, 256}  # those of 64 elements take less
+
+
+def test_the_workspace_is_enough(pkg, launches):
+    """The size that the library names is all that a call can use: more changes no launch.
+    Decoded tokens without cu_seqlens are one a sequence; their keys are split."""
+    calls = [_call(D, B * most if cu else B, B, most, Hk=Hk, cu=cu, width=width, page=16, window=w)
+             for D in (64, 128, 256) for Hk in (2, 8) for B in (1, 5, 64, 256, 512)
+             for cu, most in ((False, 1), (True, 1), (True, 6), (True, 40)) for width in (20, 32, 1000)
+             for w in (0, 100)]
+    exact, more = launches(calls), launches([dict(c, more=1 << 40) for c in calls])
+    for c, a, b in zip(calls, exact, more):
+        assert a["rc"] == 0 and a["launches"] == b["launches"], c
+        if not c["cu"] and c["width"] > 24:
+            assert a["work"] and len(a["launches"]) == 2, c
