@@ -67,25 +67,45 @@ class PagedKVCache:
         if any(-(-t // self.page_size) > block_tables.shape[1] for t in total):
             raise ValueError(f"a sequence of {max(total)} tokens needs more than "
                              f"{block_tables.shape[1]} pages of {self.page_size}")
-        dev = self.k.device
-        seq = [s for s, n in enumerate(new) for _ in range(n)]
-        pos = [p for n, t in zip(new, total) for p in range(t - n, t)]
+        dev, width, shift = self.k.device, block_tables.shape[1], self.page_size.bit_length() - 1
+        pos, at = [], []  # positions, and the place of each token's page in the tables
+        for s, (n, t) in enumerate(zip(new, total)):
+            first = s * width
+            pos += range(t - n, t)
+            at += [first + (p >> shift) for p in range(t - n, t)]
         cu = [0]
         for n in new:
             cu.append(cu[-1] + n)
-        # one copy to the device: sequences, positions, lengths, bounds
-        host = torch.tensor(seq + pos + list(total) + cu, dtype=torch.int32)
+        # one copy to the device: places, positions, lengths, bounds
+        host = torch.tensor(at + pos + list(total) + cu, dtype=torch.int32)
         ints = (host.pin_memory() if dev.type == "cuda" else host).to(dev, non_blocking=True)
-        seq, pos, lens, cu = ints.split([len(seq), len(seq), len(total), len(cu)])
+        at, pos, lens, cu = ints.split([len(at), len(at), len(total), len(cu)])
         tables = ops._int32(block_tables).to(dev)
-        return Step(pos, self.slots(tables, seq, pos), tables, lens, cu, max(new, default=0))
+        slots = self._place(tables.reshape(-1).index_select(0, at), pos)
+        return Step(pos, slots, tables, lens, cu, max(new, default=0))
 
     def slots(self, block_tables: torch.Tensor, sequences: torch.Tensor,
               positions: torch.Tensor) -> torch.Tensor:
-        """int32 slots of tokens at `positions` of `sequences` (rows of block_tables)."""
+        """int32 slots of tokens at `positions` of `sequences` (rows of block_tables).  A token
+        that has none gets one outside the cache, which append drops: its position is negative
+        (padding) or past the table, its sequence not in the table or its page not in the
+        cache."""
+        if block_tables.numel() == 0:
+            return torch.full_like(positions, -1, dtype=torch.int32)
+        rows, width = block_tables.shape
         shift = self.page_size.bit_length() - 1
-        page = block_tables[sequences.long(), (positions >> shift).long()]
-        return ((page << shift) + (positions & (self.page_size - 1))).to(torch.int32)
+        column, sequences = positions.long() >> shift, sequences.long()
+        row, at = sequences.clamp(0, rows - 1), column.clamp(0, width - 1)
+        page = torch.where((row == sequences) & (at == column), block_tables[row, at], -1)
+        return self._place(page, positions)
+
+    def _place(self, page: torch.Tensor, position: torch.Tensor) -> torch.Tensor:
+        """int32 slots of tokens in their pages.  A page that is not in the cache counts as the
+        one before the first or behind the last, whose slots 32 bits hold too: a larger number
+        could wrap to a valid slot."""
+        page = page.clamp(-1, self.num_pages).to(torch.int32)
+        offset = (position & (self.page_size - 1)).to(torch.int32)
+        return torch.add(offset, page, alpha=self.page_size)
 
     def append(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, step: Step,
                cos_sin: torch.Tensor | None = None, q_weight: torch.Tensor | None = None,
