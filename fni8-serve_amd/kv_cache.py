@@ -15,6 +15,7 @@ synchronises, and a step's tensors may be filled anew between replays of a graph
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 
 import torch
@@ -126,11 +127,14 @@ class PagedKVCache:
                                    v_scale=self.v_scale, scale=scale, window=window)
 
     def read(self, slots: torch.Tensor):
-        """Keys and values at `slots`, as the numbers they stand for: fp32 [n, heads, head_dim]."""
+        """Keys and values at `slots`, as the numbers they stand for: fp32 [n, heads, head_dim],
+        NaN for a slot outside the cache."""
         slots = slots.long()
-        page, at = slots // self.page_size, slots % self.page_size
+        row = slots.clamp(0, self.num_pages * self.page_size - 1)
+        page, at, outside = row // self.page_size, row % self.page_size, (row != slots)[:, None, None]
         out = []
         for x, s in ((self.k, self.k_scale), (self.v, self.v_scale)):
             rows = x[page, :, at].float()
-            out.append(rows if s is None else rows * s[page, :, at].unsqueeze(-1))
+            rows = rows if s is None else rows * s[page, :, at].unsqueeze(-1)
+            out.append(rows.masked_fill(outside, math.nan))
         return out[0], out[1]

@@ -56,3 +56,21 @@ def test_a_step_with_a_page_outside_the_cache(pkg):
         tables = torch.tensor([[7, 1 << 28], [1 << 30, 3], [-1, 10]], dtype=dtype)
         step = cache.step(tables, [2, 3, 2], [17, 18, 17])
         assert _known(cache, step.slots).tolist() == [7 * 16 + 15, -1, -1, 3 * 16, 3 * 16 + 1, -1, -1]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.int8])
+def test_reading_outside_the_cache(pkg, dtype):
+    """Slots of padding and past the cache read as NaN, beside those that are there."""
+    cache = pkg.PagedKVCache(3, 16, 2, 32, dtype, device="cpu")
+    for x in (cache.k, cache.v):
+        x.copy_(torch.randint(-9, 9, x.shape, generator=torch.Generator().manual_seed(1)))
+    if dtype == torch.int8:
+        cache.k_scale.fill_(0.5), cache.v_scale.fill_(0.25)
+    slots = torch.tensor([-1, 47, 48, -(1 << 31), (1 << 31) - 1, 5], dtype=torch.int32)
+    for got, x, s in zip(cache.read(slots), (cache.k, cache.v), (0.5, 0.25)):
+        s = s if dtype == torch.int8 else 1.0
+        assert got[[0, 2, 3, 4]].isnan().all()
+        assert torch.equal(got[1], x[2, :, 15].float() * s)
+        assert torch.equal(got[5], x[0, :, 5].float() * s)
+    assert cache.read(slots[:0])[0].shape == (0, 2, 32)
+    assert cache.read(torch.tensor([1 << 40]))[1].isnan().all()
