@@ -10,8 +10,9 @@ caller's (a block table a sequence); a token's slot is page * page_size + offset
     q = cache.append(q, k, v, step, cos_sin, q_weight=..., k_weight=...)
     out = cache.attend(q, step)
 
-The arithmetic runs in `ops.rope_append` and `ops.paged_attention`; nothing here
-synchronises, and a step's tensors may be filled anew between replays of a graph.
+The arithmetic runs in `ops.rope_append` and `ops.paged_attention`; nothing here waits for
+the GPU (`step` sends what lies on the host, its block tables among it, from pinned memory in
+one copy), and a step's tensors may be filled anew between replays of a graph.
 """
 from __future__ import annotations
 
@@ -59,7 +60,8 @@ class PagedKVCache:
 
     def step(self, block_tables: torch.Tensor, new: list[int], total: list[int]) -> Step:
         """The step that brings `new[s]` tokens to sequence s, the last of its `total[s]`.
-        block_tables [sequences, pages]: the pages of each sequence's tokens, in order."""
+        block_tables [sequences, pages], on the GPU or the host: the pages of each sequence's
+        tokens, in order."""
         if len(new) != len(total) or len(new) != block_tables.shape[0]:
             raise ValueError(f"{len(new)} new and {len(total)} total lengths for "
                              f"{block_tables.shape[0]} block tables")
@@ -77,11 +79,17 @@ class PagedKVCache:
         cu = [0]
         for n in new:
             cu.append(cu[-1] + n)
-        # one copy to the device: places, positions, lengths, bounds
+        # one copy to the device, from pinned memory: places, positions, lengths, bounds, tables
+        # that lie on the host
         host = torch.tensor(at + pos + list(total) + cu, dtype=torch.int32)
+        tables = ops._int32(block_tables)
+        packed = tables.device != dev and tables.device.type == "cpu"
+        if packed:
+            host = torch.cat([host, tables.reshape(-1)])
         ints = (host.pin_memory() if dev.type == "cuda" else host).to(dev, non_blocking=True)
-        at, pos, lens, cu = ints.split([len(at), len(at), len(total), len(cu)])
-        tables = ops._int32(block_tables).to(dev)
+        at, pos, lens, cu, flat = ints.split([len(at), len(at), len(total), len(cu),
+                                              len(ints) - 2 * len(at) - len(total) - len(cu)])
+        tables = flat.view(tables.shape) if packed else tables.to(dev)
         slots = self._place(tables.reshape(-1).index_select(0, at), pos)
         return Step(pos, slots, tables, lens, cu, max(new, default=0))
 
