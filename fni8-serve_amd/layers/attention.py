@@ -8,15 +8,21 @@ of prompts, mixed) through the QKV linear; the norm of every query and key head,
 rotation and the append to the cache in one launch; attention over the cache; and the O
 linear (gqa_attention.py:62-100, :143-157).  Nothing synchronises, so a decode step can be
 captured in a graph with its tensors filled anew between replays.
+
+Where calling a norm or the rotation does more than its class defines (a hook, a forward of
+its own, a subclass) or the norms are not of one kind, the modules are called one after the
+other; a normed head is then rounded to fp16 before it is rotated.
 """
 from __future__ import annotations
 
 import torch
 import torch.nn as nn
+from torch.nn.modules.module import _has_any_global_hook
 
 from ..kv_cache import PagedKVCache, Step
 from ..qtensor import QTensor
 from .linear import LinearW8A8
+from .mlp import bare
 from .norm import RMSNorm
 from .rotary import RotaryEmbedding
 
@@ -52,13 +58,29 @@ class GQAAttention(nn.Module):
         cache afterwards."""
         D, nq, nk = self.head_dim, self.num_heads * self.head_dim, self.num_kv_heads * self.head_dim
         q, k, v = (t.unflatten(-1, (-1, D)) for t in self.qkv_proj(x).split([nq, nk, nk], -1))
-        norm = self.q_norm if self.q_norm is not None else self.k_norm
-        rotary = self.rotary
-        q = cache.append(q, k, v, step, None if rotary is None else rotary.cos_sin,
-                         q_weight=None if self.q_norm is None else self.q_norm.weight,
-                         k_weight=None if self.k_norm is None else self.k_norm.weight,
-                         eps=1e-6 if norm is None else norm.eps,
-                         interleaved=rotary is not None and rotary.interleaved,
-                         unit_offset=norm is not None and norm.add_unit_offset)
+        q_norm, k_norm, rotary = self.q_norm, self.k_norm, self.rotary
+        if self._in_one_launch():
+            norm = q_norm if q_norm is not None else k_norm
+            q = cache.append(q, k, v, step, None if rotary is None else rotary.cos_sin,
+                             q_weight=None if q_norm is None else q_norm.weight,
+                             k_weight=None if k_norm is None else k_norm.weight,
+                             eps=1e-6 if norm is None else norm.eps,
+                             interleaved=rotary is not None and rotary.interleaved,
+                             unit_offset=norm is not None and norm.add_unit_offset)
+        else:
+            q = q if q_norm is None else q_norm(q)
+            k = k if k_norm is None else k_norm(k)
+            if rotary is not None:
+                q, k = rotary(q, k, step.positions)
+            q = cache.append(q, k, v, step)
         out = cache.attend(q, step, scale=self.scale, window=self.window)
         return self.o_proj(out.flatten(1))
+
+    def _in_one_launch(self) -> bool:
+        """Whether the norms and the rotation are what the append computes on its way."""
+        norms = [n for n in (self.q_norm, self.k_norm) if n is not None]
+        return ((self.rotary is None or bare(self.rotary, RotaryEmbedding))
+                and all(bare(n, RMSNorm) and n.weight.dtype == torch.float16
+                        and n.eps == norms[0].eps
+                        and n.add_unit_offset == norms[0].add_unit_offset for n in norms)
+                and not _has_any_global_hook())

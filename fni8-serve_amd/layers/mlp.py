@@ -19,6 +19,8 @@ from .. import ops
 from ..qtensor import QTensor
 from .activation import GeluAndMul, SiluAndMul, fused_act, get_act_and_mul
 from .linear import LinearW8A8
+from .norm import RMSNorm
+from .rotary import RotaryEmbedding
 
 # Rows from which the fused activation + quantization feeds the down projection.
 # Below it the unfused chain is faster: up to 4 rows the down projection's
@@ -33,7 +35,7 @@ FUSE_MIN_ROWS = 5
 # a linear, the rule that it asks.
 _CALL = getattr(nn.Module, "_wrapped_call_impl", None)
 _DEFINED = {cls: (cls.forward, getattr(cls, "_int8_ok", None))
-            for cls in (LinearW8A8, SiluAndMul, GeluAndMul)}
+            for cls in (LinearW8A8, SiluAndMul, GeluAndMul, RMSNorm, RotaryEmbedding)}
 
 
 def bare(m: nn.Module, cls: type) -> bool:
