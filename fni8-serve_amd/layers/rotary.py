@@ -16,8 +16,8 @@ stretches the positions for long contexts:
                                         attention_factor (Peng et al., YaRN, 2023)
 
 forward(q, k, positions) rotates [T, heads, head_dim] tensors into new ones: fp16 on the
-GPU through the kernel (`ops.rope`), anything else in fp32 by torch, as RMSNorm does.  A
-position outside the table gives NaN.
+GPU, of a head_dim that is a multiple of 8 and at most 256, through the kernel (`ops.rope`),
+anything else in fp32 by torch, as RMSNorm does.  A position outside the table gives NaN.
 """
 from __future__ import annotations
 
@@ -99,6 +99,7 @@ class RotaryEmbedding(nn.Module):
         return torch.cat([turn, rest], -1).to(x.dtype)
 
     def forward(self, q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor):
-        if q.is_cuda and q.dtype == torch.float16 and k.dtype == torch.float16:
+        if (q.is_cuda and q.dtype == torch.float16 and k.dtype == torch.float16
+                and self.head_dim % 8 == 0 and self.head_dim <= 256):
             return ops.rope(q, k, positions, self.cos_sin, interleaved=self.interleaved)
         return self._rotate(q, positions), self._rotate(k, positions)
