@@ -59,6 +59,8 @@ def _frequencies(rotary_dim: int, base: float, scaling: dict | None):
     high = min(math.ceil(pair_of(slow)), rotary_dim - 1)
     ramp = ((torch.arange(rotary_dim // 2, dtype=torch.float64) - low)
             / max(high - low, 0.001)).clamp(0, 1)
+    if high <= 0:  # the first pair already turns less than `slow` times
+        ramp = torch.ones_like(ramp)
     factor_of = scaling.get("attention_factor")
     return (freq / factor * ramp + freq * (1 - ramp),
             0.1 * math.log(factor) + 1.0 if factor_of is None else float(factor_of))
