@@ -1626,10 +1626,10 @@ int launch_paged_attention(const PagedAttention& p, hipStream_t st) {
     const int64_t context = p.max_pages * p.page_size;
     const Plan plan = plan_of(p.T, p.Hq, p.Hk, p.D, p.B, p.max_seqlen, context, p.window);
     const int64_t group = p.Hq / p.Hk;
-    // the units' sums are 32 bits, a grid has 2^32 threads
+    // the units' sums, rounded up to the workers', are 32 bits, a grid has 2^32 threads
     const int64_t items = (p.B + 1 + (plan.use_tile ? 0 : p.T * group / (16 * plan.rb))) * p.Hk;
     const int64_t blocks = items + (plan.use_tile ? plan.tiles * p.Hk * plan.splits : 0);
-    if (items * ((context + kUnit) / kUnit + 1) >= (int64_t)1 << 31 || blocks >= (int64_t)1 << 24) {
+    if (items * ((context + kUnit) / kUnit + 1) + kWorkers > (int64_t)1 << 31 || blocks >= (int64_t)1 << 24) {
         set_error_detail("T=%lld tokens of %lld sequences and %lld keys are too many for one call",
                          (long long)p.T, (long long)p.B, (long long)context);
         return FNI8_ERR_SHAPE;

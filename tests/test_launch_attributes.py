@@ -142,3 +142,15 @@ def test_the_workspace_is_enough(pkg, launches):
         assert a["rc"] == 0 and a["launches"] == b["launches"], c
         if not c["cu"] and c["width"] > 24:
             assert a["work"] and len(a["launches"]) == 2, c
+
+
+def test_the_sum_of_units_and_workers_stays_in_32_bits(pkg, launches):
+    """Units close to 2^31: the workgroups' run of units, their number rounded up, is computed
+    from the sum of both."""
+    call = _call(64, 40438, 40438, 1, Hq=1, Hk=1, cu=False, page=128, width=49979)
+    items, units = 40438 + 1 + 40438 // 16, 49979 + 2
+    assert 2 ** 31 - 768 <= items * units < 2 ** 31
+    few = dict(call, width=49979 - 20)  # a million units fewer
+    refused, taken = launches([call, few])
+    assert refused["rc"] == -2 and not refused["launches"]
+    assert taken["rc"] == 0 and len(taken["launches"]) == 2
