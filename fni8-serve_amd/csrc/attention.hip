@@ -730,7 +730,11 @@ __device__ __forceinline__ void few_work(const Attn& a, const int worker, char* 
             }
         }
         if (!full && tile == 0 && threadIdx.x == 0) {  // this run begins an item, others end it
-            const int w0 = worker, w1 = (u + f.tiles - 1) / upw;
+            // (a cu_seqlens that is not one can have more units than the list's 32-bit sum says:
+            // the join reads no part behind the last workgroup's)
+            int w1 = (u + f.tiles - 1) / upw;
+            w1 = w1 < a.workers ? w1 : a.workers - 1;
+            const int w0 = worker;
             a.joins[w0] = Join{w1 - w0 + 1, 2 * w0 + (first_unit == u ? 0 : 1), 2 * w0 + 2, 2,
                                f.q.start, row0, nrows, h, f.q.L - f.q.n};
         }
