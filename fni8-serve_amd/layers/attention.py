@@ -39,7 +39,7 @@ class GQAAttention(nn.Module):
         self.rotary, self.q_norm, self.k_norm = rotary, q_norm, k_norm
         self.scale, self.window = scale, window
         wide = (num_heads + 2 * num_kv_heads) * head_dim
-        if num_heads % num_kv_heads:
+        if num_heads < 1 or num_kv_heads < 1 or num_heads % num_kv_heads:
             raise ValueError(f"{num_heads} query heads are no multiple of {num_kv_heads} key heads")
         if self.qkv_proj.out_features != wide or self.o_proj.in_features != num_heads * head_dim:
             raise ValueError(f"qkv has {self.qkv_proj.out_features} outputs and o "
