@@ -15,10 +15,17 @@
 // long as both operands agree, so the keys of P stay where S^T left them, and V^T is read
 // from row-major V in LDS with transposing reads (4 keys x 16 elements) in the same order.
 //
+// The weights P are rounded to fp16 before their product with V, the one rounding below fp32
+// between the inputs and the result: that product's MFMA takes 16-bit operands, and P in two
+// halves would double its count, half of all products.  l adds the weights unrounded.  Each
+// is off by 2^-11 of itself at most (2^-25 of 1 where it is small); the measured cases are
+// 2.3e-4 to 2.9e-4 from 64 bits in their norm, of which the result's own rounding to fp16
+// makes 2.1e-4.
+//
 // 8 bits: the codes go through the matrix cores as fp16 integers (exact).  A key's scale
 // multiplies its column of S.  A value's scale v_s joins the exponent instead of P:
-// P' = 2^(s + log2 v_s - m) with m the maximum of s + log2 v_s, so P' <= 1 rounds to fp16
-// like P does whatever the scale's size, and l adds P' / v_s.
+// P' = 2^(s + log2 v_s - m) with m the maximum of s + log2 v_s (or up to kLag below it), so P'
+// rounds to fp16 like P does whatever the scale's size, and l adds P' / v_s.
 //
 // few_work takes sequences with few rows (decode, drafted tokens): memory bounds it, each
 // cached row is read once.  The keys of all sequences are one list of units of 128 keys,

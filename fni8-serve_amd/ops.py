@@ -12,7 +12,8 @@ never synchronises, so the calls can be captured in a HIP graph.  GPU tensors
 are required: there is no CPU or PyTorch fallback here.
 
 `linear`, `gemm_w8a8`, `gemm_w4a8`, `rmsnorm`, `rmsnorm_quant`, `rope`, `qk_norm_rope`,
-`rope_append`, `paged_attention` and the chains `gated_mlp` and `sparse_moe` run in native host code (`_host`, csrc/host.cpp) when
+`rope_append`, `paged_attention` and the chains `gated_mlp` and `sparse_moe` run in native
+host code (`_host`, csrc/host.cpp) when
 every tensor is a plain GPU tensor in the layout the kernels take; the Python below
 is the general way (strided, converted or refused arguments).  A LinearW8A8 call at
 one token took 17 us of Python for 4.3 us of kernel on an MI355X host; natively a
@@ -749,13 +750,15 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     (fni8serve/layers/gqa_attention.py:87,123,131,154,278).
 
     Sequence s owns tokens cu_seqlens[s] .. cu_seqlens[s + 1] of q (from 0 on, not
-    decreasing; None: one token a sequence), the last of its context_lens[s] tokens; their keys and values are in the cache
-    already, token c of the sequence in page block_tables[s, c // page_size].  Query head h
+    decreasing; None: one token a sequence), the last of its context_lens[s] tokens; their keys
+    and values are in the cache already, token c of the sequence in page
+    block_tables[s, c // page_size].  Query head h
     reads key head h // (Hq / Hk).  max_seqlen bounds the new tokens of a sequence (None: not
     known; giving it saves time for decoded tokens; without cu_seqlens it is 1 whatever it
     says).  scale defaults to D ** -0.5; window
     is the number of keys that a query sees, itself among them.  A query without keys and
-    tokens past cu_seqlens[-1] give 0; a token whose page is not in the cache counts as NaN."""
+    tokens past cu_seqlens[-1] give 0; a token whose page is not in the cache, or past the block
+    table, counts as NaN.  The weights of the values are rounded to fp16, sums are fp32."""
     if q.is_cuda:
         out = _lib.host().paged_attention(q, k_cache, v_cache, k_scale, v_scale, block_tables,
                                           context_lens, cu_seqlens, max_seqlen, scale, window)
