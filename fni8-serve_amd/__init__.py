@@ -20,6 +20,9 @@ callers):
                                   attention over that cache
     LinearW8A8, GatedMLP, SparseMoE, LMHead, RMSNorm, RotaryEmbedding, GQAAttention
                                   and the weight helpers
+    lora_plan, lora_add           each request's own low-rank adapter beside a linear
+                                  (training/lora.py:14-170), all of a batch in one call
+    sample                        a token a row of logits (sampler.py:20-87)
     PagedKVCache, Step            the cache, fp16 or int8, and one call's tokens
     save_fni8, FQWriter, FQReader the `.fni8` checkpoint container
     load_fni8_checkpoint, load_fni8_state_dict, checkpoint_info
@@ -38,6 +41,9 @@ from .ops import (  # noqa: F401
     gemm_w8a8_grouped,
     linear,
     linear_with_intermediates,
+    lora_add,
+    lora_plan,
+    LoraPlan,
     moe_combine,
     moe_sort,
     paged_attention,
@@ -47,6 +53,7 @@ from .ops import (  # noqa: F401
     rmsnorm_quant,
     rope,
     rope_append,
+    sample,
 )
 from .qtensor import QTensor  # noqa: F401
 from .container import FQReader, FQWriter, save_fni8  # noqa: F401
@@ -81,5 +88,5 @@ __all__ = [
     "load_fni8_state_dict", "checkpoint_info", "act_and_mul", "act_and_mul_quant", "rmsnorm",
     "rmsnorm_quant", "RMSNorm", "SiluAndMul", "GeluAndMul", "get_act_and_mul", "gemm_w4a8",
     "gemm_quantized", "rope", "qk_norm_rope", "rope_append", "paged_attention", "PagedKVCache",
-    "Step", "RotaryEmbedding", "GQAAttention",
+    "Step", "RotaryEmbedding", "GQAAttention", "LoraPlan", "lora_plan", "lora_add", "sample",
 ]

@@ -237,6 +237,17 @@ int check_cache(const void* k_cache, const void* v_cache, const float* k_scale,
     return FNI8_OK;
 }
 
+constexpr int64_t kMaxWidth = (int64_t)1 << 23;
+
+bool lora_in_range(int64_t T, int64_t K, int64_t S, int64_t all_rank) {
+    return T >= 0 && T <= kMaxTokens && K > 0 && K < (int64_t)1 << 24 && S > 0 && S <= 65534 &&
+           all_rank > 0 && all_rank <= 256 * FNI8_LORA_MAX_PARTS;
+}
+
+bool sample_in_range(int64_t B, int64_t V) {
+    return B >= 0 && B <= (int64_t)1 << 20 && V > 0 && V <= (int64_t)1 << 22;
+}
+
 }  // namespace
 
 extern "C" {
@@ -808,6 +819,92 @@ int64_t fni8_paged_attention_workspace_bytes(int64_t T, int64_t Hq, int64_t Hk, 
         return 0;
     return fni8h::paged_attention_workspace_bytes(T, Hq, Hk, D, B, max_seqlen < T ? max_seqlen : T,
                                                   max_context);
+}
+
+int fni8_lora_add_f16(const void* x, int64_t ldx, int64_t T, int64_t K, const void* a,
+                      const void* b, int64_t S, int64_t rank, const int64_t* splits,
+                      int64_t parts, const float* scaling, const int32_t* seg_off,
+                      const int32_t* rows, const void* y, int64_t ldy, void* out, int64_t ldo,
+                      void* workspace, int64_t workspace_bytes, void* stream) {
+    fni8h::g_detail[0] = 0;
+    REQUIRE(x && a && b && splits && seg_off && rows && y && out, FNI8_ERR_NULL,
+            "x, a, b, splits, seg_off, rows, y and out are required");
+    REQUIRE(rank > 0 && rank <= 256 && rank % 8 == 0, FNI8_ERR_SHAPE,
+            "rank=%lld must be a multiple of 8, at most 256", (long long)rank);
+    REQUIRE(parts > 0 && parts <= FNI8_LORA_MAX_PARTS, FNI8_ERR_SHAPE, "parts=%lld (1 to %d)",
+            (long long)parts, FNI8_LORA_MAX_PARTS);
+    REQUIRE(lora_in_range(T, K, S, parts * rank), FNI8_ERR_SHAPE,
+            "T=%lld K=%lld S=%lld out of range (T <= 2^23, K < 2^24, S <= 65534)", (long long)T,
+            (long long)K, (long long)S);
+    int64_t N = 0;
+    for (int64_t i = 0; i < parts; i++) {
+        REQUIRE(splits[i] > 0 && splits[i] < kMaxWidth, FNI8_ERR_SHAPE,
+                "splits[%lld]=%lld out of range", (long long)i, (long long)splits[i]);
+        N += splits[i];
+    }
+    REQUIRE(N < kMaxWidth, FNI8_ERR_SHAPE, "N=%lld out of range (< 2^23)", (long long)N);
+    REQUIRE(ldx >= K && ldy >= N && ldo >= N, FNI8_ERR_STRIDE,
+            "ldx=%lld < K=%lld, or ldy=%lld or ldo=%lld < N=%lld", (long long)ldx, (long long)K,
+            (long long)ldy, (long long)ldo, (long long)N);
+    REQUIRE(out != y || ldo == ldy, FNI8_ERR_STRIDE, "out is y, with ldo=%lld and ldy=%lld",
+            (long long)ldo, (long long)ldy);
+    REQUIRE(aligned(x, 2) && aligned(y, 2) && aligned(out, 2) && aligned(a, 16) &&
+                aligned(b, 16) && aligned(scaling, 4) && aligned(seg_off, 4) && aligned(rows, 4),
+            FNI8_ERR_ALIGN, "a and b must be 16-byte aligned, the others element-aligned");
+    const int64_t need = fni8h::lora_workspace_bytes(T, K, S, parts * rank);
+    REQUIRE(!need || (workspace && aligned(workspace, 256)), FNI8_ERR_ALIGN,
+            "a 256-byte aligned workspace is required");
+    REQUIRE(workspace_bytes >= need, FNI8_ERR_SHAPE, "workspace of %lld bytes, %lld needed",
+            (long long)workspace_bytes, (long long)need);
+    int rc = check_device();
+    if (rc) return rc;
+    fni8h::LoraAdd l{};
+    l.x = (const uint16_t*)x; l.ldx = ldx; l.T = T; l.K = K;
+    l.a = (const uint16_t*)a; l.b = (const uint16_t*)b; l.S = S; l.rank = rank;
+    l.splits = splits; l.parts = parts; l.scaling = scaling; l.seg_off = seg_off; l.rows = rows;
+    l.y = (const uint16_t*)y; l.ldy = ldy; l.out = (uint16_t*)out; l.ldo = ldo;
+    l.work = static_cast<float*>(workspace);
+    return fni8h::launch_lora_add(l, (hipStream_t)stream);
+}
+
+int64_t fni8_lora_workspace_bytes(int64_t T, int64_t K, int64_t S, int64_t all_rank) {
+    return lora_in_range(T, K, S, all_rank) ? fni8h::lora_workspace_bytes(T, K, S, all_rank) : 0;
+}
+
+int fni8_sample(const void* logits, int fp32, int64_t B, int64_t V, int64_t ldl, const float* u,
+                const float* temperature, float temperature_all, const int32_t* top_k,
+                int64_t top_k_all, const float* top_p, float top_p_all, const float* min_p,
+                float min_p_all, int64_t* tokens, float* logprobs, void* workspace,
+                int64_t workspace_bytes, void* stream) {
+    fni8h::g_detail[0] = 0;
+    REQUIRE(logits && tokens, FNI8_ERR_NULL, "logits and tokens are required");
+    REQUIRE(sample_in_range(B, V), FNI8_ERR_SHAPE,
+            "B=%lld V=%lld out of range (B <= 2^20, 1 <= V <= 2^22)", (long long)B, (long long)V);
+    REQUIRE(ldl >= V, FNI8_ERR_STRIDE, "ldl=%lld < V=%lld", (long long)ldl, (long long)V);
+    REQUIRE(aligned(logits, fp32 ? 4 : 2) && aligned(u, 4) && aligned(temperature, 4) &&
+                aligned(top_k, 4) && aligned(top_p, 4) && aligned(min_p, 4) &&
+                aligned(tokens, 8) && aligned(logprobs, 4),
+            FNI8_ERR_ALIGN, "a tensor is not aligned to its elements");
+    const int64_t need = fni8h::sample_workspace_bytes(B, V);
+    REQUIRE(!need || (workspace && aligned(workspace, 256)), FNI8_ERR_ALIGN,
+            "a 256-byte aligned workspace is required");
+    REQUIRE(workspace_bytes >= need, FNI8_ERR_SHAPE, "workspace of %lld bytes, %lld needed",
+            (long long)workspace_bytes, (long long)need);
+    int rc = check_device();
+    if (rc) return rc;
+    fni8h::Sample a{};
+    a.logits = logits; a.fp32 = fp32 != 0; a.B = B; a.V = V; a.ld = ldl; a.u = u;
+    a.temperature = temperature; a.temperature1 = temperature_all;
+    a.top_k = top_k;
+    a.top_k1 = (int32_t)(top_k_all < 0 ? 0 : top_k_all > V ? 0 : top_k_all);
+    a.top_p = top_p; a.top_p1 = top_p_all; a.min_p = min_p; a.min_p1 = min_p_all;
+    a.tokens = tokens; a.logprobs = logprobs;
+    a.work = static_cast<int8_t*>(workspace);
+    return fni8h::launch_sample(a, (hipStream_t)stream);
+}
+
+int64_t fni8_sample_workspace_bytes(int64_t B, int64_t V) {
+    return sample_in_range(B, V) ? fni8h::sample_workspace_bytes(B, V) : 0;
 }
 
 }  // extern "C"

@@ -547,5 +547,39 @@ struct PagedAttention {
 int launch_paged_attention(const PagedAttention& a, hipStream_t st);
 int64_t paged_attention_workspace_bytes(int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t B,
                                         int64_t max_seqlen, int64_t max_context);
+struct LoraAdd {
+    const uint16_t* x;
+    int64_t ldx, T, K;
+    const uint16_t *a, *b;
+    int64_t S, rank;
+    const int64_t* splits;  // host memory
+    int64_t parts;
+    const float* scaling;
+    const int32_t *seg_off, *rows;
+    const uint16_t* y;
+    int64_t ldy;
+    uint16_t* out;
+    int64_t ldo;
+    float* work;
+};
+int launch_lora_add(const LoraAdd& l, hipStream_t st);
+int64_t lora_workspace_bytes(int64_t T, int64_t K, int64_t S, int64_t R);
+// Settings NULL: the number beside them for every row.
+struct Sample {
+    const void* logits;
+    int fp32;
+    int64_t B, V, ld;
+    const float* u;
+    const float* temperature;
+    const int32_t* top_k;
+    const float *top_p, *min_p;
+    float temperature1, top_p1, min_p1;
+    int32_t top_k1;
+    int64_t* tokens;
+    float* logprobs;
+    int8_t* work;
+};
+int launch_sample(const Sample& a, hipStream_t st);
+int64_t sample_workspace_bytes(int64_t B, int64_t V);
 void set_error_detail(const char* fmt, ...);
 }  // namespace fni8h

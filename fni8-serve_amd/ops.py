@@ -22,6 +22,9 @@ pass takes 6.1 us.
 from __future__ import annotations
 
 import ctypes
+import math
+from collections.abc import Sequence
+from typing import NamedTuple
 
 import torch
 
@@ -803,3 +806,153 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                   ctypes.c_float(D ** -0.5 if scale is None else scale), window or 0, _ptr(out),
                   _ptr(work), nw, _stream(dev))
     return out
+
+
+class LoraPlan(NamedTuple):
+    """Which tokens belong to which adapter: those of adapter e are
+    rows[seg_off[e]:seg_off[e + 1]], those without one segment S; both int32, on the GPU."""
+    seg_off: torch.Tensor
+    rows: torch.Tensor
+
+
+def lora_plan(ids: torch.Tensor, num_adapters: int) -> LoraPlan:
+    """The plan of a step's tokens, ids int [T]: each token's adapter, or any number outside
+    [0, num_adapters) for none.  Made once a step: every projection of every layer shares it."""
+    if not 0 < num_adapters <= 65534:
+        raise ValueError(f"num_adapters {num_adapters} must be from 1 to 65534")
+    _require_cuda("lora_plan", ids)
+    ids = _index("ids", ids, None)
+    if ids.numel() == 0:
+        return LoraPlan(ids.new_zeros(num_adapters + 2), ids.new_empty(0))
+    ids = torch.where((ids < 0) | (ids >= num_adapters), num_adapters, ids)
+    seg_off, rows, _ = moe_sort(ids.unsqueeze(1), num_adapters + 1)
+    return LoraPlan(seg_off, rows)
+
+
+def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, plan: LoraPlan,
+             scaling: torch.Tensor | None = None, splits: Sequence[int] | None = None,
+             out: torch.Tensor | None = None) -> torch.Tensor:
+    """y plus each token's own low-rank product, y fp16 [..., N] -> fp16 [..., N] in one call
+    for all adapters (the unmerged forward of fni8serve/training/lora.py:14-170):
+
+        out[t, n] = y[t, n] + scaling[e] * sum_j b[e, n, j] * (a[e] x[t])[p(n) * rank + j]
+
+    x fp16 [..., K] (the input of the projection that made y), b fp16 [S, N, rank], a fp16
+    [S, parts * rank, K], plan = lora_plan(ids, S).  splits: the widths of the parts of a
+    merged projection, p(n) the part of column n (None: one part).  scaling fp32 [S] (None: 1).
+    out: where the result goes; y itself adds in place and leaves rows without an adapter
+    untouched; None allocates it.  rank is a multiple of 8, at most 256 (zeros fill up).
+    Sums are fp32; the result is rounded once."""
+    for name, t, dims in (("y", y, 0), ("x", x, 0), ("a", a, 3), ("b", b, 3)):
+        if t.dtype != _f16 or t.dim() < 1 or (dims and (t.dim() != dims or not t.is_contiguous())):
+            raise ValueError(f"{name} must be {'a contiguous' if dims else 'an'} fp16 tensor"
+                             f"{' of 3 dimensions' if dims else ''} (got {t.dtype}, "
+                             f"{tuple(t.shape)})")
+    S, N, rank = b.shape
+    K = x.shape[-1]
+    splits = [N] if splits is None else [int(n) for n in splits]
+    if a.shape != (S, len(splits) * rank, K) or y.shape[-1] != N or sum(splits) != N:
+        raise ValueError(f"a {tuple(a.shape)} and b {tuple(b.shape)} do not fit x "
+                         f"{tuple(x.shape)}, y {tuple(y.shape)} and splits {splits}")
+    if scaling is not None:
+        if scaling.dtype != torch.float32 or scaling.numel() != S:
+            raise ValueError(f"scaling must be fp32 with {S} entries")
+        scaling = scaling.reshape(-1).contiguous()
+    seg_off, rows = plan
+    for name, t, n in (("seg_off", seg_off, S + 2), ("rows", rows, y.numel() // max(N, 1))):
+        if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+            raise ValueError(f"plan.{name} must be a contiguous int32 tensor with {n} entries "
+                             f"(got {t.dtype}, {tuple(t.shape)}): lora_plan({n} ids, {S})")
+    if x.shape[:-1] != y.shape[:-1]:
+        raise ValueError(f"x {tuple(x.shape)} and y {tuple(y.shape)} differ in tokens")
+    if rank % 8 or not 0 < rank <= 256:
+        raise ValueError(f"rank {rank} must be a multiple of 8, at most 256 (zeros fill up)")
+    dev = _require_cuda("lora_add", y, x, a, b, seg_off, rows, scaling, out)
+    x2, ldx = _rows(x, K)
+    if out is None:
+        y2, ldy = _rows(y, N)
+        out = torch.empty(y.shape, dtype=_f16, device=dev)
+        o2, ldo = out, N
+    else:
+        if out.dtype != _f16 or out.shape != y.shape:
+            raise ValueError(f"out must be fp16 with y's shape {tuple(y.shape)}")
+        o2, ldo = _rows(out, N)
+        if o2.numel() and o2.data_ptr() != out.data_ptr():
+            raise ValueError("out's rows must be evenly spaced, with unit inner stride")
+        y2, ldy = (o2, ldo) if out is y else _rows(y, N)
+        if y2.numel() and y2.data_ptr() == o2.data_ptr() and ldy != ldo:
+            raise ValueError("out lies in y's memory with other strides")
+    T = x2.shape[0]
+    if T == 0:
+        return out
+    nw = int(_lib.load().fni8_lora_workspace_bytes(T, K, S, len(splits) * rank))
+    work = torch.empty(nw, dtype=torch.uint8, device=dev) if nw else None
+    with torch.cuda.device(dev):
+        _lib.call("fni8_lora_add_f16", _ptr(x2), ldx, T, K, _ptr(a), _ptr(b), S, rank,
+                  (ctypes.c_int64 * len(splits))(*splits), len(splits), _ptr(scaling),
+                  _ptr(seg_off), _ptr(rows), _ptr(y2), ldy, _ptr(o2), ldo, _ptr(work), nw,
+                  _stream(dev))
+    return out
+
+
+def _setting(name: str, v, B: int, dtype: torch.dtype, least: float, most: float):
+    """A sampling setting: one number for all rows (checked), or a tensor with one a row."""
+    if torch.is_tensor(v):
+        if v.numel() != B or v.dtype == torch.bool or v.is_complex() \
+                or v.is_floating_point() != dtype.is_floating_point:
+            raise ValueError(f"{name} must be a number or a {dtype} tensor with {B} entries (got "
+                             f"{v.dtype}, {tuple(v.shape)})")
+        v = _int32(v) if dtype == torch.int32 else v.to(dtype)
+        return v.reshape(-1).contiguous(), 0
+    if not least <= v <= most:
+        raise ValueError(f"{name} {v} must be from {least} to {most}")
+    return None, v
+
+
+def sample(logits: torch.Tensor, u: torch.Tensor | None = None, temperature=1.0, top_k=0,
+           top_p=1.0, min_p=0.0, return_logprobs: bool = False):
+    """One token a row, logits fp16 or fp32 [..., V] -> int64 [...], drawn with the random
+    numbers u fp32 [...] in [0, 1) (fni8serve/layers/sampler.py:20-87).
+
+    Tokens are ordered by logit, ties by the lower index; their weights are exp((x - max) /
+    temperature).  top_k keeps the first k, top_p a token while the mass before it is less than
+    top_p times the mass that top_k keeps, min_p those with at least min_p times the largest
+    weight: the shortest of these runs is kept, the first token always.  The token is the first
+    kept one, in index order, at which the running mass exceeds u times the kept mass.
+
+    Each setting is a number, or a tensor with one for each row.  temperature 0 takes the
+    largest logit (u may be None where it is the number 0); top_k 0, top_p 1 and min_p 0 filter
+    nothing; tensors may hold values outside these ranges, which mean the nearest one inside
+    (a temperature that is NaN: see below).  A logit of minus infinity is never drawn.  A row
+    with a NaN, or of minus infinity alone, gives -1 and the log-probability NaN.
+
+    return_logprobs: (tokens, fp32 [...]), the logarithm of the token's share of the kept mass."""
+    if logits.dtype not in (_f16, torch.float32) or logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"logits must be fp16 or fp32 [..., V] (got {logits.dtype}, "
+                         f"{tuple(logits.shape)})")
+    lead, V = logits.shape[:-1], logits.shape[-1]
+    B = math.prod(lead)
+    settings = [_setting(name, v, B, dtype, least, most) for name, v, dtype, least, most in (
+        ("temperature", temperature, torch.float32, 0.0, 3e38),
+        ("top_k", top_k, torch.int32, 0, 2 ** 31 - 1), ("top_p", top_p, torch.float32, 0.0, 1.0),
+        ("min_p", min_p, torch.float32, 0.0, 1.0))]
+    if u is None:
+        if torch.is_tensor(temperature) or temperature != 0:
+            raise ValueError("u is required where the temperature is not the number 0")
+    elif u.dtype != torch.float32 or u.shape != lead:
+        raise ValueError(f"u must be fp32 {tuple(lead)} (got {u.dtype}, {tuple(u.shape)})")
+    dev = _require_cuda("sample", logits, u, *(t for t, _ in settings))
+    x2, ldl = _rows(logits, V)
+    u = None if u is None else u.reshape(-1).contiguous()
+    tokens = torch.empty(lead, dtype=torch.int64, device=dev)
+    logprobs = torch.empty(lead, dtype=torch.float32, device=dev) if return_logprobs else None
+    if B:
+        (ts, t1), (ks, k1), (ps, p1), (ms, m1) = settings
+        nw = int(_lib.load().fni8_sample_workspace_bytes(B, V))
+        work = torch.empty(nw, dtype=torch.uint8, device=dev) if nw else None
+        with torch.cuda.device(dev):
+            _lib.call("fni8_sample", _ptr(x2), int(logits.dtype == torch.float32), B, V, ldl,
+                      _ptr(u), _ptr(ts), ctypes.c_float(t1), _ptr(ks), int(k1), _ptr(ps),
+                      ctypes.c_float(p1), _ptr(ms), ctypes.c_float(m1), _ptr(tokens),
+                      _ptr(logprobs), _ptr(work), nw, _stream(dev))
+    return (tokens, logprobs) if return_logprobs else tokens

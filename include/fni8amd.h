@@ -522,6 +522,81 @@ int fni8_paged_attention_f16(const void* q, int64_t ldq, int64_t hsq, int64_t T,
 int64_t fni8_paged_attention_workspace_bytes(int64_t T, int64_t Hq, int64_t Hk, int64_t D,
                                              int64_t B, int64_t max_seqlen, int64_t max_context);
 
+/* Parts of a merged projection at most (fni8_lora_add_f16). */
+#define FNI8_LORA_MAX_PARTS 8
+
+/*
+ * Low-rank adapters of many requests beside one projection (the unmerged
+ * forward of fni8serve/training/lora.py:14-170, for a batch whose tokens have
+ * different adapters):
+ *   out[t, n] = fp16(y[t, n] + scaling[e] * sum_j b[e, n, j] * h[t, p * rank + j]),
+ *   h[t]      = a[e] x[t]
+ * with e the adapter of token t and p the part of the projection that column n
+ * is in.  Sums are fp32, h enters the second product with 22 bits, and a result
+ * is rounded once.
+ *   x        fp16 [T, K], row stride ldx
+ *   a        fp16 [S, parts * rank, K]; b fp16 [S, N, rank]
+ *   splits   HOST array of `parts` widths that add up to N (Q, K and V of a
+ *            merged projection have a's rows p * rank .. of their own); at most
+ *            FNI8_LORA_MAX_PARTS
+ *   scaling  fp32 [S], or NULL for 1
+ *   seg_off  int32 [S + 2] and rows int32 [T]: the tokens sorted by adapter, those
+ *            of adapter e at rows[seg_off[e] .. seg_off[e + 1]), those without one
+ *            last, as segment S (fni8_moe_sort with k = 1 over S + 1 experts); no
+ *            token may be there twice
+ *   y        fp16 [T, N], row stride ldy; out fp16 [T, N], row stride ldo: other
+ *            memory than y, or y itself (with ldo = ldy), whose rows without an
+ *            adapter then stay as they are
+ *   workspace  device memory, 256-byte aligned, of at least
+ *            fni8_lora_workspace_bytes(T, K, S, parts * rank) bytes; any contents;
+ *            one per stream
+ * rank is a multiple of 8, at most 256; a and b are 16-byte aligned.  Any K; multiples
+ * of 8 with 16-byte aligned rows of x and a are read in whole vectors.
+ */
+int fni8_lora_add_f16(const void* x, int64_t ldx, int64_t T, int64_t K, const void* a,
+                      const void* b, int64_t S, int64_t rank, const int64_t* splits,
+                      int64_t parts, const float* scaling, const int32_t* seg_off,
+                      const int32_t* rows, const void* y, int64_t ldy, void* out, int64_t ldo,
+                      void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Bytes of fni8_lora_add_f16's workspace (0 where its arguments are out of range). */
+int64_t fni8_lora_workspace_bytes(int64_t T, int64_t K, int64_t S, int64_t all_rank);
+
+/*
+ * One token a row of logits (fni8serve/layers/sampler.py:20-87), from given
+ * random numbers.  Tokens are ordered by logit, ties by the lower index, and
+ * w_i = exp((x_i - max) / temperature).  top_k keeps the first k; top_p a token
+ * while the mass before it is less than top_p times the mass that top_k keeps;
+ * min_p those with w_i >= min_p: each keeps a first run of the order, the
+ * shortest counts, and the first token is always in it.  The token drawn is the
+ * first kept one, in index order, at which the running mass exceeds u times the
+ * kept mass.  Masses are integers of 62 bits: the same inputs give the same token.
+ *   logits   fp16 or (fp32 != 0) fp32 [B, V], row stride ldl; V <= 2^22
+ *   u        fp32 [B] in [0, 1) (below: as 0, NaN too; 1 and above: the last kept
+ *            token), or NULL: 0
+ *   temperature, top_k, top_p, min_p
+ *            [B] each, or NULL: the number after it for every row.  temperature 0 or
+ *            less: the largest logit, the lowest index of equal ones.  top_k of 0 or
+ *            less, top_p of 1 or more and min_p of 0 or less filter nothing; top_p of
+ *            0 or less keeps the first token, min_p of more than 1 the tokens of the
+ *            largest logit.
+ *   tokens   int64 [B]; logprobs fp32 [B] or NULL: the logarithm of the drawn token's
+ *            share of the kept mass (0 at temperature 0)
+ *   workspace  device memory, 256-byte aligned, of at least
+ *            fni8_sample_workspace_bytes(B, V) bytes; any contents; one per stream
+ * Minus infinity is never drawn; several plus infinities share the mass.  A row with
+ * a NaN (logit or temperature), or of minus infinity alone, gives the token -1 and the
+ * logprob NaN.
+ */
+int fni8_sample(const void* logits, int fp32, int64_t B, int64_t V, int64_t ldl, const float* u,
+                const float* temperature, float temperature_all, const int32_t* top_k,
+                int64_t top_k_all, const float* top_p, float top_p_all, const float* min_p,
+                float min_p_all, int64_t* tokens, float* logprobs, void* workspace,
+                int64_t workspace_bytes, void* stream);
+
+/* Bytes of fni8_sample's workspace (0 where its arguments are out of range). */
+int64_t fni8_sample_workspace_bytes(int64_t B, int64_t V);
+
 #ifdef __cplusplus
 }
 #endif
