@@ -192,3 +192,43 @@ def test_rows_far_apart(pkg, cuda):
     src, u = logits(3, 1000, seed=9)
     x.copy_(src)
     assert torch.equal(pkg.sample(x, u, top_p=0.9), pkg.sample(src, u, top_p=0.9))
+
+
+@pytest.mark.parametrize("fp32", [False, True])
+@pytest.mark.parametrize("spread,kw", [
+    (1.0, dict(temperature=1.5, top_p=0.98)), (0.3, dict(top_p=0.999999)), (1.0, dict(top_k=5000)),
+    (2.0, dict(top_k=1500, top_p=0.5)), (1.0, dict(top_k=40000, top_p=0.9, min_p=1e-3)),
+    (0.01, dict(top_p=0.5)), (0.01, dict(top_k=77777)), (1.0, dict(min_p=0.03)),
+    (3.0, dict(min_p=1e-12)), (1.0, dict(top_p=0.97, min_p=0.2)), (2.0, dict(top_k=700)),
+    (2.5, dict(top_k=1000, top_p=0.999, min_p=0.01)), (4.0, dict(temperature=0.3, top_k=100000)),
+    (1.0, dict(top_k=600, min_p=0.5)), (1.5, dict(top_k=60, top_p=0.97, min_p=0.6))])
+def test_long_prefixes(pkg, cuda, spread, kw, fp32):
+    """Kept prefixes from dozens of tokens to most of the vocabulary."""
+    for V, peaks in ((151936, 0), (100003, 5)):
+        x, u = logits(4, V, seed=V + peaks, fp32=fp32, spread=spread, peaks=max(peaks, 1))
+        check(pkg, x, u, **kw)
+
+
+def test_neighbouring_peaks(pkg, cuda):
+    """The tokens that matter side by side, in one group of a thread or in one part."""
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(6, 60000, generator=g).half()
+    x[0, 800:804] = 15.0
+    x[1, 800:832] = torch.linspace(14, 15, 32).half()
+    x[2, [100, 2148, 4196, 6244]] = 15.0       # the four vectors of one thread
+    x[3, 8190:8194] = 15.0                     # across a border of parts
+    x[4, 59992:60000] = 15.0                   # the end of the row
+    x[5, 0:8] = torch.linspace(15, 12, 8).half()
+    for kw in (dict(top_p=0.95), dict(top_k=3), dict(top_k=20, top_p=0.9), dict(min_p=0.3), dict(),
+               dict(top_p=0.9999), dict(temperature=0.0)):
+        for seed in range(3):
+            check(pkg, x.cuda(), torch.rand(6, generator=g).cuda(), **kw)
+
+
+def test_a_row_is_the_same_in_every_batch(pkg, cuda):
+    x, u = logits(300, 20011, seed=8)
+    for kw in (dict(), dict(top_p=0.9), dict(top_k=40)):
+        got, logp = pkg.sample(x, u, return_logprobs=True, **kw)
+        for i in (0, 7, 299):
+            one, logp1 = pkg.sample(x[i:i + 1], u[i:i + 1], return_logprobs=True, **kw)
+            assert one[0] == got[i] and logp1[0] == logp[i]
