@@ -29,47 +29,39 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int kPart = 8192, kScanThreads = 256, kVec = 8;   // logits of a part; a thread's vectors
-constexpr int kSteps = kPart / (kScanThreads * kVec);       // vectors of a thread
-constexpr int kThreads = 1024, kWaves = 16;                 // draw
-constexpr int kBins = 2048;   // steps of weight; the last one: weights that round to 0
-constexpr int kList = 2048;   // candidates in LDS
-constexpr int kPairs = 512;   // up to here every pair of candidates is compared
-constexpr int kHits = 4096;   // groups that are read again
-constexpr int kEnough = 1024; // maxima that a top-p bound may take before the list is tried
+constexpr int kVec = 8, kPart = 8192, kScanThreads = 256;  // logits: of a load, of a part
+constexpr int kSteps = kPart / (kScanThreads * kVec);      // loads of a scan thread
+constexpr int kThreads = 512, kWaves = 8;                  // draw
+constexpr int kBins = 2048;    // steps of weight; the last one: weights that round to 0
+constexpr int kList = 2048;    // candidates in LDS
+constexpr int kMini = 64;      // candidates that one wave compares with each other
+constexpr int kHits = 4096;    // groups that are read again
+constexpr int kEnough = 1024;  // maxima that a top-p bound may take before the list is tried
 
-// 2^t for t <= 0: t = n + f, |f| <= 1/2; 2^f by its Taylor polynomial in f ln 2, degree 11 (the
-// first term left out is below 2^-47).
-__device__ __forceinline__ double exp2_part(double t, int& n) {
-    const double r = __builtin_rint(t), f = t - r;
-    n = (int)r;
-    double p = 4.4455382718708101e-10;               // ln2^11 / 11!
-    p = __builtin_fma(p, f, 7.0549116208011209e-9);  // ln2^10 / 10!
-    p = __builtin_fma(p, f, 1.0178086009239696e-7);
-    p = __builtin_fma(p, f, 1.3215486790144305e-6);
-    p = __builtin_fma(p, f, 1.5252733804059838e-5);
-    p = __builtin_fma(p, f, 1.5403530393381606e-4);
-    p = __builtin_fma(p, f, 1.3333558146428441e-3);
-    p = __builtin_fma(p, f, 9.6181291076284769e-3);
-    p = __builtin_fma(p, f, 5.5504108664821576e-2);
-    p = __builtin_fma(p, f, 0.24022650695910070);
-    p = __builtin_fma(p, f, 0.69314718055994531);
-    return __builtin_fma(p, f, 1.0);
+// 2^(t + s) for -1000 <= t <= 0.  t = n + f, |f| <= 1/2, by the addition that leaves n + s in
+// the low bits; 2^f = 1 + f q(f), q the polynomial of degree 9 through (2^f - 1) / f at the
+// Chebyshev nodes (error below 2^-50 of the value; exactly 1 at 0); n + s goes into the
+// exponent.
+__device__ __forceinline__ double exp2_at(double t, int s) {
+    const double magic = 0x1.8p52 + s, tn = t + magic, f = t - (tn - magic);
+    double q = 7.070977866508138e-09;
+    q = __builtin_fma(q, f, 1.0205905413765595e-07);
+    q = __builtin_fma(q, f, 1.3215451633221434e-06);
+    q = __builtin_fma(q, f, 1.5252672924850737e-05);
+    q = __builtin_fma(q, f, 1.5403530424776529e-04);
+    q = __builtin_fma(q, f, 1.3333558200794592e-03);
+    q = __builtin_fma(q, f, 9.618129107618665e-03);
+    q = __builtin_fma(q, f, 5.550410866465167e-02);
+    q = __builtin_fma(q, f, 0.24022650695910075);
+    q = __builtin_fma(q, f, 0.6931471805599462);
+    q = __builtin_fma(q, f, 1.0);
+    const u64 n = (u64)(uint32_t)__builtin_bit_cast(u64, tn) << 52;
+    return __builtin_bit_cast(double, __builtin_bit_cast(u64, q) + n);
 }
 
-__device__ __forceinline__ double exp2_neg(double t) {
-    if (!(t > -256.0)) return 0.0;  // nothing beside a largest weight of 1
-    int n;
-    const double p = exp2_part(t, n);
-    return __builtin_ldexp(p, n);
-}
-
-// 2^t * 2^s as an integer, rounded, for s <= 50: adding 2^52 leaves it in the sum's low bits.
+// The same as an integer, rounded, for s <= 50: adding 2^52 leaves it in the sum's low bits.
 __device__ __forceinline__ u64 exp2_fixed(double t, int s) {
-    if (!(t > -(double)(s + 2))) return 0;
-    int n;
-    const double p = exp2_part(t, n);
-    return __builtin_bit_cast(u64, __builtin_ldexp(p, n + s) + 0x1p52) & 0xfffffffffffffull;
+    return __builtin_bit_cast(u64, exp2_at(t, s) + 0x1p52) & 0xfffffffffffffull;
 }
 
 // Order of floats as unsigned numbers; -0 counts as +0, NaN above everything.
@@ -109,8 +101,8 @@ __device__ __forceinline__ void load8(const E* x, int i, int V, float (&v)[kVec]
 struct Row {
     float T, p, least, u, top;
     int k, s;
-    double rate;
-    bool inf, by_k, by_p, by_m;
+    double rate, base, cap, step;
+    bool by_k, by_p, by_m;
 
     __device__ Row(const fni8h::Sample& a, int64_t row, int V) {
         T = a.temperature ? a.temperature[row] : a.temperature1;
@@ -125,23 +117,27 @@ struct Row {
         // bits of a weight's fraction: V weights of at most 1 add up to less than 2^62
         s = 30 + __builtin_clz(V);
         s = s < 50 ? s : 50;
+        step = (kBins - 2) / (double)(s + 2);
     }
     // Every weight of the row is summed: for top-p without top-k, and without any filter.
     __device__ bool summed() const { return T > 0.0f && !by_k && (by_p || !by_m); }
+    // Plus infinity counts as 10^300 with a rate that leaves nothing of any finite logit.
     __device__ void largest(float x) {
         top = x;
-        inf = x == __builtin_inff();
+        const bool inf = x == __builtin_inff();
         rate = 1.4426950408889634 / (double)T;
+        if (inf && rate < 1e-200) rate = 1e-200;
+        cap = inf ? 1e300 : 1e200;
+        base = inf ? 1e300 : (double)x;
     }
-    // log2 of a logit's weight
+    // log2 of a logit's weight, at least -1000 (minus infinity too, whatever the rate)
     __device__ __forceinline__ double power(float v) const {
-        if (inf) return v == top ? 0.0 : -__builtin_inf();
-        if (v == -__builtin_inff()) return -__builtin_inf();
-        return ((double)v - (double)top) * rate;
+        return __builtin_fmax((__builtin_fmin((double)v, cap) - base) * rate, -1000.0);
     }
+    __device__ __forceinline__ u64 mass(float v) const { return exp2_fixed(power(v), s); }
     // Step of a weight, rising as it falls; kBins - 1 for weights that round to 0.
     __device__ __forceinline__ int bin(double power) const {
-        const double d = -power * ((kBins - 2) / (double)(s + 2));
+        const double d = -power * step;
         return d < (double)(kBins - 1) ? (int)d : kBins - 1;
     }
 };
@@ -198,14 +194,16 @@ __global__ __launch_bounds__(kScanThreads) void scan_kernel(const fni8h::Sample 
 #pragma unroll
     for (int i = 0; i < kSteps; i++)
         load8(x, part * kPart + (i * kScanThreads + (int)threadIdx.x) * kVec, V, v[i]);
-    uint32_t best = 0;
+    float most = -__builtin_inff();
+    bool nan = false;
 #pragma unroll
     for (int i = 0; i < kSteps; i++)
 #pragma unroll
         for (int j = 0; j < kVec; j++) {
-            const uint32_t key = key_of(v[i][j]);
-            best = key > best ? key : best;
+            nan |= v[i][j] != v[i][j];
+            most = __builtin_fmaxf(most, v[i][j]);
         }
+    uint32_t best = nan ? 0xffffffffu : key_of(most);
     w.top[part * kScanThreads + threadIdx.x] = best;
     best = fni8::wave_max_u32(best);
     if (lane == 0) tops[wave] = best;
@@ -219,7 +217,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_kernel(const fni8h::Sample 
 #pragma unroll
     for (int i = 0; i < kSteps; i++)
 #pragma unroll
-        for (int j = 0; j < kVec; j++) sum += exp2_neg(r.power(v[i][j]));
+        for (int j = 0; j < kVec; j++) sum += exp2_at(r.power(v[i][j]), 0);
     sum = wave_sum(sum);
     if (lane == 0) sums[wave] = sum;
     __syncthreads();
@@ -230,6 +228,8 @@ struct Candidate {
     u64 order;  // key << 32 | ~index: larger ones come first
     u64 mass;
 };
+__device__ __forceinline__ uint32_t key_at(const Candidate& c) { return (uint32_t)(c.order >> 32); }
+__device__ __forceinline__ uint32_t place_at(const Candidate& c) { return (uint32_t)c.order; }
 
 struct Shared {
     union {
@@ -238,77 +238,59 @@ struct Shared {
             uint32_t count[kBins];
         } h;
         uint32_t hits[kHits];
-        struct {
-            u64 before[kPairs];
-            uint32_t rank[kPairs];
-        } pair;
+        u64 hist[256];
     };
-    Candidate list[kList];
-    u64 hist[256];
-    u64 part[kWaves];
-    double sums[kWaves];
-    u64 need, total, kept, all;
+    Candidate list[kList], mini[kMini];
+    u64 part[2][kWaves], range[kWaves];
+    double sums[2][kWaves], before;
+    int ints[2][kWaves], counts[kWaves], highs[kWaves];
+    u64 need, found;
     uint32_t key;
-    int index, n, hits_n, bin;
+    int index, n, hits_n, bin, bin2;
 };
 
-// The sum over the workgroup, the same in every thread, added in one order.
-template <class N>
-__device__ N block_sum(N* part, N v) {
+// Sums over the workgroup take turns with two rows of LDS, so that none has to wait before it
+// writes: who writes a row again has passed the barrier of the sum between.
+struct Turn {
+    int t = 0;
+    __device__ int next() { return t ^= 1; }
+};
+
+__device__ __forceinline__ u64 block_sum(Shared& sh, Turn& turn, u64 v) {
+    const int row = turn.next();
     v = wave_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 0) sh.part[row][threadIdx.x >> 6] = v;
     __syncthreads();
     v = 0;
-    for (int w = 0; w < kWaves; w++) v += part[w];
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) v += sh.part[row][w];
     return v;
 }
 
-template <class F>
-__device__ u64 sum_of(Shared& sh, int n, F f) {
-    u64 s = 0;
-    for (int i = threadIdx.x; i < n; i += kThreads) s += f(i);
-    return block_sum(sh.part, s);
-}
-
-// The first index at which the running sum of f reaches `need` (1 to the sum of all).
-template <class F>
-__device__ int find_index(Shared& sh, int n, u64 need, F f) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int lo = 0, hi = n;
-    while (hi - lo > kThreads) {
-        const int per = ((hi - lo + kWaves - 1) / kWaves + 63) & ~63;
-        const int i0 = lo + wave * per, i1 = i0 + per < hi ? i0 + per : hi;
-        u64 s = 0;
-        for (int i = i0 + lane; i < i1; i += 64) s += f(i);
-        s = wave_sum(s);
-        __syncthreads();
-        if (lane == 0) sh.part[wave] = s;
-        __syncthreads();
-        int w = 0;
-        for (; w < kWaves - 1 && lo + (w + 1) * per < hi && sh.part[w] < need; w++)
-            need -= sh.part[w];
-        lo += w * per;
-        hi = lo + per < hi ? lo + per : hi;
+// Running sum over the threads, this one's among it, and the sum of all.
+template <class N>
+__device__ __forceinline__ N block_scan(N (&rows)[2][kWaves], Turn& turn, N v, N& all) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = turn.next();
+    v = wave_scan(v, lane);
+    if (lane == 63) rows[row][wave] = v;
+    __syncthreads();
+    N before = 0;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) {
+        const N p = rows[row][w];
+        before += w < wave ? p : 0;
+        all += p;
     }
-    const int i = lo + threadIdx.x;
-    const u64 own = i < hi ? f(i) : 0;
-    u64 run = wave_scan(own, lane);
-    __syncthreads();
-    if (lane == 63) sh.part[wave] = run;
-    if (threadIdx.x == 0) sh.index = hi - 1;
-    __syncthreads();
-    for (int w = 0; w < wave; w++) run += sh.part[w];
-    if (run >= need && run - own < need) sh.index = i;
-    __syncthreads();
-    return sh.index;
+    return before + v;
 }
 
 // The largest key such that the sum of f over keys no smaller reaches `need` (at least 1; no
 // more than the sum of all, or it is lowered to that); `need` is then what the items of that
-// key have to bring, `total` what they hold.
+// key have to bring.  Four passes over the items, eight bits of the key each: for lists that
+// are too long otherwise (thousands of equal logits).
 template <class K, class F>
-__device__ uint32_t find_key(Shared& sh, int n, u64& need, u64& total, K key, F f) {
+__device__ uint32_t find_key(Shared& sh, int n, u64& need, K key, F f) {
     uint32_t prefix = 0;
     for (int shift = 24; shift >= 0; shift -= 8) {
         __syncthreads();
@@ -322,236 +304,345 @@ __device__ uint32_t find_key(Shared& sh, int n, u64& need, u64& total, K key, F 
         }
         __syncthreads();
         if (threadIdx.x < 64) {
-            const int lane = threadIdx.x;
-            u64 h[4], own = 0;
-#pragma unroll
-            for (int j = 0; j < 4; j++) own += h[j] = sh.hist[255 - 4 * lane - j];
-            u64 run = wave_scan(own, lane);
+            const int b = 255 - 4 * (int)threadIdx.x;
+            const u64 h0 = sh.hist[b], h1 = sh.hist[b - 1], h2 = sh.hist[b - 2], h3 = sh.hist[b - 3];
+            u64 run = wave_scan(h0 + h1 + h2 + h3, (int)threadIdx.x);
             const u64 all = __shfl(run, 63, 64);
             if (need > all) need = all;
-            run -= own;
-            if (run < need && run + own >= need) {
-                for (int j = 0; j < 4; j++) {
-                    if (run + h[j] >= need) {
-                        sh.key = prefix | (uint32_t)(255 - 4 * lane - j) << shift;
-                        sh.need = need - run;
-                        sh.total = h[j];
-                        break;
-                    }
-                    run += h[j];
-                }
+            const u64 r3 = run - h3, r2 = r3 - h2, r1 = r2 - h1, r0 = r1 - h0;
+            if (r0 < need && run >= need) {
+                const int j = r1 >= need ? 0 : r2 >= need ? 1 : r3 >= need ? 2 : 3;
+                sh.key = prefix | (uint32_t)(b - j) << shift;
+                sh.need = need - (j == 0 ? r0 : j == 1 ? r1 : j == 2 ? r2 : r3);
             }
         }
         __syncthreads();
         prefix = sh.key;
         need = sh.need;
     }
-    total = sh.total;
     return prefix;
+}
+
+// Finds the first bin of the histogram h.mass at which the running sum reaches `need`, lowered
+// to the sum of all; `need` is then what that bin has to bring.
+__device__ int find_bin(Shared& sh, Turn& turn, u64& need) {
+    constexpr int B = kBins / kThreads;
+    u64 h[B], own = 0, all;
+#pragma unroll
+    for (int j = 0; j < B; j++) own += h[j] = sh.h.mass[threadIdx.x * B + j];
+    u64 run = block_scan(sh.part, turn, own, all) - own;
+    if (need > all) need = all;
+#pragma unroll
+    for (int j = 0; j < B; j++) {
+        if (run < need && run + h[j] >= need) {
+            sh.bin = threadIdx.x * B + j;
+            sh.need = need - run;
+        }
+        run += h[j];
+    }
+    __syncthreads();
+    need = sh.need;
+    return sh.bin;
+}
+
+__device__ __forceinline__ void clear_bins(Shared& sh) {
+    for (int i = threadIdx.x; i < kBins; i += kThreads) sh.h.mass[i] = 0;
+    __syncthreads();
+}
+
+// The candidate of list[0 .. n) at which the running sum of f, in the order of `rank` (larger
+// ones first, all different), reaches `need`: by buckets (rising in that order), then one wave
+// for those of the bucket.  Returns its order.
+template <class B, class R, class F>
+__device__ u64 find_item(Shared& sh, Turn& turn, int n, u64 need, B bucket, R rank, F f) {
+    const int tid = threadIdx.x;
+    __syncthreads();
+    clear_bins(sh);
+    for (int i = tid; i < n; i += kThreads) {
+        const u64 w = f(sh.list[i]);
+        if (w) atomicAdd(&sh.h.mass[bucket(sh.list[i])], w);
+    }
+    if (tid == 0) sh.n = 0;
+    __syncthreads();
+    const int bin = find_bin(sh, turn, need);
+    for (int i = tid; i < n; i += kThreads) {
+        const Candidate c = sh.list[i];
+        const u64 w = f(c);
+        if (!w || bucket(c) != bin) continue;
+        const int at = atomicAdd(&sh.n, 1);
+        if (at < kMini) sh.mini[at] = {c.order, w};
+    }
+    __syncthreads();
+    const int m = sh.n;
+    if (m > kMini) {  // by the upper, then the lower half of the rank
+        auto in = [&](int i) { return bucket(sh.list[i]) == bin ? f(sh.list[i]) : 0; };
+        const uint32_t hi = find_key(
+            sh, n, need, [&](int i) { return (uint32_t)(rank(sh.list[i].order) >> 32); }, in);
+        const uint32_t lo = find_key(
+            sh, n, need, [&](int i) { return (uint32_t)rank(sh.list[i].order); },
+            [&](int i) { return (uint32_t)(rank(sh.list[i].order) >> 32) == hi ? in(i) : 0; });
+        for (int i = tid; i < n; i += kThreads)
+            if (rank(sh.list[i].order) == ((u64)hi << 32 | lo)) sh.found = sh.list[i].order;
+    } else if (tid < m) {
+        const Candidate me = sh.mini[tid];
+        u64 before = 0;
+        for (int j = 0; j < m; j++)
+            before += rank(sh.mini[j].order) > rank(me.order) ? sh.mini[j].mass : 0;
+        if (before < need && before + me.mass >= need) sh.found = me.order;
+    }
+    __syncthreads();
+    return sh.found;
 }
 
 // A place in the order: all keys above `key`, and those equal to it up to index `last`.
 struct Cut {
-    uint32_t key;
-    int last;
+    uint32_t key = 0;
+    int last = 0x7fffffff;
     __device__ __forceinline__ bool keeps(uint32_t k, int i) const {
         return k > key || (k == key && i <= last);
     }
 };
-
-// The place in the order of the whole row at which the running sum of f(index, key, power)
-// reaches `need`: a histogram over the steps of weight, then the tokens of one step as a list;
-// over the row again where that list is too long (many equal logits).
-template <class E, class F>
-__device__ Cut cut_row(Shared& sh, const E* x, int V, const Row& r, u64 need, F f) {
-    for (int i = threadIdx.x; i < kBins; i += kThreads) sh.h.mass[i] = 0;
-    if (threadIdx.x == 0) sh.n = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < V; i += kThreads) {
-        const float v = value(x[i]);
-        const double t = r.power(v);
-        const u64 w = f(i, key_of(v), t);
-        if (w) atomicAdd(&sh.h.mass[r.bin(t)], w);
-    }
-    __syncthreads();
-    if (threadIdx.x < 64) {
-        const int lane = threadIdx.x, b0 = lane * (kBins / 64);
-        u64 own = 0;
-        for (int b = 0; b < kBins / 64; b++) own += sh.h.mass[b0 + b];
-        u64 run = wave_scan(own, lane);
-        const u64 all = __shfl(run, 63, 64);
-        if (need > all) need = all;
-        run -= own;
-        if (run < need && run + own >= need) {
-            int b = b0;
-            for (; run + sh.h.mass[b] < need; b++) run += sh.h.mass[b];
-            sh.bin = b;
-            sh.need = need - run;
-        }
-    }
-    __syncthreads();
-    const int bin = sh.bin;
-    need = sh.need;
-    for (int i = threadIdx.x; i < V; i += kThreads) {
-        const float v = value(x[i]);
-        const double t = r.power(v);
-        if (r.bin(t) != bin) continue;
-        const uint32_t key = key_of(v);
-        const u64 w = f(i, key, t);
-        if (!w) continue;
-        const int at = atomicAdd(&sh.n, 1);
-        if (at < kList) sh.list[at] = {(u64)key << 32 | (uint32_t)~i, w};
-    }
-    __syncthreads();
-    const int n = sh.n;
+__device__ __forceinline__ Cut cut_at(u64 order) {
     Cut c;
-    u64 total;
-    if (n > kList) {
-        auto key = [&](int i) { return key_of(value(x[i])); };
-        auto in = [&](int i) {
-            const float v = value(x[i]);
-            const double t = r.power(v);
-            return r.bin(t) == bin ? f(i, key_of(v), t) : 0;
-        };
-        c.key = find_key(sh, V, need, total, key, in);
-        c.last = find_index(sh, V, need, [&](int i) { return key(i) == c.key ? in(i) : 0; });
-    } else {
-        c.key = find_key(sh, n, need, total, [&](int i) { return (uint32_t)(sh.list[i].order >> 32); },
-                         [&](int i) { return sh.list[i].mass; });
-        c.last = (int)~find_key(
-            sh, n, need, total, [&](int i) { return (uint32_t)sh.list[i].order; },
-            [&](int i) { return (uint32_t)(sh.list[i].order >> 32) == c.key ? sh.list[i].mass : 0; });
-    }
-    __syncthreads();
+    c.key = (uint32_t)(order >> 32);
+    c.last = (int)~(uint32_t)order;
     return c;
 }
 
-// What a running mass has to reach for u of `all`.
-__device__ __forceinline__ u64 drawn_need(float u, u64 all) {
+// Calls fn(index, logit) for the row's logits i0 .. i1, eight a lane; i0 a multiple of 8.
+template <class E, class F>
+__device__ __forceinline__ void each(const E* x, int V, int i0, int i1, int who, int threads, F fn) {
+    float next[kVec];
+    int i = i0 + who * kVec;
+    if (i < i1) load8(x, i, V, next);
+    while (i < i1) {
+        float v[kVec];
+#pragma unroll
+        for (int j = 0; j < kVec; j++) v[j] = next[j];
+        const int at = i;
+        i += threads * kVec;
+        if (i < i1) load8(x, i, V, next);
+#pragma unroll
+        for (int j = 0; j < kVec; j++) fn(at + j, v[j]);
+    }
+}
+
+// A wave's run of the row's [lo, hi), in whole loads of a wave.
+__device__ __forceinline__ int run_of(int lo, int hi) {
+    constexpr int W = 64 * kVec;
+    return ((hi - lo + kWaves - 1) / kWaves + W - 1) / W * W;
+}
+
+// The first index at which the running sum of f(index, logit) over the row reaches `need` (at
+// most the sum of all), the sums of the waves' runs being in sh.range.
+template <class E, class F>
+__device__ int find_index(Shared& sh, Turn& turn, const E* x, int V, u64 need, F f) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int lo = 0, hi = V;
+    for (;;) {
+        const int per = run_of(lo, hi);
+        int w = 0;
+        for (; w < kWaves - 1 && lo + (w + 1) * per < hi && sh.range[w] < need; w++)
+            need -= sh.range[w];
+        lo += w * per;
+        hi = lo + per < hi ? lo + per : hi;
+        if (hi - lo <= kThreads * kVec) break;
+        const int next = run_of(lo, hi), i0 = lo + wave * next;
+        u64 s = 0;
+        each(x, V, i0, i0 + next < hi ? i0 + next : hi, lane, 64,
+             [&](int i, float v) { s += f(i, v); });
+        s = wave_sum(s);
+        __syncthreads();
+        if (lane == 0) sh.range[wave] = s;
+        __syncthreads();
+    }
+    u64 m[kVec], own = 0, all;
+    const int i0 = lo + (int)threadIdx.x * kVec;
+    float v[kVec];
+    if (i0 < hi) load8(x, i0, V, v);
+#pragma unroll
+    for (int j = 0; j < kVec; j++) own += m[j] = i0 + j < hi ? f(i0 + j, v[j]) : 0;
+    u64 run = block_scan(sh.part, turn, own, all) - own;
+    if (need > all) need = all;
+#pragma unroll
+    for (int j = 0; j < kVec; j++) {
+        if (run < need && run + m[j] >= need) sh.index = i0 + j;
+        run += m[j];
+    }
+    __syncthreads();
+    return sh.index;
+}
+
+// The place in the order of the whole row at which the running sum of f(index, logit) reaches
+// `need`: a histogram over the steps of weight, then the tokens of one step as a list; over
+// the row again where that list is too long.
+template <class E, class F>
+__device__ Cut cut_row(Shared& sh, Turn& turn, const E* x, int V, const Row& r, u64 need, F f) {
+    __syncthreads();
+    clear_bins(sh);
+    each(x, V, 0, V, threadIdx.x, kThreads, [&](int i, float v) {
+        const u64 w = f(i, v);
+        if (w) atomicAdd(&sh.h.mass[r.bin(r.power(v))], w);
+    });
+    if (threadIdx.x == 0) sh.n = 0;
+    __syncthreads();
+    const int bin = find_bin(sh, turn, need);
+    each(x, V, 0, V, threadIdx.x, kThreads, [&](int i, float v) {
+        if (r.bin(r.power(v)) != bin) return;
+        const u64 w = f(i, v);
+        if (!w) return;
+        const int at = atomicAdd(&sh.n, 1);
+        if (at < kList) sh.list[at] = {(u64)key_of(v) << 32 | (uint32_t)~i, w};
+    });
+    __syncthreads();
+    const int n = sh.n;
+    if (n <= kList)
+        return cut_at(find_item(
+            sh, turn, n, need,
+            [&](const Candidate& c) {
+                const double d = -r.power(value_of(key_at(c))) * r.step - bin;
+                return (int)(d * (kBins - 1));
+            },
+            [](u64 order) { return order; }, [](const Candidate& c) { return c.mass; }));
+    auto in = [&](int i) {
+        const float v = value(x[i]);
+        return r.bin(r.power(v)) == bin ? f(i, v) : 0;
+    };
+    auto key = [&](int i) { return key_of(value(x[i])); };
+    Cut c;
+    c.key = find_key(sh, V, need, key, in);
+    c.last = (int)~find_key(sh, V, need, [](int i) { return ~(uint32_t)i; },
+                            [&](int i) { return key(i) == c.key ? in(i) : 0; });
+    return c;
+}
+
+// What a running mass has to reach: the place p of `all`, for top-p; the place of u, for a draw.
+__device__ __forceinline__ u64 top_need(float p, double all) {
+    const u64 need = p > 0.0f ? (u64)__builtin_ceil((double)p * all) : 1;
+    return need ? need : 1;
+}
+__device__ __forceinline__ u64 draw_need(float u, u64 all) {
     const u64 need = u > 0.0f ? (u64)((double)(u < 1.0f ? u : 1.0f) * (double)all) + 1 : 1;
     return need < all ? need : all;
 }
 
-static_assert(kThreads * kVec == kPart && kPart == kSteps * kScanThreads * kVec, "parts");
+static_assert(kThreads * 2 * kVec == kPart && kPart == kSteps * kScanThreads * kVec, "parts");
 
 template <class E>
 __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, int parts) {
     __shared__ Shared sh;
+    Turn turn;
     const int64_t row = blockIdx.x;
     const E* x = (const E*)a.logits + row * a.ld;
-    const int V = (int)a.V, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int V = (int)a.V, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const Work w = work_of(a.work, row, parts);
-    Row r(a, row, V);
 
-    const uint32_t own = (int)threadIdx.x < parts ? w.part[threadIdx.x] : 0;
+    // parts <= kThreads: a thread each
+    const uint32_t own = tid < parts ? w.part[tid] : 0;
+    const double own_sum = tid < parts ? w.sum[tid] : 0.0;  // used where the row is summed
+    Row r(a, row, V);
     uint32_t best = fni8::wave_max_u32(own);
-    if (lane == 0) sh.part[wave] = best;
+    if (lane == 0) sh.counts[wave] = (int)best;
     __syncthreads();
-    for (int i = 0; i < kWaves; i++) best = sh.part[i] > best ? (uint32_t)sh.part[i] : best;
+#pragma unroll
+    for (int i = 0; i < kWaves; i++) best = (uint32_t)sh.counts[i] > best ? (uint32_t)sh.counts[i] : best;
     const float top = value_of(best);
-    auto answer = [&](int token, u64 all, double mass) {
-        // one thread: the token, and the logarithm of its share of the mass
-        a.tokens[row] = token;
-        if (a.logprobs)
-            a.logprobs[row] = (float)(r.power(value(x[token])) * 0.69314718055994531 -
-                                      log(all ? (double)all * __builtin_ldexp(1.0, -r.s) : mass));
-    };
     if (best == 0xffffffffu || r.T != r.T || top == -__builtin_inff()) {
-        if (threadIdx.x == 0) {  // a NaN, or nothing to draw
+        if (tid == 0) {  // a NaN, or nothing to draw
             a.tokens[row] = -1;
             if (a.logprobs) a.logprobs[row] = __builtin_nanf("");
         }
         return;
     }
     r.largest(top);
+    auto answer = [&](int token, double share) {  // one thread; the mass in units of the largest
+        a.tokens[row] = token;
+        if (a.logprobs)
+            a.logprobs[row] = (float)(r.power(value(x[token])) * 0.69314718055994531 - log(share));
+    };
+    // The lowest of the threads' numbers (rising with the thread) that have `first`; where none
+    // has, the highest that has `any`.
+    auto pick = [&](bool first, bool any, int number) {
+        const u64 f = __ballot(first), g = __ballot(any);
+        const int lo = __shfl(number, f ? __builtin_ctzll(f) : 0, 64);
+        const int hi = __shfl(number, g ? 63 - __builtin_clzll(g) : 0, 64);
+        __syncthreads();
+        if (lane == 0) {
+            sh.counts[wave] = f ? lo : 0x7fffffff;
+            sh.highs[wave] = g ? hi : -1;
+        }
+        __syncthreads();
+        int l = 0x7fffffff, h = -1;
+#pragma unroll
+        for (int i = 0; i < kWaves; i++) {
+            l = sh.counts[i] < l ? sh.counts[i] : l;
+            h = sh.highs[i] > h ? sh.highs[i] : h;
+        }
+        return l != 0x7fffffff ? l : h;
+    };
+    auto load16 = [&](int i0, float (&v)[2 * kVec]) {
+        float lo[kVec], hi[kVec];
+        load8(x, i0, V, lo);
+        load8(x, i0 + kVec, V, hi);
+#pragma unroll
+        for (int j = 0; j < kVec; j++) {
+            v[j] = lo[j];
+            v[j + kVec] = hi[j];
+        }
+    };
     if (!(r.T > 0.0f)) {  // the first of the largest, in the first part that holds one
-        if (threadIdx.x == 0) sh.index = V;
-        __syncthreads();
-        if (own == best) atomicMin(&sh.index, (int)threadIdx.x);
-        __syncthreads();
-        const int first = sh.index * kPart;
-        float v[kVec];
-        load8(x, first + (int)threadIdx.x * kVec, V, v);
-        __syncthreads();
-        if (threadIdx.x == 0) sh.index = V;
-        __syncthreads();
-        int at = V;
-        for (int j = kVec - 1; j >= 0; j--)
-            if (key_of(v[j]) == best) at = first + (int)threadIdx.x * kVec + j;
-        if (at < V) atomicMin(&sh.index, at);
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            a.tokens[row] = sh.index;
+        const int i0 = pick(own == best, false, tid) * kPart + tid * 2 * kVec;
+        float v[2 * kVec];
+        load16(i0, v);
+        int at = -1;
+#pragma unroll
+        for (int j = 2 * kVec - 1; j >= 0; j--)
+            if (v[j] == top) at = i0 + j;
+        at = pick(at >= 0, false, at);
+        if (tid == 0) {
+            a.tokens[row] = at;
             if (a.logprobs) a.logprobs[row] = 0.0f;
         }
         return;
     }
-    double mass = 0.0, part = 0.0;  // of the row, of this thread's part; relative to the largest
+    double mass = 0.0, part = 0.0, run = 0.0;  // of the row, of this thread's part, up to it
     if (r.summed()) {
-        if ((int)threadIdx.x < parts)
-            part = w.sum[threadIdx.x] * exp2_neg(r.power(value_of(own)));
-        mass = block_sum(sh.sums, part);
+        if (tid < parts) part = own_sum * exp2_at(r.power(value_of(own)), 0);
+        run = block_scan(sh.sums, turn, part, mass);
     }
     if (!r.by_k && !r.by_p && !r.by_m) {  // no filter: the part, then the token in it
+        // the first whose end passes `want`; where rounding leaves none, the last with mass
         const double want = (double)(r.u > 0.0f ? r.u < 1.0f ? r.u : 1.0f : 0.0f) * mass;
-        double run = wave_scan(part, lane);
-        __syncthreads();
-        if (lane == 63) sh.sums[wave] = run;
-        if (threadIdx.x == 0) sh.index = -1;
-        __syncthreads();
-        for (int i = 0; i < wave; i++) run += sh.sums[i];
-        // the first part whose end passes `want`; rounding may leave none: the last with mass
-        const bool past = run > want && part > 0.0;
-        if (threadIdx.x == 0) sh.bin = parts;
-        __syncthreads();
-        if (past) atomicMin(&sh.bin, (int)threadIdx.x);
-        if (part > 0.0) atomicMax(&sh.index, (int)threadIdx.x);
-        __syncthreads();
-        const int p = sh.bin < parts ? sh.bin : sh.index;
-        if ((int)threadIdx.x == p) sh.sums[0] = run - part;
-        __syncthreads();
-        const double before = sh.sums[0];
-        float v[kVec];
-        double m[kVec], sum = 0.0;
-        const int i0 = p * kPart + (int)threadIdx.x * kVec;
-        load8(x, i0, V, v);
+        const bool live = part > 0x1p-900;
+        const int p = pick(live && run > want, live, tid);
+        if (tid == p) sh.before = run - part;
+        const int i0 = p * kPart + tid * 2 * kVec;
+        float v[2 * kVec];
+        load16(i0, v);
+        double m[2 * kVec], sum = 0.0, all;
 #pragma unroll
-        for (int j = 0; j < kVec; j++) sum += m[j] = exp2_neg(r.power(v[j]));
-        run = wave_scan(sum, lane);
-        __syncthreads();
-        if (lane == 63) sh.sums[wave] = run;
-        if (threadIdx.x == 0) {
-            sh.index = -1;
-            sh.bin = V;
-        }
-        __syncthreads();
-        double base = before;
-        for (int i = 0; i < wave; i++) base += sh.sums[i];
-        run = base + (run - sum);
-        int at = V, last = -1;
+        for (int j = 0; j < 2 * kVec; j++) sum += m[j] = exp2_at(r.power(v[j]), 0);
+        run = block_scan(sh.sums, turn, sum, all);
+        run = sh.before + (run - sum);
+        int at = -1, last = -1;
 #pragma unroll
-        for (int j = 0; j < kVec; j++) {
+        for (int j = 0; j < 2 * kVec; j++) {
             run += m[j];
-            if (m[j] > 0.0) {
+            if (m[j] > 0x1p-900) {
                 last = i0 + j;
-                if (run > want && at == V) at = i0 + j;
+                at = at < 0 && run > want ? last : at;
             }
         }
-        if (at < V) atomicMin(&sh.bin, at);
-        if (last >= 0) atomicMax(&sh.index, last);
-        __syncthreads();
-        if (threadIdx.x == 0) answer(sh.bin < V ? sh.bin : sh.index, 0, mass);
+        const int token = pick(at >= 0, last >= 0, at >= 0 ? at : last);
+        if (tid == 0) answer(token, mass);
         return;
     }
 
     // ---- a bound on the kept prefix, from the threads' maxima
     const double unit = __builtin_ldexp(1.0, r.s);
     const int groups = parts * kScanThreads;
-    u64 need_p = 0;
-    if (r.by_p && !r.by_k) {
-        need_p = r.p > 0.0f ? (u64)__builtin_ceil((double)r.p * (mass * unit)) : 1;
-        need_p = need_p ? need_p : 1;
-    }
+    const bool whole = r.by_p && !r.by_k;  // top-p of the whole mass
+    const u64 need_p = whole ? top_need(r.p, mass * unit) : 0;
     const u64 floor = (u64)__builtin_rint((double)r.least * unit);
     // The step in which min-p ends, and one more for log2's own rounding: no token further down
     // has a mass that rounds to `floor`.  Top-p after top-k needs the whole mass of top-k.
@@ -561,48 +652,51 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, i
         bound = least = least < bound ? least : bound;
     }
     if (r.by_k || r.by_p) {
-        for (int i = threadIdx.x; i < kBins; i += kThreads) {
+        for (int i = tid; i < kBins; i += kThreads) {
             sh.h.mass[i] = 0;
             sh.h.count[i] = 0;
         }
-        if (threadIdx.x == 0) sh.bin = kBins;
+        if (tid == 0) sh.bin = sh.bin2 = kBins;
         __syncthreads();
-        for (int i = threadIdx.x; i < groups; i += kThreads) {
+        for (int i = tid; i < groups; i += kThreads) {
             const double t = r.power(value_of(w.top[i]));
             const int b = r.bin(t);
             if (b > bound) continue;
             atomicAdd(&sh.h.count[b], 1u);
-            if (!r.by_k) atomicAdd(&sh.h.mass[b], exp2_fixed(t, r.s));
+            if (whole) atomicAdd(&sh.h.mass[b], exp2_fixed(t, r.s));
         }
         __syncthreads();
-        // two steps a thread; the first at which the count or the mass is there
-        const uint32_t want = r.by_k ? (uint32_t)r.k : kEnough;
-        const int b = 2 * threadIdx.x;
-        const uint32_t c0 = sh.h.count[b], c1 = sh.h.count[b + 1];
-        const u64 m0 = sh.h.mass[b], m1 = sh.h.mass[b + 1];
-        int runc = fni8::wave_incl_scan_i32((int)(c0 + c1), lane);
-        u64 runm = wave_scan(m0 + m1, lane);
-        __shared__ int counts[kWaves];
-        if (lane == 63) {
-            counts[wave] = runc;
-            sh.part[wave] = runm;
+        // the step at which the count is there, or the mass
+        constexpr int B = kBins / kThreads;
+        const int want = r.by_k ? r.k : kEnough;
+        int c[B], some = 0, total;
+#pragma unroll
+        for (int j = 0; j < B; j++) some += c[j] = (int)sh.h.count[tid * B + j];
+        int rank = block_scan(sh.ints, turn, some, total) - some;
+#pragma unroll
+        for (int j = 0; j < B; j++) {
+            if (rank < want && rank + c[j] >= want) sh.bin = tid * B + j;
+            rank += c[j];
         }
-        __syncthreads();
-        for (int i = 0; i < wave; i++) {
-            runc += counts[i];
-            runm += sh.part[i];
+        if (whole) {
+            u64 m[B], some = 0, total;
+#pragma unroll
+            for (int j = 0; j < B; j++) some += m[j] = sh.h.mass[tid * B + j];
+            u64 to = block_scan(sh.part, turn, some, total) - some;
+#pragma unroll
+            for (int j = 0; j < B; j++) {
+                if (to < need_p && to + m[j] >= need_p) sh.bin2 = tid * B + j;
+                to += m[j];
+            }
         }
-        auto there = [&](uint32_t c, u64 m) { return c >= want || (!r.by_k && m >= need_p); };
-        if (there((uint32_t)runc - c1, runm - m1)) atomicMin(&sh.bin, b);
-        else if (there((uint32_t)runc, runm)) atomicMin(&sh.bin, b + 1);
         __syncthreads();
         bound = sh.bin < bound ? sh.bin : bound;
+        bound = sh.bin2 < bound ? sh.bin2 : bound;
     }
     // ---- the tokens down to the bound, from the groups whose maximum reaches it
+    if (tid == 0) sh.n = sh.hits_n = 0;
     __syncthreads();
-    if (threadIdx.x == 0) sh.n = sh.hits_n = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < groups; i += kThreads) {
+    for (int i = tid; i < groups; i += kThreads) {
         if (r.bin(r.power(value_of(w.top[i]))) > bound) continue;
         const int at = atomicAdd(&sh.hits_n, 1);
         if (at < kHits) sh.hits[at] = i;
@@ -610,7 +704,7 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, i
     __syncthreads();
     const int hits = sh.hits_n;
     if (hits <= kHits) {
-        for (int q = threadIdx.x; q < hits * kSteps; q += kThreads) {
+        for (int q = tid; q < hits * kSteps; q += kThreads) {
             const int group = sh.hits[q / kSteps];
             const int i0 = group / kScanThreads * kPart +
                            (q % kSteps * kScanThreads + group % kScanThreads) * kVec;
@@ -626,147 +720,108 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, i
                 if (at < kList) sh.list[at] = {(u64)key_of(v[j]) << 32 | (uint32_t)~(i0 + j), m};
             }
         }
-        __syncthreads();
     }
+    __syncthreads();
     int n = hits <= kHits ? sh.n : kList + 1;
-    if (n <= kList && r.by_p && !r.by_k && bound < least) {
+    if (n <= kList && whole && bound < least) {
         // top-p may end below the bound, and does unless the list has the mass
-        const u64 listed = sum_of(sh, n, [&](int i) { return sh.list[i].mass; });
-        if (listed < need_p) n = kList + 1;
+        u64 listed = 0;
+        for (int i = tid; i < n; i += kThreads) listed += sh.list[i].mass;
+        if (block_sum(sh, turn, listed) < need_p) n = kList + 1;
+    }
+    if (n <= kMini) {
+        // one wave, every pair: a token's rank and the mass before it, then its mass by index
+        if (wave) return;
+        const Candidate me = lane < n ? sh.list[lane] : Candidate{0, 0};
+        const int key = (int)key_at(me), place = (int)place_at(me);
+        auto other = [&](u64 v, int j) {
+            return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), j) << 32 |
+                   (uint32_t)__builtin_amdgcn_readlane((int)v, j);
+        };
+        int rank = 0;
+        u64 before = 0;
+        for (int j = 0; j < n; j++) {
+            const uint32_t k = (uint32_t)__builtin_amdgcn_readlane(key, j);
+            const uint32_t p = (uint32_t)__builtin_amdgcn_readlane(place, j);
+            const bool first = k > (uint32_t)key || (k == (uint32_t)key && p > (uint32_t)place);
+            rank += first;
+            before += first ? other(me.mass, j) : 0;
+        }
+        bool keep = lane < n && (!r.by_k || rank < r.k);
+        const u64 ranked = wave_sum(keep ? me.mass : 0);
+        if (r.by_p) keep = keep && before < (whole ? need_p : top_need(r.p, (double)ranked));
+        keep = keep && me.mass >= floor;
+        const u64 mine = keep ? me.mass : 0, all = wave_sum(mine), need = draw_need(r.u, all);
+        u64 to = 0;
+        for (int j = 0; j < n; j++) {
+            const uint32_t p = (uint32_t)__builtin_amdgcn_readlane(place, j);
+            to += p >= (uint32_t)place ? other(mine, j) : 0;
+        }
+        if (keep && to >= need && to - mine < need) answer((int)~place_at(me), (double)all / unit);
+        return;
     }
     u64 all;
     int token;
-    if (n <= kPairs) {
-        // every pair: a token's rank and the mass before it; then its mass up to it by index
-        int wide = 64;
-        while (wide < n) wide *= 2;
-        const int i = (threadIdx.x & (wide - 1)), ways = kThreads / wide, way = threadIdx.x / wide;
-        if ((int)threadIdx.x < kPairs) {
-            sh.pair.before[threadIdx.x] = 0;
-            sh.pair.rank[threadIdx.x] = 0;
-        }
-        if (threadIdx.x == 0) sh.kept = sh.all = 0;
-        __syncthreads();
-        Candidate me{0, 0};
-        if (i < n) {
-            me = sh.list[i];
-            uint32_t rank = 0;
-            u64 before = 0;
-            for (int j = way; j < n; j += ways) {
-                const Candidate c = sh.list[j];
-                if (c.order > me.order) {
-                    rank++;
-                    before += c.mass;
-                }
-            }
-            atomicAdd(&sh.pair.rank[i], rank);
-            atomicAdd(&sh.pair.before[i], before);
-        }
-        __syncthreads();
-        bool keep = i < n;
-        if (keep && r.by_k) {
-            keep = (int)sh.pair.rank[i] < r.k;
-            if (r.by_p && keep && way == 0) atomicAdd(&sh.kept, me.mass);
-        }
-        __syncthreads();
-        if (keep && r.by_p) {
-            u64 need = need_p;
-            if (r.by_k) {
-                need = r.p > 0.0f ? (u64)__builtin_ceil((double)r.p * (double)sh.kept) : 1;
-                need = need ? need : 1;
-            }
-            keep = sh.pair.before[i] < need;
-        }
-        keep = keep && me.mass >= floor;
-        __syncthreads();
-        if (way == 0 && i < n) {
-            if (keep) atomicAdd(&sh.all, me.mass);
-            else sh.list[i].mass = 0;
-            sh.pair.before[i] = 0;
-        }
-        __syncthreads();
-        all = sh.all;
-        const u64 need = drawn_need(r.u, all);
-        if (keep) {
-            u64 run = 0;
-            for (int j = way; j < n; j += ways) {
-                const Candidate c = sh.list[j];
-                if ((uint32_t)c.order >= (uint32_t)me.order) run += c.mass;
-            }
-            atomicAdd(&sh.pair.before[i], run);
-        }
-        __syncthreads();
-        if (keep && way == 0) {
-            const u64 run = sh.pair.before[i];
-            if (run >= need && run - me.mass < need) sh.index = (int)~(uint32_t)me.order;
-        }
-        __syncthreads();
-        token = sh.index;
-    } else if (n <= kList) {
-        auto key = [&](int i) { return (uint32_t)(sh.list[i].order >> 32); };
-        auto place = [&](int i) { return (uint32_t)sh.list[i].order; };
-        Cut c{0, V - 1};
-        auto kept = [&](int i) {
-            return c.keeps(key(i), (int)~place(i)) ? sh.list[i].mass : 0;
+    Cut c;
+    if (n <= kList) {
+        auto bucket = [&](const Candidate& i) { return r.bin(r.power(value_of(key_at(i)))); };
+        auto order = [](u64 o) { return o; };
+        auto kept = [&](const Candidate& i) {
+            return c.keeps(key_at(i), (int)~place_at(i)) ? i.mass : 0;
         };
-        u64 total;
-        if (r.by_k && r.k < n) {
-            u64 need = r.k;
-            const uint32_t k = find_key(sh, n, need, total, key, [](int) { return 1ull; });
-            const uint32_t l = find_key(sh, n, need, total, place,
-                                        [&](int i) { return (u64)(key(i) == k); });
-            c = {k, (int)~l};
-        }
+        if (r.by_k)
+            c = cut_at(find_item(sh, turn, n, r.k, bucket, order, [](const Candidate&) { return 1ull; }));
+        auto sum_of = [&](u64 least) {
+            u64 s = 0;
+            for (int i = tid; i < n; i += kThreads) {
+                const u64 m = kept(sh.list[i]);
+                s += m >= least ? m : 0;
+            }
+            return block_sum(sh, turn, s);
+        };
         if (r.by_p) {
-            u64 need = need_p;
-            if (r.by_k) {
-                const u64 sum = sum_of(sh, n, kept);
-                need = r.p > 0.0f ? (u64)__builtin_ceil((double)r.p * (double)sum) : 1;
-                need = need ? need : 1;
-            }
-            const uint32_t k = find_key(sh, n, need, total, key, kept);
-            const uint32_t l = find_key(sh, n, need, total, place,
-                                        [&](int i) { return key(i) == k ? kept(i) : 0; });
-            c = {k, (int)~l};
+            const u64 need = whole ? need_p : top_need(r.p, (double)sum_of(0));
+            c = cut_at(find_item(sh, turn, n, need, bucket, order, kept));
         }
-        auto drawn = [&](int i) {
-            const u64 m = kept(i);
-            return m >= floor ? m : 0;
-        };
-        all = sum_of(sh, n, drawn);
-        u64 need = drawn_need(r.u, all);
-        token = (int)~find_key(sh, n, need, total, place, drawn);
+        all = sum_of(floor);
+        const int shift = 32 - __builtin_clz(V) > 11 ? 32 - __builtin_clz(V) - 11 : 0;
+        token = (int)~(uint32_t)find_item(
+            sh, turn, n, draw_need(r.u, all),
+            [&](const Candidate& i) { return (int)(~place_at(i) >> shift); },
+            [](u64 o) { return (u64)(uint32_t)o; },
+            [&](const Candidate& i) {
+                const u64 m = kept(i);
+                return m >= floor ? m : 0;
+            });
     } else {
-        Cut c{0, V - 1};
-        auto kept = [&](int i, uint32_t key, double t) {
-            return c.keeps(key, i) ? exp2_fixed(t, r.s) : 0;
-        };
-        if (r.by_k) {
-            auto some = [&](int, uint32_t, double t) { return (u64)(exp2_fixed(t, r.s) != 0); };
-            auto at = [&](int i) { return some(i, 0, r.power(value(x[i]))); };
-            if (sum_of(sh, V, at) > (u64)r.k) c = cut_row(sh, x, V, r, r.k, some);
-        }
-        if (r.by_p) {
-            u64 need = need_p;
-            if (r.by_k) {
-                const u64 sum = sum_of(sh, V, [&](int i) {
-                    const float v = value(x[i]);
-                    return kept(i, key_of(v), r.power(v));
-                });
-                need = r.p > 0.0f ? (u64)__builtin_ceil((double)r.p * (double)sum) : 1;
-                need = need ? need : 1;
-            }
-            c = cut_row(sh, x, V, r, need, kept);
-        }
-        auto drawn = [&](int i) {
-            const float v = value(x[i]);
-            const u64 m = kept(i, key_of(v), r.power(v));
+        auto kept = [&](int i, float v) { return c.keeps(key_of(v), i) ? r.mass(v) : 0; };
+        auto drawn = [&](int i, float v) {
+            const u64 m = kept(i, v);
             return m >= floor ? m : 0;
         };
-        all = sum_of(sh, V, drawn);
-        token = find_index(sh, V, drawn_need(r.u, all), drawn);
+        auto sum_of = [&](auto f) {  // and the sums of the waves' runs
+            const int per = run_of(0, V), i0 = wave * per;
+            u64 s = 0;
+            each(x, V, i0, i0 + per < V ? i0 + per : V, lane, 64,
+                 [&](int i, float v) { s += f(i, v); });
+            s = wave_sum(s);
+            __syncthreads();
+            if (lane == 0) sh.range[wave] = s;
+            __syncthreads();
+            s = 0;
+#pragma unroll
+            for (int i = 0; i < kWaves; i++) s += sh.range[i];
+            return s;
+        };
+        if (r.by_k)
+            c = cut_row(sh, turn, x, V, r, r.k,
+                        [&](int, float v) { return (u64)(r.power(v) > -(double)(r.s + 1)); });
+        if (r.by_p)
+            c = cut_row(sh, turn, x, V, r, whole ? need_p : top_need(r.p, (double)sum_of(kept)), kept);
+        all = sum_of(drawn);
+        token = find_index(sh, turn, x, V, draw_need(r.u, all), drawn);
     }
-    if (threadIdx.x == 0) answer(token, all, 0.0);
+    if (tid == 0) answer(token, (double)all / unit);
 }
 
 template <class E>
