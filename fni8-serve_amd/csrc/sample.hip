@@ -55,8 +55,10 @@ __device__ __forceinline__ double exp2_at(double t, int s) {
     q = __builtin_fma(q, f, 0.24022650695910075);
     q = __builtin_fma(q, f, 0.6931471805599462);
     q = __builtin_fma(q, f, 1.0);
-    const u64 n = (u64)(uint32_t)__builtin_bit_cast(u64, tn) << 52;
-    return __builtin_bit_cast(double, __builtin_bit_cast(u64, q) + n);
+    // n + s times 2^20 onto the upper word
+    const u64 b = __builtin_bit_cast(u64, q);
+    const uint32_t n = (uint32_t)__builtin_bit_cast(u64, tn);
+    return __builtin_bit_cast(double, (u64)((uint32_t)(b >> 32) + (n << 20)) << 32 | (uint32_t)b);
 }
 
 // The same as an integer, rounded, for s <= 50: adding 2^52 leaves it in the sum's low bits.
@@ -101,10 +103,10 @@ __device__ __forceinline__ void load8(const E* x, int i, int V, float (&v)[kVec]
 struct Row {
     float T, p, least, u, top;
     int k, s;
-    double rate, base, cap, step;
-    bool by_k, by_p, by_m;
+    double rate, base, step;
+    bool by_k, by_p, by_m, inf;
 
-    __device__ Row(const fni8h::Sample& a, int64_t row, int V) {
+    __device__ __forceinline__ Row(const fni8h::Sample& a, int64_t row, int V) {
         T = a.temperature ? a.temperature[row] : a.temperature1;
         k = a.top_k ? a.top_k[row] : a.top_k1;
         p = a.top_p ? a.top_p[row] : a.top_p1;
@@ -120,19 +122,25 @@ struct Row {
         step = (kBins - 2) / (double)(s + 2);
     }
     // Every weight of the row is summed: for top-p without top-k, and without any filter.
-    __device__ bool summed() const { return T > 0.0f && !by_k && (by_p || !by_m); }
-    // Plus infinity counts as 10^300 with a rate that leaves nothing of any finite logit.
-    __device__ void largest(float x) {
-        top = x;
-        const bool inf = x == __builtin_inff();
+    __device__ __forceinline__ bool summed() const { return T > 0.0f && !by_k && (by_p || !by_m); }
+    __device__ __forceinline__ void largest(float x) {
+        inf = x == __builtin_inff();
+        top = inf ? 0.0f : x;
+        base = top == -__builtin_inff() ? 0.0 : (double)top;
         rate = 1.4426950408889634 / (double)T;
-        if (inf && rate < 1e-200) rate = 1e-200;
-        cap = inf ? 1e300 : 1e200;
-        base = inf ? 1e300 : (double)x;
+        rate = rate > 1e-300 ? rate : 1e-300;
     }
-    // log2 of a logit's weight, at least -1000 (minus infinity too, whatever the rate)
+    // Beside plus infinity nothing else has weight: it counts as 0, the rest as minus infinity.
+    __device__ __forceinline__ float seen(float v) const {
+        return !inf ? v : v == __builtin_inff() ? 0.0f : -__builtin_inff();
+    }
+    // log2 of a seen logit's weight, down to -1000 (minus infinity too): of two negative numbers
+    // the lower has the larger upper word.
     __device__ __forceinline__ double power(float v) const {
-        return __builtin_fmax((__builtin_fmin((double)v, cap) - base) * rate, -1000.0);
+        const u64 t = __builtin_bit_cast(u64, ((double)v - base) * rate);
+        uint32_t hi = (uint32_t)(t >> 32);
+        hi = hi < 0xc08f4000u ? hi : 0xc08f4000u;
+        return __builtin_bit_cast(double, (u64)hi << 32 | (uint32_t)t);
     }
     __device__ __forceinline__ u64 mass(float v) const { return exp2_fixed(power(v), s); }
     // Step of a weight, rising as it falls; kBins - 1 for weights that round to 0.
@@ -141,6 +149,16 @@ struct Row {
         return d < (double)(kBins - 1) ? (int)d : kBins - 1;
     }
 };
+
+// Eight seen logits.
+template <class E>
+__device__ __forceinline__ void load8(const E* x, int i, int V, const Row& r, float (&v)[kVec]) {
+    load8(x, i, V, v);
+    if (r.inf) {
+#pragma unroll
+        for (int j = 0; j < kVec; j++) v[j] = r.seen(v[j]);
+    }
+}
 
 // What scan leaves of a row, in the workspace.
 struct Work {
@@ -152,7 +170,7 @@ __host__ __device__ inline int64_t parts_of(int64_t V) { return (V + kPart - 1) 
 __host__ __device__ inline int64_t row_bytes(int64_t parts) {
     return (parts * (8 + 4 + 4 * kScanThreads) + 15) / 16 * 16;
 }
-__device__ inline Work work_of(int8_t* w, int64_t row, int64_t parts) {
+__device__ __forceinline__ Work work_of(int8_t* w, int64_t row, int64_t parts) {
     w += row * row_bytes(parts);
     Work r;
     r.sum = reinterpret_cast<double*>(w);
@@ -213,6 +231,12 @@ __global__ __launch_bounds__(kScanThreads) void scan_kernel(const fni8h::Sample 
     if (threadIdx.x == 0) w.part[part] = best;
     if (!r.summed()) return;
     r.largest(value_of(best));
+    if (r.inf) {
+#pragma unroll
+        for (int i = 0; i < kSteps; i++)
+#pragma unroll
+            for (int j = 0; j < kVec; j++) v[i][j] = r.seen(v[i][j]);
+    }
     double sum = 0.0;
 #pragma unroll
     for (int i = 0; i < kSteps; i++)
@@ -235,10 +259,12 @@ struct Shared {
     union {
         struct {
             u64 mass[kBins];
-            uint32_t count[kBins];
+            union {
+                uint32_t count[kBins];
+                u64 hist[256];
+            };
         } h;
         uint32_t hits[kHits];
-        u64 hist[256];
     };
     Candidate list[kList], mini[kMini];
     u64 part[2][kWaves], range[kWaves];
@@ -253,7 +279,7 @@ struct Shared {
 // writes: who writes a row again has passed the barrier of the sum between.
 struct Turn {
     int t = 0;
-    __device__ int next() { return t ^= 1; }
+    __device__ __forceinline__ int next() { return t ^= 1; }
 };
 
 __device__ __forceinline__ u64 block_sum(Shared& sh, Turn& turn, u64 v) {
@@ -290,22 +316,22 @@ __device__ __forceinline__ N block_scan(N (&rows)[2][kWaves], Turn& turn, N v, N
 // key have to bring.  Four passes over the items, eight bits of the key each: for lists that
 // are too long otherwise (thousands of equal logits).
 template <class K, class F>
-__device__ uint32_t find_key(Shared& sh, int n, u64& need, K key, F f) {
+__device__ __forceinline__ uint32_t find_key(Shared& sh, int n, u64& need, K key, F f) {
     uint32_t prefix = 0;
     for (int shift = 24; shift >= 0; shift -= 8) {
         __syncthreads();
-        if (threadIdx.x < 256) sh.hist[threadIdx.x] = 0;
+        if (threadIdx.x < 256) sh.h.hist[threadIdx.x] = 0;
         __syncthreads();
         for (int i = threadIdx.x; i < n; i += kThreads) {
             const uint32_t k = key(i);
             if (shift < 24 && (k ^ prefix) >> (shift + 8)) continue;
             const u64 w = f(i);
-            if (w) atomicAdd(&sh.hist[(k >> shift) & 255], w);
+            if (w) atomicAdd(&sh.h.hist[(k >> shift) & 255], w);
         }
         __syncthreads();
         if (threadIdx.x < 64) {
             const int b = 255 - 4 * (int)threadIdx.x;
-            const u64 h0 = sh.hist[b], h1 = sh.hist[b - 1], h2 = sh.hist[b - 2], h3 = sh.hist[b - 3];
+            const u64 h0 = sh.h.hist[b], h1 = sh.h.hist[b - 1], h2 = sh.h.hist[b - 2], h3 = sh.h.hist[b - 3];
             u64 run = wave_scan(h0 + h1 + h2 + h3, (int)threadIdx.x);
             const u64 all = __shfl(run, 63, 64);
             if (need > all) need = all;
@@ -325,7 +351,7 @@ __device__ uint32_t find_key(Shared& sh, int n, u64& need, K key, F f) {
 
 // Finds the first bin of the histogram h.mass at which the running sum reaches `need`, lowered
 // to the sum of all; `need` is then what that bin has to bring.
-__device__ int find_bin(Shared& sh, Turn& turn, u64& need) {
+__device__ __forceinline__ int find_bin(Shared& sh, Turn& turn, u64& need) {
     constexpr int B = kBins / kThreads;
     u64 h[B], own = 0, all;
 #pragma unroll
@@ -350,11 +376,27 @@ __device__ __forceinline__ void clear_bins(Shared& sh) {
     __syncthreads();
 }
 
+// The candidate of list[0 .. n), weighed by h.mass, at which the running sum reaches `need`, in
+// their order or by index; its order goes to `found`.  Not inlined: for buckets with more
+// than 64 candidates, mostly equal logits.
+__device__ __attribute__((noinline)) void radix_item(Shared* sh, int n, u64 need, bool by_value) {
+    __syncthreads();
+    auto mass = [&](int i) { return sh->h.mass[i]; };
+    uint32_t hi = 0;
+    if (by_value) hi = find_key(*sh, n, need, [&](int i) { return key_at(sh->list[i]); }, mass);
+    const uint32_t lo = find_key(
+        *sh, n, need, [&](int i) { return place_at(sh->list[i]); },
+        [&](int i) { return !by_value || key_at(sh->list[i]) == hi ? mass(i) : 0; });
+    for (int i = threadIdx.x; i < n; i += kThreads)
+        if (place_at(sh->list[i]) == lo && (!by_value || key_at(sh->list[i]) == hi))
+            sh->found = sh->list[i].order;
+}
+
 // The candidate of list[0 .. n) at which the running sum of f, in the order of `rank` (larger
 // ones first, all different), reaches `need`: by buckets (rising in that order), then one wave
 // for those of the bucket.  Returns its order.
 template <class B, class R, class F>
-__device__ u64 find_item(Shared& sh, Turn& turn, int n, u64 need, B bucket, R rank, F f) {
+__device__ __forceinline__ u64 find_item(Shared& sh, Turn& turn, int n, u64 need, B bucket, R rank, F f) {
     const int tid = threadIdx.x;
     __syncthreads();
     clear_bins(sh);
@@ -374,15 +416,10 @@ __device__ u64 find_item(Shared& sh, Turn& turn, int n, u64 need, B bucket, R ra
     }
     __syncthreads();
     const int m = sh.n;
-    if (m > kMini) {  // by the upper, then the lower half of the rank
-        auto in = [&](int i) { return bucket(sh.list[i]) == bin ? f(sh.list[i]) : 0; };
-        const uint32_t hi = find_key(
-            sh, n, need, [&](int i) { return (uint32_t)(rank(sh.list[i].order) >> 32); }, in);
-        const uint32_t lo = find_key(
-            sh, n, need, [&](int i) { return (uint32_t)rank(sh.list[i].order); },
-            [&](int i) { return (uint32_t)(rank(sh.list[i].order) >> 32) == hi ? in(i) : 0; });
+    if (m > kMini) {
         for (int i = tid; i < n; i += kThreads)
-            if (rank(sh.list[i].order) == ((u64)hi << 32 | lo)) sh.found = sh.list[i].order;
+            sh.h.mass[i] = bucket(sh.list[i]) == bin ? f(sh.list[i]) : 0;
+        radix_item(&sh, n, need, rank(~0ull) >> 32 != 0);
     } else if (tid < m) {
         const Candidate me = sh.mini[tid];
         u64 before = 0;
@@ -411,17 +448,18 @@ __device__ __forceinline__ Cut cut_at(u64 order) {
 
 // Calls fn(index, logit) for the row's logits i0 .. i1, eight a lane; i0 a multiple of 8.
 template <class E, class F>
-__device__ __forceinline__ void each(const E* x, int V, int i0, int i1, int who, int threads, F fn) {
+__device__ __forceinline__ void each(const E* x, int V, const Row& r, int i0, int i1, int who,
+                                     int threads, F fn) {
     float next[kVec];
     int i = i0 + who * kVec;
-    if (i < i1) load8(x, i, V, next);
+    if (i < i1) load8(x, i, V, r, next);
     while (i < i1) {
         float v[kVec];
 #pragma unroll
         for (int j = 0; j < kVec; j++) v[j] = next[j];
         const int at = i;
         i += threads * kVec;
-        if (i < i1) load8(x, i, V, next);
+        if (i < i1) load8(x, i, V, r, next);
 #pragma unroll
         for (int j = 0; j < kVec; j++) fn(at + j, v[j]);
     }
@@ -436,7 +474,8 @@ __device__ __forceinline__ int run_of(int lo, int hi) {
 // The first index at which the running sum of f(index, logit) over the row reaches `need` (at
 // most the sum of all), the sums of the waves' runs being in sh.range.
 template <class E, class F>
-__device__ int find_index(Shared& sh, Turn& turn, const E* x, int V, u64 need, F f) {
+__device__ __forceinline__ int find_index(Shared& sh, Turn& turn, const E* x, int V, const Row& r,
+                                          u64 need, F f) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int lo = 0, hi = V;
     for (;;) {
@@ -449,7 +488,7 @@ __device__ int find_index(Shared& sh, Turn& turn, const E* x, int V, u64 need, F
         if (hi - lo <= kThreads * kVec) break;
         const int next = run_of(lo, hi), i0 = lo + wave * next;
         u64 s = 0;
-        each(x, V, i0, i0 + next < hi ? i0 + next : hi, lane, 64,
+        each(x, V, r, i0, i0 + next < hi ? i0 + next : hi, lane, 64,
              [&](int i, float v) { s += f(i, v); });
         s = wave_sum(s);
         __syncthreads();
@@ -459,7 +498,7 @@ __device__ int find_index(Shared& sh, Turn& turn, const E* x, int V, u64 need, F
     u64 m[kVec], own = 0, all;
     const int i0 = lo + (int)threadIdx.x * kVec;
     float v[kVec];
-    if (i0 < hi) load8(x, i0, V, v);
+    if (i0 < hi) load8(x, i0, V, r, v);
 #pragma unroll
     for (int j = 0; j < kVec; j++) own += m[j] = i0 + j < hi ? f(i0 + j, v[j]) : 0;
     u64 run = block_scan(sh.part, turn, own, all) - own;
@@ -477,17 +516,17 @@ __device__ int find_index(Shared& sh, Turn& turn, const E* x, int V, u64 need, F
 // `need`: a histogram over the steps of weight, then the tokens of one step as a list; over
 // the row again where that list is too long.
 template <class E, class F>
-__device__ Cut cut_row(Shared& sh, Turn& turn, const E* x, int V, const Row& r, u64 need, F f) {
+__device__ __forceinline__ Cut cut_row(Shared& sh, Turn& turn, const E* x, int V, const Row& r, u64 need, F f) {
     __syncthreads();
     clear_bins(sh);
-    each(x, V, 0, V, threadIdx.x, kThreads, [&](int i, float v) {
+    each(x, V, r, 0, V, threadIdx.x, kThreads, [&](int i, float v) {
         const u64 w = f(i, v);
         if (w) atomicAdd(&sh.h.mass[r.bin(r.power(v))], w);
     });
     if (threadIdx.x == 0) sh.n = 0;
     __syncthreads();
     const int bin = find_bin(sh, turn, need);
-    each(x, V, 0, V, threadIdx.x, kThreads, [&](int i, float v) {
+    each(x, V, r, 0, V, threadIdx.x, kThreads, [&](int i, float v) {
         if (r.bin(r.power(v)) != bin) return;
         const u64 w = f(i, v);
         if (!w) return;
@@ -505,10 +544,10 @@ __device__ Cut cut_row(Shared& sh, Turn& turn, const E* x, int V, const Row& r, 
             },
             [](u64 order) { return order; }, [](const Candidate& c) { return c.mass; }));
     auto in = [&](int i) {
-        const float v = value(x[i]);
+        const float v = r.seen(value(x[i]));
         return r.bin(r.power(v)) == bin ? f(i, v) : 0;
     };
-    auto key = [&](int i) { return key_of(value(x[i])); };
+    auto key = [&](int i) { return key_of(r.seen(value(x[i]))); };
     Cut c;
     c.key = find_key(sh, V, need, key, in);
     c.last = (int)~find_key(sh, V, need, [](int i) { return ~(uint32_t)i; },
@@ -558,7 +597,7 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, i
     auto answer = [&](int token, double share) {  // one thread; the mass in units of the largest
         a.tokens[row] = token;
         if (a.logprobs)
-            a.logprobs[row] = (float)(r.power(value(x[token])) * 0.69314718055994531 - log(share));
+            a.logprobs[row] = (float)(r.power(r.seen(value(x[token]))) * 0.69314718055994531 - log(share));
     };
     // The lowest of the threads' numbers (rising with the thread) that have `first`; where none
     // has, the highest that has `any`.
@@ -582,8 +621,8 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, i
     };
     auto load16 = [&](int i0, float (&v)[2 * kVec]) {
         float lo[kVec], hi[kVec];
-        load8(x, i0, V, lo);
-        load8(x, i0 + kVec, V, hi);
+        load8(x, i0, V, r, lo);
+        load8(x, i0 + kVec, V, r, hi);
 #pragma unroll
         for (int j = 0; j < kVec; j++) {
             v[j] = lo[j];
@@ -597,7 +636,7 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, i
         int at = -1;
 #pragma unroll
         for (int j = 2 * kVec - 1; j >= 0; j--)
-            if (v[j] == top) at = i0 + j;
+            if (v[j] == r.top) at = i0 + j;
         at = pick(at >= 0, false, at);
         if (tid == 0) {
             a.tokens[row] = at;
@@ -607,7 +646,7 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, i
     }
     double mass = 0.0, part = 0.0, run = 0.0;  // of the row, of this thread's part, up to it
     if (r.summed()) {
-        if (tid < parts) part = own_sum * exp2_at(r.power(value_of(own)), 0);
+        if (tid < parts) part = own_sum * exp2_at(r.power(r.seen(value_of(own))), 0);
         run = block_scan(sh.sums, turn, part, mass);
     }
     if (!r.by_k && !r.by_p && !r.by_m) {  // no filter: the part, then the token in it
@@ -659,7 +698,7 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, i
         if (tid == 0) sh.bin = sh.bin2 = kBins;
         __syncthreads();
         for (int i = tid; i < groups; i += kThreads) {
-            const double t = r.power(value_of(w.top[i]));
+            const double t = r.power(r.seen(value_of(w.top[i])));
             const int b = r.bin(t);
             if (b > bound) continue;
             atomicAdd(&sh.h.count[b], 1u);
@@ -697,7 +736,7 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, i
     if (tid == 0) sh.n = sh.hits_n = 0;
     __syncthreads();
     for (int i = tid; i < groups; i += kThreads) {
-        if (r.bin(r.power(value_of(w.top[i]))) > bound) continue;
+        if (r.bin(r.power(r.seen(value_of(w.top[i])))) > bound) continue;
         const int at = atomicAdd(&sh.hits_n, 1);
         if (at < kHits) sh.hits[at] = i;
     }
@@ -709,7 +748,7 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, i
             const int i0 = group / kScanThreads * kPart +
                            (q % kSteps * kScanThreads + group % kScanThreads) * kVec;
             float v[kVec];
-            load8(x, i0, V, v);
+            load8(x, i0, V, r, v);
 #pragma unroll
             for (int j = 0; j < kVec; j++) {
                 const double t = r.power(v[j]);
@@ -802,7 +841,7 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, i
         auto sum_of = [&](auto f) {  // and the sums of the waves' runs
             const int per = run_of(0, V), i0 = wave * per;
             u64 s = 0;
-            each(x, V, i0, i0 + per < V ? i0 + per : V, lane, 64,
+            each(x, V, r, i0, i0 + per < V ? i0 + per : V, lane, 64,
                  [&](int i, float v) { s += f(i, v); });
             s = wave_sum(s);
             __syncthreads();
@@ -819,7 +858,7 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, i
         if (r.by_p)
             c = cut_row(sh, turn, x, V, r, whole ? need_p : top_need(r.p, (double)sum_of(kept)), kept);
         all = sum_of(drawn);
-        token = find_index(sh, turn, x, V, draw_need(r.u, all), drawn);
+        token = find_index(sh, turn, x, V, r, draw_need(r.u, all), drawn);
     }
     if (tid == 0) answer(token, (double)all / unit);
 }
