@@ -14,14 +14,19 @@
 // a neighbour of the token that the sums mean.  A rank, a mass and a place among equal logits
 // are all the same search: the first key at which a running sum of integers reaches a number.
 //
-// Two launches:
-//   scan  reads the logits once, 8192 to a workgroup: the largest logit of each thread's 32
-//         and, where a row needs its whole mass, the sum of the part's weights in 64 bits
-//   draw  one workgroup a row: the threads' maxima bound the kept prefix from below (k of them
-//         are k tokens; those down to some logit have a mass), so only the few groups of 32
-//         that reach over that bound are read again, and all searches run over a short list
-// A row whose prefix is long (thousands of tokens) is searched whole: a histogram of its mass
-// in steps of 1/40 bit of weight, then the list of one step.
+// Launches:
+//   scan    reads the logits once, 8192 to an item: the largest logit of each thread's 32 and,
+//           where a row needs its whole mass, the sum of the part's weights in 64 bits
+//   draw    one workgroup a row: the threads' maxima bound the kept prefix from below (k of
+//           them are k tokens, and have a mass), so only the few groups of 32 that reach over
+//           that bound are read again, and all searches run over a short list
+// and, unless the host knows that every prefix is short, for rows where it is not:
+//   gather  all workgroups: the parts' masses above the place where top-p ends, as far as
+//           samples tell, and a list of the tokens around that place (min-p: the kept mass)
+//   finish  one workgroup a row: top-p's end in the list, the part that the draw falls into, and
+//           the token in it
+// A row whose list does not fit (thousands of equal logits, top-k of thousands) is searched whole
+// by its workgroup: a histogram of its mass in 2048 steps of weight, then the list of one step.
 // Nothing depends on the number of rows: a row's token is the same in every batch.
 #include "common.h"
 
@@ -36,14 +41,19 @@ constexpr int kBins = 2048;    // steps of weight; the last one: weights that ro
 constexpr int kList = 2048;    // candidates in LDS
 constexpr int kMini = 64;      // candidates that one wave compares with each other
 constexpr int kHits = 4096;    // groups that are read again
-constexpr int kEnough = 1024;  // maxima that a top-p bound may take before the list is tried
+constexpr int kShort = 256;    // thread maxima that a bound is taken from (of kThreads)
+constexpr int kKeep = 10;      // groups of a draw thread in registers
+constexpr int kAround = 8192;  // tokens around a row's end of top-p, in the workspace
 
-// 2^(t + s) for -1000 <= t <= 0.  t = n + f, |f| <= 1/2, by the addition that leaves n + s in
-// the low bits; 2^f = 1 + f q(f), q the polynomial of degree 9 through (2^f - 1) / f at the
-// Chebyshev nodes (error below 2^-50 of the value; exactly 1 at 0); n + s goes into the
-// exponent.
-__device__ __forceinline__ double exp2_at(double t, int s) {
-    const double magic = 0x1.8p52 + s, tn = t + magic, f = t - (tn - magic);
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+// 2^(d rate + s) for -1000 <= d rate <= 0.  d rate = n + f, |f| <= 1/2, by the addition that
+// leaves n + s in the low bits; 2^f = 1 + f q(f), q the polynomial of degree 9 through
+// (2^f - 1) / f at the Chebyshev nodes (error below 2^-50 of the value; exactly 1 at 0); n + s
+// goes into the exponent.
+__device__ __forceinline__ double exp2_at(double d, double rate, int s) {
+    const double magic = 0x1.8p52 + s, tn = __builtin_fma(d, rate, magic);
+    const double f = __builtin_fma(d, rate, -(tn - magic));
     double q = 7.070977866508138e-09;
     q = __builtin_fma(q, f, 1.0205905413765595e-07);
     q = __builtin_fma(q, f, 1.3215451633221434e-06);
@@ -55,15 +65,10 @@ __device__ __forceinline__ double exp2_at(double t, int s) {
     q = __builtin_fma(q, f, 0.24022650695910075);
     q = __builtin_fma(q, f, 0.6931471805599462);
     q = __builtin_fma(q, f, 1.0);
-    // n + s times 2^20 onto the upper word
-    const u64 b = __builtin_bit_cast(u64, q);
-    const uint32_t n = (uint32_t)__builtin_bit_cast(u64, tn);
-    return __builtin_bit_cast(double, (u64)((uint32_t)(b >> 32) + (n << 20)) << 32 | (uint32_t)b);
-}
-
-// The same as an integer, rounded, for s <= 50: adding 2^52 leaves it in the sum's low bits.
-__device__ __forceinline__ u64 exp2_fixed(double t, int s) {
-    return __builtin_bit_cast(u64, exp2_at(t, s) + 0x1p52) & 0xfffffffffffffull;
+    u32x2 b = __builtin_bit_cast(u32x2, q);
+    const u32x2 n = __builtin_bit_cast(u32x2, tn);
+    b.y += n.x << 20;
+    return __builtin_bit_cast(double, b);
 }
 
 // Order of floats as unsigned numbers; -0 counts as +0, NaN above everything.
@@ -79,6 +84,12 @@ template <class E>
 __device__ __forceinline__ float value(E e) {
     if constexpr (sizeof(E) == 2) return fni8::h2f(e);
     else return e;
+}
+
+template <class E>
+__device__ __forceinline__ E lowest_of() {  // minus infinity
+    if constexpr (sizeof(E) == 2) return (E)0xfc00;
+    else return -__builtin_inff();
 }
 
 // Eight logits from index i on, -inf past the row's end.  Rows need no more than their
@@ -104,6 +115,7 @@ struct Row {
     float T, p, least, u, top;
     int k, s;
     double rate, base, step;
+    uint32_t low;
     bool by_k, by_p, by_m, inf;
 
     __device__ __forceinline__ Row(const fni8h::Sample& a, int64_t row, int V) {
@@ -128,21 +140,33 @@ struct Row {
         top = inf ? 0.0f : x;
         base = top == -__builtin_inff() ? 0.0 : (double)top;
         rate = 1.4426950408889634 / (double)T;
-        rate = rate > 1e-300 ? rate : 1e-300;
+        rate = rate > 1e-280 ? rate : 1e-280;
+        low = __builtin_bit_cast(u32x2, -1000.0 / rate).y;
     }
     // Beside plus infinity nothing else has weight: it counts as 0, the rest as minus infinity.
     __device__ __forceinline__ float seen(float v) const {
         return !inf ? v : v == __builtin_inff() ? 0.0f : -__builtin_inff();
     }
-    // log2 of a seen logit's weight, down to -1000 (minus infinity too): of two negative numbers
-    // the lower has the larger upper word.
-    __device__ __forceinline__ double power(float v) const {
-        const u64 t = __builtin_bit_cast(u64, ((double)v - base) * rate);
-        uint32_t hi = (uint32_t)(t >> 32);
-        hi = hi < 0xc08f4000u ? hi : 0xc08f4000u;
-        return __builtin_bit_cast(double, (u64)hi << 32 | (uint32_t)t);
+    // A seen logit's distance from the largest, down to that of weight 2^-1000 (minus infinity
+    // too): of two negative numbers the lower has the larger upper word.
+    __device__ __forceinline__ double away(float v) const {
+        u32x2 d = __builtin_bit_cast(u32x2, (double)v - base);
+        d.y = d.y < low ? d.y : low;
+        return __builtin_bit_cast(double, d);
     }
-    __device__ __forceinline__ u64 mass(float v) const { return exp2_fixed(power(v), s); }
+    // log2 of its weight; the weight; the weight as an integer, rounded: adding 2^52 leaves it in
+    // the low bits of the sum.
+    __device__ __forceinline__ double power(float v) const { return away(v) * rate; }
+    __device__ __forceinline__ double weight(float v) const { return exp2_at(away(v), rate, 0); }
+    __device__ __forceinline__ u64 mass(float v) const {
+        u32x2 m = __builtin_bit_cast(u32x2, exp2_at(away(v), rate, s) + 0x1p52);
+        m.y &= 0xfffffu;
+        return __builtin_bit_cast(u64, m);
+    }
+    // What a mass has to be for min-p.
+    __device__ __forceinline__ u64 floor() const {
+        return (u64)__builtin_rint((double)least * __builtin_ldexp(1.0, s));
+    }
     // Step of a weight, rising as it falls; kBins - 1 for weights that round to 0.
     __device__ __forceinline__ int bin(double power) const {
         const double d = -power * step;
@@ -160,22 +184,43 @@ __device__ __forceinline__ void load8(const E* x, int i, int V, const Row& r, fl
     }
 }
 
-// What scan leaves of a row, in the workspace.
+// A row in the workspace.  scan fills top, part, sum and pick; draw the long prefix's state;
+// gather its above and around.
+enum { kDone, kTopP, kMinP, kWhole };  // what is left to do
+struct Long {
+    u64 need;        // top-p: the mass to reach
+    float high, low; // logits that the end of top-p lies between
+    int kind, around;
+};
 struct Work {
-    uint32_t* top;   // [parts][256] keys of the threads' largest logits
-    uint32_t* part;  // [parts] keys of the parts' largest
     double* sum;     // [parts] masses, relative to the part's largest logit
+    u64 *above;      // [parts] masses of what is kept for certain
+    u64* around;     // [kAround] orders of the tokens from low up to high
+    uint32_t* top;   // [parts][256] keys of the threads' largest logits
+    uint32_t* pick;  // [parts][256] two of the 32, as bfloat16
+    uint32_t* part;  // [parts] keys of the parts' largest
+    Long* more;
 };
 __host__ __device__ inline int64_t parts_of(int64_t V) { return (V + kPart - 1) / kPart; }
-__host__ __device__ inline int64_t row_bytes(int64_t parts) {
-    return (parts * (8 + 4 + 4 * kScanThreads) + 15) / 16 * 16;
+// Tokens around an end that a row has room for: no row of up to kList tokens needs any.
+__host__ __device__ inline int64_t around_of(int64_t V) {
+    return V <= kList ? 0 : V < kAround ? V : kAround;
 }
-__device__ __forceinline__ Work work_of(int8_t* w, int64_t row, int64_t parts) {
-    w += row * row_bytes(parts);
+__host__ __device__ inline int64_t row_bytes(int64_t V) {
+    return (parts_of(V) * (8 + 8 + 8 * kScanThreads + 4) + around_of(V) * 8 + (int64_t)sizeof(Long) +
+            15) / 16 * 16;
+}
+__device__ __forceinline__ Work work_of(int8_t* w, int64_t row, int64_t V) {
+    const int64_t parts = parts_of(V);
+    w += row * row_bytes(V);
     Work r;
     r.sum = reinterpret_cast<double*>(w);
-    r.top = reinterpret_cast<uint32_t*>(w + parts * 8);
-    r.part = r.top + parts * kScanThreads;
+    r.above = reinterpret_cast<u64*>(w + parts * 8);
+    r.around = r.above + parts;
+    r.more = reinterpret_cast<Long*>(r.around + around_of(V));
+    r.top = reinterpret_cast<uint32_t*>(r.more + 1);
+    r.pick = r.top + parts * kScanThreads;
+    r.part = r.pick + parts * kScanThreads;
     return r;
 }
 
@@ -189,6 +234,19 @@ __device__ __forceinline__ u64 wave_sum(u64 v) {
     for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
     return v;
 }
+__device__ __forceinline__ float wave_sum_f32(float v) {
+    auto add = [&](int o) { v += __builtin_bit_cast(float, o); };
+    add(fni8::dpp<fni8::kDppXor1>(__builtin_bit_cast(int, v)));
+    add(fni8::dpp<fni8::kDppXor2>(__builtin_bit_cast(int, v)));
+    add(fni8::dpp<fni8::kDppHalfMirror>(__builtin_bit_cast(int, v)));
+    add(fni8::dpp<fni8::kDppMirror>(__builtin_bit_cast(int, v)));
+    const int b = __builtin_bit_cast(int, v);
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 64; i += 16)
+        sum += __builtin_bit_cast(float, __builtin_amdgcn_readlane(b, i));
+    return sum;
+}
 template <class N>
 __device__ __forceinline__ N wave_scan(N v, int lane) {
 #pragma unroll
@@ -199,53 +257,92 @@ __device__ __forceinline__ N wave_scan(N v, int lane) {
     return v;
 }
 
+// An item is a part of a row; a workgroup walks items, the loads of the next on their way while
+// it computes: 32 exponentials of 64 bits a thread take longer than its 64 or 128 bytes.
 template <class E>
 __global__ __launch_bounds__(kScanThreads) void scan_kernel(const fni8h::Sample a, int parts) {
-    __shared__ uint32_t tops[4];
-    __shared__ double sums[4];
-    const int part = blockIdx.x, V = (int)a.V, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t row = blockIdx.y + (int64_t)blockIdx.z * 32768;
-    if (row >= a.B) return;
-    const E* x = (const E*)a.logits + row * a.ld;
-    const Work w = work_of(a.work, row, parts);
-    float v[kSteps][kVec];
+    typedef E vec __attribute__((ext_vector_type(8), aligned(sizeof(E))));
+    __shared__ uint32_t tops[2][4];
+    __shared__ double sums[2][4];
+    const int V = (int)a.V, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int items = (int)a.B * parts;  // fewer than 2^30
+    vec next[kSteps];
+    auto fetch = [&](int item) {
+        const int row = item / parts;
+        const E* x = (const E*)a.logits + row * a.ld;
+        const int i0 = (item - row * parts) * kPart + tid * kVec;
 #pragma unroll
-    for (int i = 0; i < kSteps; i++)
-        load8(x, part * kPart + (i * kScanThreads + (int)threadIdx.x) * kVec, V, v[i]);
-    float most = -__builtin_inff();
-    bool nan = false;
+        for (int i = 0; i < kSteps; i++) {
+            const int at = i0 + i * kScanThreads * kVec;
+            if (at + kVec <= V) {
+                next[i] = *reinterpret_cast<const vec*>(x + at);
+            } else {
 #pragma unroll
-    for (int i = 0; i < kSteps; i++)
-#pragma unroll
-        for (int j = 0; j < kVec; j++) {
-            nan |= v[i][j] != v[i][j];
-            most = __builtin_fmaxf(most, v[i][j]);
+                for (int j = 0; j < kVec; j++) {
+                    E e = lowest_of<E>();
+                    if (at + j < V) e = x[at + j];
+                    next[i][j] = e;
+                }
+            }
         }
-    uint32_t best = nan ? 0xffffffffu : key_of(most);
-    w.top[part * kScanThreads + threadIdx.x] = best;
-    best = fni8::wave_max_u32(best);
-    if (lane == 0) tops[wave] = best;
-    Row r(a, row, V);
-    __syncthreads();
-    for (int i = 0; i < 4; i++) best = tops[i] > best ? tops[i] : best;
-    if (threadIdx.x == 0) w.part[part] = best;
-    if (!r.summed()) return;
-    r.largest(value_of(best));
-    if (r.inf) {
+    };
+    const int step = gridDim.x;
+    int item = blockIdx.x;
+    if (item < items) fetch(item);
+    for (int turn = 0; item < items; item += step, turn ^= 1) {
+        const int row = item / parts, part = item - row * parts;
+        const Work w = work_of(a.work, row, V);
+        float v[kSteps][kVec];
+        float most = -__builtin_inff();
+        bool nan = false;
 #pragma unroll
         for (int i = 0; i < kSteps; i++)
 #pragma unroll
-            for (int j = 0; j < kVec; j++) v[i][j] = r.seen(v[i][j]);
+            for (int j = 0; j < kVec; j++) {
+                const E e = next[i][j];
+                v[i][j] = value(e);
+                nan |= v[i][j] != v[i][j];
+                most = __builtin_fmaxf(most, v[i][j]);
+            }
+        if (item + step < items) fetch(item + step);
+        uint32_t best = nan ? 0xffffffffu : key_of(most);
+        w.top[part * kScanThreads + tid] = best;
+        best = fni8::wave_max_u32(best);
+        if (lane == 0) tops[turn][wave] = best;
+        Row r(a, row, V);
+        __syncthreads();
+        for (int i = 0; i < 4; i++) best = tops[turn][i] > best ? tops[turn][i] : best;
+        if (tid == 0) w.part[part] = best;
+        if (!r.summed()) continue;
+        r.largest(value_of(best));
+        if (r.inf) {
+#pragma unroll
+            for (int i = 0; i < kSteps; i++)
+#pragma unroll
+                for (int j = 0; j < kVec; j++) v[i][j] = r.seen(v[i][j]);
+        }
+        if (r.by_p) {  // samples, of loads that differ from wave to wave
+            float p = 0.0f, q = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kSteps; i++)
+                if (i == (wave & (kSteps - 1))) {
+                    p = v[i][1];
+                    q = v[(i + kSteps / 2) % kSteps][6];
+                }
+            w.pick[part * kScanThreads + tid] =
+                (__builtin_bit_cast(uint32_t, p) + 0x8000u) >> 16 |
+                ((__builtin_bit_cast(uint32_t, q) + 0x8000u) & 0xffff0000u);
+        }
+        double sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < kSteps; i++)
+#pragma unroll
+            for (int j = 0; j < kVec; j++) sum += r.weight(v[i][j]);
+        sum = wave_sum(sum);
+        if (lane == 0) sums[turn][wave] = sum;
+        __syncthreads();
+        if (tid == 0) w.sum[part] = sums[turn][0] + sums[turn][1] + sums[turn][2] + sums[turn][3];
     }
-    double sum = 0.0;
-#pragma unroll
-    for (int i = 0; i < kSteps; i++)
-#pragma unroll
-        for (int j = 0; j < kVec; j++) sum += exp2_at(r.power(v[i][j]), 0);
-    sum = wave_sum(sum);
-    if (lane == 0) sums[wave] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) w.sum[part] = sums[0] + sums[1] + sums[2] + sums[3];
 }
 
 struct Candidate {
@@ -265,12 +362,15 @@ struct Shared {
             };
         } h;
         uint32_t hits[kHits];
+        int bins[kThreads];
+        u64 above[kThreads];
     };
     Candidate list[kList], mini[kMini];
     u64 part[2][kWaves], range[kWaves];
     double sums[2][kWaves], before;
+    float floats[2][kWaves];
     int ints[2][kWaves], counts[kWaves], highs[kWaves];
-    u64 need, found;
+    u64 need, all, found;
     uint32_t key;
     int index, n, hits_n, bin, bin2;
 };
@@ -350,13 +450,14 @@ __device__ __forceinline__ uint32_t find_key(Shared& sh, int n, u64& need, K key
 }
 
 // Finds the first bin of the histogram h.mass at which the running sum reaches `need`, lowered
-// to the sum of all; `need` is then what that bin has to bring.
+// to the sum of all (left in `all`); `need` is then what that bin has to bring.
 __device__ __forceinline__ int find_bin(Shared& sh, Turn& turn, u64& need) {
     constexpr int B = kBins / kThreads;
     u64 h[B], own = 0, all;
 #pragma unroll
     for (int j = 0; j < B; j++) own += h[j] = sh.h.mass[threadIdx.x * B + j];
     u64 run = block_scan(sh.part, turn, own, all) - own;
+    if (threadIdx.x == 0) sh.all = all;
     if (need > all) need = all;
 #pragma unroll
     for (int j = 0; j < B; j++) {
@@ -565,18 +666,115 @@ __device__ __forceinline__ u64 draw_need(float u, u64 all) {
     return need < all ? need : all;
 }
 
+// The token of a row that is searched whole, and the kept mass.
+template <class E>
+__device__ __forceinline__ int search_row(Shared& sh, Turn& turn, const E* x, int V, const Row& r,
+                                          u64 need_p, u64& all) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const u64 floor = r.floor();
+    const bool whole = r.by_p && !r.by_k;
+    Cut c;
+    auto kept = [&](int i, float v) { return c.keeps(key_of(v), i) ? r.mass(v) : 0; };
+    auto drawn = [&](int i, float v) {
+        const u64 m = kept(i, v);
+        return m >= floor ? m : 0;
+    };
+    auto sum_of = [&](auto f) {  // and the sums of the waves' runs
+        const int per = run_of(0, V), i0 = wave * per;
+        u64 s = 0;
+        each(x, V, r, i0, i0 + per < V ? i0 + per : V, lane, 64,
+             [&](int i, float v) { s += f(i, v); });
+        s = wave_sum(s);
+        __syncthreads();
+        if (lane == 0) sh.range[wave] = s;
+        __syncthreads();
+        s = 0;
+#pragma unroll
+        for (int i = 0; i < kWaves; i++) s += sh.range[i];
+        return s;
+    };
+    if (r.by_k)
+        c = cut_row(sh, turn, x, V, r, r.k,
+                    [&](int, float v) { return (u64)(r.power(v) > -(double)(r.s + 1)); });
+    if (r.by_p)
+        c = cut_row(sh, turn, x, V, r, whole ? need_p : top_need(r.p, (double)sum_of(kept)), kept);
+    all = sum_of(drawn);
+    return find_index(sh, turn, x, V, r, draw_need(r.u, all), drawn);
+}
+
+// The logits that the end of top-p lies between, as far as the samples tell: two of each
+// group of 32, so the mass below a logit is 16 times that of the samples below it, counted in
+// steps of weight.  Of `tail`, the mass that top-p leaves out (in units of the largest weight),
+// the estimate is off by sqrt(16 w tail) at most (one standard deviation; w the weight at the
+// end, the largest of the tail): five of them on either side, and a step for their rounding.
+__device__ __forceinline__ void find_ends(Shared& sh, Turn& turn, const Work& w, int groups,
+                                          const Row& r, double tail, Long& more) {
+    constexpr int B = kBins / kThreads;
+    constexpr float f = 16.0f;
+    for (int i = threadIdx.x; i < kBins; i += kThreads) sh.h.count[i] = 0;
+    if (threadIdx.x == 0) sh.bin = kBins - 2;
+    __syncthreads();
+    const float rate = (float)(r.rate * r.step);
+    auto count = [&](uint32_t bits) {
+        const float d = (r.top - __builtin_bit_cast(float, bits)) * rate;
+        if (d < (float)(kBins - 1)) atomicAdd(&sh.h.count[d > 0.0f ? (int)d : 0], 1u);
+    };
+    for (int i = threadIdx.x; i < groups; i += kThreads) {
+        const uint32_t two = w.pick[i];
+        count(two << 16);
+        count(two & 0xffff0000u);
+    }
+    __syncthreads();
+    // from the bottom: a thread's steps are last - j
+    const int last = kBins - 1 - (int)threadIdx.x * B;
+    const float unit = 1.0f / (float)r.step, goal = (float)tail;
+    float m[B], own = 0.0f, all;
+#pragma unroll
+    for (int j = 0; j < B; j++) {
+        const int b = last - j;
+        own += m[j] = f * (float)sh.h.count[b] * __builtin_amdgcn_exp2f(-((float)b + 0.5f) * unit);
+    }
+    const float before = block_scan(sh.floats, turn, own, all) - own;
+    // the step in which the mass from the bottom reaches x
+    auto reach = [&](float x, int& where) {
+        float to = before;
+#pragma unroll
+        for (int j = 0; j < B; j++) {
+            if (to < x && to + m[j] >= x) where = last - j;
+            to += m[j];
+        }
+    };
+    reach(goal, sh.bin);
+    __syncthreads();
+    const int end = sh.bin;
+    const float dev = 5.0f * __builtin_sqrtf(f * __builtin_amdgcn_exp2f(-(float)end * unit) * goal);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        sh.bin = kBins - 3;  // the lowest step with weight, where the tail is too thin to tell
+        sh.bin2 = 0;
+    }
+    __syncthreads();
+    reach(goal - dev, sh.bin);
+    reach(goal + dev, sh.bin2);
+    __syncthreads();
+    more.low = r.top - (float)(sh.bin + 2) / rate;
+    more.high = sh.bin2 > 0 ? r.top - (float)(sh.bin2 - 1) / rate : r.top;
+}
+
 static_assert(kThreads * 2 * kVec == kPart && kPart == kSteps * kScanThreads * kVec, "parts");
 
-template <class E>
+// ALONE: no other launch follows, and a row whose list does not fit is searched whole.
+template <class E, bool ALONE>
 __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, int parts) {
     __shared__ Shared sh;
     Turn turn;
     const int64_t row = blockIdx.x;
     const E* x = (const E*)a.logits + row * a.ld;
     const int V = (int)a.V, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const Work w = work_of(a.work, row, parts);
+    const Work w = work_of(a.work, row, V);
 
     // parts <= kThreads: a thread each
+    if (!ALONE && tid == 0) w.more->kind = kDone;
     const uint32_t own = tid < parts ? w.part[tid] : 0;
     const double own_sum = tid < parts ? w.sum[tid] : 0.0;  // used where the row is summed
     Row r(a, row, V);
@@ -646,7 +844,7 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, i
     }
     double mass = 0.0, part = 0.0, run = 0.0;  // of the row, of this thread's part, up to it
     if (r.summed()) {
-        if (tid < parts) part = own_sum * exp2_at(r.power(r.seen(value_of(own))), 0);
+        if (tid < parts) part = own_sum * r.weight(r.seen(value_of(own)));
         run = block_scan(sh.sums, turn, part, mass);
     }
     if (!r.by_k && !r.by_p && !r.by_m) {  // no filter: the part, then the token in it
@@ -660,7 +858,7 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, i
         load16(i0, v);
         double m[2 * kVec], sum = 0.0, all;
 #pragma unroll
-        for (int j = 0; j < 2 * kVec; j++) sum += m[j] = exp2_at(r.power(v[j]), 0);
+        for (int j = 0; j < 2 * kVec; j++) sum += m[j] = r.weight(v[j]);
         run = block_scan(sh.sums, turn, sum, all);
         run = sh.before + (run - sum);
         int at = -1, last = -1;
@@ -682,7 +880,7 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, i
     const int groups = parts * kScanThreads;
     const bool whole = r.by_p && !r.by_k;  // top-p of the whole mass
     const u64 need_p = whole ? top_need(r.p, mass * unit) : 0;
-    const u64 floor = (u64)__builtin_rint((double)r.least * unit);
+    const u64 floor = r.floor();
     // The step in which min-p ends, and one more for log2's own rounding: no token further down
     // has a mass that rounds to `floor`.  Top-p after top-k needs the whole mass of top-k.
     int bound = kBins - 2, least = kBins - 2;
@@ -690,55 +888,92 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, i
         least = r.bin(log2((double)floor - 0.5) - r.s) + 1;
         bound = least = least < bound ? least : bound;
     }
-    if (r.by_k || r.by_p) {
-        for (int i = tid; i < kBins; i += kThreads) {
-            sh.h.mass[i] = 0;
-            sh.h.count[i] = 0;
-        }
-        if (tid == 0) sh.bin = sh.bin2 = kBins;
+    uint32_t keep[kKeep], most = 0;
+#pragma unroll
+    for (int j = 0; j < kKeep; j++) {
+        const int i = tid + j * kThreads;
+        keep[j] = i < groups ? w.top[i] : 0;
+        most = keep[j] > most ? keep[j] : most;
+    }
+    for (int i = tid + kKeep * kThreads; i < groups; i += kThreads) {
+        const uint32_t key = w.top[i];
+        most = key > most ? key : most;
+    }
+    auto bin_of = [&](uint32_t key) { return r.bin(r.power(r.seen(value_of(key)))); };
+    const int mine = most ? bin_of(most) : kBins - 1;
+    if (r.by_k && r.k > kShort) {  // the groups' maxima, counted in steps
+        for (int i = tid; i < kBins; i += kThreads) sh.h.count[i] = 0;
+        if (tid == 0) sh.bin = kBins;
         __syncthreads();
-        for (int i = tid; i < groups; i += kThreads) {
-            const double t = r.power(r.seen(value_of(w.top[i])));
-            const int b = r.bin(t);
-            if (b > bound) continue;
-            atomicAdd(&sh.h.count[b], 1u);
-            if (whole) atomicAdd(&sh.h.mass[b], exp2_fixed(t, r.s));
-        }
+        if (mine <= bound)
+            for (int i = tid; i < groups; i += kThreads) {
+                const int b = bin_of(w.top[i]);
+                if (b <= bound) atomicAdd(&sh.h.count[b], 1u);
+            }
         __syncthreads();
-        // the step at which the count is there, or the mass
         constexpr int B = kBins / kThreads;
-        const int want = r.by_k ? r.k : kEnough;
         int c[B], some = 0, total;
 #pragma unroll
         for (int j = 0; j < B; j++) some += c[j] = (int)sh.h.count[tid * B + j];
         int rank = block_scan(sh.ints, turn, some, total) - some;
 #pragma unroll
         for (int j = 0; j < B; j++) {
-            if (rank < want && rank + c[j] >= want) sh.bin = tid * B + j;
+            if (rank < r.k && rank + c[j] >= r.k) sh.bin = tid * B + j;
             rank += c[j];
-        }
-        if (whole) {
-            u64 m[B], some = 0, total;
-#pragma unroll
-            for (int j = 0; j < B; j++) some += m[j] = sh.h.mass[tid * B + j];
-            u64 to = block_scan(sh.part, turn, some, total) - some;
-#pragma unroll
-            for (int j = 0; j < B; j++) {
-                if (to < need_p && to + m[j] >= need_p) sh.bin2 = tid * B + j;
-                to += m[j];
-            }
         }
         __syncthreads();
         bound = sh.bin < bound ? sh.bin : bound;
-        bound = sh.bin2 < bound ? sh.bin2 : bound;
+    } else if (r.by_k || whole) {
+        // One wave, the maxima of the threads' groups: by bisection the first step down to which
+        // they are k, or bring top-p's mass (in 32 bits, with room for its error: that only
+        // moves the bound), or are kShort.
+        sh.bins[tid] = mine;
+        __syncthreads();
+        if (wave == 0) {
+            constexpr int B = kThreads / 64;
+            int b[B];
+            float m[B];
+#pragma unroll
+            for (int j = 0; j < B; j++) {
+                b[j] = sh.bins[lane + 64 * j];
+                m[j] = whole && b[j] < kBins - 1
+                           ? __builtin_amdgcn_exp2f(-(float)(b[j] + 1) / (float)r.step) : 0.0f;
+            }
+            const int want = whole ? kShort : r.k;
+            const float goal = (float)((double)need_p / unit) * 1.0001f;
+            int lo = 0, hi = bound;  // the answer, if there is one, is in [lo, hi]
+            while (lo < hi) {
+                const int mid = (lo + hi) / 2;
+                int count = 0;
+                float sum = 0.0f;
+#pragma unroll
+                for (int j = 0; j < B; j++) {
+                    count += __builtin_popcountll(__ballot(b[j] <= mid));
+                    sum += b[j] <= mid ? m[j] : 0.0f;
+                }
+                bool there = count >= want;
+                if (whole && !there) there = wave_sum_f32(sum) >= goal;
+                if (there) hi = mid;
+                else lo = mid + 1;
+            }
+            if (lane == 0) sh.bin = lo;
+        }
+        __syncthreads();
+        bound = sh.bin;
     }
     // ---- the tokens down to the bound, from the groups whose maximum reaches it
     if (tid == 0) sh.n = sh.hits_n = 0;
     __syncthreads();
-    for (int i = tid; i < groups; i += kThreads) {
-        if (r.bin(r.power(r.seen(value_of(w.top[i])))) > bound) continue;
+    auto hit = [&](uint32_t key, int i) {
+        if (bin_of(key) > bound) return;
         const int at = atomicAdd(&sh.hits_n, 1);
         if (at < kHits) sh.hits[at] = i;
+    };
+    if (mine <= bound) {
+#pragma unroll
+        for (int j = 0; j < kKeep; j++)
+            if (tid + j * kThreads < groups) hit(keep[j], tid + j * kThreads);
+        for (int i = tid + kKeep * kThreads; i < groups; i += kThreads) hit(w.top[i], i);
     }
     __syncthreads();
     const int hits = sh.hits_n;
@@ -751,9 +986,8 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, i
             load8(x, i0, V, r, v);
 #pragma unroll
             for (int j = 0; j < kVec; j++) {
-                const double t = r.power(v[j]);
-                if (r.bin(t) > bound) continue;
-                const u64 m = exp2_fixed(t, r.s);
+                if (r.bin(r.power(v[j])) > bound) continue;
+                const u64 m = r.mass(v[j]);
                 if (!m) continue;
                 const int at = atomicAdd(&sh.n, 1);
                 if (at < kList) sh.list[at] = {(u64)key_of(v[j]) << 32 | (uint32_t)~(i0 + j), m};
@@ -801,8 +1035,8 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, i
     }
     u64 all;
     int token;
-    Cut c;
     if (n <= kList) {
+        Cut c;
         auto bucket = [&](const Candidate& i) { return r.bin(r.power(value_of(key_at(i)))); };
         auto order = [](u64 o) { return o; };
         auto kept = [&](const Candidate& i) {
@@ -832,50 +1066,248 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, i
                 const u64 m = kept(i);
                 return m >= floor ? m : 0;
             });
-    } else {
-        auto kept = [&](int i, float v) { return c.keeps(key_of(v), i) ? r.mass(v) : 0; };
-        auto drawn = [&](int i, float v) {
-            const u64 m = kept(i, v);
-            return m >= floor ? m : 0;
-        };
-        auto sum_of = [&](auto f) {  // and the sums of the waves' runs
-            const int per = run_of(0, V), i0 = wave * per;
-            u64 s = 0;
-            each(x, V, r, i0, i0 + per < V ? i0 + per : V, lane, 64,
-                 [&](int i, float v) { s += f(i, v); });
-            s = wave_sum(s);
-            __syncthreads();
-            if (lane == 0) sh.range[wave] = s;
-            __syncthreads();
-            s = 0;
-#pragma unroll
-            for (int i = 0; i < kWaves; i++) s += sh.range[i];
-            return s;
-        };
-        if (r.by_k)
-            c = cut_row(sh, turn, x, V, r, r.k,
-                        [&](int, float v) { return (u64)(r.power(v) > -(double)(r.s + 1)); });
-        if (r.by_p)
-            c = cut_row(sh, turn, x, V, r, whole ? need_p : top_need(r.p, (double)sum_of(kept)), kept);
-        all = sum_of(drawn);
-        token = find_index(sh, turn, x, V, r, draw_need(r.u, all), drawn);
+    } else if constexpr (ALONE) {
+        token = search_row(sh, turn, x, V, r, need_p, all);
+    } else {  // the long way
+        Long more{need_p, 0.0f, 0.0f, kWhole, 0};
+        if (!r.by_k && !r.by_p) more.kind = kMinP;
+        if (whole && !r.by_m) {
+            more.kind = kTopP;
+            find_ends(sh, turn, w, groups, r, mass - (double)need_p / unit, more);
+        }
+        if (tid == 0) *w.more = more;
+        return;
     }
     if (tid == 0) answer(token, (double)all / unit);
 }
 
+// One part of a row with a long prefix: the mass of what is kept for certain, and the tokens
+// around the end of top-p.
+template <class E>
+__global__ __launch_bounds__(kScanThreads) void gather_kernel(const fni8h::Sample a, int parts) {
+    __shared__ u64 sums[4];
+    __shared__ int counts[4], base;
+    const int items = (int)a.B * parts, V = (int)a.V;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    for (int item = blockIdx.x; item < items; item += gridDim.x) {
+        const int row = item / parts, part = item - row * parts;
+        const Work w = work_of(a.work, row, V);
+        const Long more = *w.more;
+        if (more.kind != kTopP && more.kind != kMinP) continue;
+        const E* x = (const E*)a.logits + (int64_t)row * a.ld;
+        Row r(a, row, V);
+        uint32_t best = 0;
+        for (int i = tid; i < parts; i += kScanThreads) best = w.part[i] > best ? w.part[i] : best;
+        best = fni8::wave_max_u32(best);
+        if (lane == 0) counts[wave] = (int)best;
+        __syncthreads();
+        for (int i = 0; i < 4; i++) best = (uint32_t)counts[i] > best ? (uint32_t)counts[i] : best;
+        r.largest(value_of(best));
+        __syncthreads();
+        float v[kSteps][kVec];
+        u64 sum = 0;
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < kSteps; i++)
+            load8(x, part * kPart + (i * kScanThreads + tid) * kVec, V, r, v[i]);
+        if (more.kind == kTopP) {
+#pragma unroll
+            for (int i = 0; i < kSteps; i++)
+#pragma unroll
+                for (int j = 0; j < kVec; j++) {
+                    n += v[i][j] < more.high && v[i][j] >= more.low;
+                    sum += r.mass(v[i][j] >= more.high ? v[i][j] : -__builtin_inff());
+                }
+        } else {
+            const u64 floor = r.floor();
+#pragma unroll
+            for (int i = 0; i < kSteps; i++)
+#pragma unroll
+                for (int j = 0; j < kVec; j++) {
+                    const u64 m = r.mass(v[i][j]);
+                    sum += m >= floor ? m : 0;
+                }
+        }
+        sum = wave_sum(sum);
+        const int run = fni8::wave_incl_scan_i32(n, lane);
+        if (lane == 63) {
+            sums[wave] = sum;
+            counts[wave] = run;
+        }
+        __syncthreads();
+        if (tid == 0) {
+            w.above[part] = sums[0] + sums[1] + sums[2] + sums[3];
+            const int all = counts[0] + counts[1] + counts[2] + counts[3];
+            base = all ? atomicAdd(&w.more->around, all) : 0;
+        }
+        __syncthreads();
+        int at = base + run - n;
+        for (int i = 0; i < wave; i++) at += counts[i];
+        if (n) {
+#pragma unroll
+            for (int i = 0; i < kSteps; i++)
+#pragma unroll
+                for (int j = 0; j < kVec; j++)
+                    if (v[i][j] < more.high && v[i][j] >= more.low) {
+                        const int index = part * kPart + (i * kScanThreads + tid) * kVec + j;
+                        if (at < around_of(V))
+                            w.around[at] = (u64)key_of(v[i][j]) << 32 | (uint32_t)~index;
+                        at++;
+                    }
+        }
+        __syncthreads();  // sums and counts are the next item's
+    }
+}
+
+template <class E>
+__global__ __launch_bounds__(kThreads) void finish_kernel(const fni8h::Sample a, int parts) {
+    __shared__ Shared sh;
+    Turn turn;
+    const int64_t row = blockIdx.x;
+    const int V = (int)a.V;
+    const Work w = work_of(a.work, row, V);
+    const Long more = *w.more;
+    if (more.kind == kDone) return;
+    const E* x = (const E*)a.logits + row * a.ld;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    Row r(a, row, V);
+    const uint32_t own = tid < parts ? w.part[tid] : 0;
+    uint32_t best = fni8::wave_max_u32(own);
+    if (lane == 0) sh.counts[wave] = (int)best;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWaves; i++) best = (uint32_t)sh.counts[i] > best ? (uint32_t)sh.counts[i] : best;
+    r.largest(value_of(best));
+    const u64 floor = r.floor();
+    u64 all = 0;
+    int token = -1;
+    bool found = false;
+    if (more.kind != kWhole) {
+        u64 mine = tid < parts ? w.above[tid] : 0;
+        Cut c;
+        found = true;
+        if (more.kind == kTopP) {
+            // the end of top-p in the list: a step of weight, then the tokens of that step
+            const u64 certain = block_sum(sh, turn, mine);
+            const int n = more.around;
+            found = certain < more.need && n <= around_of(V);
+            if (found) {
+                const double p0 = r.power(more.high);
+                // no token of the list weighs less than 2^-(s + 2)
+                const double p1 = r.power(more.low), deep = -(double)(r.s + 2);
+                const double steps = (kBins - 1) / (p0 - (p1 > deep ? p1 : deep));
+                auto bin = [&](double t) {
+                    const double d = (p0 - t) * steps;
+                    return d < (double)(kBins - 1) ? (int)d : kBins - 1;
+                };
+                auto logit = [](u64 order) { return value_of((uint32_t)(order >> 32)); };
+                clear_bins(sh);
+                for (int i = tid; i < n; i += kThreads) {
+                    const float v = logit(w.around[i]);
+                    atomicAdd(&sh.h.mass[bin(r.power(v))], r.mass(v));
+                }
+                if (tid == 0) sh.n = 0;
+                __syncthreads();
+                u64 need = more.need - certain;
+                const u64 wanted = need;
+                const int b = find_bin(sh, turn, need);
+                for (int i = tid; i < n; i += kThreads) {
+                    const u64 order = w.around[i];
+                    if (bin(r.power(logit(order))) != b) continue;
+                    const int at = atomicAdd(&sh.n, 1);
+                    if (at < kList) sh.list[at] = {order, r.mass(logit(order))};
+                }
+                __syncthreads();
+                const int few = sh.n;
+                found = few <= kList && sh.all >= wanted;
+                if (found)
+                    c = cut_at(find_item(
+                        sh, turn, few, need,
+                        [&](const Candidate& i) {
+                            const double d = (p0 - r.power(logit(i.order))) * steps - b;
+                            return d < 1.0 ? (int)(d * (kBins - 1)) : kBins - 1;
+                        },
+                        [](u64 o) { return o; }, [](const Candidate& i) { return i.mass; }));
+                // what the list brings to each part
+                __syncthreads();
+                sh.above[tid] = mine;
+                __syncthreads();
+                if (found)
+                    for (int i = tid; i < n; i += kThreads) {
+                        const u64 order = w.around[i];
+                        const int index = (int)~(uint32_t)order;
+                        if (c.keeps((uint32_t)(order >> 32), index))
+                            atomicAdd(&sh.above[index / kPart], r.mass(logit(order)));
+                    }
+                __syncthreads();
+                mine = sh.above[tid];
+            }
+        }
+        if (found) {  // the part, then the token in it
+            u64 run = block_scan(sh.part, turn, mine, all);
+            u64 need = draw_need(r.u, all);
+            if (run >= need && run - mine < need) {
+                sh.bin = tid;
+                sh.need = need - (run - mine);
+            }
+            __syncthreads();
+            need = sh.need;
+            const int i0 = sh.bin * kPart + tid * 2 * kVec;
+            u64 m[2 * kVec], some = 0, total;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                float v[kVec];
+                load8(x, i0 + h * kVec, V, r, v);
+#pragma unroll
+                for (int j = 0; j < kVec; j++) {
+                    const u64 q = c.keeps(key_of(v[j]), i0 + h * kVec + j) ? r.mass(v[j]) : 0;
+                    some += m[h * kVec + j] = q >= floor ? q : 0;
+                }
+            }
+            run = block_scan(sh.part, turn, some, total) - some;
+#pragma unroll
+            for (int j = 0; j < 2 * kVec; j++) {
+                if (run < need && run + m[j] >= need) sh.index = i0 + j;
+                run += m[j];
+            }
+            __syncthreads();
+            token = sh.index;
+        }
+    }
+    if (!found) token = search_row(sh, turn, x, V, r, more.need, all);
+    if (tid == 0) {
+        a.tokens[row] = token;
+        if (a.logprobs)
+            a.logprobs[row] = (float)(r.power(r.seen(value(x[token]))) * 0.69314718055994531 -
+                                      log((double)all * __builtin_ldexp(1.0, -r.s)));
+    }
+}
+
 template <class E>
 void launch(const fni8h::Sample& a, hipStream_t st) {
-    const int64_t parts = parts_of(a.V), deep = (a.B + 32767) / 32768;
-    const dim3 grid((uint32_t)parts, (uint32_t)(a.B < 32768 ? a.B : 32768), (uint32_t)deep);
-    scan_kernel<E><<<grid, kScanThreads, 0, st>>>(a, (int)parts);
-    draw_kernel<E><<<(uint32_t)a.B, kThreads, 0, st>>>(a, (int)parts);
+    const int parts = (int)parts_of(a.V);
+    const int64_t items = a.B * parts;
+    const uint32_t grid = (uint32_t)(items < 1 << 20 ? items : 1 << 20);
+    scan_kernel<E><<<grid, kScanThreads, 0, st>>>(a, parts);
+    // no filter, the largest logit, or top-k of a few: no prefix is long but for equal logits
+    const bool alone = (!a.temperature && !(a.temperature1 > 0.0f)) ||
+                       (!a.top_k && a.top_k1 > 0 && a.top_k1 <= kShort) ||
+                       (!a.top_k && !a.top_p && !a.min_p && a.top_k1 <= 0 && !(a.top_p1 < 1.0f) &&
+                        !(a.min_p1 > 0.0f));
+    if (alone) {
+        draw_kernel<E, true><<<(uint32_t)a.B, kThreads, 0, st>>>(a, parts);
+        return;
+    }
+    draw_kernel<E, false><<<(uint32_t)a.B, kThreads, 0, st>>>(a, parts);
+    gather_kernel<E><<<grid, kScanThreads, 0, st>>>(a, parts);
+    finish_kernel<E><<<(uint32_t)a.B, kThreads, 0, st>>>(a, parts);
 }
 
 }  // namespace
 
 namespace fni8h {
 
-int64_t sample_workspace_bytes(int64_t B, int64_t V) { return B * row_bytes(parts_of(V)); }
+int64_t sample_workspace_bytes(int64_t B, int64_t V) { return B * row_bytes(V); }
 
 int launch_sample(const Sample& a, hipStream_t st) {
     if (a.B == 0) return FNI8_OK;
