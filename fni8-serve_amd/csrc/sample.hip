@@ -706,7 +706,7 @@ __device__ __forceinline__ int search_row(Shared& sh, Turn& turn, const E* x, in
 // group of 32, so the mass below a logit is 16 times that of the samples below it, counted in
 // steps of weight.  Of `tail`, the mass that top-p leaves out (in units of the largest weight),
 // the estimate is off by sqrt(16 w tail) at most (one standard deviation; w the weight at the
-// end, the largest of the tail): five of them on either side, and a step for their rounding.
+// end, the largest of the tail): four of them on either side, and a step for their rounding.
 __device__ __forceinline__ void find_ends(Shared& sh, Turn& turn, const Work& w, int groups,
                                           const Row& r, double tail, Long& more) {
     constexpr int B = kBins / kThreads;
@@ -747,7 +747,7 @@ __device__ __forceinline__ void find_ends(Shared& sh, Turn& turn, const Work& w,
     reach(goal, sh.bin);
     __syncthreads();
     const int end = sh.bin;
-    const float dev = 5.0f * __builtin_sqrtf(f * __builtin_amdgcn_exp2f(-(float)end * unit) * goal);
+    const float dev = 4.0f * __builtin_sqrtf(f * __builtin_amdgcn_exp2f(-(float)end * unit) * goal);
     __syncthreads();
     if (threadIdx.x == 0) {
         sh.bin = kBins - 3;  // the lowest step with weight, where the tail is too thin to tell
@@ -956,51 +956,74 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, i
                 if (there) hi = mid;
                 else lo = mid + 1;
             }
-            if (lane == 0) sh.bin = lo;
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < B; j++) sum += b[j] <= lo ? m[j] : 0.0f;
+            sum = wave_sum_f32(sum);
+            // the list has more than these maxima: it is tried unless they are far from the mass
+            if (lane == 0) sh.bin = whole && lo < least && 4.0f * sum < goal ? -1 : lo;
         }
         __syncthreads();
         bound = sh.bin;
     }
     // ---- the tokens down to the bound, from the groups whose maximum reaches it
-    if (tid == 0) sh.n = sh.hits_n = 0;
-    __syncthreads();
-    auto hit = [&](uint32_t key, int i) {
-        if (bin_of(key) > bound) return;
-        const int at = atomicAdd(&sh.hits_n, 1);
-        if (at < kHits) sh.hits[at] = i;
-    };
-    if (mine <= bound) {
+    int n = kList + 1;
+    if (bound >= 0) {
+        // as a logit, a little lower: the list is a first run of the order, at least to the bound
+        const double down = r.base - (double)(bound + 1) / (r.step * r.rate);
+        const float edge = __builtin_fmaxf((float)(down - __builtin_fabs(down) * 0x1p-22), -0x1.fffffep127f);
+        const uint32_t least_key = key_of(r.inf ? __builtin_inff() : edge);
+        if (tid == 0) sh.n = sh.hits_n = 0;
+        __syncthreads();
+        auto hit = [&](uint32_t key, int i) {
+            if (key < least_key) return;
+            const int at = atomicAdd(&sh.hits_n, 1);
+            if (at < kHits) sh.hits[at] = i;
+        };
+        if (most >= least_key) {
 #pragma unroll
-        for (int j = 0; j < kKeep; j++)
-            if (tid + j * kThreads < groups) hit(keep[j], tid + j * kThreads);
-        for (int i = tid + kKeep * kThreads; i < groups; i += kThreads) hit(w.top[i], i);
-    }
-    __syncthreads();
-    const int hits = sh.hits_n;
-    if (hits <= kHits) {
-        for (int q = tid; q < hits * kSteps; q += kThreads) {
-            const int group = sh.hits[q / kSteps];
-            const int i0 = group / kScanThreads * kPart +
-                           (q % kSteps * kScanThreads + group % kScanThreads) * kVec;
-            float v[kVec];
-            load8(x, i0, V, r, v);
+            for (int j = 0; j < kKeep; j++)
+                if (tid + j * kThreads < groups) hit(keep[j], tid + j * kThreads);
+            for (int i = tid + kKeep * kThreads; i < groups; i += kThreads) hit(w.top[i], i);
+        }
+        __syncthreads();
+        const int hits = sh.hits_n;
+        if (hits <= kHits) {
+            auto first_of = [&](int q) {
+                const int group = sh.hits[q / kSteps];
+                return group / kScanThreads * kPart +
+                       (q % kSteps * kScanThreads + group % kScanThreads) * kVec;
+            };
+            auto list = [&](int i0, const float (&v)[kVec]) {
 #pragma unroll
-            for (int j = 0; j < kVec; j++) {
-                if (r.bin(r.power(v[j])) > bound) continue;
-                const u64 m = r.mass(v[j]);
-                if (!m) continue;
-                const int at = atomicAdd(&sh.n, 1);
-                if (at < kList) sh.list[at] = {(u64)key_of(v[j]) << 32 | (uint32_t)~(i0 + j), m};
+                for (int j = 0; j < kVec; j++) {
+                    if (v[j] < edge) continue;
+                    const int at = atomicAdd(&sh.n, 1);
+                    if (at < kList) sh.list[at].order = (u64)key_of(v[j]) << 32 | (uint32_t)~(i0 + j);
+                }
+            };
+            for (int q = tid; q < hits * kSteps; q += 2 * kThreads) {  // two loads on their way
+                float v[2][kVec];
+                const int q1 = q + kThreads, i0 = first_of(q), i1 = first_of(q1 < hits * kSteps ? q1 : q);
+                load8(x, i0, V, r, v[0]);
+                load8(x, i1, V, r, v[1]);
+                list(i0, v[0]);
+                if (q1 < hits * kSteps) list(i1, v[1]);
             }
         }
-    }
-    __syncthreads();
-    int n = hits <= kHits ? sh.n : kList + 1;
-    if (n <= kList && whole && bound < least) {
-        // top-p may end below the bound, and does unless the list has the mass
-        u64 listed = 0;
-        for (int i = tid; i < n; i += kThreads) listed += sh.list[i].mass;
-        if (block_sum(sh, turn, listed) < need_p) n = kList + 1;
+        __syncthreads();
+        n = hits <= kHits ? sh.n : kList + 1;
+        if (n <= kList) {
+            u64 listed = 0;
+            for (int i = tid; i < n; i += kThreads)
+                listed += sh.list[i].mass = r.mass(value_of(key_at(sh.list[i])));
+            // top-p may end below the bound, and does unless the list has the mass
+            if (whole && bound < least) {
+                if (block_sum(sh, turn, listed) < need_p) n = kList + 1;
+            } else {
+                __syncthreads();
+            }
+        }
     }
     if (n <= kMini) {
         // one wave, every pair: a token's rank and the mass before it, then its mass by index
@@ -1070,7 +1093,10 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, i
         token = search_row(sh, turn, x, V, r, need_p, all);
     } else {  // the long way
         Long more{need_p, 0.0f, 0.0f, kWhole, 0};
-        if (!r.by_k && !r.by_p) more.kind = kMinP;
+        if (!r.by_k && !r.by_p) {
+            more.kind = kMinP;
+            more.low = (float)(r.base - (double)(bound + 2) / (r.step * r.rate));
+        }
         if (whole && !r.by_m) {
             more.kind = kTopP;
             find_ends(sh, turn, w, groups, r, mass - (double)need_p / unit, more);
@@ -1082,13 +1108,19 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, i
 }
 
 // One part of a row with a long prefix: the mass of what is kept for certain, and the tokens
-// around the end of top-p.
+// around the end of top-p.  Each wave first packs the logits that matter (down to `low`) into its
+// LDS, so that their exponentials, 25 operations of 64 bits, are not computed for the others.
 template <class E>
 __global__ __launch_bounds__(kScanThreads) void gather_kernel(const fni8h::Sample a, int parts) {
+    constexpr int W = 64 * kVec;  // logits of a wave's load
+    __shared__ float packed[4][W];
+    __shared__ uint16_t where[4][W];
     __shared__ u64 sums[4];
-    __shared__ int counts[4], base;
+    __shared__ uint32_t tops[4];
     const int items = (int)a.B * parts, V = (int)a.V;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const u64 below = ((u64)1 << lane) - 1;
     for (int item = blockIdx.x; item < items; item += gridDim.x) {
         const int row = item / parts, part = item - row * parts;
         const Work w = work_of(a.work, row, V);
@@ -1096,66 +1128,68 @@ __global__ __launch_bounds__(kScanThreads) void gather_kernel(const fni8h::Sampl
         if (more.kind != kTopP && more.kind != kMinP) continue;
         const E* x = (const E*)a.logits + (int64_t)row * a.ld;
         Row r(a, row, V);
+        float v[kSteps][kVec];
+#pragma unroll
+        for (int i = 0; i < kSteps; i++)
+            load8(x, part * kPart + (i * kScanThreads + tid) * kVec, V, v[i]);
         uint32_t best = 0;
         for (int i = tid; i < parts; i += kScanThreads) best = w.part[i] > best ? w.part[i] : best;
         best = fni8::wave_max_u32(best);
-        if (lane == 0) counts[wave] = (int)best;
+        if (lane == 0) tops[wave] = best;
         __syncthreads();
-        for (int i = 0; i < 4; i++) best = (uint32_t)counts[i] > best ? (uint32_t)counts[i] : best;
+        for (int i = 0; i < 4; i++) best = tops[i] > best ? tops[i] : best;
         r.largest(value_of(best));
-        __syncthreads();
-        float v[kSteps][kVec];
-        u64 sum = 0;
-        int n = 0;
+        const u64 floor = more.kind == kMinP ? r.floor() : 0;
+        const float high = more.kind == kMinP ? -__builtin_inff() : more.high;
+        const float low = __builtin_fmaxf(more.low, -0x1.fffffep127f);
+        int around = 0;  // of the wave
 #pragma unroll
         for (int i = 0; i < kSteps; i++)
-            load8(x, part * kPart + (i * kScanThreads + tid) * kVec, V, r, v[i]);
-        if (more.kind == kTopP) {
 #pragma unroll
-            for (int i = 0; i < kSteps; i++)
+            for (int j = 0; j < kVec; j++) {
+                v[i][j] = r.seen(v[i][j]);
+                around += __builtin_popcountll(__ballot(v[i][j] >= low && v[i][j] < high));
+            }
+        int to = 0;
+        if (around && lane == 0) to = atomicAdd(&w.more->around, around);
+        u64 sum = 0;
 #pragma unroll
-                for (int j = 0; j < kVec; j++) {
-                    n += v[i][j] < more.high && v[i][j] >= more.low;
-                    sum += r.mass(v[i][j] >= more.high ? v[i][j] : -__builtin_inff());
+        for (int i = 0; i < kSteps; i++) {
+            int n = 0;
+#pragma unroll
+            for (int j = 0; j < kVec; j++) {
+                const u64 has = __ballot(v[i][j] >= low);
+                if (v[i][j] >= low) {
+                    const int at = n + __builtin_popcountll(has & below);
+                    packed[wave][at] = v[i][j];
+                    where[wave][at] = (uint16_t)(lane * kVec + j);
                 }
-        } else {
-            const u64 floor = r.floor();
-#pragma unroll
-            for (int i = 0; i < kSteps; i++)
-#pragma unroll
-                for (int j = 0; j < kVec; j++) {
-                    const u64 m = r.mass(v[i][j]);
-                    sum += m >= floor ? m : 0;
+                n += __builtin_popcountll(has);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            for (int t = lane; t < n; t += 64) {
+                const float q = packed[wave][t];
+                const u64 m = r.mass(q);
+                const bool certain = q >= high;
+                sum += certain && m >= floor ? m : 0;
+                if (!around) continue;
+                const u64 has = __ballot(!certain);
+                const int base = __builtin_amdgcn_readfirstlane(to);  // of lane 0
+                const int at = base + __builtin_popcountll(has & below);
+                if (!certain && at < around_of(V)) {
+                    const int index = part * kPart + (i * kScanThreads + wave * 64) * kVec +
+                                      where[wave][t];
+                    w.around[at] = (u64)key_of(q) << 32 | (uint32_t)~index;
                 }
+                to = base + __builtin_popcountll(has);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
         sum = wave_sum(sum);
-        const int run = fni8::wave_incl_scan_i32(n, lane);
-        if (lane == 63) {
-            sums[wave] = sum;
-            counts[wave] = run;
-        }
+        if (lane == 0) sums[wave] = sum;
         __syncthreads();
-        if (tid == 0) {
-            w.above[part] = sums[0] + sums[1] + sums[2] + sums[3];
-            const int all = counts[0] + counts[1] + counts[2] + counts[3];
-            base = all ? atomicAdd(&w.more->around, all) : 0;
-        }
-        __syncthreads();
-        int at = base + run - n;
-        for (int i = 0; i < wave; i++) at += counts[i];
-        if (n) {
-#pragma unroll
-            for (int i = 0; i < kSteps; i++)
-#pragma unroll
-                for (int j = 0; j < kVec; j++)
-                    if (v[i][j] < more.high && v[i][j] >= more.low) {
-                        const int index = part * kPart + (i * kScanThreads + tid) * kVec + j;
-                        if (at < around_of(V))
-                            w.around[at] = (u64)key_of(v[i][j]) << 32 | (uint32_t)~index;
-                        at++;
-                    }
-        }
-        __syncthreads();  // sums and counts are the next item's
+        if (tid == 0) w.above[part] = sums[0] + sums[1] + sums[2] + sums[3];
+        __syncthreads();  // tops and sums are the next item's
     }
 }
 
