@@ -22,6 +22,7 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 
+#include <array>
 #include <cmath>
 
 #include "../../include/fni8amd.h"
@@ -643,11 +644,130 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// lora_add(y, x, a, b, seg_off, rows, scaling, splits, in_place)
+PyObject* py_lora_add(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return entry(a, n, 9, [](PyObject* const* a) {
+        const Tensor &y = plain(a[0]), &x = plain(a[1]), &la = plain(a[2]), &lb = plain(a[3]);
+        const Rows ry = rows(y, at::kHalf), rx = rows(x, at::kHalf);
+        same(la, y, at::kHalf);
+        same(lb, y, at::kHalf);
+        need(x.device() == y.device() && x.dim() == y.dim() &&
+             x.sizes().slice(0, x.dim() - 1) == y.sizes().slice(0, y.dim() - 1));
+        need(la.dim() == 3 && lb.dim() == 3 && la.size(0) == lb.size(0) && la.size(2) == rx.K &&
+             lb.size(1) == ry.K && la.numel() > 0 && lb.numel() > 0);
+        const int64_t S = lb.size(0), rank = lb.size(2);
+        std::array<int64_t, FNI8_LORA_MAX_PARTS> splits{};
+        int64_t parts = 1, sum = 0;
+        if (a[7] == Py_None) {
+            splits[0] = sum = ry.K;
+        } else {
+            need(PyList_Check(a[7]) || PyTuple_Check(a[7]));
+            parts = PySequence_Fast_GET_SIZE(a[7]);
+            need(parts >= 1 && parts <= FNI8_LORA_MAX_PARTS);
+            for (int64_t i = 0; i < parts; i++) {
+                PyObject* o = PySequence_Fast_GET_ITEM(a[7], i);
+                need(PyLong_CheckExact(o));
+                splits[i] = integer(o);
+                need(splits[i] > 0 && splits[i] <= ry.K);
+                sum += splits[i];
+            }
+        }
+        need(sum == ry.K && la.size(1) == parts * rank);
+        const int32_t *seg = index32(plain(a[4]), y, S + 2), *order = index32(plain(a[5]), y, ry.M);
+        const float* scaling = nullptr;
+        if (a[6] != Py_None) {
+            const Tensor& s = plain(a[6]);
+            same(s, y, at::kFloat);
+            need(s.numel() == S);
+            scaling = static_cast<const float*>(s.data_ptr());
+        }
+        const bool in_place = a[8] == Py_True;
+        return [y, rx, ry, la, lb, S, rank, splits, parts, seg, order, scaling, in_place] {
+            c10::DeviceGuard guard(y.device());
+            Tensor out = in_place ? y : at::empty(y.sizes(), y.options());
+            const int64_t nw = fni8_lora_workspace_bytes(rx.M, rx.K, S, parts * rank);
+            Scratch sc;
+            sc.take(nw);
+            sc.alloc(y);
+            check("fni8_lora_add_f16",
+                  fni8_lora_add_f16(rx.p, rx.ld, rx.M, rx.K, la.data_ptr(), lb.data_ptr(), S, rank,
+                                    splits.data(), parts, scaling, seg, order, ry.p, ry.ld,
+                                    out.data_ptr(), in_place ? ry.ld : ry.K, sc.at_<void>(0), nw,
+                                    stream_of(y)));
+            return One{out};
+        };
+    });
+}
+
+// A sampling setting: a number for every row, or a tensor with one a row.
+struct Setting {
+    const void* p = nullptr;
+    double v = 0;
+};
+Setting setting(PyObject* o, const Tensor& x, int64_t B, at::ScalarType type, double most) {
+    Setting s;
+    if (PyFloat_CheckExact(o) || PyLong_CheckExact(o)) {
+        s.v = type == at::kInt ? (double)integer(o) : real(o);
+        need(s.v >= 0 && s.v <= most && (type != at::kInt || PyLong_CheckExact(o)));
+        return s;
+    }
+    const Tensor& t = plain(o);
+    same(t, x, type);
+    need(t.numel() == B);
+    s.p = t.data_ptr();
+    return s;
+}
+
+// sample(logits, u, temperature, top_k, top_p, min_p, return_logprobs)
+PyObject* py_sample(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return entry(a, n, 7, [](PyObject* const* a) {
+        const Tensor& x = plain(a[0]);
+        const bool fp32 = x.scalar_type() == at::kFloat;
+        const Rows r = rows(x, fp32 ? at::kFloat : at::kHalf);
+        const auto lead = x.sizes().slice(0, x.dim() - 1);
+        const Setting t = setting(a[2], x, r.M, at::kFloat, 3e38);
+        const Setting k = setting(a[3], x, r.M, at::kInt, 2147483647.0);
+        const Setting p = setting(a[4], x, r.M, at::kFloat, 1.0);
+        const Setting m = setting(a[5], x, r.M, at::kFloat, 1.0);
+        const float* u = nullptr;
+        if (a[1] == Py_None) {
+            need(!t.p && t.v == 0);
+        } else {
+            const Tensor& ut = plain(a[1]);
+            same(ut, x, at::kFloat);
+            need(ut.sizes() == lead);
+            u = static_cast<const float*>(ut.data_ptr());
+        }
+        const bool logprobs = PyObject_IsTrue(a[6]) == 1;
+        return [x, fp32, r, t, k, p, m, u, logprobs] {
+            c10::DeviceGuard guard(x.device());
+            const auto lead = x.sizes().slice(0, x.dim() - 1);
+            Several out;
+            out.t[out.n++] = at::empty(lead, x.options().dtype(at::kLong));
+            if (logprobs) out.t[out.n++] = at::empty(lead, x.options().dtype(at::kFloat));
+            const int64_t nw = fni8_sample_workspace_bytes(r.M, r.K);
+            Scratch sc;
+            sc.take(nw);
+            sc.alloc(x);
+            check("fni8_sample",
+                  fni8_sample(r.p, fp32, r.M, r.K, r.ld, u, static_cast<const float*>(t.p), (float)t.v,
+                              static_cast<const int32_t*>(k.p), (int64_t)k.v,
+                              static_cast<const float*>(p.p), (float)p.v,
+                              static_cast<const float*>(m.p), (float)m.v,
+                              static_cast<int64_t*>(out.t[0].data_ptr()),
+                              logprobs ? static_cast<float*>(out.t[1].data_ptr()) : nullptr,
+                              sc.at_<void>(0), nw, stream_of(x)));
+            return out;
+        };
+    });
+}
+
 #define FNI8_METHOD(name) \
     {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FNI8_METHOD(linear), FNI8_METHOD(gemm), FNI8_METHOD(mlp),
                          FNI8_METHOD(rmsnorm), FNI8_METHOD(moe), FNI8_METHOD(norm_rope),
-                         FNI8_METHOD(rope_append), FNI8_METHOD(paged_attention), {nullptr, nullptr, 0, nullptr}};
+                         FNI8_METHOD(rope_append), FNI8_METHOD(paged_attention),
+                         FNI8_METHOD(lora_add), FNI8_METHOD(sample), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods,
                       nullptr, nullptr, nullptr, nullptr};
 

@@ -12,7 +12,7 @@ never synchronises, so the calls can be captured in a HIP graph.  GPU tensors
 are required: there is no CPU or PyTorch fallback here.
 
 `linear`, `gemm_w8a8`, `gemm_w4a8`, `rmsnorm`, `rmsnorm_quant`, `rope`, `qk_norm_rope`,
-`rope_append`, `paged_attention` and the chains `gated_mlp` and `sparse_moe` run in native
+`rope_append`, `paged_attention`, `lora_add`, `sample` and the chains `gated_mlp` and `sparse_moe` run in native
 host code (`_host`, csrc/host.cpp) when
 every tensor is a plain GPU tensor in the layout the kernels take; the Python below
 is the general way (strided, converted or refused arguments).  A LinearW8A8 call at
@@ -843,6 +843,10 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     out: where the result goes; y itself adds in place and leaves rows without an adapter
     untouched; None allocates it.  rank is a multiple of 8, at most 256 (zeros fill up).
     Sums are fp32; the result is rounded once."""
+    if y.is_cuda and (out is None or out is y):
+        z = _lib.host().lora_add(y, x, a, b, plan[0], plan[1], scaling, splits, out is y)
+        if z is not None:
+            return y if out is y else z
     for name, t, dims in (("y", y, 0), ("x", x, 0), ("a", a, 3), ("b", b, 3)):
         if t.dtype != _f16 or t.dim() < 1 or (dims and (t.dim() != dims or not t.is_contiguous())):
             raise ValueError(f"{name} must be {'a contiguous' if dims else 'an'} fp16 tensor"
@@ -927,6 +931,10 @@ def sample(logits: torch.Tensor, u: torch.Tensor | None = None, temperature=1.0,
     with a NaN, or of minus infinity alone, gives -1 and the log-probability NaN.
 
     return_logprobs: (tokens, fp32 [...]), the logarithm of the token's share of the kept mass."""
+    if logits.is_cuda:
+        out = _lib.host().sample(logits, u, temperature, top_k, top_p, min_p, return_logprobs)
+        if out is not None:
+            return out
     if logits.dtype not in (_f16, torch.float32) or logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"logits must be fp16 or fp32 [..., V] (got {logits.dtype}, "
                          f"{tuple(logits.shape)})")
