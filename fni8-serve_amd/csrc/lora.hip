@@ -6,10 +6,14 @@
 // n belongs to.  Tokens come sorted by adapter (seg_off, rows); a tile is a run of one
 // adapter's tokens.  Two launches:
 //
-//   shrink  h = A x, a tile's tokens by a group of 16-row blocks of A by a part of K.  Waves
-//           split the part and add up in LDS; the parts' sums go to the workspace in fp32.
+//   shrink  h = A x: 16 or 64 tokens by up to 96 rows of A; K split over the eight waves of a
+//           tile of 16, and over workgroups where there are few tiles; fp32 sums to the workspace
 //   expand  adds the parts, then B h on the matrix cores, 16 tokens by a strip of columns a
-//           wave, and y in the same pass.
+//           wave, and y in the same pass
+//
+// Both wait for memory only.  A call of few tokens is a chain of dependent loads (which tile,
+// which rows, their data), so each wave finds its tile by itself, without LDS or a barrier, and
+// everything that depends on the tile alone is on its way at once.
 //
 // h enters the second product as two fp16 numbers, h * 2^k = hi + lo with one k a token that
 // brings the largest |h| to 2^8: the pair keeps 2^-22 of the largest h, so nothing overflows or
@@ -21,7 +25,8 @@ namespace {
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kThreads = 256, kWaves = 4;
+constexpr int kShrinkWaves = 8;            // of a workgroup
+constexpr int kThreads = 256, kWaves = 4;  // expand
 
 struct Args {
     const uint16_t *x, *y, *a, *b;
@@ -32,7 +37,7 @@ struct Args {
     float* h;            // [kparts][T][R]
     int T, K, S, rank, R, kparts;
     int copy;            // out is not y: tokens without an adapter are copied
-    int parts, cols;     // parts of the projection; columns of a workgroup
+    int parts, cols, blocks;  // parts of the projection; columns of a workgroup, their number
     int start[FNI8_LORA_MAX_PARTS + 1];  // first column of each part
 };
 
@@ -50,187 +55,521 @@ __device__ __forceinline__ h8 load8(const uint16_t* p, int64_t n) {
     return v;
 }
 
-template <int JT, int NT, bool WIDE>
-__global__ __launch_bounds__(kThreads) void shrink_kernel(const Args a) {
-    __shared__ f32x4 red[kWaves][JT * NT][64];
+// Inclusive sum over the lanes, by data movement within the vector unit.
+__device__ __forceinline__ int lane_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31
+    return v;
+}
+
+// Tile `slot` of the segments 0 .. E - 1, cut into tiles of BM tokens: its adapter and its tokens
+// r0 .. r1, or false past the last.  Bounded by T whatever seg_off holds.
+template <int BM>
+__device__ __forceinline__ bool find_tile(const Args& a, int E, int slot, int& e, int& r0, int& r1) {
+    const int lane = threadIdx.x & 63;
+    int base = 0;
+    for (int c = 0; c < E; c += 64) {
+        const int i = c + lane;
+        const int lo = i < E ? a.seg_off[i] : 0, hi = i < E ? a.seg_off[i + 1] : 0;
+        const int tiles = hi > lo ? (hi - lo + BM - 1) / BM : 0, end = base + lane_scan(tiles);
+        const uint64_t who = __ballot(slot < end && slot >= end - tiles);
+        if (who) {
+            const int l = __builtin_ctzll(who);
+            const int first = __builtin_amdgcn_readlane(end - tiles, l);
+            const int from = __builtin_amdgcn_readlane(lo, l), to = __builtin_amdgcn_readlane(hi, l);
+            e = c + l;
+            r0 = from + (slot - first) * BM;
+            r1 = r0 + BM < to ? r0 + BM : to;
+            r1 = r1 < a.T ? r1 : a.T;
+            return r0 >= 0 && r0 < r1;
+        }
+        base = __builtin_amdgcn_readlane(end, 63);
+    }
+    return false;
+}
+
+// The token at position r0 + i (i below count; else the last one's), -1 where rows holds none.
+// `ahead` is lane l's rows[l], loaded with the segments: enough for 64 tokens.
+__device__ __forceinline__ int token_at(const Args& a, int ahead, int r0, int i, int count) {
+    const int p = r0 + (i < count ? i : count - 1);
+    const int row = a.T <= 64 ? __shfl(ahead, p, 64) : a.rows[p];
+    return (unsigned)row < (unsigned)a.T ? row : -1;
+}
+__device__ __forceinline__ int rows_ahead(const Args& a) {
+    const int lane = threadIdx.x & 63;
+    return a.rows[lane < a.T ? lane : a.T - 1];
+}
+
+template <int JT, bool WIDE>
+__global__ __launch_bounds__(kShrinkWaves * 64) void shrink_kernel(const Args a) {
+    constexpr int HALF = kShrinkWaves / 2;
+    __shared__ f32x4 red[HALF][JT][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int ahead = rows_ahead(a);
     int e, r0, r1;
-    if (!fni8::find_group_tile(a.seg_off, a.S, 16 * NT, blockIdx.x, a.T, e, r0, r1)) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (!find_tile<16>(a, a.S, blockIdx.x, e, r0, r1)) return;
     const int j0 = blockIdx.y * 16 * JT, count = r1 - r0;
 
-    const uint16_t *xr[NT], *ar[JT];
-#pragma unroll
-    for (int t = 0; t < NT; t++) {
-        const int i = t * 16 + (lane & 15);
-        int row = a.rows[r0 + (i < count ? i : count - 1)];
-        row = row < 0 ? 0 : row < a.T ? row : a.T - 1;
-        xr[t] = a.x + (int64_t)row * a.ldx;
-    }
+    const int row = token_at(a, ahead, r0, lane & 15, count);
+    const uint16_t *xr = a.x + (int64_t)(row < 0 ? 0 : row) * a.ldx, *ar[JT];
 #pragma unroll
     for (int j = 0; j < JT; j++) {
         const int i = j0 + j * 16 + (lane & 15);
         ar[j] = a.a + ((int64_t)e * a.R + (i < a.R ? i : a.R - 1)) * a.K;
     }
-    f32x4 acc[JT][NT];
+    f32x4 acc[JT];
 #pragma unroll
-    for (int j = 0; j < JT; j++)
-#pragma unroll
-        for (int t = 0; t < NT; t++) acc[j][t] = f32x4{0, 0, 0, 0};
+    for (int j = 0; j < JT; j++) acc[j] = f32x4{0, 0, 0, 0};
 
     // steps of 32 elements of K, a run of them for each wave of each part
-    const int steps = (a.K + 31) / 32, ways = a.kparts * kWaves;
+    const int steps = (a.K + 31) / 32, ways = a.kparts * kShrinkWaves;
     const int per = (steps + ways - 1) / ways;
-    const int s0 = (blockIdx.z * kWaves + wave) * per;
+    const int s0 = (blockIdx.z * kShrinkWaves + wave) * per;
     const int s1 = s0 + per < steps ? s0 + per : steps;
-#pragma unroll WIDE ? 2 : 1
-    for (int s = s0; s < s1; s++) {
+    constexpr int AHEAD = !WIDE ? 1 : JT > 4 ? 2 : 4;  // steps whose loads are on their way
+    h8 xf[AHEAD], af[AHEAD][JT];
+    auto fetch = [&](int s, h8& xs, h8 (&as)[JT]) {
+        const h8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (s >= s1) {
+            xs = zero;
+#pragma unroll
+            for (int j = 0; j < JT; j++) as[j] = zero;
+            return;
+        }
         const int k = s * 32 + 8 * (lane >> 4);
-        h8 xf[NT], af[JT];
+        if (WIDE && s * 32 + 32 <= a.K) {
+            xs = *reinterpret_cast<const h8*>(xr + k);
 #pragma unroll
-        for (int t = 0; t < NT; t++) xf[t] = load8<WIDE>(xr[t] + k, a.K - k);
+            for (int j = 0; j < JT; j++) as[j] = *reinterpret_cast<const h8*>(ar[j] + k);
+        } else {
+            xs = load8<WIDE>(xr + k, a.K - k);
 #pragma unroll
-        for (int j = 0; j < JT; j++) af[j] = load8<WIDE>(ar[j] + k, a.K - k);
+            for (int j = 0; j < JT; j++) as[j] = load8<WIDE>(ar[j] + k, a.K - k);
+        }
+    };
 #pragma unroll
-        for (int j = 0; j < JT; j++)
+    for (int i = 0; i < AHEAD; i++) fetch(s0 + i, xf[i], af[i]);
+    for (int s = s0; s < s1; s += AHEAD) {
 #pragma unroll
-            for (int t = 0; t < NT; t++)
-                acc[j][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(af[j], xf[t], acc[j][t], 0, 0, 0);
+        for (int i = 0; i < AHEAD; i++) {
+#pragma unroll
+            for (int j = 0; j < JT; j++)
+                acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(af[i][j], xf[i], acc[j], 0, 0, 0);
+            fetch(s + AHEAD + i, xf[i], af[i]);
+        }
     }
+    // half of the waves' sums go through LDS to the other half, then those by all threads
+    auto keep = [&](int w) {
 #pragma unroll
-    for (int j = 0; j < JT; j++)
-#pragma unroll
-        for (int t = 0; t < NT; t++) red[wave][j * NT + t][lane] = acc[j][t];
+        for (int j = 0; j < JT; j++) red[w][j][lane] = acc[j];
+    };
+    if (wave >= HALF) keep(wave - HALF);
     __syncthreads();
-    for (int i = threadIdx.x; i < JT * NT * 64; i += kThreads) {
-        const int tile = i >> 6, l = i & 63, t = (tile % NT) * 16 + (l & 15);
-        const int j = j0 + (tile / NT) * 16 + 4 * (l >> 4);
+    if (wave < HALF) {
+#pragma unroll
+        for (int j = 0; j < JT; j++) acc[j] += red[wave][j][lane];
+        keep(wave);  // its own slots
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < JT * 64; i += kShrinkWaves * 64) {
+        const int tile = i >> 6, l = i & 63, t = l & 15, j = j0 + tile * 16 + 4 * (l >> 4);
         f32x4 v = red[0][tile][l];
 #pragma unroll
-        for (int w = 1; w < kWaves; w++) v += red[w][tile][l];
+        for (int w = 1; w < HALF; w++) v += red[w][tile][l];
         if (t < count && j < a.R)
             *reinterpret_cast<f32x4*>(a.h + ((int64_t)blockIdx.z * a.T + r0 + t) * a.R + j) = v;
     }
 }
 
-// KS: 32-element steps of the rank.  A strip is 16 * QT columns; lane (t, g) of a wave ends up
-// with the 4 * QT consecutive columns 4 * QT * g .. of token t, one to two 16-byte accesses.
-template <int KS, int NT>
-__global__ __launch_bounds__(kThreads) void expand_kernel(const Args a) {
-    constexpr int TM = 16 * NT, QT = KS <= 4 ? 4 : 2, UNITS = (TM * KS * 4 + kThreads - 1) / kThreads;
-    __shared__ h8 hs[NT * KS * 2][64];
-    __shared__ uint32_t top[TM];
-    __shared__ float back[TM];
-    __shared__ int token[TM];
+// 64 tokens by up to 32 * JW rows of A, for whole vectors: chunks of 128 elements of K go through
+// LDS, the next one's loads on their way.  A row's 256 bytes are read by 16 lanes side by side;
+// fragments loaded straight from memory take 64 bytes from each of 16 rows, which lie a power of
+// two apart and so in one channel of the cache (8192 tokens, K = 4096, 96 rows: 49 us that way).
+// Wave w has token group w % 4 and the rows' half w / 4, so no sums are added up.
+template <int JW>
+__global__ __launch_bounds__(512) void shrink_tile_kernel(const Args a) {
+    constexpr int TM = 64, JR = 32 * JW, CK = 128, ROW = 2 * CK + 16;  // bytes of a padded row
+    constexpr int LOADS = (TM + JR) * 16 / 512;                       // 16 bytes each, a thread
+    __shared__ __align__(16) uint8_t lds[(TM + JR) * ROW];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int ahead = rows_ahead(a);
     int e, r0, r1;
-    if (!fni8::find_group_tile(a.seg_off, a.S + 1, TM, blockIdx.x, a.T, e, r0, r1)) return;
-    const bool bare = e == a.S;
-    if (bare && !a.copy) return;
-    const int count = r1 - r0, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    // the part that this workgroup's columns are of
-    int part = 0, n0 = 0, block = blockIdx.y;
-    for (; part < a.parts; part++) {
+    if (!find_tile<TM>(a, a.S, blockIdx.x, e, r0, r1)) return;
+    const int j0 = blockIdx.y * JR, count = r1 - r0;
+    // a thread's loads: 16 bytes (tid % 16) of rows tid / 16 + 32 i, tokens first
+    const uint16_t* src[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; i++) {
+        const int r = (tid >> 4) + 32 * i;
+        if (r < TM) {
+            const int row = token_at(a, ahead, r0, r, count);
+            src[i] = a.x + (int64_t)(row < 0 ? 0 : row) * a.ldx;
+        } else {
+            const int j = j0 + r - TM;
+            src[i] = a.a + ((int64_t)e * a.R + (j < a.R ? j : a.R - 1)) * a.K;
+        }
+        src[i] += 8 * (tid & 15);
+    }
+    const int chunks = (a.K + CK - 1) / CK, per = (chunks + a.kparts - 1) / a.kparts;
+    const int c0 = blockIdx.z * per, c1 = c0 + per < chunks ? c0 + per : chunks;
+    h8 next[LOADS];
+    auto fetch = [&](int c) {
+        if (c >= c1) return;
+        const int k = c * CK;
+        if (k + CK <= a.K) {
+#pragma unroll
+            for (int i = 0; i < LOADS; i++) next[i] = *reinterpret_cast<const h8*>(src[i] + k);
+        } else {
+#pragma unroll
+            for (int i = 0; i < LOADS; i++) next[i] = load8<true>(src[i] + k, a.K - k - 8 * (tid & 15));
+        }
+    };
+    f32x4 acc[JW];
+#pragma unroll
+    for (int j = 0; j < JW; j++) acc[j] = f32x4{0, 0, 0, 0};
+    fetch(c0);
+    const uint8_t* xs = lds + ((wave & 3) * 16 + (lane & 15)) * ROW + 16 * (lane >> 4);
+    const uint8_t* as = lds + (TM + (wave >> 2) * 16 * JW + (lane & 15)) * ROW + 16 * (lane >> 4);
+    for (int c = c0; c < c1; c++) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < LOADS; i++)
+            *reinterpret_cast<h8*>(lds + ((tid >> 4) + 32 * i) * ROW + 16 * (tid & 15)) = next[i];
+        __syncthreads();
+        fetch(c + 1);
+#pragma unroll
+        for (int s = 0; s < CK / 32; s++) {
+            const h8 x = *reinterpret_cast<const h8*>(xs + 64 * s);
+#pragma unroll
+            for (int j = 0; j < JW; j++)
+                acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                    *reinterpret_cast<const h8*>(as + j * 16 * ROW + 64 * s), x, acc[j], 0, 0, 0);
+        }
+    }
+    const int t = (wave & 3) * 16 + (lane & 15);
+#pragma unroll
+    for (int j = 0; j < JW; j++) {
+        const int i = j0 + ((wave >> 2) * JW + j) * 16 + 4 * (lane >> 4);
+        if (t < count && i < a.R)
+            *reinterpret_cast<f32x4*>(a.h + ((int64_t)blockIdx.z * a.T + r0 + t) * a.R + i) = acc[j];
+    }
+}
+
+// What a workgroup's column block is of: the part, and the columns n0 .. n1 of it.
+__device__ __forceinline__ bool find_block(const Args& a, int block, int& part, int& n0, int& n1) {
+    for (part = 0; part < a.parts; part++) {
         const int width = a.start[part + 1] - a.start[part], blocks = (width + a.cols - 1) / a.cols;
         if (block < blocks) break;
         block -= blocks;
     }
-    if (part == a.parts) return;
+    if (part == a.parts) return false;
     n0 = a.start[part] + block * a.cols;
     const int end = a.start[part + 1];
-    const int n1 = n0 + a.cols < end ? n0 + a.cols : end;
+    n1 = n0 + a.cols < end ? n0 + a.cols : end;
+    return true;
+}
 
-    for (int t = threadIdx.x; t < TM; t += kThreads) {
-        const int row = t < count ? a.rows[r0 + t] : -1;
-        token[t] = row < a.T ? row : -1;
-        top[t] = 0;
+// Eight consecutive values of a token's low-rank row, the parts added in order (MANY of them on
+// their way at once), scaled.
+template <int MANY>
+__device__ __forceinline__ void low_rank(const Args& a, int pos, int part, int j, float scale,
+                                         float (&v)[8]) {
+    const float* h = a.h + (int64_t)pos * a.R + part * a.rank + j;
+    const int64_t step = (int64_t)a.T * a.R;
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = 0.0f;
+    for (int p = 0; p < a.kparts; p += MANY) {
+        f32x4 lo[MANY], hi[MANY];
+#pragma unroll
+        for (int i = 0; i < MANY; i++) {
+            const bool has = p + i < a.kparts;
+            const float* q = h + (has ? i * step : 0);
+            lo[i] = *reinterpret_cast<const f32x4*>(q);
+            hi[i] = *reinterpret_cast<const f32x4*>(q + 4);
+            if (!has) lo[i] = hi[i] = f32x4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int i = 0; i < MANY; i++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                v[k] += lo[i][k];
+                v[k + 4] += hi[i][k];
+            }
+        h += MANY * step;
     }
-    __syncthreads();
-    if (bare) {
-        for (int t = wave; t < count; t += kWaves) {
-            if (token[t] < 0) continue;
-            const uint16_t* y = a.y + (int64_t)token[t] * a.ldy;
-            uint16_t* o = a.out + (int64_t)token[t] * a.ldo;
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] *= scale;
+}
+
+__device__ __forceinline__ uint32_t top_of(const float (&v)[8]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const uint32_t w = __builtin_bit_cast(uint32_t, v[j]) & 0x7fffffffu;
+        m = w > m ? w : m;
+    }
+    return m;
+}
+
+// The power of two that brings a token's largest |h| (its bits) to 2^8; 0 for a row of zeros and
+// one with infinities or NaN.
+__device__ __forceinline__ int shift_of(uint32_t top) {
+    const int up = 135 - (int)(top >> 23);
+    return top >= 0x7f800000u || top == 0 ? 0 : up > 120 ? 120 : up;
+}
+
+__device__ __forceinline__ void split8(const float (&v)[8], uint32_t top, h8& hi, h8& lo) {
+    const int up = shift_of(top);
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const float w = __builtin_ldexpf(v[j], up);
+        const _Float16 h = (_Float16)w;
+        hi[j] = h;
+        lo[j] = top < 0x7f800000u ? (_Float16)(w - (float)h) : (_Float16)0.0f;
+    }
+}
+
+// A strip of a wave: 16 * QT columns from n on, the rows of B for it.  Row i of the q-th product
+// is column 32 (q / 2) + 8 (i / 4) + 4 (q & 1) + i % 4, which leaves lane (t, g) with columns
+// 8 g .. 8 g + 7 of every 32: a load of 16 bytes a lane takes 64 in a row of each token.
+// b: B of the adapter; whole: the strip ends before n1.
+template <int KS, int QT>
+__device__ __forceinline__ void load_b(const Args& a, const uint16_t* b, int n, int n1, bool whole,
+                                       int lane, h8 (&bf)[QT][KS]) {
+    const int i = lane & 15, g = lane >> 4, mine = 8 * (i >> 2) + (i & 3);
+    const uint16_t* base = b + (int64_t)n * a.rank;  // the same for the wave
+#pragma unroll
+    for (int q = 0; q < QT; q++) {
+        const int c = 32 * (q >> 1) + 4 * (q & 1);
+        const uint16_t* from = base + c * a.rank;
+        int off = mine * a.rank + 8 * g;
+        if (!whole) off = ((n + c + mine < n1 ? c + mine : n1 - 1 - n) - c) * a.rank + 8 * g;
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            // past the rank: the row's first values, then zeros
+            const bool has = 32 * s + 8 * g < a.rank;
+            bf[q][s] = *reinterpret_cast<const h8*>(from + off + (has ? 32 * s : -8 * g));
+            if (a.rank < 32 * (s + 1) && !has) bf[q][s] = h8{0, 0, 0, 0, 0, 0, 0, 0};
+        }
+    }
+}
+
+// y: the lane's first column of the strip, `left` columns before the end; whole (the same for
+// the wave): all of the strip is there, in whole vectors.
+template <int QT>
+__device__ __forceinline__ void load_y(const uint16_t* y, int left, bool whole, h8 (&in)[QT / 2]) {
+    if (whole) {
+#pragma unroll
+        for (int q = 0; q < QT / 2; q++) in[q] = *reinterpret_cast<const h8*>(y + 32 * q);
+    } else {
+#pragma unroll
+        for (int q = 0; q < QT / 2; q++) in[q] = load8<false>(y + 32 * q, left - 32 * q);
+    }
+}
+
+// down is a power of two: the product is exact, the sum rounded once to 32 bits, then to 16.
+template <int QT>
+__device__ __forceinline__ void store_y(uint16_t* o, int left, bool whole, const h8 (&in)[QT / 2],
+                                        const f32x4 (&acc)[QT], float down) {
+#pragma unroll
+    for (int q = 0; q < QT / 2; q++) {
+        h8 z;
+#pragma unroll
+        for (int r = 0; r < 8; r++)
+            z[r] = (_Float16)__builtin_fmaf(acc[2 * q + r / 4][r & 3], down, (float)in[q][r]);
+        if (whole) {
+            *reinterpret_cast<h8*>(o + 32 * q) = z;
+        } else {
+#pragma unroll
+            for (int r = 0; r < 8; r++) {
+                const _Float16 f = z[r];  // an element is no lvalue to bit_cast
+                if (32 * q + r < left) o[32 * q + r] = __builtin_bit_cast(uint16_t, f);
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ bool aligned8(const Args& a, int n0) {
+    return (a.ldy | a.ldo | n0) % 8 == 0 && (((uintptr_t)a.y | (uintptr_t)a.out) & 15) == 0;
+}
+
+// Tokens without an adapter: out is y.
+__device__ __forceinline__ void copy_rows(const Args& a, int ahead, int r0, int count, int n0, int n1) {
+    const int lane = threadIdx.x & 63;
+    for (int t = threadIdx.x >> 6; t < count; t += kWaves) {
+        const int row = token_at(a, ahead, r0, t, count);
+        if (row < 0) continue;
+        const uint16_t* y = a.y + (int64_t)row * a.ldy;
+        uint16_t* o = a.out + (int64_t)row * a.ldo;
+        if (aligned8(a, n0) && (n1 - n0) % 8 == 0) {
+            for (int n = n0 + lane * 8; n < n1; n += 512)
+                *reinterpret_cast<h8*>(o + n) = *reinterpret_cast<const h8*>(y + n);
+        } else {
             for (int n = n0 + lane; n < n1; n += 64) o[n] = y[n];
         }
+    }
+}
+
+// KS: 32-element steps of the rank.  Tiles of 16 tokens; a wave keeps the low-rank rows in
+// registers and goes through its strips, the loads of the next on their way.
+template <int KS>
+__global__ __launch_bounds__(kThreads, KS <= 2 ? 4 : KS == 4 ? 2 : 1) void expand_few_kernel(const Args a) {
+    constexpr int QT = KS == 1 ? 4 : 2;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int ahead = rows_ahead(a);
+    int e, r0, r1, part, n0, n1;
+    if (!find_tile<16>(a, a.S + 1, blockIdx.x, e, r0, r1)) return;
+    if (!find_block(a, blockIdx.y, part, n0, n1)) return;
+    const int count = r1 - r0, t = lane & 15, g = lane >> 4;
+    if (e == a.S) {
+        if (a.copy) copy_rows(a, ahead, r0, count, n0, n1);
         return;
     }
+    const int row = token_at(a, ahead, r0, t, count);
+    const bool live = t < count && row >= 0, wide = aligned8(a, n0);
+    // lanes without a token load another's row, and store nothing
+    const uint16_t* y = a.y + (int64_t)(row < 0 ? 0 : row) * a.ldy + 8 * g;
+    uint16_t* o = a.out + (int64_t)(row < 0 ? 0 : row) * a.ldo + 8 * g;
+    const uint16_t* rows_b = a.b + (int64_t)e * a.start[a.parts] * a.rank;
+    constexpr int STEP = kWaves * 16 * QT;
+    h8 bf[2][QT][KS], in[2][QT / 2];
+    auto fetch = [&](int n, h8 (&b)[QT][KS], h8 (&z)[QT / 2]) {
+        if (n >= n1) return;
+        load_b<KS, QT>(a, rows_b, n, n1, n + 16 * QT <= n1, lane, b);
+        load_y<QT>(y + n, n1 - n - 8 * g, wide && n + 16 * QT <= n1, z);
+    };
+    int n = n0 + wave * 16 * QT;
+    // the low-rank rows before y and B: loads come back in order, and these come from the cache
+    const float scale = a.scaling ? a.scaling[e] : 1.0f;
+    float v[KS][8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+        const int j = s * 32 + 8 * g;
+        if (t < count && j < a.rank) {
+            low_rank<KS == 1 ? 8 : 4>(a, r0 + t, part, j, scale, v[s]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[s][i] = 0.0f;
+        }
+        const uint32_t m = top_of(v[s]);
+        top = m > top ? m : top;
+    }
+    fetch(n, bf[0], in[0]);
+#pragma unroll
+    for (int d = 16; d < 64; d *= 2) {
+        const uint32_t m = (uint32_t)__shfl_xor((int)top, d, 64);
+        top = m > top ? m : top;
+    }
+    h8 hi[KS], lo[KS];
+#pragma unroll
+    for (int s = 0; s < KS; s++) split8(v[s], top, hi[s], lo[s]);
+    const float down = __builtin_ldexpf(1.0f, -shift_of(top));
+    fetch(n + STEP, bf[1], in[1]);
+    auto strip = [&](int n, h8 (&b)[QT][KS], h8 (&z)[QT / 2]) {
+        if (n >= n1) return;
+        f32x4 acc[QT];
+#pragma unroll
+        for (int q = 0; q < QT; q++) acc[q] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int q = 0; q < QT; q++) {
+                acc[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b[q][s], lo[s], acc[q], 0, 0, 0);
+                acc[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b[q][s], hi[s], acc[q], 0, 0, 0);
+            }
+        h8 was[QT / 2];
+#pragma unroll
+        for (int q = 0; q < QT / 2; q++) was[q] = z[q];
+        fetch(n + 2 * STEP, b, z);
+        if (live)
+            store_y<QT>(o + n, n1 - n - 8 * g, wide && n + 16 * QT <= n1, was, acc, down);
+    };
+    for (; n < n1; n += 2 * STEP) {
+        strip(n, bf[0], in[0]);
+        strip(n + STEP, bf[1], in[1]);
+    }
+}
+
+// The same for tiles of 16 * NT tokens: the low-rank rows lie in LDS, a strip's rows of B serve
+// all NT groups of 16.
+template <int KS, int NT>
+__global__ __launch_bounds__(kThreads) void expand_kernel(const Args a) {
+    constexpr int TM = 16 * NT, QT = KS <= 2 ? 4 : 2;
+    constexpr int UNITS = (TM * KS * 4 + kThreads - 1) / kThreads;
+    __shared__ h8 hs[NT * KS * 2][64];
+    __shared__ uint32_t top[TM];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int ahead = rows_ahead(a);
+    int e, r0, r1, part, n0, n1;
+    // the column blocks of a tile side by side
+    const int tile = blockIdx.x / (uint32_t)a.blocks;
+    if (!find_tile<TM>(a, a.S + 1, tile, e, r0, r1)) return;
+    if (!find_block(a, blockIdx.x - tile * a.blocks, part, n0, n1)) return;
+    const int count = r1 - r0, g = lane >> 4;
+    if (e == a.S) {
+        if (a.copy) copy_rows(a, ahead, r0, count, n0, n1);
+        return;
+    }
+    int row[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        const int i = t * 16 + (lane & 15), r = token_at(a, ahead, r0, i, count);
+        row[t] = i < count ? r : -1;  // -1: loads row 0, stores nothing
+    }
+    const bool wide = aligned8(a, n0);
+    const uint16_t* rows_b = a.b + (int64_t)e * a.start[a.parts] * a.rank;
+    h8 bf[QT][KS], in[NT][QT / 2];
+    auto fetch = [&](int n) {
+        const bool whole = wide && n + 16 * QT <= n1;
+        load_b<KS, QT>(a, rows_b, n, n1, n + 16 * QT <= n1, lane, bf);
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+            load_y<QT>(a.y + (int64_t)(row[t] < 0 ? 0 : row[t]) * a.ldy + n + 8 * g, n1 - n - 8 * g,
+                       whole, in[t]);
+    };
+    // the low-rank rows before y: loads come back in order, and these come from the cache
+    const float scale = a.scaling ? a.scaling[e] : 1.0f;
     float v[UNITS][8];
 #pragma unroll
     for (int i = 0; i < UNITS; i++) {
-        const int u = threadIdx.x + i * kThreads, t = u / (KS * 4), g = u % (KS * 4);
+        const int u = threadIdx.x + i * kThreads, t = u / (KS * 4), j = u % (KS * 4) * 8;
+        if (t < count && j < a.rank) {
+            low_rank<4>(a, r0 + t, part, j, scale, v[i]);
+        } else {
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[i][j] = 0.0f;
-        if (t >= count || g * 8 >= a.rank) continue;
-        const float* h = a.h + (int64_t)(r0 + t) * a.R + part * a.rank + g * 8;
-        for (int p = 0; p < a.kparts; p++, h += (int64_t)a.T * a.R) {
-            const f32x4 lo = *reinterpret_cast<const f32x4*>(h);
-            const f32x4 hi = *reinterpret_cast<const f32x4*>(h + 4);
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                v[i][j] += lo[j];
-                v[i][j + 4] += hi[j];
-            }
+            for (int k = 0; k < 8; k++) v[i][k] = 0.0f;
         }
-        uint32_t m = 0;
+    }
+    int n = n0 + wave * 16 * QT;
+    if (n < n1) fetch(n);
+    for (int t = threadIdx.x; t < TM; t += kThreads) top[t] = 0;
+    __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const uint32_t w = __builtin_bit_cast(uint32_t, v[i][j]) & 0x7fffffffu;
-            m = w > m ? w : m;
-        }
-        atomicMax(&top[t], m);
+    for (int i = 0; i < UNITS; i++) {
+        const int t = (threadIdx.x + i * kThreads) / (KS * 4);
+        if (t < count) atomicMax(&top[t], top_of(v[i]));
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < UNITS; i++) {
-        const int u = threadIdx.x + i * kThreads, t = u / (KS * 4), g = u % (KS * 4);
+        const int u = threadIdx.x + i * kThreads, t = u / (KS * 4), k = u % (KS * 4);
         if (t >= TM) continue;
-        const uint32_t m = top[t];
-        const bool finite = m < 0x7f800000u;
-        int up = 135 - (int)(m >> 23);  // brings the largest to 2^8
-        up = !finite || m == 0 ? 0 : up > 120 ? 120 : up;
-        h8 hi, lo;
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const float w = __builtin_ldexpf(v[i][j], up);
-            hi[j] = (_Float16)w;
-            lo[j] = finite ? (_Float16)(w - (float)hi[j]) : (_Float16)0.0f;
-        }
-        const int at = ((t >> 4) * KS + (g >> 2)) * 2, l = (t & 15) + 16 * (g & 3);
-        hs[at][l] = hi;
-        hs[at + 1][l] = lo;
-        if (g == 0) back[t] = __builtin_ldexpf(1.0f, -up);
+        const int at = ((t >> 4) * KS + (k >> 2)) * 2, l = (t & 15) + 16 * (k & 3);
+        split8(v[i], top[t], hs[at][l], hs[at + 1][l]);
     }
     __syncthreads();
-
-    const float scale = a.scaling ? a.scaling[e] : 1.0f;
-    const int g = lane >> 4;
-    const bool wide = (a.ldy | a.ldo | n0) % 8 == 0 &&
-                      (((uintptr_t)a.y | (uintptr_t)a.out) & 15) == 0;
-    for (int n = n0 + wave * 16 * QT; n < n1; n += kWaves * 16 * QT) {
-        h8 bf[QT][KS];
-        const int i = lane & 15;
+    float down[NT];
 #pragma unroll
-        for (int q = 0; q < QT; q++) {
-            // row i of the q-th product: the column that brings lane (t, g) its runs
-            int c = n + 4 * QT * (i >> 2) + 4 * q + (i & 3);
-            c = c < n1 ? c : n1 - 1;
-            const uint16_t* b = a.b + ((int64_t)e * a.start[a.parts] + c) * a.rank;
-#pragma unroll
-            for (int s = 0; s < KS; s++) bf[q][s] = load8<true>(b + s * 32 + 8 * g, a.rank - s * 32 - 8 * g);
-        }
-        const int c0 = n + 4 * QT * g;
+    for (int t = 0; t < NT; t++) down[t] = __builtin_ldexpf(1.0f, -shift_of(top[t * 16 + (lane & 15)]));
+    while (n < n1) {
+        const bool whole = wide && n + 16 * QT <= n1;
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-            if (t * 16 >= count) break;
-            const int row = token[t * 16 + i];
-            const bool live = row >= 0;
-            const uint16_t* y = a.y + (int64_t)(live ? row : 0) * a.ldy + c0;
-            uint16_t* o = a.out + (int64_t)(live ? row : 0) * a.ldo + c0;
-            const bool whole = wide && n + 16 * QT <= n1;
-            h8 in[QT / 2];
-#pragma unroll
-            for (int q = 0; q < QT / 2; q++)
-                in[q] = whole ? load8<true>(y + 8 * q, live ? 8 : 0)
-                              : load8<false>(y + 8 * q, live ? n1 - c0 - 8 * q : 0);
             f32x4 acc[QT];
 #pragma unroll
             for (int q = 0; q < QT; q++) acc[q] = f32x4{0, 0, 0, 0};
@@ -243,34 +582,18 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(const Args a) {
                     acc[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bf[q][s], hi, acc[q], 0, 0, 0);
                 }
             }
-            const float down = back[t * 16 + i];
-#pragma unroll
-            for (int q = 0; q < QT; q++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const float d = acc[q][r] * down * scale;
-                    const int z = (q & 1) * 4 + r;
-                    in[q >> 1][z] = __builtin_bit_cast(_Float16, fni8::f2h((float)in[q >> 1][z] + d));
-                }
-            if (!live) continue;
-#pragma unroll
-            for (int q = 0; q < QT / 2; q++) {
-                if (whole) {
-                    *reinterpret_cast<h8*>(o + 8 * q) = in[q];
-                } else {
-#pragma unroll
-                    for (int r = 0; r < 8; r++) {
-                        const _Float16 z = in[q][r];  // an element is no lvalue to bit_cast
-                        if (c0 + 8 * q + r < n1) o[8 * q + r] = __builtin_bit_cast(uint16_t, z);
-                    }
-                }
-            }
+            if (row[t] >= 0)
+                store_y<QT>(a.out + (int64_t)row[t] * a.ldo + n + 8 * g, n1 - n - 8 * g, whole, in[t],
+                            acc, down[t]);
         }
+        n += kWaves * 16 * QT;
+        if (n < n1) fetch(n);
     }
 }
 
-// Tiles of 16 tokens, or of 64 where an adapter has that many on average.
-bool big_tiles(int64_t T, int64_t S) { return T >= 64 * (S < 16 ? S : 16) && T >= 256; }
+// Tiles of 16 tokens, or of 64 where an adapter has that many on average and there are enough of
+// them.
+bool big_tiles(int64_t T, int64_t S) { return T >= 64 * (S < 16 ? S : 16) && T >= 1024; }
 
 int64_t tiles_of(int64_t T, int64_t groups, int64_t bm) {
     return T / bm + (groups < T ? groups : T);
@@ -278,36 +601,73 @@ int64_t tiles_of(int64_t T, int64_t groups, int64_t bm) {
 
 struct Plan {
     bool big;
-    int jt;
+    int jt;  // blocks of 16 rows of A in a workgroup: x is read once for each group of them
     int64_t jgroups, tiles, kparts;
 };
 Plan plan_of(int64_t T, int64_t K, int64_t S, int64_t R) {
     Plan p{};
     p.big = big_tiles(T, S);
-    p.jt = R <= 16 ? 1 : R <= 32 ? 2 : 3;
-    p.jgroups = (R + 16 * p.jt - 1) / (16 * p.jt);
+    const int64_t blocks = (R + 15) / 16;
     p.tiles = tiles_of(T, S, p.big ? 64 : 16);
-    // enough workgroups for two on each CU, no wave with less than two steps of K
-    const int64_t want = 512 / (p.tiles * p.jgroups) + 1, most = (K + 255) / 256;
+    if (p.big) {
+        p.jt = blocks <= 2 ? 2 : blocks <= 4 || blocks == 7 || blocks == 8 ? 4 : 6;
+        p.jgroups = (blocks + p.jt - 1) / p.jt;
+        // parts of K that leave the 256 CUs evenly loaded; each costs its share of the sums' way
+        // through memory
+        double best = 1e30;
+        for (int64_t k = 1; k <= 8 && (k == 1 || k * 256 <= K); k++) {
+            const int64_t rounds = (p.tiles * p.jgroups * k + 255) / 256;
+            const double cost = (double)rounds / k + 0.05 * k;
+            if (cost < best) {
+                best = cost;
+                p.kparts = k;
+            }
+        }
+        return p;
+    }
+    // as many blocks in a workgroup as leave 192 with eight parts of K, and parts for one on each
+    // CU; more than eight cost the expansion a round trip
+    for (int jt : {6, 4, 3, 2, 1}) {
+        p.jt = jt;
+        p.jgroups = (blocks + jt - 1) / jt;
+        if (jt == 1 || (blocks % jt == 0 && p.tiles * p.jgroups * 8 >= 192)) break;
+    }
+    const int64_t want = 256 / (p.tiles * p.jgroups) + 1, most = (K + 511) / 512;
     p.kparts = want < most ? want : most;
-    if (p.kparts > 16) p.kparts = 16;
+    if (p.kparts > 8) p.kparts = 8;
     return p;
 }
 
-template <int NT, bool WIDE>
+template <bool WIDE>
 void shrink(const Args& a, const Plan& p, hipStream_t st) {
-    const dim3 grid((uint32_t)p.tiles, (uint32_t)p.jgroups, (uint32_t)p.kparts);
-    if (p.jt == 1) shrink_kernel<1, NT, WIDE><<<grid, kThreads, 0, st>>>(a);
-    else if (p.jt == 2) shrink_kernel<2, NT, WIDE><<<grid, kThreads, 0, st>>>(a);
-    else shrink_kernel<3, NT, WIDE><<<grid, kThreads, 0, st>>>(a);
+    dim3 grid((uint32_t)p.tiles, (uint32_t)p.jgroups, (uint32_t)p.kparts);
+    constexpr int threads = kShrinkWaves * 64;
+    if (p.big && WIDE) {
+        if (p.jt == 2) shrink_tile_kernel<1><<<grid, 512, 0, st>>>(a);
+        else if (p.jt == 4) shrink_tile_kernel<2><<<grid, 512, 0, st>>>(a);
+        else shrink_tile_kernel<3><<<grid, 512, 0, st>>>(a);
+        return;
+    }
+    if (p.big) grid.x = (uint32_t)tiles_of(a.T, a.S, 16);
+    if (p.jt == 1) shrink_kernel<1, WIDE><<<grid, threads, 0, st>>>(a);
+    else if (p.jt == 2) shrink_kernel<2, WIDE><<<grid, threads, 0, st>>>(a);
+    else if (p.jt == 3) shrink_kernel<3, WIDE><<<grid, threads, 0, st>>>(a);
+    else if (p.jt == 4) shrink_kernel<4, WIDE><<<grid, threads, 0, st>>>(a);
+    else shrink_kernel<6, WIDE><<<grid, threads, 0, st>>>(a);
 }
 
-template <int NT>
+void expand_few(const Args& a, dim3 grid, hipStream_t st) {
+    if (a.rank <= 32) expand_few_kernel<1><<<grid, kThreads, 0, st>>>(a);
+    else if (a.rank <= 64) expand_few_kernel<2><<<grid, kThreads, 0, st>>>(a);
+    else if (a.rank <= 128) expand_few_kernel<4><<<grid, kThreads, 0, st>>>(a);
+    else expand_few_kernel<8><<<grid, kThreads, 0, st>>>(a);
+}
+
 void expand(const Args& a, dim3 grid, hipStream_t st) {
-    if (a.rank <= 32) expand_kernel<1, NT><<<grid, kThreads, 0, st>>>(a);
-    else if (a.rank <= 64) expand_kernel<2, NT><<<grid, kThreads, 0, st>>>(a);
-    else if (a.rank <= 128) expand_kernel<4, NT><<<grid, kThreads, 0, st>>>(a);
-    else expand_kernel<8, NT < 2 ? NT : 2><<<grid, kThreads, 0, st>>>(a);
+    if (a.rank <= 32) expand_kernel<1, 4><<<grid, kThreads, 0, st>>>(a);
+    else if (a.rank <= 64) expand_kernel<2, 4><<<grid, kThreads, 0, st>>>(a);
+    else if (a.rank <= 128) expand_kernel<4, 4><<<grid, kThreads, 0, st>>>(a);
+    else expand_kernel<8, 2><<<grid, kThreads, 0, st>>>(a);
 }
 
 }  // namespace
@@ -333,21 +693,32 @@ int launch_lora_add(const LoraAdd& l, hipStream_t st) {
     for (int i = 0; i < l.parts; i++) a.start[i + 1] = a.start[i] + (int)l.splits[i];
 
     const bool wide = l.K % 8 == 0 && l.ldx % 8 == 0 && (((uintptr_t)l.x | (uintptr_t)l.a) & 15) == 0;
-    if (p.big) wide ? shrink<4, true>(a, p, st) : shrink<4, false>(a, p, st);
-    else wide ? shrink<1, true>(a, p, st) : shrink<1, false>(a, p, st);
+    if (wide) shrink<true>(a, p, st);
+    else shrink<false>(a, p, st);
 
     const int nt = !p.big ? 1 : l.rank > 128 ? 2 : 4;
     const int64_t tiles = tiles_of(l.T, l.S + 1, 16 * nt);
-    // columns of a workgroup: four waves' strips, more where that leaves plenty of workgroups
-    const int64_t N = a.start[l.parts];
-    int64_t cols = 256;
-    while (cols < 1024 && tiles * (N / (2 * cols)) >= 1024) cols *= 2;
+    // Columns of a workgroup, whole strips of its four waves.  Tiles of 64: two strips where that
+    // leaves three workgroups to a CU (8192 tokens, 6144 columns: 54 us; 57 with one, 64 with
+    // three).  Of 16: the fewest rounds of the four that a CU holds at once, each as long as the
+    // columns and a start that takes about as long as 1024 of them.
+    const int64_t strips = kWaves * 64;
+    int64_t cols = 0, blocks = 0, best = 0;
+    for (int64_t c = strips; c <= (p.big ? 512 : 4096); c += strips) {
+        int64_t n = 0;
+        for (int i = 0; i < l.parts; i++) n += (l.splits[i] + c - 1) / c;
+        const int64_t cost = p.big ? (tiles * n >= 768 ? 1 : 2) * 4096 - c
+                                   : (tiles * n + 1023) / 1024 * (c + 1024);
+        if (!cols || cost < best) {
+            cols = c;
+            blocks = n;
+            best = cost;
+        }
+    }
     a.cols = (int)cols;
-    int64_t blocks = 0;
-    for (int i = 0; i < l.parts; i++) blocks += (l.splits[i] + cols - 1) / cols;
-    const dim3 grid((uint32_t)tiles, (uint32_t)blocks);
-    if (p.big) expand<4>(a, grid, st);
-    else expand<1>(a, grid, st);
+    a.blocks = (int)blocks;
+    if (p.big) expand(a, dim3((uint32_t)(tiles * blocks)), st);
+    else expand_few(a, dim3((uint32_t)tiles, (uint32_t)blocks), st);
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) {
         set_error_detail("lora launch: %s", hipGetErrorString(err));
