@@ -20,6 +20,8 @@ callers):
                                   attention over that cache
     LinearW8A8, GatedMLP, SparseMoE, LMHead, RMSNorm, RotaryEmbedding, GQAAttention
                                   and the weight helpers
+    AdapterBatch, LoRALinear      adapters on any of their linears, a row's own
+    Sampler                       the draw from LMHead's logits
     lora_plan, lora_add           each request's own low-rank adapter beside a linear
                                   (training/lora.py:14-170), all of a batch in one call
     sample                        a token a row of logits (sampler.py:20-87)
@@ -62,6 +64,7 @@ from .loader import checkpoint_info, load_fni8_checkpoint, load_fni8_state_dict 
 from .quant import quantize_int8_rowwise  # noqa: F401
 from .layers import (  # noqa: F401
     NF4_CODEBOOK,
+    AdapterBatch,
     GatedMLP,
     GeluAndMul,
     GQAAttention,
@@ -71,7 +74,9 @@ from .layers import (  # noqa: F401
     get_act_and_mul,
     LinearW8A8,
     LMHead,
+    LoRALinear,
     Qwen3MLP,
+    Sampler,
     SparseMoE,
     _dequant_weight,
     gate_up_weight,
@@ -89,4 +94,5 @@ __all__ = [
     "rmsnorm_quant", "RMSNorm", "SiluAndMul", "GeluAndMul", "get_act_and_mul", "gemm_w4a8",
     "gemm_quantized", "rope", "qk_norm_rope", "rope_append", "paged_attention", "PagedKVCache",
     "Step", "RotaryEmbedding", "GQAAttention", "LoraPlan", "lora_plan", "lora_add", "sample",
+    "AdapterBatch", "LoRALinear", "Sampler",
 ]

@@ -1,0 +1,151 @@
+"""Low-rank adapters of many requests beside a LinearW8A8 (the unmerged forward of
+fni8serve/training/lora.py:14-170, in serving: every token of a batch has its own adapter).
+
+    batch = AdapterBatch(num_adapters)                 one for the modules that see the same rows
+    mlp.down_proj = LoRALinear(mlp.down_proj, batch, rank=16)
+    mlp.down_proj.load(3, [(A, B)], scaling=alpha / rank)
+    batch.assign(ids)                                  once a step: each row's adapter, -1 none
+    y = mlp(x)
+
+A merged projection (QKV, gate and up) has one pair of matrices for each part of its output
+(splits).  The module takes the place of the linear that it wraps: GatedMLP, GQAAttention and
+LMHead call it as they call that.  GatedMLP then runs its projections one after the other, since
+the adapter reads what its fused kernels never write.  SparseMoE's experts are stacked at
+construction and take no adapters.
+"""
+from __future__ import annotations
+
+from collections.abc import Sequence
+
+import torch
+import torch.nn as nn
+
+from .. import ops
+from .linear import LinearW8A8
+
+
+class AdapterBatch:
+    """Which adapter each row of a step has, shared by all LoRALinear modules that see these rows
+    (an LMHead that sees the last token of each sequence needs one of its own)."""
+
+    def __init__(self, num_adapters: int):
+        if not 0 < num_adapters <= 65534:
+            raise ValueError(f"num_adapters {num_adapters} must be from 1 to 65534")
+        self.num_adapters = num_adapters
+        self.ids: torch.Tensor | None = None
+        self.plan: ops.LoraPlan | None = None
+
+    def assign(self, ids: torch.Tensor) -> None:
+        """ids int [rows]: each row's adapter, any number outside [0, num_adapters) for none.
+        The tensors of a plan for as many rows are filled anew, so that a captured graph that
+        reads them follows; nothing waits for the GPU."""
+        if ids.dim() != 1 or ids.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"ids must be int32 or int64 [rows] (got {ids.dtype}, "
+                             f"{tuple(ids.shape)})")
+        if not ids.is_cuda:
+            self.ids, self.plan = ids, None
+            return
+        plan = ops.lora_plan(ids, self.num_adapters)
+        old = self.plan
+        if old is not None and old.rows.shape == plan.rows.shape and old.rows.device == ids.device:
+            old.seg_off.copy_(plan.seg_off)
+            old.rows.copy_(plan.rows)
+        else:
+            self.plan = plan
+        self.ids = ids
+
+    def clear(self) -> None:
+        """No row has an adapter: the modules are the linears that they wrap."""
+        self.ids = self.plan = None
+
+
+class LoRALinear(nn.Module):
+    def __init__(self, base: LinearW8A8, batch: AdapterBatch, rank: int,
+                 splits: Sequence[int] | None = None):
+        """rank: the largest of any adapter; kept as the next multiple of 8, smaller ones are
+        filled with zeros.  splits: the widths of a merged projection's parts."""
+        super().__init__()
+        self.base, self.batch = base, batch
+        self.in_features, self.out_features = base.in_features, base.out_features
+        self.splits = [self.out_features] if splits is None else [int(n) for n in splits]
+        if sum(self.splits) != self.out_features or min(self.splits) < 1:
+            raise ValueError(f"splits {self.splits} do not add up to {self.out_features} outputs")
+        if not 0 < rank <= 256:
+            raise ValueError(f"rank {rank} must be from 1 to 256")
+        self.rank = -(-rank // 8) * 8
+        S, dev = batch.num_adapters, base.weight.data.device
+        zeros = lambda *s: torch.zeros(s, dtype=torch.float16, device=dev)  # noqa: E731
+        self.register_buffer("a", zeros(S, len(self.splits) * self.rank, self.in_features))
+        self.register_buffer("b", zeros(S, self.out_features, self.rank))
+        self.register_buffer("scaling", torch.zeros(S, device=dev))
+
+    # what callers read of the linear (layers/mlp.py, layers/attention.py)
+    @property
+    def weight(self):
+        return self.base.weight
+
+    @property
+    def bias(self):
+        return self.base.bias
+
+    def _int8_ok(self, x: torch.Tensor) -> bool:
+        """Its input is needed in 16 bits: the fused chains leave it to be called."""
+        return False
+
+    def load(self, slot: int, parts: Sequence[tuple[torch.Tensor, torch.Tensor] | None],
+             scaling: float = 1.0) -> None:
+        """Adapter `slot`: for each part of the output its (A [r, in], B [width, r]) with r up to
+        rank, or None for a part without one."""
+        if not 0 <= slot < self.batch.num_adapters:
+            raise ValueError(f"slot {slot} is not among {self.batch.num_adapters} adapters")
+        if len(parts) != len(self.splits):
+            raise ValueError(f"{len(parts)} pairs for {len(self.splits)} parts")
+        for pair, wide in zip(parts, self.splits):
+            if pair is not None:
+                r = pair[0].shape[0]
+                if r > self.rank or pair[0].shape != (r, self.in_features) \
+                        or pair[1].shape != (wide, r):
+                    raise ValueError(f"A {tuple(pair[0].shape)} and B {tuple(pair[1].shape)} do not "
+                                     f"fit {self.in_features} inputs, {wide} outputs and rank "
+                                     f"{self.rank}")
+        self.a[slot].zero_()
+        self.b[slot].zero_()
+        n = 0
+        for p, (pair, wide) in enumerate(zip(parts, self.splits)):
+            if pair is not None:
+                r = pair[0].shape[0]
+                self.a[slot, p * self.rank:p * self.rank + r].copy_(pair[0])
+                self.b[slot, n:n + wide, :r].copy_(pair[1])
+            n += wide
+        self.scaling[slot] = scaling
+
+    def unload(self, slot: int) -> None:
+        """Rows of this adapter get nothing added from now on."""
+        self.load(slot, [None] * len(self.splits), 0.0)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        y = self.base(x)
+        if self.batch.ids is None:
+            return y
+        if not x.is_cuda:
+            return self._on_host(x, y)
+        return ops.lora_add(y, x, self.a, self.b, self.batch.plan, scaling=self.scaling,
+                            splits=self.splits, out=y)
+
+    def _on_host(self, x: torch.Tensor, y: torch.Tensor) -> torch.Tensor:
+        """CPU tensors, beside the linear's own fallback: sums in 32 bits, rounded once."""
+        ids = self.batch.ids
+        x2, out = x.reshape(-1, self.in_features), y.reshape(-1, self.out_features).float()
+        if ids.is_cuda or ids.numel() != x2.shape[0]:
+            raise ValueError(f"{x2.shape[0]} rows on the host, {ids.numel()} ids on {ids.device}")
+        for e in range(self.batch.num_adapters):
+            at = (ids == e).nonzero().squeeze(1)
+            if at.numel():
+                low = (x2[at].float() @ self.a[e].float().t()) * self.scaling[e]
+                up, n = [], 0
+                for p, wide in enumerate(self.splits):
+                    up.append(low[:, p * self.rank:(p + 1) * self.rank]
+                              @ self.b[e, n:n + wide].float().t())
+                    n += wide
+                out[at] += torch.cat(up, 1)
+        return out.to(y.dtype).reshape(y.shape)

@@ -1,0 +1,85 @@
+"""AdapterBatch and LoRALinear on the CPU, and what they and Sampler refuse."""
+import pytest
+import torch
+
+
+def linear(pkg, out, inner, seed):
+    g = torch.Generator().manual_seed(seed)
+    q = torch.randint(-127, 128, (out, inner), generator=g, dtype=torch.int8)
+    return pkg.LinearW8A8(pkg.QTensor(q, torch.rand(out, generator=g) * 0.01, scheme="per_row_i8"))
+
+
+def pair(rank, inner, wide, seed):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(rank, inner, generator=g).half(),
+            (torch.randn(wide, rank, generator=g) * 0.1).half())
+
+
+def test_rows_get_their_own_adapter(pkg):
+    base, batch = linear(pkg, 40, 32, 1), pkg.AdapterBatch(4)
+    m = pkg.LoRALinear(base, batch, rank=6, splits=[24, 16])
+    assert (m.rank, m.in_features, m.out_features) == (8, 32, 40)
+    assert m.weight is base.weight and m.bias is base.bias
+    p0, p1 = pair(6, 32, 24, 2), pair(3, 32, 16, 3)
+    m.load(2, [p0, p1], scaling=0.5)
+    m.load(0, [None, pair(5, 32, 16, 4)], scaling=2.0)
+    x = torch.randn(5, 32).half()
+    plain = base(x)
+    assert torch.equal(m(x), plain)                      # no ids yet
+    batch.assign(torch.tensor([2, -1, 0, 4, 1]))
+    y = m(x)
+    assert torch.equal(y[[1, 3, 4]], plain[[1, 3, 4]])   # none, outside, an empty slot
+    want = plain[0].float() + 0.5 * torch.cat([(p0[1].float() @ (p0[0].float() @ x[0].float())),
+                                               (p1[1].float() @ (p1[0].float() @ x[0].float()))])
+    # sums of 32 products of a few units in 32 bits, then half a step of fp16
+    assert torch.allclose(y[0].float(), want, rtol=2.0 ** -11, atol=1e-4)
+    assert torch.equal(y[2, :24], plain[2, :24]) and not torch.equal(y[2, 24:], plain[2, 24:])
+    assert torch.equal(m(x.view(5, 1, 32)).view(5, 40), y)
+    m.unload(2)
+    assert torch.equal(m(x)[0], plain[0])
+    batch.clear()
+    assert torch.equal(m(x), plain)
+
+
+def test_refusals(pkg):
+    base, batch = linear(pkg, 40, 32, 1), pkg.AdapterBatch(4)
+    for n in (0, -1, 65535):
+        with pytest.raises(ValueError, match="num_adapters"):
+            pkg.AdapterBatch(n)
+    for kw in (dict(rank=0), dict(rank=257), dict(rank=8, splits=[20, 16]),
+               dict(rank=8, splits=[40, 0])):
+        with pytest.raises(ValueError):
+            pkg.LoRALinear(base, batch, **kw)
+    m = pkg.LoRALinear(base, batch, rank=8, splits=[24, 16])
+    good = [pair(8, 32, 24, 1), pair(8, 32, 16, 2)]
+    for slot, parts in ((4, good), (-1, good), (0, good[:1]), (0, [good[1], good[0]]),
+                        (0, [pair(9, 32, 24, 1), None]), (0, [pair(8, 31, 24, 1), None]),
+                        (0, [(good[0][0], good[0][1][:, :7]), None])):
+        with pytest.raises(ValueError):
+            m.load(slot, parts)
+    for ids in (torch.zeros(2, 2, dtype=torch.int32), torch.zeros(3)):
+        with pytest.raises(ValueError, match="ids"):
+            batch.assign(ids)
+    batch.assign(torch.tensor([0, 1]))
+    with pytest.raises(ValueError, match="rows"):
+        m(torch.zeros(3, 32).half())
+    with pytest.raises(ValueError, match="GPU"):
+        pkg.Sampler()(torch.zeros(3, 32).half())
+
+
+def test_the_mlp_calls_an_adapted_linear(pkg):
+    """GatedMLP on the CPU with both projections wrapped: the sum of its parts."""
+    up, down = linear(pkg, 48, 32, 1).weight, linear(pkg, 32, 24, 2).weight
+    mlp, batch = pkg.GatedMLP(up, down), pkg.AdapterBatch(2)
+    x = torch.randn(3, 32).half()
+    plain = mlp(x)
+    mlp.gate_up_proj = pkg.LoRALinear(mlp.gate_up_proj, batch, 8, splits=[24, 24])
+    mlp.down_proj = pkg.LoRALinear(mlp.down_proj, batch, 8)
+    assert torch.equal(mlp(x), plain)
+    mlp.gate_up_proj.load(1, [pair(8, 32, 24, 3), pair(4, 32, 24, 4)])
+    mlp.down_proj.load(1, [pair(8, 24, 32, 5)])
+    batch.assign(torch.tensor([1, -1, 0]))
+    y = mlp(x)
+    assert torch.equal(y[1:], plain[1:]) and not torch.equal(y[0], plain[0])
+    h = mlp.gate_up_proj(x)
+    assert torch.equal(mlp.down_proj(mlp.act_fn(h)), y)

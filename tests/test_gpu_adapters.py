@@ -1,0 +1,164 @@
+"""Adapters on the linears of an MLP, an attention layer and a head, and the draw from its logits,
+as a serving step runs them together."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+HIDDEN, INTER, HEADS, KV, DIM, VOCAB, RANK, SLOTS = 512, 1280, 8, 2, 64, 5003, 12, 6
+
+
+def qtensor(pkg, wl, out, inner, seed):
+    q, s = wl.weight_i8(out, inner, seed=seed)
+    return pkg.QTensor(q.cuda(), (s * 0.1).cuda(), scheme="per_row_i8")
+
+
+def fill(m, seed):
+    """Adapters in every slot but the last, of different ranks, one with a part left out."""
+    g = torch.Generator().manual_seed(seed)
+    for slot in range(SLOTS - 1):
+        r, parts = RANK - 2 * slot, []
+        for i, wide in enumerate(m.splits):
+            a = torch.randn(r, m.in_features, generator=g) * m.in_features ** -0.5
+            b = torch.randn(wide, r, generator=g) * 0.2
+            parts.append(None if slot == 1 and i == 0 else (a.half().cuda(), b.half().cuda()))
+        m.load(slot, parts, scaling=0.5 + 0.3 * slot)
+
+
+def wrap(pkg, linear, batch, seed, splits=None):
+    m = pkg.LoRALinear(linear, batch, RANK, splits=splits)
+    fill(m, seed)
+    return m
+
+
+def by_row(pkg, m, x, ids):
+    """The module's rows one by one, from its base and its matrices in 32 bits."""
+    y = m.base(x)
+    want = y.clone()
+    for t, e in enumerate(ids.tolist()):
+        if 0 <= e < SLOTS:
+            low, n = (m.a[e].float() @ x[t].float()) * m.scaling[e], 0
+            for p, wide in enumerate(m.splits):
+                up = m.b[e, n:n + wide].float() @ low[p * m.rank:(p + 1) * m.rank]
+                want[t, n:n + wide] = (y[t, n:n + wide].float() + up).half()
+                n += wide
+    return want
+
+
+def close(got, want):
+    """Two sums in 32 bits in different orders, each rounded to fp16: a step of fp16 apart at most
+    (twice half a step, 2^-10 of the value), and 2^-12 for sums of terms of a few units that
+    cancel (1e3 products of 2^-24 each)."""
+    return bool(((got.float() - want.float()).abs() <= 2.0 ** -10 * want.float().abs() + 2.0 ** -12).all())
+
+
+def test_modules_match_their_parts(pkg, wl, cuda):
+    batch = pkg.AdapterBatch(SLOTS)
+    for rows in (1, 7, 70):
+        ids = torch.arange(rows) % (SLOTS + 1) - 1
+        batch.assign(ids.cuda())
+        x = wl.activations(rows, HIDDEN, seed=rows).cuda()
+        m = wrap(pkg, pkg.LinearW8A8(qtensor(pkg, wl, 768, HIDDEN, 1)), batch, 2, [512, 128, 128])
+        got = m(x)
+        assert close(got, by_row(pkg, m, x, ids))
+        assert torch.equal(got[ids < 0], m.base(x)[ids < 0])
+        host = pkg.LoRALinear(pkg.LinearW8A8(m.weight), pkg.AdapterBatch(SLOTS), RANK)
+        assert host.a.is_cuda
+        mlp = pkg.GatedMLP(qtensor(pkg, wl, 2 * INTER, HIDDEN, 3), qtensor(pkg, wl, HIDDEN, INTER, 4))
+        mlp.gate_up_proj = wrap(pkg, mlp.gate_up_proj, batch, 5, [INTER, INTER])
+        mlp.down_proj = wrap(pkg, mlp.down_proj, batch, 6)
+        h = mlp.act_fn(mlp.gate_up_proj(x))
+        assert torch.equal(mlp(x), mlp.down_proj(h))
+        assert close(mlp.down_proj(h), by_row(pkg, mlp.down_proj, h, ids))
+    with pytest.raises(ValueError, match="rows"):
+        m(wl.activations(3, HIDDEN, seed=1).cuda())
+    batch.clear()
+    assert torch.equal(m(x), m.base(x))
+
+
+class Layer:
+    """Attention, MLP, head and sampler over one decoded token a sequence."""
+
+    def __init__(self, pkg, wl, batch):
+        rot = pkg.RotaryEmbedding(DIM, 256, device="cuda")
+        self.attn = pkg.GQAAttention(qtensor(pkg, wl, (HEADS + 2 * KV) * DIM, HIDDEN, 1),
+                                     qtensor(pkg, wl, HIDDEN, HEADS * DIM, 2), HEADS, KV, DIM, rot)
+        self.attn.qkv_proj = wrap(pkg, self.attn.qkv_proj, batch, 3,
+                                  [HEADS * DIM, KV * DIM, KV * DIM])
+        self.attn.o_proj = wrap(pkg, self.attn.o_proj, batch, 4)
+        self.mlp = pkg.GatedMLP(qtensor(pkg, wl, 2 * INTER, HIDDEN, 5),
+                                qtensor(pkg, wl, HIDDEN, INTER, 6))
+        self.mlp.gate_up_proj = wrap(pkg, self.mlp.gate_up_proj, batch, 7, [INTER, INTER])
+        self.mlp.down_proj = wrap(pkg, self.mlp.down_proj, batch, 8)
+        self.head = pkg.LMHead(qtensor(pkg, wl, VOCAB, HIDDEN, 9))
+        self.head.proj = wrap(pkg, self.head.proj, batch, 10)
+        self.sampler = pkg.Sampler(return_logprobs=True)
+
+    def __call__(self, x, cache, step, settings, u):
+        h = x + self.attn(x, cache, step)
+        h = h + self.mlp(h)
+        return self.sampler(self.head(h), *settings, u=u)
+
+
+@pytest.mark.parametrize("seqs", [1, 5, 24])
+def test_a_decode_step_in_a_graph(pkg, wl, cuda, seqs):
+    """Replays with new tokens, adapters, settings and random numbers, each against the eager
+    step."""
+    batch = pkg.AdapterBatch(SLOTS)
+    layer = Layer(pkg, wl, batch)
+    cache = pkg.PagedKVCache(2 * seqs, 16, KV, DIM)
+    tables = torch.arange(2 * seqs, dtype=torch.int32).view(seqs, 2)
+    steps = [cache.step(tables, new=[1] * seqs, total=[n] * seqs) for n in range(1, 8)]
+    step = cache.step(tables, new=[1] * seqs, total=[1] * seqs)
+    g = torch.Generator().manual_seed(seqs)
+    x = wl.activations(seqs, HIDDEN, seed=3).cuda()
+    u = torch.rand(seqs, device="cuda")
+    kinds = (torch.float32, torch.int32, torch.float32, torch.float32)
+    settings = [torch.zeros(seqs, dtype=t, device="cuda") for t in kinds]
+    batch.assign(torch.zeros(seqs, dtype=torch.int32, device="cuda"))
+
+    def renew(n):
+        x.copy_(wl.activations(seqs, HIDDEN, seed=50 + n))
+        u.copy_(torch.rand(seqs, generator=g))
+        batch.assign(torch.randint(-1, SLOTS, (seqs,), generator=g).cuda())
+        for t, v in zip(settings, ((0.0, 0.7, 1.0, 1.4), (0, 5, 40, 0), (1.0, 0.9, 0.5, 1.0),
+                                   (0.0, 0.0, 0.1, 0.02))):
+            pick = torch.randint(0, 4, (seqs,), generator=g)
+            t.copy_(torch.tensor(v)[pick].to(t.dtype))
+        for f in ("positions", "slots", "block_tables", "context_lens", "cu_seqlens"):
+            old, new = getattr(step, f), getattr(steps[n], f)
+            if old is not None:
+                old.copy_(new)
+
+    renew(0)
+    layer(x, cache, step, settings, u)                   # first calls outside the capture
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        token, logp = layer(x, cache, step, settings, u)
+    for n in range(6):
+        renew(n)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = (token.clone(), logp.clone())
+        want = layer(x, cache, step, settings, u)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), n
+        assert ((got[0] >= 0) & (got[0] < VOCAB)).all()
+
+
+def test_adapters_change_what_is_drawn(pkg, wl, cuda):
+    batch = pkg.AdapterBatch(SLOTS)
+    head = pkg.LMHead(qtensor(pkg, wl, VOCAB, HIDDEN, 9), logit_softcap=30.0)
+    head.proj = wrap(pkg, head.proj, batch, 10)
+    x = wl.activations(32, HIDDEN, seed=1).cuda()
+    greedy = pkg.Sampler()
+    plain = greedy(head(x), temperature=0.0)             # soft-capped logits are fp32
+    assert torch.equal(plain, head(x).argmax(-1))
+    batch.assign(torch.tensor([-1, 0] * 16, device="cuda"))
+    drawn = greedy(head(x), temperature=0.0)
+    assert torch.equal(drawn[::2], plain[::2]) and not torch.equal(drawn[1::2], plain[1::2])
+    torch.manual_seed(0)
+    one = greedy(head(x), top_k=50)
+    torch.manual_seed(0)
+    assert torch.equal(one, greedy(head(x), top_k=50))
