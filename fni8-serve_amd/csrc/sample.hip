@@ -92,6 +92,12 @@ __device__ __forceinline__ E lowest_of() {  // minus infinity
     else return -__builtin_inff();
 }
 
+template <class E>
+__device__ __forceinline__ E element(float v) {  // of a value that has one
+    if constexpr (sizeof(E) == 2) return fni8::f2h(v);
+    else return v;
+}
+
 // Eight logits from index i on, -inf past the row's end.  Rows need no more than their
 // elements' alignment: the loads are as wide at any address.
 template <class E>
@@ -224,37 +230,48 @@ __device__ __forceinline__ Work work_of(int8_t* w, int64_t row, int64_t V) {
     return r;
 }
 
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
-    return v;
+__device__ __forceinline__ uint32_t key_max(uint32_t key) {
+    return fni8::wave_max_uniform(key ^ 0x80000000u) ^ 0x80000000u;  // of signed numbers
 }
-__device__ __forceinline__ u64 wave_sum(u64 v) {
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
-    return v;
-}
-__device__ __forceinline__ float wave_sum_f32(float v) {
-    auto add = [&](int o) { v += __builtin_bit_cast(float, o); };
-    add(fni8::dpp<fni8::kDppXor1>(__builtin_bit_cast(int, v)));
-    add(fni8::dpp<fni8::kDppXor2>(__builtin_bit_cast(int, v)));
-    add(fni8::dpp<fni8::kDppHalfMirror>(__builtin_bit_cast(int, v)));
-    add(fni8::dpp<fni8::kDppMirror>(__builtin_bit_cast(int, v)));
-    const int b = __builtin_bit_cast(int, v);
-    float sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 64; i += 16)
-        sum += __builtin_bit_cast(float, __builtin_amdgcn_readlane(b, i));
-    return sum;
+
+// The value of the lane that a step of a running sum over the lanes adds (0 where there is none),
+// by data movement within the vector unit: a round trip through LDS takes ten times as long.
+template <int CTRL, int ROWS, class N>
+__device__ __forceinline__ N moved(N v) {
+    if constexpr (sizeof(N) == 8) {
+        u32x2 w = __builtin_bit_cast(u32x2, v);
+        w.x = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w.x, CTRL, ROWS, 0xf, false);
+        w.y = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w.y, CTRL, ROWS, 0xf, false);
+        return __builtin_bit_cast(N, w);
+    } else {
+        return __builtin_bit_cast(
+            N, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+    }
 }
 template <class N>
-__device__ __forceinline__ N wave_scan(N v, int lane) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const N o = __shfl_up(v, d, 64);
-        if (lane >= d) v += o;
-    }
+__device__ __forceinline__ N wave_scan(N v) {
+    v += moved<0x111, 0xf>(v);  // row_shr:1, within rows of 16 lanes
+    v += moved<0x112, 0xf>(v);
+    v += moved<0x114, 0xf>(v);
+    v += moved<0x118, 0xf>(v);
+    v += moved<0x142, 0xa>(v);  // row_bcast:15, a row's end to the next
+    v += moved<0x143, 0xc>(v);  // row_bcast:31
     return v;
+}
+template <class N>
+__device__ __forceinline__ N last_lane(N v) {
+    if constexpr (sizeof(N) == 8) {
+        u32x2 w = __builtin_bit_cast(u32x2, v);
+        w.x = (uint32_t)__builtin_amdgcn_readlane((int)w.x, 63);
+        w.y = (uint32_t)__builtin_amdgcn_readlane((int)w.y, 63);
+        return __builtin_bit_cast(N, w);
+    } else {
+        return __builtin_bit_cast(N, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+    }
+}
+template <class N>
+__device__ __forceinline__ N wave_sum(N v) {
+    return last_lane(wave_scan(v));
 }
 
 // An item is a part of a row; a workgroup walks items, the loads of the next on their way while
@@ -307,7 +324,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_kernel(const fni8h::Sample 
         if (item + step < items) fetch(item + step);
         uint32_t best = nan ? 0xffffffffu : key_of(most);
         w.top[part * kScanThreads + tid] = best;
-        best = fni8::wave_max_u32(best);
+        best = key_max(best);
         if (lane == 0) tops[turn][wave] = best;
         Row r(a, row, V);
         __syncthreads();
@@ -397,7 +414,7 @@ __device__ __forceinline__ u64 block_sum(Shared& sh, Turn& turn, u64 v) {
 template <class N>
 __device__ __forceinline__ N block_scan(N (&rows)[2][kWaves], Turn& turn, N v, N& all) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = turn.next();
-    v = wave_scan(v, lane);
+    v = wave_scan(v);
     if (lane == 63) rows[row][wave] = v;
     __syncthreads();
     N before = 0;
@@ -432,8 +449,8 @@ __device__ __forceinline__ uint32_t find_key(Shared& sh, int n, u64& need, K key
         if (threadIdx.x < 64) {
             const int b = 255 - 4 * (int)threadIdx.x;
             const u64 h0 = sh.h.hist[b], h1 = sh.h.hist[b - 1], h2 = sh.h.hist[b - 2], h3 = sh.h.hist[b - 3];
-            u64 run = wave_scan(h0 + h1 + h2 + h3, (int)threadIdx.x);
-            const u64 all = __shfl(run, 63, 64);
+            u64 run = wave_scan(h0 + h1 + h2 + h3);
+            const u64 all = last_lane(run);
             if (need > all) need = all;
             const u64 r3 = run - h3, r2 = r3 - h2, r1 = r2 - h1, r0 = r1 - h0;
             if (r0 < need && run >= need) {
@@ -778,7 +795,7 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, i
     const uint32_t own = tid < parts ? w.part[tid] : 0;
     const double own_sum = tid < parts ? w.sum[tid] : 0.0;  // used where the row is summed
     Row r(a, row, V);
-    uint32_t best = fni8::wave_max_u32(own);
+    uint32_t best = key_max(own);
     if (lane == 0) sh.counts[wave] = (int)best;
     __syncthreads();
 #pragma unroll
@@ -952,14 +969,14 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, i
                     sum += b[j] <= mid ? m[j] : 0.0f;
                 }
                 bool there = count >= want;
-                if (whole && !there) there = wave_sum_f32(sum) >= goal;
+                if (whole && !there) there = wave_sum(sum) >= goal;
                 if (there) hi = mid;
                 else lo = mid + 1;
             }
             float sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < B; j++) sum += b[j] <= lo ? m[j] : 0.0f;
-            sum = wave_sum_f32(sum);
+            sum = wave_sum(sum);
             // the list has more than these maxima: it is tried unless they are far from the mass
             if (lane == 0) sh.bin = whole && lo < least && 4.0f * sum < goal ? -1 : lo;
         }
@@ -1108,19 +1125,20 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, i
 }
 
 // One part of a row with a long prefix: the mass of what is kept for certain, and the tokens
-// around the end of top-p.  Each wave first packs the logits that matter (down to `low`) into its
-// LDS, so that their exponentials, 25 operations of 64 bits, are not computed for the others.
+// around the end of top-p.  Each wave first lists the logits of its 2048 that matter (down to
+// `low`), so that their exponentials, 20 operations of 64 bits, are not computed for the others
+// (256 rows of 151936, top-p 0.95, a fifth of the logits kept: 56 us with all of them).
 template <class E>
 __global__ __launch_bounds__(kScanThreads) void gather_kernel(const fni8h::Sample a, int parts) {
-    constexpr int W = 64 * kVec;  // logits of a wave's load
-    __shared__ float packed[4][W];
-    __shared__ uint16_t where[4][W];
+    constexpr int W = 64 * kVec * kSteps, AROUND = 256;  // logits of a wave; of them around the end
+    __shared__ E logit[4][W];
+    __shared__ uint16_t listed[4][W];
+    __shared__ u64 orders[4][AROUND];
     __shared__ u64 sums[4];
     __shared__ uint32_t tops[4];
     const int items = (int)a.B * parts, V = (int)a.V;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const u64 below = ((u64)1 << lane) - 1;
     for (int item = blockIdx.x; item < items; item += gridDim.x) {
         const int row = item / parts, part = item - row * parts;
         const Work w = work_of(a.work, row, V);
@@ -1129,63 +1147,74 @@ __global__ __launch_bounds__(kScanThreads) void gather_kernel(const fni8h::Sampl
         const E* x = (const E*)a.logits + (int64_t)row * a.ld;
         Row r(a, row, V);
         float v[kSteps][kVec];
+        const int i0 = part * kPart + wave * 64 * kVec;  // of the wave's first load
 #pragma unroll
         for (int i = 0; i < kSteps; i++)
-            load8(x, part * kPart + (i * kScanThreads + tid) * kVec, V, v[i]);
+            load8(x, i0 + (i * kScanThreads + lane) * kVec, V, v[i]);
         uint32_t best = 0;
         for (int i = tid; i < parts; i += kScanThreads) best = w.part[i] > best ? w.part[i] : best;
-        best = fni8::wave_max_u32(best);
+        best = key_max(best);
         if (lane == 0) tops[wave] = best;
         __syncthreads();
         for (int i = 0; i < 4; i++) best = tops[i] > best ? tops[i] : best;
         r.largest(value_of(best));
+        if (r.inf) {
+#pragma unroll
+            for (int i = 0; i < kSteps; i++)
+#pragma unroll
+                for (int j = 0; j < kVec; j++) v[i][j] = r.seen(v[i][j]);
+        }
         const u64 floor = more.kind == kMinP ? r.floor() : 0;
         const float high = more.kind == kMinP ? -__builtin_inff() : more.high;
         const float low = __builtin_fmaxf(more.low, -0x1.fffffep127f);
-        int around = 0;  // of the wave
+        int n = 0;
 #pragma unroll
         for (int i = 0; i < kSteps; i++)
 #pragma unroll
             for (int j = 0; j < kVec; j++) {
-                v[i][j] = r.seen(v[i][j]);
-                around += __builtin_popcountll(__ballot(v[i][j] >= low && v[i][j] < high));
-            }
-        int to = 0;
-        if (around && lane == 0) to = atomicAdd(&w.more->around, around);
-        u64 sum = 0;
-#pragma unroll
-        for (int i = 0; i < kSteps; i++) {
-            int n = 0;
-#pragma unroll
-            for (int j = 0; j < kVec; j++) {
+                const int mine = (i * 64 + lane) * kVec + j;
+                logit[wave][mine] = element<E>(v[i][j]);
                 const u64 has = __ballot(v[i][j] >= low);
                 if (v[i][j] >= low) {
-                    const int at = n + __builtin_popcountll(has & below);
-                    packed[wave][at] = v[i][j];
-                    where[wave][at] = (uint16_t)(lane * kVec + j);
+                    const int before = __builtin_amdgcn_mbcnt_hi(
+                        (uint32_t)(has >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)has, n));
+                    listed[wave][before] = (uint16_t)mine;
                 }
                 n += __builtin_popcountll(has);
             }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            for (int t = lane; t < n; t += 64) {
-                const float q = packed[wave][t];
-                const u64 m = r.mass(q);
-                const bool certain = q >= high;
-                sum += certain && m >= floor ? m : 0;
-                if (!around) continue;
-                const u64 has = __ballot(!certain);
-                const int base = __builtin_amdgcn_readfirstlane(to);  // of lane 0
-                const int at = base + __builtin_popcountll(has & below);
-                if (!certain && at < around_of(V)) {
-                    const int index = part * kPart + (i * kScanThreads + wave * 64) * kVec +
-                                      where[wave][t];
-                    w.around[at] = (u64)key_of(q) << 32 | (uint32_t)~index;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        u64 sum = 0;
+        int around = 0;
+        for (int t0 = 0; t0 < n; t0 += 64) {
+            const bool live = t0 + lane < n;
+            const int mine = listed[wave][live ? t0 + lane : 0];
+            const float q = value(logit[wave][mine]);
+            const u64 m = r.mass(q);
+            const bool certain = live && q >= high;
+            sum += certain && m >= floor ? m : 0;
+            const u64 has = __ballot(live && !certain);
+            if (has) {
+                const int at = __builtin_amdgcn_mbcnt_hi(
+                    (uint32_t)(has >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)has, around));
+                if (live && !certain && at < AROUND) {
+                    const int index = i0 + (mine / (64 * kVec)) * kScanThreads * kVec +
+                                      mine % (64 * kVec);
+                    orders[wave][at] = (u64)key_of(q) << 32 | (uint32_t)~index;
                 }
-                to = base + __builtin_popcountll(has);
+                around += __builtin_popcountll(has);
             }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
         sum = wave_sum(sum);
+        if (around) {
+            // more than there is room for: the count tells finish, which searches the whole row
+            int at = 0;
+            if (lane == 0) at = atomicAdd(&w.more->around, around <= AROUND ? around : kAround + 1);
+            at = __builtin_amdgcn_readfirstlane(at);
+            const int room = around_of(V);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            for (int t = lane; t < around && around <= AROUND && at + t < room; t += 64)
+                w.around[at + t] = orders[wave][t];
+        }
         if (lane == 0) sums[wave] = sum;
         __syncthreads();
         if (tid == 0) w.above[part] = sums[0] + sums[1] + sums[2] + sums[3];
@@ -1206,7 +1235,7 @@ __global__ __launch_bounds__(kThreads) void finish_kernel(const fni8h::Sample a,
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     Row r(a, row, V);
     const uint32_t own = tid < parts ? w.part[tid] : 0;
-    uint32_t best = fni8::wave_max_u32(own);
+    uint32_t best = key_max(own);
     if (lane == 0) sh.counts[wave] = (int)best;
     __syncthreads();
 #pragma unroll
@@ -1222,6 +1251,7 @@ __global__ __launch_bounds__(kThreads) void finish_kernel(const fni8h::Sample a,
         found = true;
         if (more.kind == kTopP) {
             // the end of top-p in the list: a step of weight, then the tokens of that step
+            constexpr int HELD = kAround / kThreads;
             const u64 certain = block_sum(sh, turn, mine);
             const int n = more.around;
             found = certain < more.need && n <= around_of(V);
@@ -1235,22 +1265,30 @@ __global__ __launch_bounds__(kThreads) void finish_kernel(const fni8h::Sample a,
                     return d < (double)(kBins - 1) ? (int)d : kBins - 1;
                 };
                 auto logit = [](u64 order) { return value_of((uint32_t)(order >> 32)); };
+                u64 order[HELD], m[HELD];  // the list: read once, weighed once
+#pragma unroll
+                for (int j = 0; j < HELD; j++)
+                    if (j * kThreads < n)
+                        order[j] = tid + j * kThreads < n ? w.around[tid + j * kThreads] : 0;
                 clear_bins(sh);
-                for (int i = tid; i < n; i += kThreads) {
-                    const float v = logit(w.around[i]);
-                    atomicAdd(&sh.h.mass[bin(r.power(v))], r.mass(v));
-                }
+#pragma unroll
+                for (int j = 0; j < HELD; j++)
+                    if (j * kThreads < n) {
+                        const float v = logit(order[j]);
+                        m[j] = order[j] ? r.mass(v) : 0;
+                        if (m[j]) atomicAdd(&sh.h.mass[bin(r.power(v))], m[j]);
+                    }
                 if (tid == 0) sh.n = 0;
                 __syncthreads();
                 u64 need = more.need - certain;
                 const u64 wanted = need;
                 const int b = find_bin(sh, turn, need);
-                for (int i = tid; i < n; i += kThreads) {
-                    const u64 order = w.around[i];
-                    if (bin(r.power(logit(order))) != b) continue;
-                    const int at = atomicAdd(&sh.n, 1);
-                    if (at < kList) sh.list[at] = {order, r.mass(logit(order))};
-                }
+#pragma unroll
+                for (int j = 0; j < HELD; j++)
+                    if (j * kThreads < n && m[j] && bin(r.power(logit(order[j]))) == b) {
+                        const int at = atomicAdd(&sh.n, 1);
+                        if (at < kList) sh.list[at] = {order[j], m[j]};
+                    }
                 __syncthreads();
                 const int few = sh.n;
                 found = few <= kList && sh.all >= wanted;
@@ -1266,13 +1304,23 @@ __global__ __launch_bounds__(kThreads) void finish_kernel(const fni8h::Sample a,
                 __syncthreads();
                 sh.above[tid] = mine;
                 __syncthreads();
-                if (found)
-                    for (int i = tid; i < n; i += kThreads) {
-                        const u64 order = w.around[i];
-                        const int index = (int)~(uint32_t)order;
-                        if (c.keeps((uint32_t)(order >> 32), index))
-                            atomicAdd(&sh.above[index / kPart], r.mass(logit(order)));
-                    }
+                if (found) {
+#pragma unroll
+                    for (int j = 0; j < HELD; j++)
+                        if (j * kThreads < n) {
+                            // neighbours in the list are of one part, or of a few: a sum for each
+                            const int index = (int)~(uint32_t)order[j];
+                            const bool keep = m[j] && c.keeps((uint32_t)(order[j] >> 32), index);
+                            const int part = index / kPart;
+                            for (u64 left = __ballot(keep); left;) {
+                                const int p = __builtin_amdgcn_readlane(part, __builtin_ctzll(left));
+                                const u64 same = __ballot(keep && part == p);
+                                const u64 some = wave_sum(keep && part == p ? m[j] : 0);
+                                if (lane == 0) atomicAdd(&sh.above[p], some);
+                                left &= ~same;
+                            }
+                        }
+                }
                 __syncthreads();
                 mine = sh.above[tid];
             }
