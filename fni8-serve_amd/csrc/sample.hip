@@ -28,6 +28,8 @@
 // A row whose list does not fit (thousands of equal logits, top-k of thousands) is searched whole
 // by its workgroup: a histogram of its mass in 2048 steps of weight, then the list of one step.
 // Nothing depends on the number of rows: a row's token is the same in every batch.
+#include <type_traits>
+
 #include "common.h"
 
 namespace {
@@ -48,22 +50,20 @@ constexpr int kAround = 8192;  // tokens around a row's end of top-p, in the wor
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 // 2^(d rate + s) for -1000 <= d rate <= 0.  d rate = n + f, |f| <= 1/2, by the addition that
-// leaves n + s in the low bits; 2^f = 1 + f q(f), q the polynomial of degree 9 through
-// (2^f - 1) / f at the Chebyshev nodes (error below 2^-50 of the value; exactly 1 at 0); n + s
-// goes into the exponent.
+// leaves n + s in the low bits; 2^f = 1 + f q(f), q the polynomial of degree 7 through
+// (2^f - 1) / f at the Chebyshev nodes (exactly 1 at 0, else off by 2.2e-12 of the value at
+// most; a row of 151936 equal shares has 6.6e-6 for each); n + s goes into the exponent.
 __device__ __forceinline__ double exp2_at(double d, double rate, int s) {
     const double magic = 0x1.8p52 + s, tn = __builtin_fma(d, rate, magic);
     const double f = __builtin_fma(d, rate, -(tn - magic));
-    double q = 7.070977866508138e-09;
-    q = __builtin_fma(q, f, 1.0205905413765595e-07);
-    q = __builtin_fma(q, f, 1.3215451633221434e-06);
-    q = __builtin_fma(q, f, 1.5252672924850737e-05);
-    q = __builtin_fma(q, f, 1.5403530424776529e-04);
-    q = __builtin_fma(q, f, 1.3333558200794592e-03);
-    q = __builtin_fma(q, f, 9.618129107618665e-03);
-    q = __builtin_fma(q, f, 5.550410866465167e-02);
-    q = __builtin_fma(q, f, 0.24022650695910075);
-    q = __builtin_fma(q, f, 0.6931471805599462);
+    double q = 1.325080551750225e-06;
+    q = __builtin_fma(q, f, 1.5303700711365693e-05);
+    q = __builtin_fma(q, f, 1.5403475186530786e-04);
+    q = __builtin_fma(q, f, 1.3333478473685416e-03);
+    q = __builtin_fma(q, f, 9.61812913523614e-03);
+    q = __builtin_fma(q, f, 5.5504109063258665e-02);
+    q = __builtin_fma(q, f, 0.24022650695888503);
+    q = __builtin_fma(q, f, 0.6931471805568324);
     q = __builtin_fma(q, f, 1.0);
     u32x2 b = __builtin_bit_cast(u32x2, q);
     const u32x2 n = __builtin_bit_cast(u32x2, tn);
@@ -279,6 +279,9 @@ __device__ __forceinline__ N wave_sum(N v) {
 template <class E>
 __global__ __launch_bounds__(kScanThreads) void scan_kernel(const fni8h::Sample a, int parts) {
     typedef E vec __attribute__((ext_vector_type(8), aligned(sizeof(E))));
+    // maxima keep a NaN, and take two or three 16-bit numbers an operation
+    typedef std::conditional_t<sizeof(E) == 2, _Float16, float> number
+        __attribute__((ext_vector_type(8)));
     __shared__ uint32_t tops[2][4];
     __shared__ double sums[2][4];
     const int V = (int)a.V, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -310,19 +313,22 @@ __global__ __launch_bounds__(kScanThreads) void scan_kernel(const fni8h::Sample 
         const int row = item / parts, part = item - row * parts;
         const Work w = work_of(a.work, row, V);
         float v[kSteps][kVec];
-        float most = -__builtin_inff();
-        bool nan = false;
+        number many = __builtin_bit_cast(number, next[0]);
+#pragma unroll
+        for (int i = 1; i < kSteps; i++)
+            many = __builtin_elementwise_maximum(many, __builtin_bit_cast(number, next[i]));
 #pragma unroll
         for (int i = 0; i < kSteps; i++)
 #pragma unroll
             for (int j = 0; j < kVec; j++) {
                 const E e = next[i][j];
                 v[i][j] = value(e);
-                nan |= v[i][j] != v[i][j];
-                most = __builtin_fmaxf(most, v[i][j]);
             }
         if (item + step < items) fetch(item + step);
-        uint32_t best = nan ? 0xffffffffu : key_of(most);
+        auto most = many[0];
+#pragma unroll
+        for (int j = 1; j < kVec; j++) most = __builtin_elementwise_maximum(most, many[j]);
+        uint32_t best = key_of((float)most);
         w.top[part * kScanThreads + tid] = best;
         best = key_max(best);
         if (lane == 0) tops[turn][wave] = best;
@@ -977,8 +983,8 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, i
 #pragma unroll
             for (int j = 0; j < B; j++) sum += b[j] <= lo ? m[j] : 0.0f;
             sum = wave_sum(sum);
-            // the list has more than these maxima: it is tried unless they are far from the mass
-            if (lane == 0) sh.bin = whole && lo < least && 4.0f * sum < goal ? -1 : lo;
+            // the list has some more than these maxima: it is tried unless they are far from the mass
+            if (lane == 0) sh.bin = whole && lo < least && 2.0f * sum < goal ? -1 : lo;
         }
         __syncthreads();
         bound = sh.bin;
@@ -1131,7 +1137,7 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, i
 template <class E>
 __global__ __launch_bounds__(kScanThreads) void gather_kernel(const fni8h::Sample a, int parts) {
     constexpr int W = 64 * kVec * kSteps, AROUND = 256;  // logits of a wave; of them around the end
-    __shared__ E logit[4][W];
+    __shared__ __attribute__((aligned(16))) E logit[4][W];
     __shared__ uint16_t listed[4][W];
     __shared__ u64 orders[4][AROUND];
     __shared__ u64 sums[4];
@@ -1167,21 +1173,23 @@ __global__ __launch_bounds__(kScanThreads) void gather_kernel(const fni8h::Sampl
         const u64 floor = more.kind == kMinP ? r.floor() : 0;
         const float high = more.kind == kMinP ? -__builtin_inff() : more.high;
         const float low = __builtin_fmaxf(more.low, -0x1.fffffep127f);
-        int n = 0;
+        uint32_t bits = 0;  // this lane's that matter
 #pragma unroll
-        for (int i = 0; i < kSteps; i++)
+        for (int i = 0; i < kSteps; i++) {
+            typedef E run __attribute__((ext_vector_type(8)));
+            run q;
 #pragma unroll
             for (int j = 0; j < kVec; j++) {
-                const int mine = (i * 64 + lane) * kVec + j;
-                logit[wave][mine] = element<E>(v[i][j]);
-                const u64 has = __ballot(v[i][j] >= low);
-                if (v[i][j] >= low) {
-                    const int before = __builtin_amdgcn_mbcnt_hi(
-                        (uint32_t)(has >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)has, n));
-                    listed[wave][before] = (uint16_t)mine;
-                }
-                n += __builtin_popcountll(has);
+                q[j] = element<E>(v[i][j]);
+                bits |= (uint32_t)(v[i][j] >= low) << (i * kVec + j);
             }
+            *reinterpret_cast<run*>(&logit[wave][(i * 64 + lane) * kVec]) = q;
+        }
+        const int some = __builtin_popcount(bits), upto = wave_scan(some), n = last_lane(upto);
+        for (int at = upto - some; bits; bits &= bits - 1, at++) {
+            const int b = __builtin_ctz(bits);
+            listed[wave][at] = (uint16_t)((b / kVec * 64 + lane) * kVec + b % kVec);
+        }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         u64 sum = 0;
         int around = 0;
