@@ -1136,10 +1136,8 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, i
 // (256 rows of 151936, top-p 0.95, a fifth of the logits kept: 56 us with all of them).
 template <class E>
 __global__ __launch_bounds__(kScanThreads) void gather_kernel(const fni8h::Sample a, int parts) {
-    constexpr int W = 64 * kVec * kSteps, AROUND = 256;  // logits of a wave; of them around the end
-    __shared__ __attribute__((aligned(16))) E logit[4][W];
-    __shared__ uint16_t listed[4][W];
-    __shared__ u64 orders[4][AROUND];
+    constexpr int W = 64 * kVec * kSteps;  // logits of a wave
+    __shared__ E logit[4][W];
     __shared__ u64 sums[4];
     __shared__ uint32_t tops[4];
     const int items = (int)a.B * parts, V = (int)a.V;
@@ -1171,57 +1169,45 @@ __global__ __launch_bounds__(kScanThreads) void gather_kernel(const fni8h::Sampl
                 for (int j = 0; j < kVec; j++) v[i][j] = r.seen(v[i][j]);
         }
         const u64 floor = more.kind == kMinP ? r.floor() : 0;
-        const float high = more.kind == kMinP ? -__builtin_inff() : more.high;
         const float low = __builtin_fmaxf(more.low, -0x1.fffffep127f);
-        uint32_t bits = 0;  // this lane's that matter
+        const float high = more.kind == kMinP ? low : __builtin_fmaxf(more.high, low);
+        uint32_t sure = 0, near = 0;  // this lane's, kept for certain and around the end
 #pragma unroll
-        for (int i = 0; i < kSteps; i++) {
-            typedef E run __attribute__((ext_vector_type(8)));
-            run q;
+        for (int i = 0; i < kSteps; i++)
 #pragma unroll
             for (int j = 0; j < kVec; j++) {
-                q[j] = element<E>(v[i][j]);
-                bits |= (uint32_t)(v[i][j] >= low) << (i * kVec + j);
+                sure |= (uint32_t)(v[i][j] >= high) << (i * kVec + j);
+                near |= (uint32_t)(v[i][j] >= low) << (i * kVec + j);
             }
-            *reinterpret_cast<run*>(&logit[wave][(i * 64 + lane) * kVec]) = q;
-        }
-        const int some = __builtin_popcount(bits), upto = wave_scan(some), n = last_lane(upto);
-        for (int at = upto - some; bits; bits &= bits - 1, at++) {
-            const int b = __builtin_ctz(bits);
-            listed[wave][at] = (uint16_t)((b / kVec * 64 + lane) * kVec + b % kVec);
-        }
+        near &= ~sure;
+        const int some = __builtin_popcount(sure) | __builtin_popcount(near) << 16;
+        const int upto = wave_scan(some), counts = last_lane(upto);
+        const int n = counts & 0xffff, around = counts >> 16;
+        // where there is no room for them the count tells finish, which searches the whole row
+        int first = 0;  // on its way while the sums are made
+        if (around && lane == 0) first = atomicAdd(&w.more->around, around);
+        int at = (upto - some) & 0xffff;
+#pragma unroll
+        for (int i = 0; i < kSteps; i++)
+#pragma unroll
+            for (int j = 0; j < kVec; j++)
+                if (v[i][j] >= high) logit[wave][at++] = element<E>(v[i][j]);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         u64 sum = 0;
-        int around = 0;
-        for (int t0 = 0; t0 < n; t0 += 64) {
-            const bool live = t0 + lane < n;
-            const int mine = listed[wave][live ? t0 + lane : 0];
-            const float q = value(logit[wave][mine]);
-            const u64 m = r.mass(q);
-            const bool certain = live && q >= high;
-            sum += certain && m >= floor ? m : 0;
-            const u64 has = __ballot(live && !certain);
-            if (has) {
-                const int at = __builtin_amdgcn_mbcnt_hi(
-                    (uint32_t)(has >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)has, around));
-                if (live && !certain && at < AROUND) {
-                    const int index = i0 + (mine / (64 * kVec)) * kScanThreads * kVec +
-                                      mine % (64 * kVec);
-                    orders[wave][at] = (u64)key_of(q) << 32 | (uint32_t)~index;
-                }
-                around += __builtin_popcountll(has);
-            }
+        for (int t = lane; t < n; t += 64) {
+            const u64 m = r.mass(value(logit[wave][t]));
+            sum += m >= floor ? m : 0;
         }
         sum = wave_sum(sum);
         if (around) {
-            // more than there is room for: the count tells finish, which searches the whole row
-            int at = 0;
-            if (lane == 0) at = atomicAdd(&w.more->around, around <= AROUND ? around : kAround + 1);
-            at = __builtin_amdgcn_readfirstlane(at);
             const int room = around_of(V);
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            for (int t = lane; t < around && around <= AROUND && at + t < room; t += 64)
-                w.around[at + t] = orders[wave][t];
+            int to = __builtin_amdgcn_readfirstlane(first) + ((upto - some) >> 16);
+            for (; near; near &= near - 1, to++) {
+                const int b = __builtin_ctz(near);
+                const int index = i0 + (b / kVec * kScanThreads + lane) * kVec + b % kVec;
+                if (to < room)
+                    w.around[to] = (u64)key_of(r.seen(value(x[index]))) << 32 | (uint32_t)~index;
+            }
         }
         if (lane == 0) sums[wave] = sum;
         __syncthreads();
