@@ -34,25 +34,27 @@ class AdapterBatch:
         self.num_adapters = num_adapters
         self.ids: torch.Tensor | None = None
         self.plan: ops.LoraPlan | None = None
+        self._kept: dict[tuple[torch.device, int], ops.LoraPlan] = {}
 
     def assign(self, ids: torch.Tensor) -> None:
         """ids int [rows]: each row's adapter, any number outside [0, num_adapters) for none.
-        The tensors of a plan for as many rows are filled anew, so that a captured graph that
-        reads them follows; nothing waits for the GPU."""
+        Nothing waits for the GPU.  The plan lies in memory that is kept, one for each power of
+        two of rows: captured graphs of several batch sizes each read what the last assign of
+        that many rows left there, so assign before a replay, on its stream."""
         if ids.dim() != 1 or ids.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"ids must be int32 or int64 [rows] (got {ids.dtype}, "
                              f"{tuple(ids.shape)})")
-        if not ids.is_cuda:
-            self.ids, self.plan = ids, None
-            return
-        plan = ops.lora_plan(ids, self.num_adapters)
-        old = self.plan
-        if old is not None and old.rows.shape == plan.rows.shape and old.rows.device == ids.device:
-            old.seg_off.copy_(plan.seg_off)
-            old.rows.copy_(plan.rows)
-        else:
-            self.plan = plan
-        self.ids = ids
+        self.ids, self.plan = ids, None
+        if ids.is_cuda:
+            plan = ops.lora_plan(ids, self.num_adapters)
+            n = ids.numel()
+            key = ids.device, n.bit_length()
+            kept = self._kept.get(key)
+            if kept is None:
+                kept = self._kept[key] = ops.LoraPlan(torch.empty_like(plan.seg_off),
+                                                      plan.rows.new_empty(1 << n.bit_length()))
+            self.plan = ops.LoraPlan(kept.seg_off.copy_(plan.seg_off),
+                                     kept.rows[:n].copy_(plan.rows))
 
     def clear(self) -> None:
         """No row has an adapter: the modules are the linears that they wrap."""
@@ -129,6 +131,9 @@ class LoRALinear(nn.Module):
             return y
         if not x.is_cuda:
             return self._on_host(x, y)
+        if self.batch.plan is None:
+            raise ValueError(f"the batch's ids are on {self.batch.ids.device}, the rows on "
+                             f"{x.device}")
         return ops.lora_add(y, x, self.a, self.b, self.batch.plan, scaling=self.scaling,
                             splits=self.splits, out=y)
 

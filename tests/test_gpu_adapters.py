@@ -162,3 +162,39 @@ def test_adapters_change_what_is_drawn(pkg, wl, cuda):
     one = greedy(head(x), top_k=50)
     torch.manual_seed(0)
     assert torch.equal(one, greedy(head(x), top_k=50))
+
+
+def test_graphs_of_several_batch_sizes_share_a_batch(pkg, wl, cuda):
+    """One captured graph for each number of rows, as a server keeps them: each follows what is
+    assigned before its replay, whatever was assigned, and freed, in between."""
+    batch = pkg.AdapterBatch(SLOTS)
+    m = wrap(pkg, pkg.LinearW8A8(qtensor(pkg, wl, 640, HIDDEN, 81)), batch, 82, splits=[512, 128])
+    g = torch.Generator().manual_seed(83)
+    ids_of = lambda n: torch.randint(-1, SLOTS, (n,), generator=g)  # noqa: E731
+    graphs = {}
+    for n in (4, 7, 16, 200):
+        x = wl.activations(n, HIDDEN, seed=n).cuda()
+        batch.assign(ids_of(n).cuda())
+        m(x)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = m(x)
+        graphs[n] = graph, x, y
+    for n in (16, 4, 200, 7, 4, 16, 7, 200):
+        ids, (graph, x, y) = ids_of(n), graphs[n]
+        batch.assign(ids_of(33).cuda())                    # an eager step of another size
+        other = [torch.full((64,), 1 << 20, dtype=torch.int32, device="cuda") for _ in range(8)]
+        batch.assign(ids.cuda())
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, m(x)) and close(y, by_row(pkg, m, x, ids)), n
+        del other
+
+
+def test_ids_on_the_host_beside_rows_on_the_gpu_are_refused(pkg, wl, cuda):
+    batch = pkg.AdapterBatch(SLOTS)
+    m = wrap(pkg, pkg.LinearW8A8(qtensor(pkg, wl, 640, HIDDEN, 84)), batch, 85)
+    batch.assign(torch.zeros(4, dtype=torch.int64))
+    with pytest.raises(ValueError):
+        m(wl.activations(4, HIDDEN, seed=86).cuda())
