@@ -715,6 +715,11 @@ int launch_lora_add(const LoraAdd& l, hipStream_t st) {
             best = cost;
         }
     }
+    while (p.big && tiles * blocks >= 1 << 24) {  // a launch has fewer than 2^32 threads
+        cols *= 2;
+        blocks = 0;
+        for (int i = 0; i < l.parts; i++) blocks += (l.splits[i] + cols - 1) / cols;
+    }
     a.cols = (int)cols;
     a.blocks = (int)blocks;
     if (p.big) expand(a, dim3((uint32_t)(tiles * blocks)), st);
