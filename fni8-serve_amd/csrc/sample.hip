@@ -275,7 +275,9 @@ __device__ __forceinline__ N wave_sum(N v) {
 }
 
 // An item is a part of a row; a workgroup walks items, the loads of the next on their way while
-// it computes: 32 exponentials of 64 bits a thread take longer than its 64 or 128 bytes.
+// it computes.  256 rows of 151936 fp16 (77.8 MB): 15.3 us without sums (5.1 TB/s; a read alone
+// reaches 6.1), 35 with them, where the vector unit bounds it: 18 operations a logit and its sum,
+// 15 of them of 64 bits.
 template <class E>
 __global__ __launch_bounds__(kScanThreads) void scan_kernel(const fni8h::Sample a, int parts) {
     typedef E vec __attribute__((ext_vector_type(8), aligned(sizeof(E))));
@@ -786,6 +788,9 @@ __device__ __forceinline__ void find_ends(Shared& sh, Turn& turn, const Work& w,
 
 static_assert(kThreads * 2 * kVec == kPart && kPart == kSteps * kScanThreads * kVec, "parts");
 
+// One workgroup a row: a chain of searches, each a few round trips to LDS and the cache, so it is
+// bound by their latency and by the way of its own code from memory, not by bytes (a list of 50
+// of 151936: 10.3 us for one row; of hundreds, 64 rows: 19 us; no filter, 256 rows: 6.8 us).
 // ALONE: no other launch follows, and a row whose list does not fit is searched whole.
 template <class E, bool ALONE>
 __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, int parts) {
@@ -1131,9 +1136,11 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, i
 }
 
 // One part of a row with a long prefix: the mass of what is kept for certain, and the tokens
-// around the end of top-p.  Each wave first lists the logits of its 2048 that matter (down to
-// `low`), so that their exponentials, 20 operations of 64 bits, are not computed for the others
-// (256 rows of 151936, top-p 0.95, a fifth of the logits kept: 56 us with all of them).
+// around the end of top-p.  Each wave first moves the logits of its 2048 that are certain next to
+// each other in LDS, so that their exponentials, 18 operations, are not computed for the others;
+// the few around the end are read again.  256 rows of 151936 fp16 with top-p 0.95, a fifth of
+// the logits kept: 43 us (56 with the exponentials of all), half of it the vector unit, half
+// waiting for the chain settings, logits, lists.
 template <class E>
 __global__ __launch_bounds__(kScanThreads) void gather_kernel(const fni8h::Sample a, int parts) {
     constexpr int W = 64 * kVec * kSteps;  // logits of a wave
@@ -1216,6 +1223,10 @@ __global__ __launch_bounds__(kScanThreads) void gather_kernel(const fni8h::Sampl
     }
 }
 
+// One workgroup a row with a long prefix: the list that gather left, in registers, gives the end
+// of top-p; the masses of the parts, with what the list brings to each, the part that the draw
+// falls into; its 8192 logits the token.  Bound by the latency of these steps, as draw is: 21 us
+// for one row and 23 for 256 of 151936.
 template <class E>
 __global__ __launch_bounds__(kThreads) void finish_kernel(const fni8h::Sample a, int parts) {
     __shared__ Shared sh;
