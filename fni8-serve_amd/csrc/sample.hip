@@ -197,6 +197,7 @@ struct Long {
     u64 need;        // top-p: the mass to reach
     float high, low; // logits that the end of top-p lies between
     int kind, around;
+    uint32_t top;    // key of the row's largest logit
 };
 struct Work {
     double* sum;     // [parts] masses, relative to the part's largest logit
@@ -744,10 +745,18 @@ __device__ __forceinline__ void find_ends(Shared& sh, Turn& turn, const Work& w,
         const float d = (r.top - __builtin_bit_cast(float, bits)) * rate;
         if (d < (float)(kBins - 1)) atomicAdd(&sh.h.count[d > 0.0f ? (int)d : 0], 1u);
     };
-    for (int i = threadIdx.x; i < groups; i += kThreads) {
-        const uint32_t two = w.pick[i];
-        count(two << 16);
-        count(two & 0xffff0000u);
+    for (int i0 = threadIdx.x; i0 < groups; i0 += kKeep * kThreads) {
+        uint32_t two[kKeep];  // all on their way at once
+#pragma unroll
+        for (int j = 0; j < kKeep; j++) {
+            const int i = i0 + j * kThreads;
+            two[j] = i < groups ? w.pick[i] : 0xff80ff80u;  // minus infinity
+        }
+#pragma unroll
+        for (int j = 0; j < kKeep; j++) {
+            count(two[j] << 16);
+            count(two[j] & 0xffff0000u);
+        }
     }
     __syncthreads();
     // from the bottom: a thread's steps are last - j
@@ -790,7 +799,7 @@ static_assert(kThreads * 2 * kVec == kPart && kPart == kSteps * kScanThreads * k
 
 // One workgroup a row: a chain of searches, each a few round trips to LDS and the cache, so it is
 // bound by their latency and by the way of its own code from memory, not by bytes (a list of 50
-// of 151936: 10.3 us for one row; of hundreds, 64 rows: 19 us; no filter, 256 rows: 6.8 us).
+// of 151936: 10.6 us for one row; of hundreds, 64 rows: 17 us; no filter, 256 rows: 6.8 us).
 // ALONE: no other launch follows, and a row whose list does not fit is searched whole.
 template <class E, bool ALONE>
 __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, int parts) {
@@ -1120,7 +1129,7 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, i
     } else if constexpr (ALONE) {
         token = search_row(sh, turn, x, V, r, need_p, all);
     } else {  // the long way
-        Long more{need_p, 0.0f, 0.0f, kWhole, 0};
+        Long more{need_p, 0.0f, 0.0f, kWhole, 0, best};
         if (!r.by_k && !r.by_p) {
             more.kind = kMinP;
             more.low = (float)(r.base - (double)(bound + 2) / (r.step * r.rate));
@@ -1139,66 +1148,76 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, i
 // around the end of top-p.  Each wave first moves the logits of its 2048 that are certain next to
 // each other in LDS, so that their exponentials, 18 operations, are not computed for the others;
 // the few around the end are read again.  256 rows of 151936 fp16 with top-p 0.95, a fifth of
-// the logits kept: 43 us (56 with the exponentials of all), half of it the vector unit, half
-// waiting for the chain settings, logits, lists.
+// the logits kept: 36 us; 56 with the exponentials of all, 43 with the logits loaded only once
+// the row is known to need them and the row's largest found again by each workgroup.
 template <class E>
 __global__ __launch_bounds__(kScanThreads) void gather_kernel(const fni8h::Sample a, int parts) {
     constexpr int W = 64 * kVec * kSteps;  // logits of a wave
+    typedef E vec __attribute__((ext_vector_type(8), aligned(sizeof(E))));
     __shared__ E logit[4][W];
     __shared__ u64 sums[4];
-    __shared__ uint32_t tops[4];
     const int items = (int)a.B * parts, V = (int)a.V;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     for (int item = blockIdx.x; item < items; item += gridDim.x) {
         const int row = item / parts, part = item - row * parts;
+        Row r(a, row, V);
+        if (!(r.T > 0.0f) || r.by_k || !(r.by_p || r.by_m)) continue;
         const Work w = work_of(a.work, row, V);
+        // with top-p, the logits are on their way before it is known that the row needs them
+        if (!r.by_p && w.more->kind != kMinP) continue;
+        const E* x = (const E*)a.logits + (int64_t)row * a.ld;
+        const int i0 = part * kPart + wave * 64 * kVec;  // of the wave's first load
+        vec v[kSteps];
+#pragma unroll
+        for (int i = 0; i < kSteps; i++) {
+            const int at = i0 + (i * kScanThreads + lane) * kVec;
+            if (at + kVec <= V) {
+                v[i] = *reinterpret_cast<const vec*>(x + at);
+            } else {
+#pragma unroll
+                for (int j = 0; j < kVec; j++) {
+                    E e = lowest_of<E>();
+                    if (at + j < V) e = x[at + j];
+                    v[i][j] = e;
+                }
+            }
+        }
         const Long more = *w.more;
         if (more.kind != kTopP && more.kind != kMinP) continue;
-        const E* x = (const E*)a.logits + (int64_t)row * a.ld;
-        Row r(a, row, V);
-        float v[kSteps][kVec];
-        const int i0 = part * kPart + wave * 64 * kVec;  // of the wave's first load
-#pragma unroll
-        for (int i = 0; i < kSteps; i++)
-            load8(x, i0 + (i * kScanThreads + lane) * kVec, V, v[i]);
-        uint32_t best = 0;
-        for (int i = tid; i < parts; i += kScanThreads) best = w.part[i] > best ? w.part[i] : best;
-        best = key_max(best);
-        if (lane == 0) tops[wave] = best;
-        __syncthreads();
-        for (int i = 0; i < 4; i++) best = tops[i] > best ? tops[i] : best;
-        r.largest(value_of(best));
+        r.largest(value_of(more.top));
         if (r.inf) {
 #pragma unroll
             for (int i = 0; i < kSteps; i++)
 #pragma unroll
-                for (int j = 0; j < kVec; j++) v[i][j] = r.seen(v[i][j]);
+                for (int j = 0; j < kVec; j++) {
+                    const E e = v[i][j];
+                    v[i][j] = element<E>(r.seen(value(e)));
+                }
         }
         const u64 floor = more.kind == kMinP ? r.floor() : 0;
         const float low = __builtin_fmaxf(more.low, -0x1.fffffep127f);
         const float high = more.kind == kMinP ? low : __builtin_fmaxf(more.high, low);
-        uint32_t sure = 0, near = 0;  // this lane's, kept for certain and around the end
+        int n = 0;
+        uint32_t near = 0;  // this lane's around the end
 #pragma unroll
         for (int i = 0; i < kSteps; i++)
 #pragma unroll
             for (int j = 0; j < kVec; j++) {
-                sure |= (uint32_t)(v[i][j] >= high) << (i * kVec + j);
-                near |= (uint32_t)(v[i][j] >= low) << (i * kVec + j);
+                const E e = v[i][j];
+                const float q = value(e);
+                const bool sure = q >= high;
+                const u64 has = __ballot(sure);
+                if (sure)
+                    logit[wave][__builtin_amdgcn_mbcnt_hi(
+                        (uint32_t)(has >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)has, n))] = e;
+                n += __builtin_popcountll(has);
+                near |= (uint32_t)(q >= low && !sure) << (i * kVec + j);
             }
-        near &= ~sure;
-        const int some = __builtin_popcount(sure) | __builtin_popcount(near) << 16;
-        const int upto = wave_scan(some), counts = last_lane(upto);
-        const int n = counts & 0xffff, around = counts >> 16;
+        const int some = __builtin_popcount(near), upto = wave_scan(some), around = last_lane(upto);
         // where there is no room for them the count tells finish, which searches the whole row
         int first = 0;  // on its way while the sums are made
         if (around && lane == 0) first = atomicAdd(&w.more->around, around);
-        int at = (upto - some) & 0xffff;
-#pragma unroll
-        for (int i = 0; i < kSteps; i++)
-#pragma unroll
-            for (int j = 0; j < kVec; j++)
-                if (v[i][j] >= high) logit[wave][at++] = element<E>(v[i][j]);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         u64 sum = 0;
         for (int t = lane; t < n; t += 64) {
@@ -1208,7 +1227,7 @@ __global__ __launch_bounds__(kScanThreads) void gather_kernel(const fni8h::Sampl
         sum = wave_sum(sum);
         if (around) {
             const int room = around_of(V);
-            int to = __builtin_amdgcn_readfirstlane(first) + ((upto - some) >> 16);
+            int to = __builtin_amdgcn_readfirstlane(first) + upto - some;
             for (; near; near &= near - 1, to++) {
                 const int b = __builtin_ctz(near);
                 const int index = i0 + (b / kVec * kScanThreads + lane) * kVec + b % kVec;
@@ -1219,14 +1238,15 @@ __global__ __launch_bounds__(kScanThreads) void gather_kernel(const fni8h::Sampl
         if (lane == 0) sums[wave] = sum;
         __syncthreads();
         if (tid == 0) w.above[part] = sums[0] + sums[1] + sums[2] + sums[3];
-        __syncthreads();  // tops and sums are the next item's
+        __syncthreads();  // the sums are the next item's
     }
 }
 
 // One workgroup a row with a long prefix: the list that gather left, in registers, gives the end
 // of top-p; the masses of the parts, with what the list brings to each, the part that the draw
-// falls into; its 8192 logits the token.  Bound by the latency of these steps, as draw is: 21 us
-// for one row and 23 for 256 of 151936.
+// falls into; its 8192 logits the token.  Bound by the latency of these steps, as draw is: 12 us
+// for 5 rows of 50257, 20 for 256 of 151936 (23 with the list's neighbours in different threads,
+// whose sums then have to be joined by the wave).
 template <class E>
 __global__ __launch_bounds__(kThreads) void finish_kernel(const fni8h::Sample a, int parts) {
     __shared__ Shared sh;
@@ -1237,15 +1257,9 @@ __global__ __launch_bounds__(kThreads) void finish_kernel(const fni8h::Sample a,
     const Long more = *w.more;
     if (more.kind == kDone) return;
     const E* x = (const E*)a.logits + row * a.ld;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x;
     Row r(a, row, V);
-    const uint32_t own = tid < parts ? w.part[tid] : 0;
-    uint32_t best = key_max(own);
-    if (lane == 0) sh.counts[wave] = (int)best;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kWaves; i++) best = (uint32_t)sh.counts[i] > best ? (uint32_t)sh.counts[i] : best;
-    r.largest(value_of(best));
+    r.largest(value_of(more.top));
     const u64 floor = r.floor();
     u64 all = 0;
     int token = -1;
@@ -1270,15 +1284,16 @@ __global__ __launch_bounds__(kThreads) void finish_kernel(const fni8h::Sample a,
                     return d < (double)(kBins - 1) ? (int)d : kBins - 1;
                 };
                 auto logit = [](u64 order) { return value_of((uint32_t)(order >> 32)); };
-                u64 order[HELD], m[HELD];  // the list: read once, weighed once
+                // the list: read once, weighed once, neighbours to a thread
+                u64 order[HELD], m[HELD];
+                const int per = (n + kThreads - 1) / kThreads;
 #pragma unroll
                 for (int j = 0; j < HELD; j++)
-                    if (j * kThreads < n)
-                        order[j] = tid + j * kThreads < n ? w.around[tid + j * kThreads] : 0;
+                    if (j < per) order[j] = tid * per + j < n ? w.around[tid * per + j] : 0;
                 clear_bins(sh);
 #pragma unroll
                 for (int j = 0; j < HELD; j++)
-                    if (j * kThreads < n) {
+                    if (j < per) {
                         const float v = logit(order[j]);
                         m[j] = order[j] ? r.mass(v) : 0;
                         if (m[j]) atomicAdd(&sh.h.mass[bin(r.power(v))], m[j]);
@@ -1290,7 +1305,7 @@ __global__ __launch_bounds__(kThreads) void finish_kernel(const fni8h::Sample a,
                 const int b = find_bin(sh, turn, need);
 #pragma unroll
                 for (int j = 0; j < HELD; j++)
-                    if (j * kThreads < n && m[j] && bin(r.power(logit(order[j]))) == b) {
+                    if (j < per && m[j] && bin(r.power(logit(order[j]))) == b) {
                         const int at = atomicAdd(&sh.n, 1);
                         if (at < kList) sh.list[at] = {order[j], m[j]};
                     }
@@ -1309,22 +1324,21 @@ __global__ __launch_bounds__(kThreads) void finish_kernel(const fni8h::Sample a,
                 __syncthreads();
                 sh.above[tid] = mine;
                 __syncthreads();
-                if (found) {
+                if (found) {  // neighbours are of one part, or of a few: a sum for each
+                    u64 some = 0;
+                    int at = 0;
 #pragma unroll
                     for (int j = 0; j < HELD; j++)
-                        if (j * kThreads < n) {
-                            // neighbours in the list are of one part, or of a few: a sum for each
+                        if (j < per && m[j]) {
                             const int index = (int)~(uint32_t)order[j];
-                            const bool keep = m[j] && c.keeps((uint32_t)(order[j] >> 32), index);
-                            const int part = index / kPart;
-                            for (u64 left = __ballot(keep); left;) {
-                                const int p = __builtin_amdgcn_readlane(part, __builtin_ctzll(left));
-                                const u64 same = __ballot(keep && part == p);
-                                const u64 some = wave_sum(keep && part == p ? m[j] : 0);
-                                if (lane == 0) atomicAdd(&sh.above[p], some);
-                                left &= ~same;
+                            if (index / kPart != at) {
+                                if (some) atomicAdd(&sh.above[at], some);
+                                some = 0;
+                                at = index / kPart;
                             }
+                            some += c.keeps((uint32_t)(order[j] >> 32), index) ? m[j] : 0;
                         }
+                    if (some) atomicAdd(&sh.above[at], some);
                 }
                 __syncthreads();
                 mine = sh.above[tid];
