@@ -82,6 +82,17 @@ def test_shapes(pkg, cuda, T, K, splits, rank, S):
     check(pkg, *make(T, K, splits, rank, S, seed=T + K), splits)
 
 
+@pytest.mark.parametrize("splits", [[128, 64], [72, 60], [2048 + 64]])
+@pytest.mark.parametrize("K,rank", [(8, 8), (136, 32), (264, 40), (130, 72), (512, 136), (96, 256)])
+def test_large_batches(pkg, cuda, K, rank, splits):
+    """Tiles of 64 tokens: each step of the rank, whole strips and parts of them, chunks of K that
+    are whole and not, several parts of K; an adapter with one token, and one with none."""
+    g = torch.Generator().manual_seed(rank)
+    ids = torch.randint(-1, 3, (1100,), generator=g)
+    ids[500] = 3
+    check(pkg, *make(1100, K, splits, rank, 5, seed=K + rank, ids=ids), splits)
+
+
 @pytest.mark.parametrize("T", [3, 70, 600])
 def test_ids_of_every_kind(pkg, cuda, T):
     """No token with an adapter, one adapter for all, one of many used, ids outside the range."""
