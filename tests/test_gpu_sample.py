@@ -2,7 +2,7 @@
 within the rounding of their last step.
 
 Tokens: a running sum is off by less than n * 2^-45 of the largest weight (integer weights,
-n <= 151936), so a random u picks another token than the 64-bit sums with a chance below
+n <= 151936) and 2^-38 of itself (the weights' polynomial), so a random u picks another token than the 64-bit sums with a chance below
 151936 * 2^-27 / 2^17 a row at the worst and about 1e-8 for the rows here; u on a border is
 tested where weights are equal, and sums exact on both sides.
 Log-probabilities: power and log in 64 bits, one rounding to fp32: 2^-24 relative, and the
@@ -232,3 +232,52 @@ def test_a_row_is_the_same_in_every_batch(pkg, cuda):
         for i in (0, 7, 299):
             one, logp1 = pkg.sample(x[i:i + 1], u[i:i + 1], return_logprobs=True, **kw)
             assert one[0] == got[i] and logp1[0] == logp[i]
+
+
+def test_the_longest_rows(pkg, cuda):
+    """2^22 logits, 512 parts; one more is refused."""
+    x, u = logits(2, 2 ** 22, seed=12, spread=1.5, peaks=3)
+    x[1, 2 ** 22 - 1] = 20.0
+    for kw in (dict(temperature=0.0), dict(), dict(top_p=0.9), dict(top_k=50, top_p=0.9),
+               dict(min_p=0.01)):
+        check(pkg, x, u, **kw)
+    with pytest.raises((ValueError, RuntimeError)):
+        pkg.sample(torch.zeros(1, 2 ** 22 + 1, dtype=torch.float16, device="cuda"), u[:1])
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(top_p=0.9), dict(top_k=5), dict(min_p=0.1)])
+def test_many_rows(pkg, cuda, kw):
+    x, u = logits(3000, 131, seed=13)
+    check(pkg, x, u, **kw)
+
+
+@pytest.mark.parametrize("fp32", [False, True])
+@pytest.mark.parametrize("low", [-30.0, -6.0, 6.0])
+def test_rows_with_a_pattern(pkg, cuda, low, fp32):
+    """Places in every eight (or every 32) that are all lower, or all higher, than the others: what
+    a few of a group's logits tell of the row is wrong."""
+    g = torch.Generator().manual_seed(14)
+    x = torch.randn(6, 120000, generator=g)
+    i = torch.arange(120000)
+    for row, at in enumerate(([1], [6], [1, 6], [0, 2, 3, 4, 5, 7])):
+        x[row, (i[:, None] % 8 == torch.tensor(at)).any(1)] += low
+    x[4, i // 2048 % 4 == 1] += low
+    x[5, i % 8192 < 4096] += low
+    x = (x if fp32 else x.half()).cuda()
+    for kw in (dict(top_p=0.9), dict(top_p=0.5), dict(top_p=0.99, temperature=2.0), dict(min_p=0.02)):
+        check(pkg, x, torch.rand(6, generator=g).cuda(), **kw)
+
+
+def test_two_streams_at_once(pkg, cuda):
+    work = [logits(40, 50257, seed=50 + i) for i in range(2)]
+    want = [pkg.sample(x, u, temperature=1.2, top_p=0.98) for x, u in work]
+    sides = [torch.cuda.Stream() for _ in work]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for rep in range(5):
+        for i, s in enumerate(sides):
+            with torch.cuda.stream(s):
+                got[i].append(pkg.sample(*work[i], temperature=1.2, top_p=0.98))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(t, want[i]) for t in got[i])
