@@ -23,6 +23,7 @@
 namespace {
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef h8 h8_anywhere __attribute__((aligned(2)));  // loads and stores are as wide at any address
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kShrinkWaves = 8;            // of a workgroup
@@ -363,12 +364,12 @@ __device__ __forceinline__ void load_b(const Args& a, const uint16_t* b, int n, 
 }
 
 // y: the lane's first column of the strip, `left` columns before the end; whole (the same for
-// the wave): all of the strip is there, in whole vectors.
+// the wave): all of the strip is there.
 template <int QT>
 __device__ __forceinline__ void load_y(const uint16_t* y, int left, bool whole, h8 (&in)[QT / 2]) {
     if (whole) {
 #pragma unroll
-        for (int q = 0; q < QT / 2; q++) in[q] = *reinterpret_cast<const h8*>(y + 32 * q);
+        for (int q = 0; q < QT / 2; q++) in[q] = *reinterpret_cast<const h8_anywhere*>(y + 32 * q);
     } else {
 #pragma unroll
         for (int q = 0; q < QT / 2; q++) in[q] = load8<false>(y + 32 * q, left - 32 * q);
@@ -386,7 +387,7 @@ __device__ __forceinline__ void store_y(uint16_t* o, int left, bool whole, const
         for (int r = 0; r < 8; r++)
             z[r] = (_Float16)__builtin_fmaf(acc[2 * q + r / 4][r & 3], down, (float)in[q][r]);
         if (whole) {
-            *reinterpret_cast<h8*>(o + 32 * q) = z;
+            *reinterpret_cast<h8_anywhere*>(o + 32 * q) = z;
         } else {
 #pragma unroll
             for (int r = 0; r < 8; r++) {
@@ -397,10 +398,6 @@ __device__ __forceinline__ void store_y(uint16_t* o, int left, bool whole, const
     }
 }
 
-__device__ __forceinline__ bool aligned8(const Args& a, int n0) {
-    return (a.ldy | a.ldo | n0) % 8 == 0 && (((uintptr_t)a.y | (uintptr_t)a.out) & 15) == 0;
-}
-
 // Tokens without an adapter: out is y.
 __device__ __forceinline__ void copy_rows(const Args& a, int ahead, int r0, int count, int n0, int n1) {
     const int lane = threadIdx.x & 63;
@@ -409,12 +406,10 @@ __device__ __forceinline__ void copy_rows(const Args& a, int ahead, int r0, int 
         if (row < 0) continue;
         const uint16_t* y = a.y + (int64_t)row * a.ldy;
         uint16_t* o = a.out + (int64_t)row * a.ldo;
-        if (aligned8(a, n0) && (n1 - n0) % 8 == 0) {
-            for (int n = n0 + lane * 8; n < n1; n += 512)
-                *reinterpret_cast<h8*>(o + n) = *reinterpret_cast<const h8*>(y + n);
-        } else {
-            for (int n = n0 + lane; n < n1; n += 64) o[n] = y[n];
-        }
+        const int whole = n0 + (n1 - n0) / 8 * 8;
+        for (int n = n0 + lane * 8; n < whole; n += 512)
+            *reinterpret_cast<h8_anywhere*>(o + n) = *reinterpret_cast<const h8_anywhere*>(y + n);
+        if (whole + lane < n1) o[whole + lane] = y[whole + lane];
     }
 }
 
@@ -435,7 +430,7 @@ __global__ __launch_bounds__(kThreads, KS <= 2 ? 4 : KS == 4 ? 2 : 1) void expan
         return;
     }
     const int row = token_at(a, ahead, r0, t, count);
-    const bool live = t < count && row >= 0, wide = aligned8(a, n0);
+    const bool live = t < count && row >= 0;
     // lanes without a token load another's row, and store nothing
     const uint16_t* y = a.y + (int64_t)(row < 0 ? 0 : row) * a.ldy + 8 * g;
     uint16_t* o = a.out + (int64_t)(row < 0 ? 0 : row) * a.ldo + 8 * g;
@@ -445,7 +440,7 @@ __global__ __launch_bounds__(kThreads, KS <= 2 ? 4 : KS == 4 ? 2 : 1) void expan
     auto fetch = [&](int n, h8 (&b)[QT][KS], h8 (&z)[QT / 2]) {
         if (n >= n1) return;
         load_b<KS, QT>(a, rows_b, n, n1, n + 16 * QT <= n1, lane, b);
-        load_y<QT>(y + n, n1 - n - 8 * g, wide && n + 16 * QT <= n1, z);
+        load_y<QT>(y + n, n1 - n - 8 * g, n + 16 * QT <= n1, z);
     };
     int n = n0 + wave * 16 * QT;
     // the low-rank rows before y and B: loads come back in order, and these come from the cache
@@ -492,7 +487,7 @@ __global__ __launch_bounds__(kThreads, KS <= 2 ? 4 : KS == 4 ? 2 : 1) void expan
         for (int q = 0; q < QT / 2; q++) was[q] = z[q];
         fetch(n + 2 * STEP, b, z);
         if (live)
-            store_y<QT>(o + n, n1 - n - 8 * g, wide && n + 16 * QT <= n1, was, acc, down);
+            store_y<QT>(o + n, n1 - n - 8 * g, n + 16 * QT <= n1, was, acc, down);
     };
     for (; n < n1; n += 2 * STEP) {
         strip(n, bf[0], in[0]);
@@ -501,7 +496,7 @@ __global__ __launch_bounds__(kThreads, KS <= 2 ? 4 : KS == 4 ? 2 : 1) void expan
 }
 
 // The same for tiles of 16 * NT tokens: the low-rank rows lie in LDS, a strip's rows of B serve
-// all NT groups of 16.  WHOLE: every strip is there to its end, in whole vectors.  8192 tokens,
+// all NT groups of 16.  WHOLE: every strip is there to its end.  8192 tokens,
 // 6144 columns (201 MB of y in and out): 50 us, 4.0 TB/s; a copy in the same order of addresses
 // alone takes 39 us, one straight through 32.
 template <int KS, int NT, bool WHOLE>
@@ -528,11 +523,10 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(const Args a) {
         const int i = t * 16 + (lane & 15), r = token_at(a, ahead, r0, i, count);
         row[t] = i < count ? r : -1;  // -1: loads row 0, stores nothing
     }
-    const bool wide = WHOLE || aligned8(a, n0);
     const uint16_t* rows_b = a.b + (int64_t)e * a.start[a.parts] * a.rank;
     h8 bf[QT][KS], in[NT][QT / 2];
     auto fetch = [&](int n) {
-        const bool whole = WHOLE || (wide && n + 16 * QT <= n1);
+        const bool whole = WHOLE || n + 16 * QT <= n1;
         load_b<KS, QT>(a, rows_b, n, n1, WHOLE || n + 16 * QT <= n1, lane, bf);
 #pragma unroll
         for (int t = 0; t < NT; t++)
@@ -574,7 +568,7 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(const Args a) {
 #pragma unroll
     for (int t = 0; t < NT; t++) down[t] = __builtin_ldexpf(1.0f, -shift_of(top[t * 16 + (lane & 15)]));
     while (n < n1) {
-        const bool whole = WHOLE || (wide && n + 16 * QT <= n1);
+        const bool whole = WHOLE || n + 16 * QT <= n1;
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             f32x4 acc[QT];
@@ -730,10 +724,9 @@ int launch_lora_add(const LoraAdd& l, hipStream_t st) {
     }
     a.cols = (int)cols;
     a.blocks = (int)blocks;
-    // Where all strips are whole and in whole vectors, the large tiles take code without the
-    // branches for others (75.4 us a call of 8192 tokens, 78.0 with them; the small tiles are as
-    // fast either way).
-    bool whole = (l.ldy | l.ldo) % 8 == 0 && (((uintptr_t)l.y | (uintptr_t)l.out) & 15) == 0;
+    // Where all strips are whole the large tiles take code without the branches for others (75.4
+    // us a call of 8192 tokens, 78.0 with them; the small tiles are as fast either way).
+    bool whole = true;
     for (int i = 0; i < l.parts; i++) whole = whole && l.splits[i] % 64 == 0;
     const uint32_t all = (uint32_t)(tiles * blocks);
     if (!p.big) expand_few(a, dim3((uint32_t)tiles, (uint32_t)blocks), st);
