@@ -447,19 +447,38 @@ __global__ __launch_bounds__(kThreads, KS <= 2 ? 4 : KS == 4 ? 2 : 1) void expan
     const float scale = a.scaling ? a.scaling[e] : 1.0f;
     float v[KS][8];
     uint32_t top = 0;
-#pragma unroll
-    for (int s = 0; s < KS; s++) {
+    auto sum = [&](int s, float (&to)[8]) {
         const int j = s * 32 + 8 * g;
         if (t < count && j < a.rank) {
-            low_rank<KS == 1 ? 8 : 4>(a, r0 + t, part, j, scale, v[s]);
+            low_rank<8>(a, r0 + t, part, j, scale, to);
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[s][i] = 0.0f;
+            for (int i = 0; i < 8; i++) to[i] = 0.0f;
         }
+    };
+    if constexpr (KS == 1) {
+        sum(0, v[0]);
+        fetch(n, bf[0], in[0]);
+    } else {  // a step or two of the rank for each wave, so that all parts are on their way
+        __shared__ f32x4 sums[KS][2][64];
+        for (int s = wave; s < KS; s += kWaves) {
+            float w[8];
+            sum(s, w);
+            sums[s][0][lane] = f32x4{w[0], w[1], w[2], w[3]};
+            sums[s][1][lane] = f32x4{w[4], w[5], w[6], w[7]};
+        }
+        fetch(n, bf[0], in[0]);
+        __syncthreads();
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[s][i] = sums[s][i / 4][lane][i % 4];
+    }
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
         const uint32_t m = top_of(v[s]);
         top = m > top ? m : top;
     }
-    fetch(n, bf[0], in[0]);
 #pragma unroll
     for (int d = 16; d < 64; d *= 2) {
         const uint32_t m = (uint32_t)__shfl_xor((int)top, d, 64);
