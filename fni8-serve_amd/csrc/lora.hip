@@ -12,7 +12,7 @@
 //           wave, and y in the same pass
 //
 // Both wait for memory only.  A call of few tokens is a chain of dependent loads (which tile,
-// which rows, their data), so each wave finds its tile by itself, without LDS or a barrier, and
+// which rows, their data), so each wave finds its tile by itself, without a barrier, and
 // everything that depends on the tile alone is on its way at once.
 //
 // h enters the second product as two fp16 numbers, h * 2^k = hi + lo with one k a token that
@@ -415,7 +415,9 @@ __device__ __forceinline__ void copy_rows(const Args& a, int ahead, int r0, int 
 
 // KS: 32-element steps of the rank.  Tiles of 16 tokens; a wave keeps the low-rank rows in
 // registers and goes through its strips, the loads of the next on their way.  48 tokens of 48
-// adapters, rank 16, 24576 columns: 13.2 us for 42 MB; 16 tokens, 151936 columns: 11.2 us.
+// adapters, rank 16, 24576 columns: 12.4 us for 42 MB; 16 tokens, 151936 columns: 11.0 us.  At
+// ranks above 32 the waves share the sums of the low-rank rows (9 tokens, rank 128, 32000
+// columns: 10.8 us; 17.7 with all sums in each wave).
 template <int KS>
 __global__ __launch_bounds__(kThreads, KS <= 2 ? 4 : KS == 4 ? 2 : 1) void expand_few_kernel(const Args a) {
     constexpr int QT = KS == 1 ? 4 : 2;
@@ -443,7 +445,7 @@ __global__ __launch_bounds__(kThreads, KS <= 2 ? 4 : KS == 4 ? 2 : 1) void expan
         load_y<QT>(y + n, n1 - n - 8 * g, n + 16 * QT <= n1, z);
     };
     int n = n0 + wave * 16 * QT;
-    // the low-rank rows before y and B: loads come back in order, and these come from the cache
+    fetch(n, bf[0], in[0]);  // comes from memory, the low-rank rows from a cache
     const float scale = a.scaling ? a.scaling[e] : 1.0f;
     float v[KS][8];
     uint32_t top = 0;
@@ -458,8 +460,7 @@ __global__ __launch_bounds__(kThreads, KS <= 2 ? 4 : KS == 4 ? 2 : 1) void expan
     };
     if constexpr (KS == 1) {
         sum(0, v[0]);
-        fetch(n, bf[0], in[0]);
-    } else {  // a step or two of the rank for each wave, so that all parts are on their way
+    } else {  // a step or two of the rank for each wave, so that all parts are on their way at once
         __shared__ f32x4 sums[KS][2][64];
         for (int s = wave; s < KS; s += kWaves) {
             float w[8];
@@ -467,7 +468,6 @@ __global__ __launch_bounds__(kThreads, KS <= 2 ? 4 : KS == 4 ? 2 : 1) void expan
             sums[s][0][lane] = f32x4{w[0], w[1], w[2], w[3]};
             sums[s][1][lane] = f32x4{w[4], w[5], w[6], w[7]};
         }
-        fetch(n, bf[0], in[0]);
         __syncthreads();
 #pragma unroll
         for (int s = 0; s < KS; s++)
