@@ -275,8 +275,7 @@ __device__ __forceinline__ N wave_sum(N v) {
     return last_lane(wave_scan(v));
 }
 
-// An item is a part of a row; a workgroup walks items, the loads of the next on their way while
-// it computes.  256 rows of 151936 fp16 (77.8 MB): 15.3 us without sums (5.1 TB/s; a read alone
+// An item is a part of a row; beyond 2^20 of them a workgroup takes more than one.  256 rows of 151936 fp16 (77.8 MB): 15.3 us without sums (5.1 TB/s; a read alone
 // reaches 6.1), 35 with them, where the vector unit bounds it: 18 operations a logit and its sum,
 // 15 of them of 64 bits.
 template <class E>
@@ -289,45 +288,39 @@ __global__ __launch_bounds__(kScanThreads) void scan_kernel(const fni8h::Sample 
     __shared__ double sums[2][4];
     const int V = (int)a.V, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int items = (int)a.B * parts;  // fewer than 2^30
-    vec next[kSteps];
-    auto fetch = [&](int item) {
-        const int row = item / parts;
+    const int step = gridDim.x;
+    for (int item = blockIdx.x, turn = 0; item < items; item += step, turn ^= 1) {
+        const int row = item / parts, part = item - row * parts;
+        const Work w = work_of(a.work, row, V);
         const E* x = (const E*)a.logits + row * a.ld;
-        const int i0 = (item - row * parts) * kPart + tid * kVec;
+        const int i0 = part * kPart + tid * kVec;
+        vec q[kSteps];
 #pragma unroll
         for (int i = 0; i < kSteps; i++) {
             const int at = i0 + i * kScanThreads * kVec;
             if (at + kVec <= V) {
-                next[i] = *reinterpret_cast<const vec*>(x + at);
+                q[i] = *reinterpret_cast<const vec*>(x + at);
             } else {
 #pragma unroll
                 for (int j = 0; j < kVec; j++) {
                     E e = lowest_of<E>();
                     if (at + j < V) e = x[at + j];
-                    next[i][j] = e;
+                    q[i][j] = e;
                 }
             }
         }
-    };
-    const int step = gridDim.x;
-    int item = blockIdx.x;
-    if (item < items) fetch(item);
-    for (int turn = 0; item < items; item += step, turn ^= 1) {
-        const int row = item / parts, part = item - row * parts;
-        const Work w = work_of(a.work, row, V);
         float v[kSteps][kVec];
-        number many = __builtin_bit_cast(number, next[0]);
+        number many = __builtin_bit_cast(number, q[0]);
 #pragma unroll
         for (int i = 1; i < kSteps; i++)
-            many = __builtin_elementwise_maximum(many, __builtin_bit_cast(number, next[i]));
+            many = __builtin_elementwise_maximum(many, __builtin_bit_cast(number, q[i]));
 #pragma unroll
         for (int i = 0; i < kSteps; i++)
 #pragma unroll
             for (int j = 0; j < kVec; j++) {
-                const E e = next[i][j];
+                const E e = q[i][j];
                 v[i][j] = value(e);
             }
-        if (item + step < items) fetch(item + step);
         auto most = many[0];
 #pragma unroll
         for (int j = 1; j < kVec; j++) most = __builtin_elementwise_maximum(most, many[j]);

@@ -281,3 +281,19 @@ def test_two_streams_at_once(pkg, cuda):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(t, want[i]) for t in got[i])
+
+
+def test_more_parts_than_workgroups(pkg, cuda):
+    """540000 rows of two parts each: workgroups take more than one part."""
+    B, V = 540000, 8200
+    x = torch.empty(B, V, dtype=torch.float16, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(7))
+    u = torch.rand(B, device="cuda", generator=torch.Generator("cuda").manual_seed(8))
+    got = pkg.sample(x, temperature=0.0)
+    assert torch.equal(x.gather(1, got[:, None])[:, 0], x.amax(1))
+    some = torch.cat([torch.arange(0, 4), torch.arange(524286, 524290), torch.arange(B - 4, B)])
+    assert got[some.cuda()].tolist() == x[some.cuda()].argmax(1).tolist()
+    for kw in (dict(top_p=0.8), dict()):
+        got = pkg.sample(x, u, **kw)[some.cuda()].tolist()
+        assert got == [w[0] for w in expected(x[some.cuda()], u[some.cuda()], **kw)]
+    del x
+    torch.cuda.empty_cache()
