@@ -276,7 +276,7 @@ __device__ __forceinline__ N wave_sum(N v) {
 }
 
 // An item is a part of a row; beyond 2^20 of them a workgroup takes more than one.  256 rows of 151936 fp16 (77.8 MB): 15.3 us without sums (5.1 TB/s; a read alone
-// reaches 6.1), 35 with them, where the vector unit bounds it: 18 operations a logit and its sum,
+// reaches 6.1), 34 with them, where the vector unit bounds it: 18 operations a logit and its sum,
 // 15 of them of 64 bits.
 template <class E>
 __global__ __launch_bounds__(kScanThreads) void scan_kernel(const fni8h::Sample a, int parts) {
