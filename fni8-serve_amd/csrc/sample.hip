@@ -791,8 +791,8 @@ __device__ __forceinline__ void find_ends(Shared& sh, Turn& turn, const Work& w,
 static_assert(kThreads * 2 * kVec == kPart && kPart == kSteps * kScanThreads * kVec, "parts");
 
 // One workgroup a row: a chain of searches, each a few round trips to LDS and the cache, so it is
-// bound by their latency and by the way of its own code from memory, not by bytes (a list of 50
-// of 151936: 10.6 us for one row; of hundreds, 64 rows: 17 us; no filter, 256 rows: 6.8 us).
+// bound by their latency, not by bytes (a list of 50 of 151936: 10.6 us for one row; of hundreds,
+// 64 rows: 17 us; no filter, 256 rows: 6.8 us).
 // ALONE: no other launch follows, and a row whose list does not fit is searched whole.
 template <class E, bool ALONE>
 __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, int parts) {
@@ -990,8 +990,10 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, i
 #pragma unroll
             for (int j = 0; j < B; j++) sum += b[j] <= lo ? m[j] : 0.0f;
             sum = wave_sum(sum);
-            // the list has some more than these maxima: it is tried unless they are far from the mass
-            if (lane == 0) sh.bin = whole && lo < least && 2.0f * sum < goal ? -1 : lo;
+            // The list has more than these maxima (of logits in no order, about 355 tokens where
+            // they are 256 of 512): it is tried unless half as much again does not reach the
+            // mass (5 us for a list in vain).
+            if (lane == 0) sh.bin = whole && lo < least && 1.5f * sum < goal ? -1 : lo;
         }
         __syncthreads();
         bound = sh.bin;
