@@ -398,18 +398,37 @@ __device__ __forceinline__ void store_y(uint16_t* o, int left, bool whole, const
     }
 }
 
-// Tokens without an adapter: out is y.
+// Tokens without an adapter: out is y.  MANY of a wave's rows are on their way at once (3323
+// tokens, 6144 columns, half of them without: 32.0 us, 34.0 with one).
+template <int MANY>
 __device__ __forceinline__ void copy_rows(const Args& a, int ahead, int r0, int count, int n0, int n1) {
-    const int lane = threadIdx.x & 63;
-    for (int t = threadIdx.x >> 6; t < count; t += kWaves) {
-        const int row = token_at(a, ahead, r0, t, count);
-        if (row < 0) continue;
-        const uint16_t* y = a.y + (int64_t)row * a.ldy;
-        uint16_t* o = a.out + (int64_t)row * a.ldo;
-        const int whole = n0 + (n1 - n0) / 8 * 8;
-        for (int n = n0 + lane * 8; n < whole; n += 512)
-            *reinterpret_cast<h8_anywhere*>(o + n) = *reinterpret_cast<const h8_anywhere*>(y + n);
-        if (whole + lane < n1) o[whole + lane] = y[whole + lane];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int whole = n0 + (n1 - n0) / 8 * 8;
+    for (int t0 = wave; t0 < count; t0 += kWaves * MANY) {
+        int row[MANY];
+#pragma unroll
+        for (int i = 0; i < MANY; i++) {
+            const int t = t0 + kWaves * i, r = token_at(a, ahead, r0, t, count);
+            row[i] = t < count ? r : -1;
+        }
+        for (int n = n0 + lane * 8; n < whole; n += 512) {
+            h8 v[MANY];
+#pragma unroll
+            for (int i = 0; i < MANY; i++)
+                if (row[i] >= 0)
+                    v[i] = *reinterpret_cast<const h8_anywhere*>(a.y + (int64_t)row[i] * a.ldy + n);
+#pragma unroll
+            for (int i = 0; i < MANY; i++)
+                if (row[i] >= 0)
+                    *reinterpret_cast<h8_anywhere*>(a.out + (int64_t)row[i] * a.ldo + n) = v[i];
+        }
+        if (whole + lane < n1) {
+#pragma unroll
+            for (int i = 0; i < MANY; i++)
+                if (row[i] >= 0)
+                    a.out[(int64_t)row[i] * a.ldo + whole + lane] =
+                        a.y[(int64_t)row[i] * a.ldy + whole + lane];
+        }
     }
 }
 
@@ -428,7 +447,7 @@ __global__ __launch_bounds__(kThreads, KS <= 2 ? 4 : KS == 4 ? 2 : 1) void expan
     if (!find_block(a, blockIdx.y, part, n0, n1)) return;
     const int count = r1 - r0, t = lane & 15, g = lane >> 4;
     if (e == a.S) {
-        if (a.copy) copy_rows(a, ahead, r0, count, n0, n1);
+        if (a.copy) copy_rows<4>(a, ahead, r0, count, n0, n1);
         return;
     }
     const int row = token_at(a, ahead, r0, t, count);
@@ -533,7 +552,7 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(const Args a) {
     if (!find_block(a, blockIdx.x - tile * a.blocks, part, n0, n1)) return;
     const int count = r1 - r0, g = lane >> 4;
     if (e == a.S) {
-        if (a.copy) copy_rows(a, ahead, r0, count, n0, n1);
+        if (a.copy) copy_rows<8>(a, ahead, r0, count, n0, n1);
         return;
     }
     int row[NT];
@@ -720,15 +739,17 @@ int launch_lora_add(const LoraAdd& l, hipStream_t st) {
     const int nt = !p.big ? 1 : l.rank > 128 ? 2 : 4;
     const int64_t tiles = tiles_of(l.T, l.S + 1, 16 * nt);
     // Columns of a workgroup, whole strips of its four waves.  Tiles of 64: two strips where that
-    // leaves three workgroups to a CU (8192 tokens, 6144 columns: 54 us; 57 with one, 64 with
-    // three).  Of 16: the fewest rounds of the four that a CU holds at once, each as long as the
-    // columns and a start that takes about as long as 1024 of them.
+    // leaves more than one workgroup to a CU (calls of 8192 tokens, 6144 columns: 58.8 us; 60.4
+    // with one strip, 67.8 with three; of 2048 tokens: 21.3, 23.3, 24.0; of 2048 tokens and
+    // columns, half a workgroup a CU: 13.3, 11.9, 14.9).  Of 16: the fewest rounds of the four
+    // that a CU holds at once, each as long as the columns and a start that takes about as long
+    // as 1024 of them.
     const int64_t strips = kWaves * 64;
     int64_t cols = 0, blocks = 0, best = 0;
     for (int64_t c = strips; c <= (p.big ? 512 : 4096); c += strips) {
         int64_t n = 0;
         for (int i = 0; i < l.parts; i++) n += (l.splits[i] + c - 1) / c;
-        const int64_t cost = p.big ? (tiles * n >= 768 ? 1 : 2) * 4096 - c
+        const int64_t cost = p.big ? (tiles * n >= 320 ? 1 : 2) * 4096 - c
                                    : (tiles * n + 1023) / 1024 * (c + 1024);
         if (!cols || cost < best) {
             cols = c;
