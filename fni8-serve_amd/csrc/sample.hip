@@ -730,6 +730,7 @@ __device__ __forceinline__ void find_ends(Shared& sh, Turn& turn, const Work& w,
                                           const Row& r, double tail, Long& more) {
     constexpr int B = kBins / kThreads;
     constexpr float f = 16.0f;
+    __syncthreads();  // where no list was tried, waves may still have to read the bound in sh.bin
     for (int i = threadIdx.x; i < kBins; i += kThreads) sh.h.count[i] = 0;
     if (threadIdx.x == 0) sh.bin = kBins - 2;
     __syncthreads();

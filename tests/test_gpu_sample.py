@@ -297,3 +297,16 @@ def test_more_parts_than_workgroups(pkg, cuda):
         assert got == [w[0] for w in expected(x[some.cuda()], u[some.cuda()], **kw)]
     del x
     torch.cuda.empty_cache()
+
+
+def test_many_long_prefixes_at_once(pkg, cuda):
+    """Flat rows under top-p, for whose prefix no list is tried: more workgroups than the device
+    holds, so that their waves run apart.  Every wave has to go the same way."""
+    x, u = logits(1500, 20011, seed=15, spread=1.0, peaks=1)
+    kw = dict(temperature=1.5, top_p=0.95)
+    got, logp = pkg.sample(x, u, return_logprobs=True, **kw)
+    some = torch.arange(0, 1500, 53, device="cuda")
+    assert got[some].tolist() == [w[0] for w in expected(x[some], u[some], **kw)]
+    for _ in range(3):
+        again, logp2 = pkg.sample(x, u, return_logprobs=True, **kw)
+        assert torch.equal(again, got) and torch.equal(logp2, logp)
