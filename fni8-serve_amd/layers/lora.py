@@ -38,23 +38,25 @@ class AdapterBatch:
 
     def assign(self, ids: torch.Tensor) -> None:
         """ids int [rows]: each row's adapter, any number outside [0, num_adapters) for none.
-        Nothing waits for the GPU.  The plan lies in memory that is kept, one for each power of
-        two of rows: captured graphs of several batch sizes each read what the last assign of
-        that many rows left there, so assign before a replay, on its stream."""
+        Nothing waits for the GPU.  The plan lies in memory that is kept, its own for every number
+        of rows (4 bytes a row and an adapter): a captured graph of so many rows reads what the
+        last assign of that many left there, so assign before a replay, on its stream."""
         if ids.dim() != 1 or ids.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"ids must be int32 or int64 [rows] (got {ids.dtype}, "
                              f"{tuple(ids.shape)})")
         self.ids, self.plan = ids, None
         if ids.is_cuda:
-            plan = ops.lora_plan(ids, self.num_adapters)
-            n = ids.numel()
-            key = ids.device, n.bit_length()
-            kept = self._kept.get(key)
-            if kept is None:
-                kept = self._kept[key] = ops.LoraPlan(torch.empty_like(plan.seg_off),
-                                                      plan.rows.new_empty(1 << n.bit_length()))
-            self.plan = ops.LoraPlan(kept.seg_off.copy_(plan.seg_off),
-                                     kept.rows[:n].copy_(plan.rows))
+            self.plan = self._keep(ops.lora_plan(ids, self.num_adapters))
+
+    def _keep(self, plan: ops.LoraPlan) -> ops.LoraPlan:
+        """The plan, copied to the memory of its number of rows."""
+        key = plan.rows.device, plan.rows.numel()
+        kept = self._kept.get(key)
+        if kept is None:
+            kept = self._kept[key] = ops.LoraPlan(*(torch.empty_like(t) for t in plan))
+        for to, t in zip(kept, plan):
+            to.copy_(t)
+        return kept
 
     def clear(self) -> None:
         """No row has an adapter: the modules are the linears that they wrap."""

@@ -83,3 +83,24 @@ def test_the_mlp_calls_an_adapted_linear(pkg):
     assert torch.equal(y[1:], plain[1:]) and not torch.equal(y[0], plain[0])
     h = mlp.gate_up_proj(x)
     assert torch.equal(mlp.down_proj(mlp.act_fn(h)), y)
+
+
+def plan_of(pkg, ids, slots):
+    """ops.lora_plan's result, made on the host."""
+    e = torch.where((ids < 0) | (ids >= slots), slots, ids)
+    off = torch.cat([torch.zeros(1, dtype=torch.long), torch.bincount(e, minlength=slots + 1).cumsum(0)])
+    return pkg.LoraPlan(off.int(), torch.argsort(e, stable=True).int())
+
+
+def test_every_number_of_rows_has_its_own_plan(pkg):
+    batch = pkg.AdapterBatch(3)
+    g = torch.Generator().manual_seed(1)
+    ids = {n: torch.randint(-1, 3, (n,), generator=g) for n in (1, 2, 3, 4, 5, 6, 7, 8)}
+    kept = {n: batch._keep(plan_of(pkg, v, 3)) for n, v in ids.items()}
+    for n, v in ids.items():
+        assert all(torch.equal(a, b) for a, b in zip(kept[n], plan_of(pkg, v, 3))), n
+    new = plan_of(pkg, torch.tensor([2, -1, 0, 1, 2]), 3)
+    again = batch._keep(new)                              # the memory of five rows, written anew
+    assert all(a.data_ptr() == b.data_ptr() for a, b in zip(again, kept[5]))
+    assert all(torch.equal(a, b) for a, b in zip(kept[5], new))
+    assert all(torch.equal(a, b) for a, b in zip(kept[6], plan_of(pkg, ids[6], 3)))

@@ -198,3 +198,29 @@ def test_ids_on_the_host_beside_rows_on_the_gpu_are_refused(pkg, wl, cuda):
     batch.assign(torch.zeros(4, dtype=torch.int64))
     with pytest.raises(ValueError):
         m(wl.activations(4, HIDDEN, seed=86).cuda())
+
+
+def test_graphs_of_neighbouring_sizes_keep_their_plans(pkg, wl, cuda):
+    """Every size assigned first, then all replayed: each graph has the plan of its own rows."""
+    batch = pkg.AdapterBatch(SLOTS)
+    m = wrap(pkg, pkg.LinearW8A8(qtensor(pkg, wl, 640, HIDDEN, 91)), batch, 92, splits=[512, 128])
+    g = torch.Generator().manual_seed(93)
+    graphs = {}
+    for n in (4, 5, 6, 7):
+        x = wl.activations(n, HIDDEN, seed=n).cuda()
+        batch.assign(torch.zeros(n, dtype=torch.int32, device="cuda"))
+        m(x)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = m(x)
+        graphs[n] = graph, x, y
+    for order in ((4, 5, 6, 7), (7, 6, 5, 4), (5, 7, 4, 6)):
+        ids = {n: torch.randint(-1, SLOTS, (n,), generator=g) for n in graphs}
+        for n in order:
+            batch.assign(ids[n].cuda())
+        for graph, _, _ in graphs.values():
+            graph.replay()
+        torch.cuda.synchronize()
+        for n, (_, x, y) in graphs.items():
+            assert close(y, by_row(pkg, m, x, ids[n])), (order, n)
