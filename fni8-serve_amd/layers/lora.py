@@ -35,6 +35,7 @@ class AdapterBatch:
         self.ids: torch.Tensor | None = None
         self.plan: ops.LoraPlan | None = None
         self._kept: dict[tuple[torch.device, int], ops.LoraPlan] = {}
+        self._assigned: set[tuple[torch.device, int]] = set()  # since the last clear
 
     def assign(self, ids: torch.Tensor) -> None:
         """ids int [rows]: each row's adapter, any number outside [0, num_adapters) for none.
@@ -56,11 +57,17 @@ class AdapterBatch:
             kept = self._kept[key] = ops.LoraPlan(*(torch.empty_like(t) for t in plan))
         for to, t in zip(kept, plan):
             to.copy_(t)
+        self._assigned.add(key)
         return kept
 
     def clear(self) -> None:
-        """No row has an adapter: the modules are the linears that they wrap."""
+        """No row has an adapter: the modules are the linears that they wrap, and a captured graph
+        adds nothing until the next assign of its number of rows."""
         self.ids = self.plan = None
+        for key in self._assigned:
+            seg_off, rows = self._kept[key]
+            seg_off.zero_()[-1:].fill_(rows.numel())      # all rows in the last segment
+        self._assigned.clear()
 
 
 class LoRALinear(nn.Module):

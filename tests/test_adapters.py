@@ -104,3 +104,15 @@ def test_every_number_of_rows_has_its_own_plan(pkg):
     assert all(a.data_ptr() == b.data_ptr() for a, b in zip(again, kept[5]))
     assert all(torch.equal(a, b) for a, b in zip(kept[5], new))
     assert all(torch.equal(a, b) for a, b in zip(kept[6], plan_of(pkg, ids[6], 3)))
+
+
+def test_clear_empties_the_kept_plans(pkg):
+    batch = pkg.AdapterBatch(3)
+    kept = [batch._keep(plan_of(pkg, torch.tensor([2, -1, 0, 1, 2])[:n], 3)) for n in (5, 3, 0)]
+    batch.clear()
+    for plan, n in zip(kept, (5, 3, 0)):
+        assert plan.seg_off.tolist() == [0, 0, 0, 0, n]
+        assert sorted(plan.rows.tolist()) == list(range(n))
+    new = plan_of(pkg, torch.tensor([0, 1, 1]), 3)
+    batch._keep(new)
+    assert all(torch.equal(a, b) for a, b in zip(kept[1], new))

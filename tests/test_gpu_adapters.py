@@ -224,3 +224,28 @@ def test_graphs_of_neighbouring_sizes_keep_their_plans(pkg, wl, cuda):
         torch.cuda.synchronize()
         for n, (_, x, y) in graphs.items():
             assert close(y, by_row(pkg, m, x, ids[n])), (order, n)
+
+
+def test_clear_reaches_captured_steps(pkg, wl, cuda):
+    batch = pkg.AdapterBatch(SLOTS)
+    m = wrap(pkg, pkg.LinearW8A8(qtensor(pkg, wl, 640, HIDDEN, 94)), batch, 95)
+    graphs = []
+    for n in (6, 70):
+        x = wl.activations(n, HIDDEN, seed=n).cuda()
+        batch.assign((torch.arange(n) % SLOTS).cuda())
+        m(x)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = m(x)
+        graphs.append((graph, x, y))
+    for rep in range(3):
+        batch.clear()
+        for graph, x, y in graphs:
+            graph.replay()
+            assert torch.equal(y, m.base(x)), rep
+        for graph, x, y in graphs:                        # and back
+            ids = (torch.arange(len(x)) + rep) % SLOTS
+            batch.assign(ids.cuda())
+            graph.replay()
+            assert close(y, by_row(pkg, m, x, ids)), rep
