@@ -54,7 +54,8 @@ class AdapterBatch:
         key = plan.rows.device, plan.rows.numel()
         kept = self._kept.get(key)
         if kept is None:
-            kept = self._kept[key] = ops.LoraPlan(*(torch.empty_like(t) for t in plan))
+            with torch.inference_mode(False):  # a later assign outside it writes these too
+                kept = self._kept[key] = ops.LoraPlan(*(torch.empty_like(t) for t in plan))
         for to, t in zip(kept, plan):
             to.copy_(t)
         self._assigned.add(key)

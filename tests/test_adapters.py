@@ -116,3 +116,17 @@ def test_clear_empties_the_kept_plans(pkg):
     new = plan_of(pkg, torch.tensor([0, 1, 1]), 3)
     batch._keep(new)
     assert all(torch.equal(a, b) for a, b in zip(kept[1], new))
+
+
+def test_plans_made_in_inference_mode_are_written_outside_it(pkg):
+    batch = pkg.AdapterBatch(3)
+    ids = torch.tensor([2, -1, 0, 1, 2])
+    with torch.inference_mode():
+        kept = batch._keep(plan_of(pkg, ids, 3))
+    new = plan_of(pkg, ids.flip(0), 3)
+    batch._keep(new)
+    assert all(torch.equal(a, b) for a, b in zip(kept, new))
+    batch.clear()
+    with torch.inference_mode():
+        batch._keep(plan_of(pkg, ids, 3))
+    assert all(torch.equal(a, b) for a, b in zip(kept, plan_of(pkg, ids, 3)))
