@@ -19,9 +19,11 @@ from collections.abc import Sequence
 
 import torch
 import torch.nn as nn
+from torch.nn.modules.module import _has_any_global_hook
 
 from .. import ops
 from .linear import LinearW8A8
+from .mlp import bare
 
 
 class AdapterBatch:
@@ -144,13 +146,16 @@ class LoRALinear(nn.Module):
         if self.batch.plan is None:
             raise ValueError(f"the batch's ids are on {self.batch.ids.device}, the rows on "
                              f"{x.device}")
+        # in place where nobody else can hold y: no hook, no forward but the linear's own
+        fresh = bare(self.base, LinearW8A8) and not _has_any_global_hook()
         return ops.lora_add(y, x, self.a, self.b, self.batch.plan, scaling=self.scaling,
-                            splits=self.splits, out=y)
+                            splits=self.splits, out=y if fresh else None)
 
     def _on_host(self, x: torch.Tensor, y: torch.Tensor) -> torch.Tensor:
         """CPU tensors, beside the linear's own fallback: sums in 32 bits, rounded once."""
         ids = self.batch.ids
-        x2, out = x.reshape(-1, self.in_features), y.reshape(-1, self.out_features).float()
+        x2, out = x.reshape(-1, self.in_features), y.reshape(-1, self.out_features)
+        out = out.to(torch.float32, copy=True)
         if ids.is_cuda or ids.numel() != x2.shape[0]:
             raise ValueError(f"{x2.shape[0]} rows on the host, {ids.numel()} ids on {ids.device}")
         for e in range(self.batch.num_adapters):

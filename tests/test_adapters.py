@@ -130,3 +130,19 @@ def test_plans_made_in_inference_mode_are_written_outside_it(pkg):
     with torch.inference_mode():
         batch._keep(plan_of(pkg, ids, 3))
     assert all(torch.equal(a, b) for a, b in zip(kept, plan_of(pkg, ids, 3)))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_what_the_base_returned_stays(pkg, dtype):
+    """A hook on the base, or a base that keeps its output, sees it as the base made it."""
+    base, batch = linear(pkg, 40, 32, 1), pkg.AdapterBatch(2)
+    m = pkg.LoRALinear(base, batch, rank=8)
+    m.load(0, [pair(8, 32, 40, 2)])
+    batch.assign(torch.tensor([0, -1, 0]))
+    x = torch.randn(3, 32).to(dtype)
+    plain, seen = base(x).clone(), []
+    handle = base.register_forward_hook(lambda mod, args, y: seen.append(y))
+    y = m(x)
+    handle.remove()
+    assert torch.equal(seen[0], plain) and not torch.equal(y[0], plain[0])
+    assert torch.equal(m(x), y)

@@ -249,3 +249,34 @@ def test_clear_reaches_captured_steps(pkg, wl, cuda):
             batch.assign(ids.cuda())
             graph.replay()
             assert close(y, by_row(pkg, m, x, ids)), rep
+
+
+class Keeps:
+    """A linear's forward of its own that hands out the same tensor again."""
+
+    def __init__(self, base):
+        self.inner, self.kept = base.forward, None
+
+    def __call__(self, x):
+        if self.kept is None:
+            self.kept = self.inner(x)
+        return self.kept
+
+
+def test_what_the_base_returned_stays(pkg, wl, cuda):
+    batch = pkg.AdapterBatch(SLOTS)
+    m = wrap(pkg, pkg.LinearW8A8(qtensor(pkg, wl, 640, HIDDEN, 96)), batch, 97)
+    x, ids = wl.activations(9, HIDDEN, seed=98).cuda(), torch.arange(9) % SLOTS - 1
+    batch.assign(ids.cuda())
+    plain, want, seen = m.base(x).clone(), m(x), []
+    keep = lambda mod, args, y: seen.append(y)  # noqa: E731
+    for register in (m.base.register_forward_hook, torch.nn.modules.module.register_module_forward_hook):
+        seen.clear()
+        handle = register(keep)
+        y = m(x)
+        handle.remove()
+        assert torch.equal(seen[0], plain) and torch.equal(y, want)
+    m.base.forward = Keeps(m.base)
+    for _ in range(3):
+        assert torch.equal(m(x), want)
+    assert torch.equal(m.base.forward.kept, plain)
