@@ -93,6 +93,14 @@ class LoRALinear(nn.Module):
         self.register_buffer("b", zeros(S, self.out_features, self.rank))
         self.register_buffer("scaling", torch.zeros(S, device=dev))
 
+    def _apply(self, fn, *args, **kw):
+        had = dict(self._buffers)  # they move with the module and keep their types in half()
+        super()._apply(fn, *args, **kw)
+        for name, t in had.items():
+            if self._buffers[name].dtype != t.dtype:
+                self._buffers[name] = t.to(self._buffers[name].device)
+        return self
+
     # what callers read of the linear (layers/mlp.py, layers/attention.py)
     @property
     def weight(self):

@@ -146,3 +146,19 @@ def test_what_the_base_returned_stays(pkg, dtype):
     handle.remove()
     assert torch.equal(seen[0], plain) and not torch.equal(y[0], plain[0])
     assert torch.equal(m(x), y)
+
+
+def test_matrices_keep_their_types(pkg):
+    """half(), float() and the like on a model that holds one: what the kernel reads stays."""
+    base, batch = linear(pkg, 40, 32, 1), pkg.AdapterBatch(2)
+    m = pkg.LoRALinear(base, batch, rank=8)
+    m.load(0, [pair(8, 32, 40, 2)], scaling=1 / 3)
+    batch.assign(torch.tensor([0, -1, 0]))
+    x = torch.randn(3, 32).half()
+    y, model = m(x), torch.nn.Sequential(m)
+    for to in (model.half, model.float, model.double, model.bfloat16, lambda: model.to(torch.float16)):
+        to()
+        assert (m.a.dtype, m.b.dtype, m.scaling.dtype) == (torch.float16, torch.float16, torch.float32)
+        assert torch.equal(m(x), y)
+    model.to("meta")
+    assert m.a.device.type == m.scaling.device.type == "meta" and m.scaling.dtype == torch.float32
