@@ -52,6 +52,8 @@ SIGNATURES = {
                                  _P, _P, _I, _I, _F, _I, _P, _P, _I, _P],
     "fni8_lora_add_f16": [_P, _I, _I, _I, _P, _P, _I, _I, _P, _I, _P, _P, _P, _P, _I, _P, _I, _P,
                           _I, _P],
+    "fni8_lora_add_ranks_f16": [_P, _I, _I, _I, _P, _P, _I, _I, _P, _I, _P, _P, _P, _P, _P, _I, _P,
+                                _I, _P, _I, _P],
     "fni8_sample": [_P, _C, _I, _I, _I, _P, _P, _F, _P, _I, _P, _F, _P, _F, _P, _P, _P, _I, _P],
 }
 STRING_FUNCS = ("fni8_strerror", "fni8_last_error", "fni8_version")

@@ -826,6 +826,17 @@ int fni8_lora_add_f16(const void* x, int64_t ldx, int64_t T, int64_t K, const vo
                       int64_t parts, const float* scaling, const int32_t* seg_off,
                       const int32_t* rows, const void* y, int64_t ldy, void* out, int64_t ldo,
                       void* workspace, int64_t workspace_bytes, void* stream) {
+    return fni8_lora_add_ranks_f16(x, ldx, T, K, a, b, S, rank, splits, parts, scaling, nullptr,
+                                   seg_off, rows, y, ldy, out, ldo, workspace, workspace_bytes,
+                                   stream);
+}
+
+int fni8_lora_add_ranks_f16(const void* x, int64_t ldx, int64_t T, int64_t K, const void* a,
+                            const void* b, int64_t S, int64_t rank, const int64_t* splits,
+                            int64_t parts, const float* scaling, const int32_t* ranks,
+                            const int32_t* seg_off, const int32_t* rows, const void* y,
+                            int64_t ldy, void* out, int64_t ldo, void* workspace,
+                            int64_t workspace_bytes, void* stream) {
     fni8h::g_detail[0] = 0;
     REQUIRE(x && a && b && splits && seg_off && rows && y && out, FNI8_ERR_NULL,
             "x, a, b, splits, seg_off, rows, y and out are required");
@@ -849,7 +860,8 @@ int fni8_lora_add_f16(const void* x, int64_t ldx, int64_t T, int64_t K, const vo
     REQUIRE(out != y || ldo == ldy, FNI8_ERR_STRIDE, "out is y, with ldo=%lld and ldy=%lld",
             (long long)ldo, (long long)ldy);
     REQUIRE(aligned(x, 2) && aligned(y, 2) && aligned(out, 2) && aligned(a, 16) &&
-                aligned(b, 16) && aligned(scaling, 4) && aligned(seg_off, 4) && aligned(rows, 4),
+                aligned(b, 16) && aligned(scaling, 4) && aligned(seg_off, 4) && aligned(rows, 4) &&
+                aligned(ranks, 4),
             FNI8_ERR_ALIGN, "a and b must be 16-byte aligned, the others element-aligned");
     const int64_t need = fni8h::lora_workspace_bytes(T, K, S, parts * rank);
     REQUIRE(!need || (workspace && aligned(workspace, 256)), FNI8_ERR_ALIGN,
@@ -862,6 +874,7 @@ int fni8_lora_add_f16(const void* x, int64_t ldx, int64_t T, int64_t K, const vo
     l.x = (const uint16_t*)x; l.ldx = ldx; l.T = T; l.K = K;
     l.a = (const uint16_t*)a; l.b = (const uint16_t*)b; l.S = S; l.rank = rank;
     l.splits = splits; l.parts = parts; l.scaling = scaling; l.seg_off = seg_off; l.rows = rows;
+    l.ranks = ranks;
     l.y = (const uint16_t*)y; l.ldy = ldy; l.out = (uint16_t*)out; l.ldo = ldo;
     l.work = static_cast<float*>(workspace);
     return fni8h::launch_lora_add(l, (hipStream_t)stream);

@@ -555,7 +555,7 @@ struct LoraAdd {
     const int64_t* splits;  // host memory
     int64_t parts;
     const float* scaling;
-    const int32_t *seg_off, *rows;
+    const int32_t *seg_off, *rows, *ranks;
     const uint16_t* y;
     int64_t ldy;
     uint16_t* out;

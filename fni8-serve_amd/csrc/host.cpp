@@ -644,9 +644,9 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
-// lora_add(y, x, a, b, seg_off, rows, scaling, splits, in_place)
+// lora_add(y, x, a, b, seg_off, rows, scaling, splits, ranks, in_place)
 PyObject* py_lora_add(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    return entry(a, n, 9, [](PyObject* const* a) {
+    return entry(a, n, 10, [](PyObject* const* a) {
         const Tensor &y = plain(a[0]), &x = plain(a[1]), &la = plain(a[2]), &lb = plain(a[3]);
         const Rows ry = rows(y, at::kHalf), rx = rows(x, at::kHalf);
         same(la, y, at::kHalf);
@@ -681,19 +681,26 @@ PyObject* py_lora_add(PyObject*, PyObject* const* a, Py_ssize_t n) {
             need(s.numel() == S);
             scaling = static_cast<const float*>(s.data_ptr());
         }
-        const bool in_place = a[8] == Py_True;
-        return [y, rx, ry, la, lb, S, rank, splits, parts, seg, order, scaling, in_place] {
+        const int32_t* ranks = nullptr;
+        if (a[8] != Py_None) {
+            const Tensor& r = plain(a[8]);
+            same(r, y, at::kInt);
+            need(r.dim() == 2 && r.size(0) == S && r.size(1) == parts);
+            ranks = static_cast<const int32_t*>(r.data_ptr());
+        }
+        const bool in_place = a[9] == Py_True;
+        return [y, rx, ry, la, lb, S, rank, splits, parts, seg, order, scaling, ranks, in_place] {
             c10::DeviceGuard guard(y.device());
             Tensor out = in_place ? y : at::empty(y.sizes(), y.options());
             const int64_t nw = fni8_lora_workspace_bytes(rx.M, rx.K, S, parts * rank);
             Scratch sc;
             sc.take(nw);
             sc.alloc(y);
-            check("fni8_lora_add_f16",
-                  fni8_lora_add_f16(rx.p, rx.ld, rx.M, rx.K, la.data_ptr(), lb.data_ptr(), S, rank,
-                                    splits.data(), parts, scaling, seg, order, ry.p, ry.ld,
-                                    out.data_ptr(), in_place ? ry.ld : ry.K, sc.at_<void>(0), nw,
-                                    stream_of(y)));
+            check("fni8_lora_add_ranks_f16",
+                  fni8_lora_add_ranks_f16(rx.p, rx.ld, rx.M, rx.K, la.data_ptr(), lb.data_ptr(), S,
+                                          rank, splits.data(), parts, scaling, ranks, seg, order,
+                                          ry.p, ry.ld, out.data_ptr(), in_place ? ry.ld : ry.K,
+                                          sc.at_<void>(0), nw, stream_of(y)));
             return One{out};
         };
     });

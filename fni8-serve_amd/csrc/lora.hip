@@ -34,7 +34,7 @@ struct Args {
     uint16_t* out;
     int64_t ldx, ldy, ldo;
     const float* scaling;
-    const int32_t *seg_off, *rows;
+    const int32_t *seg_off, *rows, *ranks;
     float* h;            // [kparts][T][R]
     int T, K, S, rank, R, kparts;
     int copy;            // out is not y: tokens without an adapter are copied
@@ -278,11 +278,17 @@ __device__ __forceinline__ bool find_block(const Args& a, int block, int& part, 
     return true;
 }
 
+// How many rows of the part are the adapter's: what the others (filled up) make of x is not
+// looked at, since 0 times an infinity is not 0.
+__device__ __forceinline__ int own_rank(const Args& a, int e, int part) {
+    return a.ranks ? a.ranks[(int64_t)e * a.parts + part] : a.rank;
+}
+
 // Eight consecutive values of a token's low-rank row, the parts added in order (MANY of them on
-// their way at once), scaled.
+// their way at once), scaled; 0 from `left` on.
 template <int MANY>
-__device__ __forceinline__ void low_rank(const Args& a, int pos, int part, int j, float scale,
-                                         float (&v)[8]) {
+__device__ __forceinline__ void low_rank(const Args& a, int pos, int part, int j, int left,
+                                         float scale, float (&v)[8]) {
     const float* h = a.h + (int64_t)pos * a.R + part * a.rank + j;
     const int64_t step = (int64_t)a.T * a.R;
 #pragma unroll
@@ -307,7 +313,7 @@ __device__ __forceinline__ void low_rank(const Args& a, int pos, int part, int j
         h += MANY * step;
     }
 #pragma unroll
-    for (int i = 0; i < 8; i++) v[i] *= scale;
+    for (int i = 0; i < 8; i++) v[i] = i < left ? v[i] * scale : 0.0f;
 }
 
 __device__ __forceinline__ uint32_t top_of(const float (&v)[8]) {
@@ -466,12 +472,13 @@ __global__ __launch_bounds__(kThreads, KS <= 2 ? 4 : KS == 4 ? 2 : 1) void expan
     int n = n0 + wave * 16 * QT;
     fetch(n, bf[0], in[0]);  // comes from memory, the low-rank rows from a cache
     const float scale = a.scaling ? a.scaling[e] : 1.0f;
+    const int own = own_rank(a, e, part);
     float v[KS][8];
     uint32_t top = 0;
     auto sum = [&](int s, float (&to)[8]) {
         const int j = s * 32 + 8 * g;
         if (t < count && j < a.rank) {
-            low_rank<8>(a, r0 + t, part, j, scale, to);
+            low_rank<8>(a, r0 + t, part, j, own - j, scale, to);
         } else {
 #pragma unroll
             for (int i = 0; i < 8; i++) to[i] = 0.0f;
@@ -573,12 +580,13 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(const Args a) {
     };
     // the low-rank rows before y: loads come back in order, and these come from the cache
     const float scale = a.scaling ? a.scaling[e] : 1.0f;
+    const int own = own_rank(a, e, part);
     float v[UNITS][8];
 #pragma unroll
     for (int i = 0; i < UNITS; i++) {
         const int u = threadIdx.x + i * kThreads, t = u / (KS * 4), j = u % (KS * 4) * 8;
         if (t < count && j < a.rank) {
-            low_rank<4>(a, r0 + t, part, j, scale, v[i]);
+            low_rank<4>(a, r0 + t, part, j, own - j, scale, v[i]);
         } else {
 #pragma unroll
             for (int k = 0; k < 8; k++) v[i][k] = 0.0f;
@@ -725,6 +733,7 @@ int launch_lora_add(const LoraAdd& l, hipStream_t st) {
     Args a{};
     a.x = l.x; a.ldx = l.ldx; a.y = l.y; a.ldy = l.ldy; a.out = l.out; a.ldo = l.ldo;
     a.a = l.a; a.b = l.b; a.scaling = l.scaling; a.seg_off = l.seg_off; a.rows = l.rows;
+    a.ranks = l.ranks;
     a.h = l.work;
     a.T = (int)l.T; a.K = (int)l.K; a.S = (int)l.S; a.rank = (int)l.rank; a.R = (int)R;
     a.kparts = (int)p.kparts;

@@ -92,6 +92,8 @@ class LoRALinear(nn.Module):
         self.register_buffer("a", zeros(S, len(self.splits) * self.rank, self.in_features))
         self.register_buffer("b", zeros(S, self.out_features, self.rank))
         self.register_buffer("scaling", torch.zeros(S, device=dev))
+        # of each part: rows that are filled up, and slots that are empty, add nothing
+        self.register_buffer("ranks", torch.zeros(S, len(self.splits), dtype=torch.int32, device=dev))
 
     def _apply(self, fn, *args, **kw):
         had = dict(self._buffers)  # they move with the module and keep their types in half()
@@ -100,6 +102,11 @@ class LoRALinear(nn.Module):
             if self._buffers[name].dtype != t.dtype:
                 self._buffers[name] = t.to(self._buffers[name].device)
         return self
+
+    def _load_from_state_dict(self, state, prefix, *args):
+        if prefix + "a" in state and prefix + "ranks" not in state:  # saved without: all rows
+            state[prefix + "ranks"] = torch.full_like(self.ranks, self.rank)
+        super()._load_from_state_dict(state, prefix, *args)
 
     # what callers read of the linear (layers/mlp.py, layers/attention.py)
     @property
@@ -140,6 +147,8 @@ class LoRALinear(nn.Module):
                 self.b[slot, n:n + wide, :r].copy_(pair[1])
             n += wide
         self.scaling[slot] = scaling
+        for p, pair in enumerate(parts):
+            self.ranks[slot, p] = 0 if pair is None else pair[0].shape[0]
 
     def unload(self, slot: int) -> None:
         """Rows of this adapter get nothing added from now on."""
@@ -157,7 +166,7 @@ class LoRALinear(nn.Module):
         # in place where nobody else can hold y: no hook, no forward but the linear's own
         fresh = bare(self.base, LinearW8A8) and not _has_any_global_hook()
         return ops.lora_add(y, x, self.a, self.b, self.batch.plan, scaling=self.scaling,
-                            splits=self.splits, out=y if fresh else None)
+                            splits=self.splits, out=y if fresh else None, ranks=self.ranks)
 
     def _on_host(self, x: torch.Tensor, y: torch.Tensor) -> torch.Tensor:
         """CPU tensors, beside the linear's own fallback: sums in 32 bits, rounded once."""
@@ -169,11 +178,10 @@ class LoRALinear(nn.Module):
         for e in range(self.batch.num_adapters):
             at = (ids == e).nonzero().squeeze(1)
             if at.numel():
-                low = (x2[at].float() @ self.a[e].float().t()) * self.scaling[e]
-                up, n = [], 0
+                rows, n = x2[at].float(), 0
                 for p, wide in enumerate(self.splits):
-                    up.append(low[:, p * self.rank:(p + 1) * self.rank]
-                              @ self.b[e, n:n + wide].float().t())
+                    r, j = int(self.ranks[e, p]), p * self.rank
+                    low = (rows @ self.a[e, j:j + r].float().t()) * self.scaling[e]
+                    out[at, n:n + wide] += low @ self.b[e, n:n + wide, :r].float().t()
                     n += wide
-                out[at] += torch.cat(up, 1)
         return out.to(y.dtype).reshape(y.shape)

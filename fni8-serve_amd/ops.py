@@ -831,7 +831,7 @@ def lora_plan(ids: torch.Tensor, num_adapters: int) -> LoraPlan:
 
 def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, plan: LoraPlan,
              scaling: torch.Tensor | None = None, splits: Sequence[int] | None = None,
-             out: torch.Tensor | None = None) -> torch.Tensor:
+             out: torch.Tensor | None = None, ranks: torch.Tensor | None = None) -> torch.Tensor:
     """y plus each token's own low-rank product, y fp16 [..., N] -> fp16 [..., N] in one call
     for all adapters (the unmerged forward of fni8serve/training/lora.py:14-170):
 
@@ -842,9 +842,12 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     merged projection, p(n) the part of column n (None: one part).  scaling fp32 [S] (None: 1).
     out: where the result goes; y itself adds in place and leaves rows without an adapter
     untouched; None allocates it.  rank is a multiple of 8, at most 256 (zeros fill up).
+    ranks int32 [S, parts]: how many of a part's rank are the adapter's own; the others add
+    nothing, also where x holds infinities, of which zeros make NaN (None: all).
     Sums are fp32; the result is rounded once."""
     if y.is_cuda and (out is None or out is y):
-        z = _lib.host().lora_add(y, x, a, b, plan[0], plan[1], scaling, splits, out is y)
+        z = _lib.host().lora_add(y, x, a, b, plan[0], plan[1], scaling, splits, ranks,
+                                 out is y)
         if z is not None:
             return y if out is y else z
     for name, t, dims in (("y", y, 0), ("x", x, 0), ("a", a, 3), ("b", b, 3)):
@@ -862,6 +865,11 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
         if scaling.dtype != torch.float32 or scaling.numel() != S:
             raise ValueError(f"scaling must be fp32 with {S} entries")
         scaling = scaling.reshape(-1).contiguous()
+    if ranks is not None:
+        if ranks.dtype != torch.int32 or ranks.shape != (S, len(splits)):
+            raise ValueError(f"ranks must be int32 [{S}, {len(splits)}] (got {ranks.dtype}, "
+                             f"{tuple(ranks.shape)})")
+        ranks = ranks.contiguous()
     seg_off, rows = plan
     for name, t, n in (("seg_off", seg_off, S + 2), ("rows", rows, y.numel() // max(N, 1))):
         if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
@@ -871,7 +879,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
         raise ValueError(f"x {tuple(x.shape)} and y {tuple(y.shape)} differ in tokens")
     if rank % 8 or not 0 < rank <= 256:
         raise ValueError(f"rank {rank} must be a multiple of 8, at most 256 (zeros fill up)")
-    dev = _require_cuda("lora_add", y, x, a, b, seg_off, rows, scaling, out)
+    dev = _require_cuda("lora_add", y, x, a, b, seg_off, rows, scaling, ranks, out)
     x2, ldx = _rows(x, K)
     if out is None:
         y2, ldy = _rows(y, N)
@@ -892,10 +900,10 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     nw = int(_lib.load().fni8_lora_workspace_bytes(T, K, S, len(splits) * rank))
     work = torch.empty(nw, dtype=torch.uint8, device=dev) if nw else None
     with torch.cuda.device(dev):
-        _lib.call("fni8_lora_add_f16", _ptr(x2), ldx, T, K, _ptr(a), _ptr(b), S, rank,
+        _lib.call("fni8_lora_add_ranks_f16", _ptr(x2), ldx, T, K, _ptr(a), _ptr(b), S, rank,
                   (ctypes.c_int64 * len(splits))(*splits), len(splits), _ptr(scaling),
-                  _ptr(seg_off), _ptr(rows), _ptr(y2), ldy, _ptr(o2), ldo, _ptr(work), nw,
-                  _stream(dev))
+                  _ptr(ranks), _ptr(seg_off), _ptr(rows), _ptr(y2), ldy, _ptr(o2), ldo,
+                  _ptr(work), nw, _stream(dev))
     return out
 
 

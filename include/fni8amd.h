@@ -559,6 +559,19 @@ int fni8_lora_add_f16(const void* x, int64_t ldx, int64_t T, int64_t K, const vo
                       const int32_t* rows, const void* y, int64_t ldy, void* out, int64_t ldo,
                       void* workspace, int64_t workspace_bytes, void* stream);
 
+/*
+ * The same where adapters have ranks of their own:
+ *   ranks    int32 [S, parts], or NULL for `rank` everywhere: how many of a part's rows of a
+ *            are the adapter's.  The others add nothing, also where x holds infinities or NaN
+ *            (0 times these is NaN); b is 0 there.  0 or less: the adapter has none in the part.
+ */
+int fni8_lora_add_ranks_f16(const void* x, int64_t ldx, int64_t T, int64_t K, const void* a,
+                            const void* b, int64_t S, int64_t rank, const int64_t* splits,
+                            int64_t parts, const float* scaling, const int32_t* ranks,
+                            const int32_t* seg_off, const int32_t* rows, const void* y,
+                            int64_t ldy, void* out, int64_t ldo, void* workspace,
+                            int64_t workspace_bytes, void* stream);
+
 /* Bytes of fni8_lora_add_f16's workspace (0 where its arguments are out of range). */
 int64_t fni8_lora_workspace_bytes(int64_t T, int64_t K, int64_t S, int64_t all_rank);
 

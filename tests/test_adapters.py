@@ -162,3 +162,47 @@ def test_matrices_keep_their_types(pkg):
         assert torch.equal(m(x), y)
     model.to("meta")
     assert m.a.device.type == m.scaling.device.type == "meta" and m.scaling.dtype == torch.float32
+
+
+def test_nothing_is_added_where_a_slot_has_nothing(pkg):
+    """Rows with infinities keep what the base makes of them in empty and unloaded slots and in
+    parts without an adapter; a rank that is filled up changes nothing."""
+    g = torch.Generator().manual_seed(6)
+    q = torch.randint(1, 128, (40, 32), generator=g, dtype=torch.int8)   # no 0: no NaN from inf
+    base = pkg.LinearW8A8(pkg.QTensor(q, torch.rand(40, generator=g) * 0.01 + 0.01, scheme="per_row_i8"))
+    batch = pkg.AdapterBatch(4)
+    m = pkg.LoRALinear(base, batch, rank=16, splits=[24, 16])
+    one, two = pair(1, 32, 24, 7), pair(1, 32, 16, 8)
+    m.load(0, [None, two])
+    m.load(1, [one, two])
+    m.load(2, [one, two])
+    m.unload(2)
+    x = torch.randn(4, 32, generator=g).half()
+    x[:, 5] = torch.inf
+    plain = base(x)
+    assert plain.isinf().all()
+    batch.assign(torch.tensor([0, 1, 2, 3]))
+    y = m(x)
+    assert torch.equal(y[2:], plain[2:]) and torch.equal(y[0, :24], plain[0, :24])
+    # one rank: an infinity of either sign times B, added to the base's plus infinity
+    for p, (n, w, (a, b)) in enumerate(((0, 24, one), (24, 16, two))):
+        up = torch.inf * torch.sign(a[0, 5].float()) * b[:, 0].float()
+        assert torch.equal(y[1, n:n + w].isinf(), up > 0) and torch.equal(y[1, n:n + w].isnan(), up < 0)
+
+
+def test_matrices_saved_without_ranks(pkg):
+    """A state without them has all rows."""
+    base = linear(pkg, 40, 32, 1)
+    m, n = (pkg.LoRALinear(base, pkg.AdapterBatch(2), rank=8) for _ in range(2))
+    m.load(1, [pair(8, 32, 40, 2)], scaling=0.5)
+    state = m.state_dict()
+    n.load_state_dict(state)
+    assert torch.equal(n.ranks, m.ranks) and n.ranks.tolist() == [[0], [8]]
+    del state["ranks"]
+    k = pkg.LoRALinear(base, pkg.AdapterBatch(2), rank=8)
+    k.load_state_dict(state)
+    x, ids = torch.randn(3, 32).half(), torch.tensor([1, -1, 0])
+    for t in (m, n, k):
+        t.batch.assign(ids)
+    assert torch.equal(n(x), m(x)) and torch.equal(k(x), m(x))
+    assert k.ranks.tolist() == [[8], [8]]

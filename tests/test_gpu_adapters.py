@@ -280,3 +280,29 @@ def test_what_the_base_returned_stays(pkg, wl, cuda):
     for _ in range(3):
         assert torch.equal(m(x), want)
     assert torch.equal(m.base.forward.kept, plain)
+
+
+def test_nothing_is_added_where_a_slot_has_nothing(pkg, wl, cuda):
+    """Rows with infinities keep what the base makes of them in empty and unloaded slots and in
+    parts without an adapter."""
+    g = torch.Generator().manual_seed(99)
+    codes = torch.randint(0, 7, (768, HIDDEN), generator=g, dtype=torch.uint8)   # all below 0
+    data = codes[:, ::2] | codes[:, 1::2] << 4
+    base = pkg.LinearW8A8(pkg.QTensor(data.cuda(), torch.full((768, HIDDEN // 64), 0.02, device="cuda"),
+                                      scheme="per_group_i4", group_size=64, codebook="nf4"))
+    batch = pkg.AdapterBatch(SLOTS)
+    m = wrap(pkg, base, batch, 100, splits=[512, 256])   # slot 1 has no first part
+    m.unload(3)
+    for rows in (6, 1200):
+        x = wl.activations(rows, HIDDEN, seed=rows).cuda()
+        ids = torch.arange(rows) % (SLOTS + 1) - 1
+        batch.assign(ids.cuda())
+        clean = m(x)
+        assert close(clean, by_row(pkg, m, x, ids))
+        x[:, 7] = torch.inf
+        plain, y = base(x), m(x)
+        assert plain.isinf().all()
+        bare = (ids < 0) | (ids == 3) | (ids == SLOTS - 1)
+        assert torch.equal(y[bare], plain[bare])
+        assert torch.equal(y[ids == 1, :512], plain[ids == 1, :512])
+        assert not y.isfinite().any()

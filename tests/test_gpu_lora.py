@@ -211,3 +211,50 @@ def test_no_tokens(pkg, cuda):
     x, y, a, b, s, ids = make(0, 64, [96], 8, 2, seed=3)
     plan = pkg.lora_plan(ids.cuda(), 2)
     assert pkg.lora_add(y.cuda(), x.cuda(), a.cuda(), b.cuda(), plan, s.cuda()).shape == (0, 96)
+
+
+@pytest.mark.parametrize("T,K,splits,rank,S", [
+    (1, 64, [72], 8, 2), (40, 136, [48, 16], 16, 5), (70, 100, [31, 8, 9], 40, 6),
+    (50, 72, [65], 136, 3), (1100, 136, [128, 64], 32, 5), (1100, 96, [72, 60], 72, 4),
+    (1100, 264, [64], 256, 3)])
+def test_ranks_of_their_own(pkg, cuda, T, K, splits, rank, S):
+    """What a's filled-up rows hold, and what they make of infinities, is not looked at."""
+    x, y, a, b, s, ids = make(T, K, splits, rank, S, seed=T + rank)
+    rng = random.Random(rank)
+    own = torch.tensor([[rng.choice((-3, 0, 1, rng.randint(1, rank), rank - 1, rank, rank + 5))
+                         for _ in splits] for _ in range(S)], dtype=torch.int32)
+    own[0, 0] = 0                                         # and one with nothing at all
+    own[S - 1] = 0
+    for e in range(S):
+        n = 0
+        for p, wide in enumerate(splits):
+            r = min(max(int(own[e, p]), 0), rank)
+            a[e, p * rank + r:(p + 1) * rank] = 0
+            b[e, n:n + wide, r:] = 0
+            n += wide
+    want = check(pkg, x, y, a, b, s, ids, splits)
+    plan = pkg.lora_plan(ids.cuda(), S)
+    bad = a.clone()
+    for e in range(S):
+        for p in range(len(splits)):
+            bad[e, p * rank + min(max(int(own[e, p]), 0), rank):(p + 1) * rank] = math.nan
+    dev = [t.cuda() for t in (y, x, bad, b)]
+    got = pkg.lora_add(*dev, plan, s.cuda(), splits, ranks=own.cuda())
+    assert torch.equal(got, want)
+    place = y.cuda()
+    pkg.lora_add(place, *dev[1:], plan, s.cuda(), splits, out=place, ranks=own.cuda())
+    assert torch.equal(place, want)
+    x[::3, K // 2] = math.inf
+    got = pkg.lora_add(y.cuda(), x.cuda(), a.cuda(), b.cuda(), plan, s.cuda(), splits,
+                       ranks=own.cuda()).cpu()
+    for t in range(0, T, 3):
+        n = 0
+        for p, wide in enumerate(splits):
+            e = int(ids[t])
+            if not 0 <= e < S or own[e, p] <= 0:
+                assert torch.equal(got[t, n:n + wide], y[t, n:n + wide]), (t, p)
+            else:
+                assert not got[t, n:n + wide].isfinite().any(), (t, p)
+            n += wide
+    clean = torch.arange(T) % 3 != 0
+    assert torch.equal(got[clean], want.cpu()[clean])

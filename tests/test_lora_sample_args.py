@@ -125,3 +125,21 @@ def test_lora_refuses(pkg):
             pkg.lora_plan(torch.zeros(4, dtype=torch.int32), n)
     with pytest.raises(ValueError, match="GPU"):
         pkg.lora_plan(torch.zeros(4, dtype=torch.int32), 2)
+
+
+def test_lora_refuses_ranks(pkg, lib):
+    h = torch.float16
+    y, x = torch.zeros(4, 48, dtype=h), torch.zeros(4, 64, dtype=h)
+    a, b = torch.zeros(2, 32, 64, dtype=h), torch.zeros(2, 48, 16, dtype=h)
+    plan = pkg.LoraPlan(torch.zeros(4, dtype=torch.int32), torch.zeros(4, dtype=torch.int32))
+    i = torch.int32
+    for bad in (torch.zeros(2, dtype=i), torch.zeros(2, 1, dtype=i), torch.zeros(3, 2, dtype=i),
+                torch.zeros(2, 2), torch.zeros(2, 2, dtype=torch.int64)):
+        with pytest.raises(ValueError, match="ranks"):
+            pkg.lora_add(y, x, a, b, plan, splits=[32, 16], ranks=bad)
+    with pytest.raises(ValueError, match="GPU"):
+        pkg.lora_add(y, x, a, b, plan, splits=[32, 16], ranks=torch.zeros(2, 2, dtype=i))
+    splits = (ctypes.c_int64 * 2)(32, 16)
+    rc = lib.fni8_lora_add_ranks_f16(FAKE, 64, 4, 64, FAKE, FAKE, 2, 16, splits, 2, None, P(0x1002),
+                                     FAKE, FAKE, FAKE, 48, FAKE, 48, FAKE, 1 << 30, None)
+    assert rc == -3 and lib.fni8_last_error()
