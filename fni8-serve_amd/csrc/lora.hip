@@ -326,11 +326,11 @@ __device__ __forceinline__ uint32_t top_of(const float (&v)[8]) {
     return m;
 }
 
-// The power of two that brings a token's largest |h| (its bits) to 2^8; 0 for a row of zeros and
-// one with infinities or NaN.
+// The power of two that brings a token's largest |h| (its bits) to 2^8; 0 for a row of zeros.
+// Beside infinities and NaN, which decide the row, whatever is finite stays so in fp16.
 __device__ __forceinline__ int shift_of(uint32_t top) {
     const int up = 135 - (int)(top >> 23);
-    return top >= 0x7f800000u || top == 0 ? 0 : up > 120 ? 120 : up;
+    return top >= 0x7f800000u ? -113 : top == 0 ? 0 : up > 120 ? 120 : up;
 }
 
 __device__ __forceinline__ void split8(const float (&v)[8], uint32_t top, h8& hi, h8& lo) {

@@ -258,3 +258,20 @@ def test_ranks_of_their_own(pkg, cuda, T, K, splits, rank, S):
             n += wide
     clean = torch.arange(T) % 3 != 0
     assert torch.equal(got[clean], want.cpu()[clean])
+
+
+@pytest.mark.parametrize("T", [5, 1100])
+def test_finite_values_beside_an_infinite_one(pkg, cuda, T):
+    """A low-rank value that overflows 32 bits, others that are finite but beyond fp16: the row is
+    infinite with that one's sign, not the difference of two infinities."""
+    h = torch.float16
+    x = torch.ones(T, 8, dtype=h)
+    a, b = torch.zeros(1, 8, 8, dtype=h), torch.zeros(1, 64, 8, dtype=h)
+    a[0, 0, 0], a[0, 1, 0], a[0, 2, 0] = 2.0, 0.5, 2.0 ** -14
+    b[0, :, 0] = torch.where(torch.arange(64) % 2 == 0, 1.0, -1.0)
+    b[0, :, 1] = -b[0, :, 0]
+    b[0, :, 2] = 3.0
+    s, y = torch.tensor([3e38]), torch.randn(T, 64).half()
+    got = pkg.lora_add(y.cuda(), x.cuda(), a.cuda(), b.cuda(),
+                       pkg.lora_plan(torch.zeros(T, dtype=torch.int32, device="cuda"), 1), s.cuda())
+    assert torch.equal(got.cpu(), (b[0, :, 0].float() * math.inf).half().expand(T, 64))
