@@ -1,4 +1,6 @@
 """AdapterBatch and LoRALinear on the CPU, and what they and Sampler refuse."""
+from types import SimpleNamespace
+
 import pytest
 import torch
 
@@ -206,3 +208,28 @@ def test_matrices_saved_without_ranks(pkg):
         t.batch.assign(ids)
     assert torch.equal(n(x), m(x)) and torch.equal(k(x), m(x))
     assert k.ranks.tolist() == [[8], [8]]
+
+
+def test_without_ids_it_has_the_rule_of_its_base(pkg):
+    """The fused chains take it as they take its base, unless calling it does more."""
+    gpu = SimpleNamespace(is_cuda=True)
+    batch = pkg.AdapterBatch(2)
+    m = pkg.LoRALinear(linear(pkg, 40, 32, 1), batch, rank=8)
+    assert m._int8_ok(gpu) and not m._int8_ok(torch.zeros(1, 32))
+    batch.assign(torch.tensor([0]))
+    assert not m._int8_ok(gpu)
+    batch.clear()
+    assert m._int8_ok(gpu)
+    for module in (m, m.base):
+        handle = module.register_forward_hook(lambda *a: None)
+        assert not m._int8_ok(gpu)
+        handle.remove()
+        assert m._int8_ok(gpu)
+    handle = torch.nn.modules.module.register_module_forward_hook(lambda *a: None)
+    assert not m._int8_ok(gpu)
+    handle.remove()
+    m.base.forward = m.base.forward
+    assert not m._int8_ok(gpu)
+    class Other(pkg.LoRALinear):
+        pass
+    assert not Other(linear(pkg, 40, 32, 1), batch, rank=8)._int8_ok(gpu)

@@ -306,3 +306,26 @@ def test_nothing_is_added_where_a_slot_has_nothing(pkg, wl, cuda):
         assert torch.equal(y[bare], plain[bare])
         assert torch.equal(y[ids == 1, :512], plain[ids == 1, :512])
         assert not y.isfinite().any()
+
+
+def test_the_mlp_fuses_again_without_adapters(pkg, wl, cuda, monkeypatch):
+    batch = pkg.AdapterBatch(SLOTS)
+    up, down = qtensor(pkg, wl, 2 * INTER, HIDDEN, 3), qtensor(pkg, wl, HIDDEN, INTER, 4)
+    plain, mlp = pkg.GatedMLP(up, down), pkg.GatedMLP(up, down)
+    mlp.gate_up_proj = wrap(pkg, mlp.gate_up_proj, batch, 5, [INTER, INTER])
+    mlp.down_proj = wrap(pkg, mlp.down_proj, batch, 6)
+    calls, fused = [], pkg.ops.act_and_mul_quant
+    monkeypatch.setattr(pkg.ops, "act_and_mul_quant", lambda *a: calls.append(1) or fused(*a))
+    for rows in (1, 4, 5, 70):
+        x = wl.activations(rows, HIDDEN, seed=rows).cuda()
+        calls.clear()
+        assert torch.equal(mlp(x), plain(x)) and len(calls) == (rows >= 5)
+        batch.assign(torch.zeros(rows, dtype=torch.int32, device="cuda"))
+        calls.clear()
+        assert not torch.equal(mlp(x), plain(x)) and not calls
+        batch.clear()
+        assert torch.equal(mlp(x), plain(x))
+        seen = []
+        handle = mlp.down_proj.register_forward_hook(lambda *a: seen.append(1))
+        assert torch.equal(mlp(x), plain(x)) and seen
+        handle.remove()
