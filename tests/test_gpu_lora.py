@@ -275,3 +275,19 @@ def test_finite_values_beside_an_infinite_one(pkg, cuda, T):
     got = pkg.lora_add(y.cuda(), x.cuda(), a.cuda(), b.cuda(),
                        pkg.lora_plan(torch.zeros(T, dtype=torch.int32, device="cuda"), 1), s.cuda())
     assert torch.equal(got.cpu(), (b[0, :, 0].float() * math.inf).half().expand(T, 64))
+
+
+@pytest.mark.parametrize("T", [3, 1100])
+def test_out_beside_y_in_the_same_rows(pkg, cuda, T):
+    """y and out as two column ranges of one tensor are other memory; shifted views are refused."""
+    x, y, a, b, s, ids = make(T, 72, [40, 16], 8, 3, seed=T)
+    plan = pkg.lora_plan(ids.cuda(), 3)
+    want = pkg.lora_add(y.cuda(), x.cuda(), a.cuda(), b.cuda(), plan, s.cuda(), [40, 16])
+    wide = torch.zeros(T, 120, dtype=torch.float16, device="cuda")
+    vy, vo = wide[:, 4:60], wide[:, 60:116]
+    vy.copy_(y)
+    assert pkg.lora_add(vy, x.cuda(), a.cuda(), b.cuda(), plan, s.cuda(), [40, 16], out=vo) is vo
+    assert torch.equal(vo, want) and torch.equal(vy.cpu(), y)
+    for bad in (wide[:, 5:61], wide[:, 59:115], wide.view(-1)[4:4 + T * 56].view(T, 56)):
+        with pytest.raises((ValueError, RuntimeError), match="overlaps|other strides"):
+            pkg.lora_add(vy, x.cuda(), a.cuda(), b.cuda(), plan, s.cuda(), [40, 16], out=bad)

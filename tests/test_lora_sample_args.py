@@ -1,6 +1,7 @@
 """What lora_plan, lora_add, sample and their C entry points refuse, without a GPU."""
 import ctypes
 import math
+import random
 from importlib import import_module
 
 import pytest
@@ -143,3 +144,29 @@ def test_lora_refuses_ranks(pkg, lib):
     rc = lib.fni8_lora_add_ranks_f16(FAKE, 64, 4, 64, FAKE, FAKE, 2, 16, splits, 2, None, P(0x1002),
                                      FAKE, FAKE, FAKE, 48, FAKE, 48, FAKE, 1 << 30, None)
     assert rc == -3 and lib.fni8_last_error()
+
+
+def test_lora_refuses_an_out_that_overlaps_y(lib):
+    """Every way that rows of two views can lie, against a set of their elements.  No workspace:
+    a call that gets past this check fails at that one."""
+    rng, seen = random.Random(1), {True: 0, False: 0}
+    for _ in range(3000):
+        T, N = rng.choice((1, 2, 3, 7)), rng.choice((1, 2, 5))
+        ldy, ldo = N + rng.randint(0, 8), N + rng.randint(0, 8)
+        if rng.random() < 0.5:
+            ldo = ldy
+        d = rng.randint(-60, 60)
+        if d == 0:
+            continue
+        y = {t * ldy + n for t in range(T) for n in range(N)}
+        out = {d + t * ldo + n for t in range(T) for n in range(N)}
+        rc = lora(lib, T=T, splits=[N], y=P(0x1000), ldy=ldy, out=P(0x1000 + 2 * d), ldo=ldo,
+                  work=None)
+        assert rc == (-4 if y & out else -3), (T, N, ldy, ldo, d)
+        seen[bool(y & out)] += 1
+    assert min(seen.values()) > 300
+    assert lora(lib, work=None) == -3                     # in place
+    far = dict(T=1 << 23, ldy=1 << 24, ldo=1 << 24, work=None)
+    assert lora(lib, **far, out=P(0x1000 + 2 * 48)) == -3   # two halves of the same rows
+    assert lora(lib, **far, out=P(0x1000 + 2 * 47)) == -4
+    assert lora(lib, **dict(far, ldo=(1 << 24) - 8), out=P(0x1000 + 2 * 48)) == -4
