@@ -244,6 +244,22 @@ bool lora_in_range(int64_t T, int64_t K, int64_t S, int64_t all_rank) {
            all_rank > 0 && all_rank <= 256 * FNI8_LORA_MAX_PARTS;
 }
 
+// Whether T rows of `wide` bytes at p, ldp bytes apart, and as many at q, ldq apart, share any.
+bool rows_meet(const void* p, int64_t ldp, const void* q, int64_t ldq, int64_t T, int64_t wide) {
+    const int64_t d = (int64_t)((uintptr_t)q - (uintptr_t)p);
+    if (T == 0 || d >= (T - 1) * ldp + wide || -d >= (T - 1) * ldq + wide) return false;
+    // rows at s of p's are met by q's at or before s, or by the next
+    auto met = [&](int64_t s, int64_t first, int64_t last) {
+        const int64_t j = s >= 0 ? s / ldq : -((-s + ldq - 1) / ldq);
+        return (j >= first && j <= last && s - j * ldq < wide) ||
+               (j + 1 >= first && j + 1 <= last && (j + 1) * ldq - s < wide);
+    };
+    if (ldp == ldq) return met(-d, 1 - T, T - 1);  // rows i of p and i + j of q
+    for (int64_t i = 0; i < T; i++)
+        if (met(i * ldp - d, 0, T - 1)) return true;
+    return false;
+}
+
 bool sample_in_range(int64_t B, int64_t V) {
     return B >= 0 && B <= (int64_t)1 << 20 && V > 0 && V <= (int64_t)1 << 22;
 }
@@ -863,6 +879,8 @@ int fni8_lora_add_ranks_f16(const void* x, int64_t ldx, int64_t T, int64_t K, co
                 aligned(b, 16) && aligned(scaling, 4) && aligned(seg_off, 4) && aligned(rows, 4) &&
                 aligned(ranks, 4),
             FNI8_ERR_ALIGN, "a and b must be 16-byte aligned, the others element-aligned");
+    REQUIRE(out == y || !rows_meet(y, 2 * ldy, out, 2 * ldo, T, 2 * N), FNI8_ERR_STRIDE,
+            "out overlaps y without being y");
     const int64_t need = fni8h::lora_workspace_bytes(T, K, S, parts * rank);
     REQUIRE(!need || (workspace && aligned(workspace, 256)), FNI8_ERR_ALIGN,
             "a 256-byte aligned workspace is required");

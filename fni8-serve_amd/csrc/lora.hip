@@ -748,17 +748,18 @@ int launch_lora_add(const LoraAdd& l, hipStream_t st) {
     const int nt = !p.big ? 1 : l.rank > 128 ? 2 : 4;
     const int64_t tiles = tiles_of(l.T, l.S + 1, 16 * nt);
     // Columns of a workgroup, whole strips of its four waves.  Tiles of 64: two strips where that
-    // leaves more than one workgroup to a CU (calls of 8192 tokens, 6144 columns: 58.8 us; 60.4
-    // with one strip, 67.8 with three; of 2048 tokens: 21.3, 23.3, 24.0; of 2048 tokens and
-    // columns, half a workgroup a CU: 13.3, 11.9, 14.9).  Of 16: the fewest rounds of the four
-    // that a CU holds at once, each as long as the columns and a start that takes about as long
-    // as 1024 of them.
+    // leaves 320 workgroups or more, else one (calls with K = 2048, rank 16, four adapters; one
+    // strip, two: 8192 tokens, 6144 columns 64.0 us, 61.0; 4096 tokens, 4096 columns 23.8, 22.1;
+    // 4096 tokens, 2048 columns 17.1, 19.7; 2048 tokens, 2048 columns 13.7, 15.7; 1024 tokens,
+    // 1024 columns 11.2, 12.7; between 320 and 550 they differ by less than 1).  Of 16: the
+    // fewest rounds of the four that a CU holds at once, each as long as the columns and a start
+    // that takes about as long as 1024 of them.
     const int64_t strips = kWaves * 64;
     int64_t cols = 0, blocks = 0, best = 0;
     for (int64_t c = strips; c <= (p.big ? 512 : 4096); c += strips) {
         int64_t n = 0;
         for (int i = 0; i < l.parts; i++) n += (l.splits[i] + c - 1) / c;
-        const int64_t cost = p.big ? (tiles * n >= 320 ? 1 : 2) * 4096 - c
+        const int64_t cost = p.big ? (tiles * n >= 320 ? -c : c)
                                    : (tiles * n + 1023) / 1024 * (c + 1024);
         if (!cols || cost < best) {
             cols = c;

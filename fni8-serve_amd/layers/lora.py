@@ -9,8 +9,8 @@ fni8serve/training/lora.py:14-170, in serving: every token of a batch has its ow
 
 A merged projection (QKV, gate and up) has one pair of matrices for each part of its output
 (splits).  The module takes the place of the linear that it wraps: GatedMLP, GQAAttention and
-LMHead call it as they call that.  GatedMLP then runs its projections one after the other, since
-the adapter reads what its fused kernels never write.  SparseMoE's experts are stacked at
+LMHead call it as they call that.  While rows have adapters GatedMLP runs its projections one after
+the other, since the adapter reads what its fused kernels never write.  SparseMoE's experts are stacked at
 construction and take no adapters.
 """
 from __future__ import annotations
@@ -23,7 +23,7 @@ from torch.nn.modules.module import _has_any_global_hook
 
 from .. import ops
 from .linear import LinearW8A8
-from .mlp import bare
+from .mlp import _DEFINED, bare
 
 
 class AdapterBatch:
@@ -118,8 +118,10 @@ class LoRALinear(nn.Module):
         return self.base.bias
 
     def _int8_ok(self, x: torch.Tensor) -> bool:
-        """Its input is needed in 16 bits: the fused chains leave it to be called."""
-        return False
+        """Where rows have adapters its input is needed in 16 bits: the fused chains leave it to be
+        called, as they do where calling it does more than the classes define."""
+        return (self.batch.ids is None and bare(self, LoRALinear) and bare(self.base, LinearW8A8)
+                and not _has_any_global_hook() and self.base._int8_ok(x))
 
     def load(self, slot: int, parts: Sequence[tuple[torch.Tensor, torch.Tensor] | None],
              scaling: float = 1.0) -> None:
@@ -185,3 +187,6 @@ class LoRALinear(nn.Module):
                     out[at, n:n + wide] += low @ self.b[e, n:n + wide, :r].float().t()
                     n += wide
         return out.to(y.dtype).reshape(y.shape)
+
+
+_DEFINED[LoRALinear] = (LoRALinear.forward, LoRALinear._int8_ok)

@@ -841,7 +841,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     [S, parts * rank, K], plan = lora_plan(ids, S).  splits: the widths of the parts of a
     merged projection, p(n) the part of column n (None: one part).  scaling fp32 [S] (None: 1).
     out: where the result goes; y itself adds in place and leaves rows without an adapter
-    untouched; None allocates it.  rank is a multiple of 8, at most 256 (zeros fill up).
+    untouched, and nothing else may share elements with y; None allocates it.  rank is a multiple of 8, at most 256 (zeros fill up).
     ranks int32 [S, parts]: how many of a part's rank are the adapter's own; the others add
     nothing, also where x holds infinities, of which zeros make NaN (None: all).
     Sums are fp32; the result is rounded once."""

@@ -545,8 +545,8 @@ int64_t fni8_paged_attention_workspace_bytes(int64_t T, int64_t Hq, int64_t Hk, 
  *            last, as segment S (fni8_moe_sort with k = 1 over S + 1 experts); no
  *            token may be there twice
  *   y        fp16 [T, N], row stride ldy; out fp16 [T, N], row stride ldo: other
- *            memory than y, or y itself (with ldo = ldy), whose rows without an
- *            adapter then stay as they are
+ *            memory than y (rows may lie between y's), or y itself (with ldo = ldy),
+ *            whose rows without an adapter then stay as they are
  *   workspace  device memory, 256-byte aligned, of at least
  *            fni8_lora_workspace_bytes(T, K, S, parts * rank) bytes; any contents;
  *            one per stream

@@ -291,3 +291,9 @@ def test_out_beside_y_in_the_same_rows(pkg, cuda, T):
     for bad in (wide[:, 5:61], wide[:, 59:115], wide.view(-1)[4:4 + T * 56].view(T, 56)):
         with pytest.raises((ValueError, RuntimeError), match="overlaps|other strides"):
             pkg.lora_add(vy, x.cuda(), a.cuda(), b.cuda(), plan, s.cuda(), [40, 16], out=bad)
+
+
+@pytest.mark.parametrize("splits", [[512], [2048], [4608, 512], [2500, 2500, 130]])
+def test_large_batches_of_every_width(pkg, cuda, splits):
+    """Tiles of 64 tokens with a workgroup for 256 columns and for 512, whole strips and not."""
+    check(pkg, *make(2100, 40, splits, 8, 3, seed=sum(splits)), splits)
