@@ -638,9 +638,14 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(const Args a) {
     }
 }
 
-// Tiles of 16 tokens, or of 64 where an adapter has that many on average and there are enough of
-// them.
-bool big_tiles(int64_t T, int64_t S) { return T >= 64 * (S < 16 ? S : 16) && T >= 1024; }
+// Tiles of 16 tokens, or of 64 from 1024 tokens on.  How many adapters share these the host does
+// not know: S counts slots, of which a step may use a few.  Tiles of 16 and of 64, calls with
+// K = 4096: 6144 columns, rank 32, 16 adapters, 1024 tokens 33.4 us, 21.5, 8192 tokens 128, 80;
+// 64 adapters, 1024 tokens 44, 31.5; 4096 columns, rank 16, 16 adapters, 1024 tokens 17.6, 15.5,
+// 8192 tokens 61, 53.  Tiles of 64 lose where an adapter has fewer than about 16 tokens: 1024
+// tokens of 128 adapters 19.8, 26.2, of 1024 adapters 77, 180; and on small projections (K = 2048,
+// 1024 columns, rank 8, 1024 tokens 10.5, 11.0).
+bool big_tiles(int64_t T) { return T >= 1024; }
 
 int64_t tiles_of(int64_t T, int64_t groups, int64_t bm) {
     return T / bm + (groups < T ? groups : T);
@@ -653,7 +658,7 @@ struct Plan {
 };
 Plan plan_of(int64_t T, int64_t K, int64_t S, int64_t R) {
     Plan p{};
-    p.big = big_tiles(T, S);
+    p.big = big_tiles(T);
     const int64_t blocks = (R + 15) / 16;
     p.tiles = tiles_of(T, S, p.big ? 64 : 16);
     if (p.big) {

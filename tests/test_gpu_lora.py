@@ -297,3 +297,12 @@ def test_out_beside_y_in_the_same_rows(pkg, cuda, T):
 def test_large_batches_of_every_width(pkg, cuda, splits):
     """Tiles of 64 tokens with a workgroup for 256 columns and for 512, whole strips and not."""
     check(pkg, *make(2100, 40, splits, 8, 3, seed=sum(splits)), splits)
+
+
+@pytest.mark.parametrize("T,S", [(1100, 200), (1024, 1024), (1500, 3000)])
+def test_large_batches_of_many_adapters(pkg, cuda, T, S):
+    """Tiles of 64 tokens with a few tokens each, slots without any among them."""
+    check(pkg, *make(T, 40, [72, 24], 8, S, seed=S), [72, 24])
+    g = torch.Generator().manual_seed(S)
+    ids = torch.randint(0, 7, (T,), generator=g) * (S // 7)
+    check(pkg, *make(T, 136, [64], 16, S, seed=S + 1, ids=ids), [64])
