@@ -217,6 +217,9 @@ __host__ __device__ inline int64_t row_bytes(int64_t V) {
     return (parts_of(V) * (8 + 8 + 8 * kScanThreads + 4) + around_of(V) * 8 + (int64_t)sizeof(Long) +
             15) / 16 * 16;
 }
+// Rows that 1 GiB of workspace holds; more take turns in it, a set of launches each (fewer than
+// 2^19 parts of rows at once).
+inline int64_t rows_at_once(int64_t V) { return ((int64_t)1 << 30) / row_bytes(V); }
 __device__ __forceinline__ Work work_of(int8_t* w, int64_t row, int64_t V) {
     const int64_t parts = parts_of(V);
     w += row * row_bytes(V);
@@ -275,8 +278,8 @@ __device__ __forceinline__ N wave_sum(N v) {
     return last_lane(wave_scan(v));
 }
 
-// An item is a part of a row; beyond 2^20 of them a workgroup takes more than one.  256 rows of 151936 fp16 (77.8 MB): 15.3 us without sums (5.1 TB/s; a read alone
-// reaches 6.1), 34 with them, where the vector unit bounds it: 18 operations a logit and its sum,
+// A workgroup has a part of a row.  256 rows of 151936 fp16 (77.8 MB): 15.3 us without sums (5.1
+// TB/s; a read alone reaches 6.1), 34 with them, where the vector unit bounds it: 18 operations a logit and its sum,
 // 15 of them of 64 bits.
 template <class E>
 __global__ __launch_bounds__(kScanThreads) void scan_kernel(const fni8h::Sample a, int parts) {
@@ -284,84 +287,80 @@ __global__ __launch_bounds__(kScanThreads) void scan_kernel(const fni8h::Sample 
     // maxima keep a NaN, and take two or three 16-bit numbers an operation
     typedef std::conditional_t<sizeof(E) == 2, _Float16, float> number
         __attribute__((ext_vector_type(8)));
-    __shared__ uint32_t tops[2][4];
-    __shared__ double sums[2][4];
+    __shared__ uint32_t tops[4];
+    __shared__ double sums[4];
     const int V = (int)a.V, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int items = (int)a.B * parts;  // fewer than 2^30
-    const int step = gridDim.x;
-    for (int item = blockIdx.x, turn = 0; item < items; item += step, turn ^= 1) {
-        const int row = item / parts, part = item - row * parts;
-        const Work w = work_of(a.work, row, V);
-        const E* x = (const E*)a.logits + row * a.ld;
-        const int i0 = part * kPart + tid * kVec;
-        vec q[kSteps];
+    const int row = blockIdx.x / (uint32_t)parts, part = blockIdx.x - row * parts;
+    const Work w = work_of(a.work, row, V);
+    const E* x = (const E*)a.logits + row * a.ld;
+    const int i0 = part * kPart + tid * kVec;
+    vec q[kSteps];
 #pragma unroll
-        for (int i = 0; i < kSteps; i++) {
-            const int at = i0 + i * kScanThreads * kVec;
-            if (at + kVec <= V) {
-                q[i] = *reinterpret_cast<const vec*>(x + at);
-            } else {
-#pragma unroll
-                for (int j = 0; j < kVec; j++) {
-                    E e = lowest_of<E>();
-                    if (at + j < V) e = x[at + j];
-                    q[i][j] = e;
-                }
-            }
-        }
-        float v[kSteps][kVec];
-        number many = __builtin_bit_cast(number, q[0]);
-#pragma unroll
-        for (int i = 1; i < kSteps; i++)
-            many = __builtin_elementwise_maximum(many, __builtin_bit_cast(number, q[i]));
-#pragma unroll
-        for (int i = 0; i < kSteps; i++)
+    for (int i = 0; i < kSteps; i++) {
+        const int at = i0 + i * kScanThreads * kVec;
+        if (at + kVec <= V) {
+            q[i] = *reinterpret_cast<const vec*>(x + at);
+        } else {
 #pragma unroll
             for (int j = 0; j < kVec; j++) {
-                const E e = q[i][j];
-                v[i][j] = value(e);
+                E e = lowest_of<E>();
+                if (at + j < V) e = x[at + j];
+                q[i][j] = e;
             }
-        auto most = many[0];
-#pragma unroll
-        for (int j = 1; j < kVec; j++) most = __builtin_elementwise_maximum(most, many[j]);
-        uint32_t best = key_of((float)most);
-        w.top[part * kScanThreads + tid] = best;
-        best = key_max(best);
-        if (lane == 0) tops[turn][wave] = best;
-        Row r(a, row, V);
-        __syncthreads();
-        for (int i = 0; i < 4; i++) best = tops[turn][i] > best ? tops[turn][i] : best;
-        if (tid == 0) w.part[part] = best;
-        if (!r.summed()) continue;
-        r.largest(value_of(best));
-        if (r.inf) {
-#pragma unroll
-            for (int i = 0; i < kSteps; i++)
-#pragma unroll
-                for (int j = 0; j < kVec; j++) v[i][j] = r.seen(v[i][j]);
         }
-        if (r.by_p) {  // samples, of loads that differ from wave to wave
-            float p = 0.0f, q = 0.0f;
+    }
+    float v[kSteps][kVec];
+    number many = __builtin_bit_cast(number, q[0]);
 #pragma unroll
-            for (int i = 0; i < kSteps; i++)
-                if (i == (wave & (kSteps - 1))) {
-                    p = v[i][1];
-                    q = v[(i + kSteps / 2) % kSteps][6];
-                }
-            w.pick[part * kScanThreads + tid] =
-                (__builtin_bit_cast(uint32_t, p) + 0x8000u) >> 16 |
-                ((__builtin_bit_cast(uint32_t, q) + 0x8000u) & 0xffff0000u);
+    for (int i = 1; i < kSteps; i++)
+        many = __builtin_elementwise_maximum(many, __builtin_bit_cast(number, q[i]));
+#pragma unroll
+    for (int i = 0; i < kSteps; i++)
+#pragma unroll
+        for (int j = 0; j < kVec; j++) {
+            const E e = q[i][j];
+            v[i][j] = value(e);
         }
-        double sum = 0.0;
+    auto most = many[0];
+#pragma unroll
+    for (int j = 1; j < kVec; j++) most = __builtin_elementwise_maximum(most, many[j]);
+    uint32_t best = key_of((float)most);
+    w.top[part * kScanThreads + tid] = best;
+    best = key_max(best);
+    if (lane == 0) tops[wave] = best;
+    Row r(a, row, V);
+    __syncthreads();
+    for (int i = 0; i < 4; i++) best = tops[i] > best ? tops[i] : best;
+    if (tid == 0) w.part[part] = best;
+    if (!r.summed()) return;
+    r.largest(value_of(best));
+    if (r.inf) {
 #pragma unroll
         for (int i = 0; i < kSteps; i++)
 #pragma unroll
-            for (int j = 0; j < kVec; j++) sum += r.weight(v[i][j]);
-        sum = wave_sum(sum);
-        if (lane == 0) sums[turn][wave] = sum;
-        __syncthreads();
-        if (tid == 0) w.sum[part] = sums[turn][0] + sums[turn][1] + sums[turn][2] + sums[turn][3];
+            for (int j = 0; j < kVec; j++) v[i][j] = r.seen(v[i][j]);
     }
+    if (r.by_p) {  // samples, of loads that differ from wave to wave
+        float p = 0.0f, q = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kSteps; i++)
+            if (i == (wave & (kSteps - 1))) {
+                p = v[i][1];
+                q = v[(i + kSteps / 2) % kSteps][6];
+            }
+        w.pick[part * kScanThreads + tid] =
+            (__builtin_bit_cast(uint32_t, p) + 0x8000u) >> 16 |
+            ((__builtin_bit_cast(uint32_t, q) + 0x8000u) & 0xffff0000u);
+    }
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < kSteps; i++)
+#pragma unroll
+        for (int j = 0; j < kVec; j++) sum += r.weight(v[i][j]);
+    sum = wave_sum(sum);
+    if (lane == 0) sums[wave] = sum;
+    __syncthreads();
+    if (tid == 0) w.sum[part] = sums[0] + sums[1] + sums[2] + sums[3];
 }
 
 struct Candidate {
@@ -1152,90 +1151,87 @@ __global__ __launch_bounds__(kScanThreads) void gather_kernel(const fni8h::Sampl
     typedef E vec __attribute__((ext_vector_type(8), aligned(sizeof(E))));
     __shared__ E logit[4][W];
     __shared__ u64 sums[4];
-    const int items = (int)a.B * parts, V = (int)a.V;
+    const int V = (int)a.V;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    for (int item = blockIdx.x; item < items; item += gridDim.x) {
-        const int row = item / parts, part = item - row * parts;
-        Row r(a, row, V);
-        if (!(r.T > 0.0f) || r.by_k || !(r.by_p || r.by_m)) continue;
-        const Work w = work_of(a.work, row, V);
-        // with top-p, the logits are on their way before it is known that the row needs them
-        if (!r.by_p && w.more->kind != kMinP) continue;
-        const E* x = (const E*)a.logits + (int64_t)row * a.ld;
-        const int i0 = part * kPart + wave * 64 * kVec;  // of the wave's first load
-        vec v[kSteps];
+    const int row = blockIdx.x / (uint32_t)parts, part = blockIdx.x - row * parts;
+    Row r(a, row, V);
+    if (!(r.T > 0.0f) || r.by_k || !(r.by_p || r.by_m)) return;
+    const Work w = work_of(a.work, row, V);
+    // with top-p, the logits are on their way before it is known that the row needs them
+    if (!r.by_p && w.more->kind != kMinP) return;
+    const E* x = (const E*)a.logits + (int64_t)row * a.ld;
+    const int i0 = part * kPart + wave * 64 * kVec;  // of the wave's first load
+    vec v[kSteps];
 #pragma unroll
-        for (int i = 0; i < kSteps; i++) {
-            const int at = i0 + (i * kScanThreads + lane) * kVec;
-            if (at + kVec <= V) {
-                v[i] = *reinterpret_cast<const vec*>(x + at);
-            } else {
+    for (int i = 0; i < kSteps; i++) {
+        const int at = i0 + (i * kScanThreads + lane) * kVec;
+        if (at + kVec <= V) {
+            v[i] = *reinterpret_cast<const vec*>(x + at);
+        } else {
 #pragma unroll
-                for (int j = 0; j < kVec; j++) {
-                    E e = lowest_of<E>();
-                    if (at + j < V) e = x[at + j];
-                    v[i][j] = e;
-                }
+            for (int j = 0; j < kVec; j++) {
+                E e = lowest_of<E>();
+                if (at + j < V) e = x[at + j];
+                v[i][j] = e;
             }
         }
-        const Long more = *w.more;
-        if (more.kind != kTopP && more.kind != kMinP) continue;
-        r.largest(value_of(more.top));
-        if (r.inf) {
-#pragma unroll
-            for (int i = 0; i < kSteps; i++)
-#pragma unroll
-                for (int j = 0; j < kVec; j++) {
-                    const E e = v[i][j];
-                    v[i][j] = element<E>(r.seen(value(e)));
-                }
-        }
-        const u64 floor = more.kind == kMinP ? r.floor() : 0;
-        const float low = __builtin_fmaxf(more.low, -0x1.fffffep127f);
-        const float high = more.kind == kMinP ? low : __builtin_fmaxf(more.high, low);
-        int n = 0;
-        uint32_t near = 0;  // this lane's around the end
+    }
+    const Long more = *w.more;
+    if (more.kind != kTopP && more.kind != kMinP) return;
+    r.largest(value_of(more.top));
+    if (r.inf) {
 #pragma unroll
         for (int i = 0; i < kSteps; i++)
 #pragma unroll
             for (int j = 0; j < kVec; j++) {
                 const E e = v[i][j];
-                const float q = value(e);
-                const bool sure = q >= high;
-                const u64 has = __ballot(sure);
-                if (sure)
-                    logit[wave][__builtin_amdgcn_mbcnt_hi(
-                        (uint32_t)(has >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)has, n))] = e;
-                n += __builtin_popcountll(has);
-                near |= (uint32_t)(q >= low && !sure) << (i * kVec + j);
+                v[i][j] = element<E>(r.seen(value(e)));
             }
-        const int some = __builtin_popcount(near), upto = wave_scan(some), around = last_lane(upto);
-        // where there is no room for them the count tells finish, which searches the whole row
-        int first = 0;  // on its way while the sums are made
-        if (around && lane == 0) first = atomicAdd(&w.more->around, around);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        u64 sum = 0;
-        for (int t = lane; t < n; t += 64) {
-            const u64 m = r.mass(value(logit[wave][t]));
-            sum += m >= floor ? m : 0;
-        }
-        sum = wave_sum(sum);
-        if (around) {
-            const int room = around_of(V);
-            int to = __builtin_amdgcn_readfirstlane(first) + upto - some;
-            for (; near; near &= near - 1, to++) {
-                const int b = __builtin_ctz(near);
-                const int index = i0 + (b / kVec * kScanThreads + lane) * kVec + b % kVec;
-                if (to < room)
-                    w.around[to] = (u64)key_of(r.seen(value(x[index]))) << 32 | (uint32_t)~index;
-            }
-        }
-        if (lane == 0) sums[wave] = sum;
-        __syncthreads();
-        if (tid == 0) w.above[part] = sums[0] + sums[1] + sums[2] + sums[3];
-        __syncthreads();  // the sums are the next item's
     }
+    const u64 floor = more.kind == kMinP ? r.floor() : 0;
+    const float low = __builtin_fmaxf(more.low, -0x1.fffffep127f);
+    const float high = more.kind == kMinP ? low : __builtin_fmaxf(more.high, low);
+    int n = 0;
+    uint32_t near = 0;  // this lane's around the end
+#pragma unroll
+    for (int i = 0; i < kSteps; i++)
+#pragma unroll
+        for (int j = 0; j < kVec; j++) {
+            const E e = v[i][j];
+            const float q = value(e);
+            const bool sure = q >= high;
+            const u64 has = __ballot(sure);
+            if (sure)
+                logit[wave][__builtin_amdgcn_mbcnt_hi(
+                    (uint32_t)(has >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)has, n))] = e;
+            n += __builtin_popcountll(has);
+            near |= (uint32_t)(q >= low && !sure) << (i * kVec + j);
+        }
+    const int some = __builtin_popcount(near), upto = wave_scan(some), around = last_lane(upto);
+    // where there is no room for them the count tells finish, which searches the whole row
+    int first = 0;  // on its way while the sums are made
+    if (around && lane == 0) first = atomicAdd(&w.more->around, around);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    u64 sum = 0;
+    for (int t = lane; t < n; t += 64) {
+        const u64 m = r.mass(value(logit[wave][t]));
+        sum += m >= floor ? m : 0;
+    }
+    sum = wave_sum(sum);
+    if (around) {
+        const int room = around_of(V);
+        int to = __builtin_amdgcn_readfirstlane(first) + upto - some;
+        for (; near; near &= near - 1, to++) {
+            const int b = __builtin_ctz(near);
+            const int index = i0 + (b / kVec * kScanThreads + lane) * kVec + b % kVec;
+            if (to < room)
+                w.around[to] = (u64)key_of(r.seen(value(x[index]))) << 32 | (uint32_t)~index;
+        }
+    }
+    if (lane == 0) sums[wave] = sum;
+    __syncthreads();
+    if (tid == 0) w.above[part] = sums[0] + sums[1] + sums[2] + sums[3];
 }
 
 // One workgroup a row with a long prefix: the list that gather left, in registers, gives the end
@@ -1383,8 +1379,7 @@ __global__ __launch_bounds__(kThreads) void finish_kernel(const fni8h::Sample a,
 template <class E>
 void launch(const fni8h::Sample& a, hipStream_t st) {
     const int parts = (int)parts_of(a.V);
-    const int64_t items = a.B * parts;
-    const uint32_t grid = (uint32_t)(items < 1 << 20 ? items : 1 << 20);
+    const uint32_t grid = (uint32_t)(a.B * parts);
     scan_kernel<E><<<grid, kScanThreads, 0, st>>>(a, parts);
     // no filter, the largest logit, or top-k of a few: no prefix is long but for equal logits
     const bool alone = (!a.temperature && !(a.temperature1 > 0.0f)) ||
@@ -1404,12 +1399,27 @@ void launch(const fni8h::Sample& a, hipStream_t st) {
 
 namespace fni8h {
 
-int64_t sample_workspace_bytes(int64_t B, int64_t V) { return B * row_bytes(V); }
+int64_t sample_workspace_bytes(int64_t B, int64_t V) {
+    const int64_t most = rows_at_once(V);
+    return (B < most ? B : most) * row_bytes(V);
+}
 
 int launch_sample(const Sample& a, hipStream_t st) {
-    if (a.B == 0) return FNI8_OK;
-    if (a.fp32) launch<float>(a, st);
-    else launch<uint16_t>(a, st);
+    const int64_t most = rows_at_once(a.V);
+    for (int64_t row = 0; row < a.B; row += most) {
+        Sample some = a;
+        some.B = a.B - row < most ? a.B - row : most;
+        some.logits = (const int8_t*)a.logits + row * a.ld * (a.fp32 ? 4 : 2);
+        if (a.u) some.u = a.u + row;
+        if (a.temperature) some.temperature = a.temperature + row;
+        if (a.top_k) some.top_k = a.top_k + row;
+        if (a.top_p) some.top_p = a.top_p + row;
+        if (a.min_p) some.min_p = a.min_p + row;
+        some.tokens = a.tokens + row;
+        if (a.logprobs) some.logprobs = a.logprobs + row;
+        if (a.fp32) launch<float>(some, st);
+        else launch<uint16_t>(some, st);
+    }
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) {
         set_error_detail("sample launch: %s", hipGetErrorString(err));

@@ -598,7 +598,8 @@ int64_t fni8_lora_workspace_bytes(int64_t T, int64_t K, int64_t S, int64_t all_r
  *   tokens   int64 [B]; logprobs fp32 [B] or NULL: the logarithm of the drawn token's
  *            share of the kept mass (0 at temperature 0)
  *   workspace  device memory, 256-byte aligned, of at least
- *            fni8_sample_workspace_bytes(B, V) bytes; any contents; one per stream
+ *            fni8_sample_workspace_bytes(B, V) bytes (at most 1 GiB: further rows take
+ *            turns in it); any contents; one per stream
  * Minus infinity is never drawn; several plus infinities share the mass.  A row with
  * a NaN (logit or temperature), or of minus infinity alone, gives the token -1 and the
  * logprob NaN.

@@ -310,3 +310,24 @@ def test_many_long_prefixes_at_once(pkg, cuda):
     for _ in range(3):
         again, logp2 = pkg.sample(x, u, return_logprobs=True, **kw)
         assert torch.equal(again, got) and torch.equal(logp2, logp)
+
+
+@pytest.mark.parametrize("fp32", [False, True])
+def test_rows_that_take_turns_in_the_workspace(pkg, cuda, fp32):
+    """More rows than 1 GiB of workspace holds: each has its own logits, number and settings."""
+    B, V = 16500, 8200
+    x, u = logits(B, V, seed=16, fp32=fp32)
+    rng = random.Random(17)
+    pick = [rng.choice(SETTINGS) for _ in range(B)]
+    col = lambda n, d, t: torch.tensor([s.get(n, d) for s in pick], dtype=t, device="cuda")  # noqa: E731
+    kw = dict(temperature=col("temperature", 1.0, torch.float32), top_k=col("top_k", 0, torch.int32),
+              top_p=col("top_p", 1.0, torch.float32), min_p=col("min_p", 0.0, torch.float32))
+    got, logp = pkg.sample(x, u, return_logprobs=True, **kw)
+    at = torch.cat([torch.arange(0, B, 211), torch.arange(15000, 15400, 7), torch.arange(B - 5, B)]).cuda()
+    some = {n: t[at] for n, t in kw.items()}
+    assert got[at].tolist() == [w[0] for w in expected(x[at], u[at], **some)]
+    for lo, hi in ((0, 300), (15100, 15400), (B - 300, B)):
+        part, logp2 = pkg.sample(x[lo:hi], u[lo:hi], return_logprobs=True,
+                                 **{n: t[lo:hi] for n, t in kw.items()})
+        assert torch.equal(part, got[lo:hi]) and torch.equal(logp2, logp[lo:hi])
+    assert torch.equal(pkg.sample(x, temperature=0.0), x.argmax(-1))

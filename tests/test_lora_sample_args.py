@@ -170,3 +170,13 @@ def test_lora_refuses_an_out_that_overlaps_y(lib):
     assert lora(lib, **far, out=P(0x1000 + 2 * 48)) == -3   # two halves of the same rows
     assert lora(lib, **far, out=P(0x1000 + 2 * 47)) == -4
     assert lora(lib, **dict(far, ldo=(1 << 24) - 8), out=P(0x1000 + 2 * 48)) == -4
+
+
+def test_sample_workspace_is_bounded(lib):
+    """Rows beyond what 1 GiB holds take turns in it."""
+    size = lib.fni8_sample_workspace_bytes
+    for V in (1, 131, 2048, 2049, 8200, 50257, 151936, 1 << 22):
+        one = size(1, V)
+        assert 0 < one < 1 << 30 and size(2, V) == 2 * one and size(0, V) == 0
+        for B in (256, 5000, 540000, 1 << 20):
+            assert size(B, V) == one * min(B, (1 << 30) // one), (B, V)
