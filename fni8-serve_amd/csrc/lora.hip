@@ -281,7 +281,9 @@ __device__ __forceinline__ bool find_block(const Args& a, int block, int& part, 
 // How many rows of the part are the adapter's: what the others (filled up) make of x is not
 // looked at, since 0 times an infinity is not 0.
 __device__ __forceinline__ int own_rank(const Args& a, int e, int part) {
-    return a.ranks ? a.ranks[(int64_t)e * a.parts + part] : a.rank;
+    int own = a.rank;
+    if (a.ranks) own = __builtin_amdgcn_readfirstlane(a.ranks[e * a.parts + part]);  // of the wave
+    return own;
 }
 
 // Eight consecutive values of a token's low-rank row, the parts added in order (MANY of them on
