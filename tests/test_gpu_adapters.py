@@ -3,6 +3,8 @@ as a serving step runs them together."""
 import pytest
 import torch
 
+import attention_ref as ref
+
 pytestmark = pytest.mark.gpu
 
 HIDDEN, INTER, HEADS, KV, DIM, VOCAB, RANK, SLOTS = 512, 1280, 8, 2, 64, 5003, 12, 6
@@ -329,3 +331,38 @@ def test_the_mlp_fuses_again_without_adapters(pkg, wl, cuda, monkeypatch):
         handle = mlp.down_proj.register_forward_hook(lambda *a: seen.append(1))
         assert torch.equal(mlp(x), plain(x)) and seen
         handle.remove()
+
+
+def test_attention_reaches_its_output_through_adapters(pkg, wl, cuda):
+    """Every stage of an attention layer with both projections adapted, over prompts and decoded
+    tokens, against its plain form from the tensors that went into it."""
+    batch = pkg.AdapterBatch(SLOTS)
+    attn = Layer(pkg, wl, batch).attn
+    cache = pkg.PagedKVCache(6, 16, KV, DIM)
+    tables = torch.arange(6, dtype=torch.int32).view(2, 3).cuda()
+    total, tab = [0, 0], attn.rotary.cos_sin.cpu()
+    for new in ([30, 7], [1, 1], [4, 1]):
+        total = [a + b for a, b in zip(total, new)]
+        T = sum(new)
+        x, ids = wl.activations(T, HIDDEN, seed=T).cuda(), torch.arange(T) % (SLOTS + 1) - 1
+        batch.assign(ids.cuda())
+        step = cache.step(tables, new, total)
+        out = attn(x, cache, step)
+        qkv = attn.qkv_proj(x)
+        assert close(qkv, by_row(pkg, attn.qkv_proj, x, ids))
+        has = (ids >= 0) & (ids < SLOTS - 1)
+        for part, base in zip(qkv[has].split(attn.qkv_proj.splits, -1),
+                              attn.qkv_proj.base(x)[has].split(attn.qkv_proj.splits, -1)):
+            assert not torch.equal(part, base)
+        q, k, v = (t.unflatten(-1, (-1, DIM)) for t in qkv.split(attn.qkv_proj.splits, -1))
+        k_got, v_got = cache.read(step.slots)
+        ref.within(k_got, *ref.norm_rope(k.cpu(), None, step.positions.cpu(), tab))
+        assert torch.equal(v_got, v.float())
+        q_got = pkg.rope(q, k, step.positions, attn.rotary.cos_sin)[0]
+        ref.within(q_got, *ref.norm_rope(q.cpu(), None, step.positions.cpu(), tab))
+        got = cache.attend(q_got, step)
+        ref.within(got, *ref.attention(q_got.cpu(), cache.k.cpu(), cache.v.cpu(), tables.cpu(), total,
+                                       [0, new[0], T], None, None))
+        low = got.flatten(1)
+        assert torch.equal(out, attn.o_proj(low)) and close(out, by_row(pkg, attn.o_proj, low, ids))
+        assert not torch.equal(out, attn.o_proj.base(low))
