@@ -68,7 +68,9 @@ __device__ __forceinline__ int lane_scan(int v) {
 }
 
 // Tile `slot` of the segments 0 .. E - 1, cut into tiles of BM tokens: its adapter and its tokens
-// r0 .. r1, or false past the last.  Bounded by T whatever seg_off holds.
+// r0 .. r1, or false past the last.  Bounded by T whatever seg_off holds.  64 segments a step, each
+// of which waits for the last: up to 64 adapters cost nothing, 512 three to four us a call, 4096
+// 37, 65534 600 (one token, and 48).
 template <int BM>
 __device__ __forceinline__ bool find_tile(const Args& a, int E, int slot, int& e, int& r0, int& r1) {
     const int lane = threadIdx.x & 63;
@@ -407,7 +409,7 @@ __device__ __forceinline__ void store_y(uint16_t* o, int left, bool whole, const
 }
 
 // Tokens without an adapter: out is y.  MANY of a wave's rows are on their way at once (3323
-// tokens, 6144 columns, half of them without: 32.0 us, 34.0 with one).
+// tokens, 6144 columns, rank 64, half of them without: 32.0 us, 34.0 with one).
 template <int MANY>
 __device__ __forceinline__ void copy_rows(const Args& a, int ahead, int r0, int count, int n0, int n1) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -543,9 +545,9 @@ __global__ __launch_bounds__(kThreads, KS <= 2 ? 4 : KS == 4 ? 2 : 1) void expan
 }
 
 // The same for tiles of 16 * NT tokens: the low-rank rows lie in LDS, a strip's rows of B serve
-// all NT groups of 16.  WHOLE: every strip is there to its end.  8192 tokens,
-// 6144 columns (201 MB of y in and out): 50 us, 4.0 TB/s; a copy in the same order of addresses
-// alone takes 39 us, one straight through 32.
+// all NT groups of 16.  WHOLE: every strip is there to its end.  8192 tokens, 6144 columns, rank
+// 32 (201 MB of y in and out): 50 us, 4.0 TB/s; a copy in the same order of addresses alone takes
+// 39 us, one straight through 32.
 template <int KS, int NT, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void expand_kernel(const Args a) {
     constexpr int TM = 16 * NT, QT = KS <= 2 ? 4 : 2;
@@ -781,8 +783,9 @@ int launch_lora_add(const LoraAdd& l, hipStream_t st) {
     }
     a.cols = (int)cols;
     a.blocks = (int)blocks;
-    // Where all strips are whole the large tiles take code without the branches for others (75.4
-    // us a call of 8192 tokens, 78.0 with them; the small tiles are as fast either way).
+    // Where all strips are whole the large tiles take code without the branches for others (a call
+    // of 8192 tokens, K = 4096, 6144 columns, rank 32: 75.4 us, 78.0 with them; the small tiles are
+    // as fast either way).
     bool whole = true;
     for (int i = 0; i < l.parts; i++) whole = whole && l.splits[i] % 64 == 0;
     const uint32_t all = (uint32_t)(tiles * blocks);

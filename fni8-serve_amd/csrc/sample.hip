@@ -25,8 +25,10 @@
 //           samples tell, and a list of the tokens around that place (min-p: the kept mass)
 //   finish  one workgroup a row: top-p's end in the list, the part that the draw falls into, and
 //           the token in it
-// A row whose list does not fit (thousands of equal logits, top-k of thousands) is searched whole
-// by its workgroup: a histogram of its mass in 2048 steps of weight, then the list of one step.
+// A row whose list does not fit is searched whole by its workgroup: a histogram of its mass in 2048
+// steps of weight, then the list of one step, 120 to 200 us for up to 64 rows of 151936.  These
+// are thousands of equal logits at an end (1.2 ms where all are equal), top-k of thousands, and
+// top-p beside min-p where the threads' maxima down to min-p's end fall short of top-p's mass.
 // Nothing depends on the number of rows: a row's token is the same in every batch.
 #include <type_traits>
 
@@ -209,7 +211,8 @@ struct Work {
     Long* more;
 };
 __host__ __device__ inline int64_t parts_of(int64_t V) { return (V + kPart - 1) / kPart; }
-// Tokens around an end that a row has room for: no row of up to kList tokens needs any.
+// Tokens around an end that a row has room for.  None for rows of up to kList tokens, which fit a
+// list whole; a flat one for which none is tried is searched whole.
 __host__ __device__ inline int64_t around_of(int64_t V) {
     return V <= kList ? 0 : V < kAround ? V : kAround;
 }
@@ -278,9 +281,9 @@ __device__ __forceinline__ N wave_sum(N v) {
     return last_lane(wave_scan(v));
 }
 
-// A workgroup has a part of a row.  256 rows of 151936 fp16 (77.8 MB): 15.3 us without sums (5.1
-// TB/s; a read alone reaches 6.1), 34 with them, where the vector unit bounds it: 18 operations a logit and its sum,
-// 15 of them of 64 bits.
+// A workgroup has a part of a row.  256 rows of 151936 fp16 (77.8 MB): 14.1 us without sums (5.5
+// TB/s; a read alone reaches 6.1), 30.9 with them and 32.5 with top-p's samples too, where the
+// vector unit bounds it: 18 operations a logit and its sum, 15 of them of 64 bits.
 template <class E>
 __global__ __launch_bounds__(kScanThreads) void scan_kernel(const fni8h::Sample a, int parts) {
     typedef E vec __attribute__((ext_vector_type(8), aligned(sizeof(E))));
@@ -791,8 +794,8 @@ __device__ __forceinline__ void find_ends(Shared& sh, Turn& turn, const Work& w,
 static_assert(kThreads * 2 * kVec == kPart && kPart == kSteps * kScanThreads * kVec, "parts");
 
 // One workgroup a row: a chain of searches, each a few round trips to LDS and the cache, so it is
-// bound by their latency, not by bytes (a list of 50 of 151936: 10.6 us for one row; of hundreds,
-// 64 rows: 17 us; no filter, 256 rows: 6.8 us).
+// bound by their latency, not by bytes (a list of 50 of 151936: 10.1 us for one row; of hundreds,
+// 64 rows: 17 us; no filter, 256 rows: 6.7 us; the largest logit, 256 rows: 4.0 us).
 // ALONE: no other launch follows, and a row whose list does not fit is searched whole.
 template <class E, bool ALONE>
 __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, int parts) {
@@ -1143,8 +1146,10 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const fni8h::Sample a, i
 // around the end of top-p.  Each wave first moves the logits of its 2048 that are certain next to
 // each other in LDS, so that their exponentials, 18 operations, are not computed for the others;
 // the few around the end are read again.  256 rows of 151936 fp16 with top-p 0.95, a fifth of
-// the logits kept: 36 us; 56 with the exponentials of all, 43 with the logits loaded only once
-// the row is known to need them and the row's largest found again by each workgroup.
+// the logits kept: 30.6 us.  While a workgroup went through several parts it was 36, 56 with the
+// exponentials of all, and 43 with the logits loaded only once the row is known to need them and
+// the row's largest found again by each workgroup (two changes at once).  The early loads are
+// in vain for rows whose prefix is short: 256 of them, 12.2 us.
 template <class E>
 __global__ __launch_bounds__(kScanThreads) void gather_kernel(const fni8h::Sample a, int parts) {
     constexpr int W = 64 * kVec * kSteps;  // logits of a wave

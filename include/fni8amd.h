@@ -583,9 +583,10 @@ int64_t fni8_lora_workspace_bytes(int64_t T, int64_t K, int64_t S, int64_t all_r
  * min_p those with w_i >= min_p: each keeps a first run of the order, the
  * shortest counts, and the first token is always in it.  The token drawn is the
  * first kept one, in index order, at which the running mass exceeds u times the
- * kept mass.  Under a filter masses are integers of 62 bits, in which a weight below
- * 2^-45 of the largest (at 151936 tokens) counts as 0, without one sums of 64-bit
- * floats in a fixed order: the same row gives the same token in any batch.
+ * kept mass.  A weight is off by at most 2.2e-12 of itself.  Under a filter masses are
+ * integers of 62 bits, in which a weight below 2^-45 of the largest (at 151936
+ * tokens) counts as 0, without one sums of 64-bit floats in a fixed order: the same
+ * row gives the same token in any batch.
  *   logits   fp16 or (fp32 != 0) fp32 [B, V], row stride ldl; V <= 2^22
  *   u        fp32 [B] in [0, 1) (below: as 0, NaN too; 1 and above: the last kept
  *            token), or NULL: 0
