@@ -1410,6 +1410,7 @@ int64_t sample_workspace_bytes(int64_t B, int64_t V) {
 }
 
 int launch_sample(const Sample& a, hipStream_t st) {
+    if (a.B == 0) return FNI8_OK;
     const int64_t most = rows_at_once(a.V);
     for (int64_t row = 0; row < a.B; row += most) {
         Sample some = a;
